@@ -362,6 +362,118 @@ int nmoe_full_attn_step_batched(const nmoe_full_attn_weights *w, int batch, cons
                                 float *out, void *workspace, void *stream);
 size_t nmoe_full_attn_batched_workspace_bytes(int batch);
 
+/* ---- Full attention over a paged cache: append, prompt, single token --------------------
+ * The reference keeps one dense cache and takes a prompt token by token (src/runtime.m:3816);
+ * these take packed prompts and decode batches over a bf16 cache in pages. Every pointer but
+ * the structs is DEVICE memory of the current device, 16-byte aligned (the int32 arrays 4).
+ *
+ * Sequences are packed: sequence b's rows are cu_rows[b] .. cu_rows[b + 1] - 1 (int32
+ * [num_seqs + 1], not decreasing, cu_rows[num_seqs] <= total_rows), and its cache holds
+ * kv_lens[b] positions (int32 [num_seqs]) once those rows are appended: its i-th row is at
+ * position kv_lens[b] - (cu_rows[b + 1] - cu_rows[b]) + i. Lengths of zero are allowed.
+ * Rows from cu_rows[num_seqs] on belong to no sequence and are left as they are. */
+typedef struct nmoe_full_attn_shape {
+    int q_heads, kv_heads; /* q_heads = 1..8 times kv_heads; query head h reads KV head h / (q_heads / kv_heads) */
+    int head_dim;          /* 128 or 256                                                       */
+    int rotary_dims;       /* rotate-half on dims 0..rotary_dims-1, pairs (t, t + rotary_dims / 2):
+                              0 (none) or a power of two from 16 to head_dim                   */
+    int gated;             /* 1: a query row holds [query | gate] per head and the attention is
+                              multiplied with sigmoid(gate); 0: [query] per head               */
+    float rope_theta;      /* > 0: pair t turns by position * theta^(-2 t / rotary_dims); the angle
+                              is reduced in 64 bits                                            */
+    float norm_eps;        /* >= 0: x * rsqrt(mean(x^2) + eps) * (w + 1), w = q_norm / k_norm (bf16
+                              [head_dim]); a NULL norm weight leaves the head as it is         */
+} nmoe_full_attn_shape;
+/* Keys and values in pages: element (page, row, head, dim) is at page * page_stride +
+ * row * row_stride + head * head_stride + dim (strides in elements, multiples of 8, the same
+ * for k and v), so [page][row][head][dim] and [page][head][row][dim] both fit. Position p of
+ * sequence b lies in page block_table[b * table_stride + p / page_size], row p % page_size, for
+ * p < max_pages * page_size (at most 2^31 - 1 positions). An entry outside [0, num_pages) is no
+ * page: nothing is written there, and its positions are left out of every softmax. */
+typedef struct nmoe_paged_kv {
+    uint16_t *k, *v;             /* bf16 */
+    int64_t page_stride, row_stride, head_stride;
+    int num_pages, page_size;
+    const int32_t *block_table;  /* [num_seqs][table_stride] */
+    int max_pages;               /* entries of a row of the table */
+    int64_t table_stride;
+} nmoe_paged_kv;
+
+/* Append the packed rows' keys (normalised with k_norm, rotated, rounded to nearest-even bf16)
+ * and values (rounded) at their positions. k_new / v_new: [total_rows][kv_heads][head_dim] in
+ * x_dtype (NMOE_DTYPE_F32 or NMOE_DTYPE_BF16), row r at r * kv_stride elements (0: packed;
+ * rows 16-byte aligned). A row whose position lies outside [0, max_pages * page_size) or in no
+ * page is skipped. Only w->k_norm is read. One launch; allocates nothing; capturable. */
+int nmoe_full_attn_append_paged(const nmoe_full_attn_weights *w, const nmoe_full_attn_shape *shape,
+                                const nmoe_paged_kv *kv, int num_seqs, int total_rows,
+                                const int32_t *cu_rows, const int32_t *kv_lens, const void *k_new,
+                                const void *v_new, int x_dtype, int64_t kv_stride, void *stream);
+
+/* Causal attention of packed prompts, or chunks of prompts, over the cache, which holds their
+ * keys and values already (nmoe_full_attn_append_paged): the row at position p attends to the
+ * positions 0..p of its sequence, scores times `scale` (0: 1 / sqrt(head_dim)). q:
+ * [total_rows][q_heads][head_dim, or 2 head_dim when gated] in x_dtype, row r at r * q_stride
+ * elements (0: packed); normalised with q_norm and rotated here (w->k_norm is not read). out:
+ * bf16 [total_rows][q_heads][head_dim]. Queries, probabilities and the cache meet in bf16
+ * tensor-core products with fp32 sums. A row that sees no position (a negative position, or no
+ * page) gets zeros. kv_lens beyond max_pages * page_size: the positions past it do not exist.
+ * A NaN or infinity in a position reaches only rows of its own sequence. workspace:
+ * nmoe_full_attn_prefill_paged_workspace_bytes(), not shared by calls that overlap.
+ * Allocates nothing; capturable. */
+int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, const nmoe_full_attn_shape *shape,
+                                 const nmoe_paged_kv *kv, int num_seqs, int total_rows,
+                                 const int32_t *cu_rows, const int32_t *kv_lens, const void *q,
+                                 int x_dtype, int64_t q_stride, float scale, uint16_t *out,
+                                 void *workspace, void *stream);
+size_t nmoe_full_attn_prefill_paged_workspace_bytes(const nmoe_full_attn_shape *shape, int num_seqs,
+                                                    int total_rows);
+
+/* One new token for each of `batch` sequences, at position kv_lens[b] - 1: its key and value
+ * are appended (as by nmoe_full_attn_append_paged) and its query attends to the positions
+ * 0..kv_lens[b] - 1. k_new and v_new may both be NULL: the cache then holds them already. q,
+ * k_new, v_new as above with one row per sequence; out [batch][q_heads][head_dim] in out_dtype
+ * (F32 or BF16). Queries and probabilities are split into bf16 parts, so sums are as exact as
+ * in fp32 (out_dtype F32) or to about 2^-17 (BF16). kv_lens[b] < 1, or beyond max_pages *
+ * page_size: zeros, nothing appended. workspace: nmoe_full_attn_step_paged_workspace_bytes(),
+ * 16-byte aligned, not shared by calls that overlap. Two launches; allocates nothing; capturable
+ * (lengths on the device: one graph serves every step). */
+int nmoe_full_attn_step_paged(const nmoe_full_attn_weights *w, const nmoe_full_attn_shape *shape,
+                              const nmoe_paged_kv *kv, int batch, const int32_t *kv_lens,
+                              const void *q, int64_t q_stride, const void *k_new, const void *v_new,
+                              int64_t kv_stride, int x_dtype, float scale, void *out, int out_dtype,
+                              void *workspace, void *stream);
+size_t nmoe_full_attn_step_paged_workspace_bytes(const nmoe_full_attn_shape *shape, int batch);
+
+/* ---- Linear attention over packed prompts -------------------------------------------------
+ * The steps of nmoe_linear_attn_step for whole prompts, or chunks of them: convolution, q/k
+ * norms, decay, gated delta rule and gated norm of every packed row (cu_rows as above), going
+ * on from each sequence's states and leaving the states that the next chunk or
+ * nmoe_linear_attn_step goes on from. Head dim 128, conv width 4; conv channels (2 key_heads +
+ * value_heads) * 128: q, then k, then v; value head h reads key head h / (value_heads /
+ * key_heads). All weights as in nmoe_linear_attn_weights for that many heads.
+ * DEVICE pointers, 16-byte aligned: qkv [total_rows][channels], z [total_rows][value_heads *
+ * 128], alpha / beta [total_rows][value_heads], all in x_dtype, row r at r * its stride in
+ * elements (0: packed; qkv and z rows 16-byte aligned). conv_in / conv_out f32
+ * [num_seqs][3][channels], delta_in / delta_out f32 [num_seqs][value_heads][128][128] (in and
+ * out may be the same buffer; in may be NULL: zeros, a new sequence). A sequence without rows
+ * gets its states unchanged. out [total_rows][value_heads * 128] in out_dtype. Sums, states and
+ * norms are fp32. workspace: nmoe_linear_attn_prefill_workspace_bytes(), 16-byte aligned, not
+ * shared by calls that overlap. Allocates nothing; capturable. */
+typedef struct nmoe_linear_attn_shape {
+    int key_heads, value_heads; /* value_heads a multiple of key_heads; Qwen3.6: 16 and 32 */
+} nmoe_linear_attn_shape;
+int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const nmoe_linear_attn_shape *shape,
+                             int num_seqs, int total_rows, const int32_t *cu_rows, const void *qkv,
+                             int64_t qkv_stride, const void *z, int64_t z_stride, const void *alpha,
+                             const void *beta, int64_t ab_stride, int x_dtype, const float *conv_in,
+                             const float *delta_in, float *conv_out, float *delta_out, void *out,
+                             int out_dtype, void *workspace, void *stream);
+size_t nmoe_linear_attn_prefill_workspace_bytes(const nmoe_linear_attn_shape *shape, int num_seqs,
+                                                int total_rows);
+/* Message of the last of the calls above that returned an error on this host thread. */
+const char *nmoe_full_attn_error(void);
+const char *nmoe_linear_attn_error(void);
+
 /* ---- Whole decode step ------------------------------------------
  * The C restatement of NMOEProcessToken (src/runtime.m:3712-3805) on the GPU: embedding
  * row, 40 layers (layer l is full attention when (l + 1) % 4 == 0, else linear attention:

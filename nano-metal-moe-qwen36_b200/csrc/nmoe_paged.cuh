@@ -1,0 +1,145 @@
+// nmoe_paged.cuh -- what the paged full-attention kernels share: the device view of a paged
+// cache, the row -> sequence search, and the preparation of one head (RMS norm, rotation).
+#pragma once
+#include <cuda_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "nmoe/moe_cuda.h"
+#include "nmoe_common.cuh"
+
+namespace nmoe {
+
+struct PagedDev {
+    uint16_t *k, *v;
+    long long page_stride, row_stride, head_stride;   // elements
+    const int *table;
+    long long table_stride;
+    int num_pages, page_size, max_pages;
+    int capacity;   // max_pages * page_size positions (checked to fit an int)
+};
+
+// Rotation frequencies theta^(-2 t / rotary_dims), t < half, in 64 bits: the angle position *
+// freq has to be reduced before it is rounded (an fp32 angle at position 32768 is off by 2e-3).
+struct RotaryDev {
+    double freq[128];
+    int half;   // rotary_dims / 2
+};
+
+struct HeadDev {
+    const uint16_t *q_norm, *k_norm;   // bf16 [head_dim] or null
+    float eps;
+};
+
+__device__ __forceinline__ float2 rotary_cs(double freq, int position) {
+    double a = (double)position * freq;
+    a -= rint(a * 0.15915494309189535) * 6.283185307179586;
+    float s, c;
+    sincosf((float)a, &s, &c);
+    return make_float2(c, s);
+}
+
+// Element offset of (sequence, position) without the head, or -1: no page holds it.
+__device__ __forceinline__ long long paged_row(const PagedDev &c, int seq, int position) {
+    if (position < 0 || position >= c.capacity) return -1;
+    const int slot = (unsigned)position / (unsigned)c.page_size;
+    const int page = c.table[(long long)seq * c.table_stride + slot];
+    if (page < 0 || page >= c.num_pages) return -1;
+    return (long long)page * c.page_stride + (long long)(position - slot * c.page_size) * c.row_stride;
+}
+
+// One warp: the sequence that holds packed row r (cu[b] <= r < cu[b + 1]), or -1 for a row
+// behind the last sequence. 32-ary search: log32(n) dependent loads.
+__device__ __forceinline__ int find_sequence(const int *cu, int n, int r, int lane) {
+    int lo = 0, len = n;   // the answer, the number of i in 1..n with cu[i] <= r, is in [lo, lo + len]
+    while (len > 0) {
+        const int step = (len + 31) / 32;
+        const int i = lo + (lane + 1) * step;
+        const bool below = (lane + 1) * step <= len && cu[i] <= r;
+        const int full = __popc(__ballot_sync(0xffffffffu, below));
+        lo += full * step;
+        len = min(step - 1, len - full * step);
+    }
+    return lo < n && cu[0] <= r ? lo : -1;
+}
+
+template <int E>
+__device__ __forceinline__ void load_elems(const void *base, long long at, bool bf16, float *v) {
+    if (bf16) {
+        const uint16_t *p = static_cast<const uint16_t *>(base) + at;
+        uint32_t w[E / 2];
+        if constexpr (E == 8) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(p);
+            w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p);
+            w[0] = u.x, w[1] = u.y;
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) v[2 * i] = bf16_lo(w[i]), v[2 * i + 1] = bf16_hi(w[i]);
+    } else {
+        const float4 *p = reinterpret_cast<const float4 *>(static_cast<const float *>(base) + at);
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) {
+            const float4 f = p[i];
+            v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t pack2_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int E>
+__device__ __forceinline__ void store_bf16(uint16_t *p, const float *v) {
+    if constexpr (E == 8)
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]),
+                                                   pack2_bf16(v[4], v[5]), pack2_bf16(v[6], v[7]));
+    else
+        *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+}
+
+// One warp prepares one head of 32 E dims, lane l holding dims E l .. E l + E - 1: RMS norm by
+// (weight + 1), then the rotation of dims 0 .. 2 half - 1 with the row's (cos, sin) table cs[half].
+// half is a power of two of at least 8 >= E, so a pair's other dim is in lane ^ (half / E).
+template <int E>
+__device__ __forceinline__ void prepare_head(float *v, const uint16_t *weight, float eps, const float2 *cs, int half,
+                                             int lane) {
+    if (weight != nullptr) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
+        const float inv = rsqrtf(warp_sum(ss) / (float)(32 * E) + eps);
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] = v[i] * inv * (bf16_to_f32(weight[E * lane + i]) + 1.0f);
+    }
+    if (half > 0) {
+        const int d = E * lane;
+        const bool second = d >= half;
+        const float2 *t = cs + (d & (half - 1));
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float other = __shfl_xor_sync(0xffffffffu, v[i], half / E);
+            if (d < 2 * half) {
+                const float2 k = t[i];
+                v[i] = second ? fmaf(other, k.y, v[i] * k.x) : fmaf(-other, k.y, v[i] * k.x);
+            }
+        }
+    }
+}
+
+// ---- host side -------------------------------------------------------------------------------
+// Fills the message of nmoe_full_attn_error() and returns `status`.
+int full_attn_fail(int status, const char *fmt, ...);
+int check_full_attn_shape(const nmoe_full_attn_weights *w, const nmoe_full_attn_shape *s);
+int check_paged_kv(const nmoe_paged_kv *kv, PagedDev *dev);
+void fill_rotary(const nmoe_full_attn_shape *s, RotaryDev *r);
+int check_x(const char *what, const void *p, int x_dtype, long long stride, long long width);
+int device_sm_count(int *sms);
+
+inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+}  // namespace nmoe

@@ -35,6 +35,9 @@ ABI_SYMBOLS = (
     "nmoe_moe_load_layer_checked", "nmoe_moe_load_layer_file_checked", "nmoe_crc32c", "nmoe_crc32c_combine",
     "nmoe_crc32c_device", "nmoe_linear_attn_step", "nmoe_full_attn_step", "nmoe_full_attn_workspace_bytes",
     "nmoe_full_attn_step_batched", "nmoe_linear_attn_step_batched", "nmoe_full_attn_batched_workspace_bytes",
+    "nmoe_full_attn_append_paged", "nmoe_full_attn_prefill_paged", "nmoe_full_attn_prefill_paged_workspace_bytes",
+    "nmoe_full_attn_step_paged", "nmoe_full_attn_step_paged_workspace_bytes", "nmoe_full_attn_error",
+    "nmoe_linear_attn_prefill", "nmoe_linear_attn_prefill_workspace_bytes", "nmoe_linear_attn_error",
     "nmoe_decoder_create", "nmoe_decoder_destroy", "nmoe_decoder_error", "nmoe_decoder_set_linear_layer",
     "nmoe_decoder_set_full_layer", "nmoe_decoder_set_globals", "nmoe_decoder_reset", "nmoe_decoder_step",
 )
@@ -70,6 +73,30 @@ class LinearAttnWeights(C.Structure):
 
 class FullAttnWeights(C.Structure):
     _fields_ = [("q_norm", C.c_void_p), ("k_norm", C.c_void_p)]
+
+
+class FullAttnShape(C.Structure):
+    """nmoe_full_attn_shape: heads, head dim and rotation of the paged full-attention calls."""
+    _fields_ = [("q_heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int), ("rotary_dims", C.c_int),
+                ("gated", C.c_int), ("rope_theta", C.c_float), ("norm_eps", C.c_float)]
+
+    def __init__(self, q_heads=16, kv_heads=2, head_dim=256, rotary_dims=64, gated=True, rope_theta=1e7,
+                 norm_eps=1e-6):
+        super().__init__(q_heads, kv_heads, head_dim, rotary_dims, int(bool(gated)), rope_theta, norm_eps)
+
+
+class PagedKVHost(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64), ("num_pages", C.c_int), ("page_size", C.c_int),
+                ("block_table", C.c_void_p), ("max_pages", C.c_int), ("table_stride", C.c_int64)]
+
+
+class LinearAttnShape(C.Structure):
+    """nmoe_linear_attn_shape: heads of nmoe_linear_attn_prefill (head dim 128)."""
+    _fields_ = [("key_heads", C.c_int), ("value_heads", C.c_int)]
+
+    def __init__(self, key_heads=16, value_heads=32):
+        super().__init__(key_heads, value_heads)
 
 
 class LinearLayerHost(C.Structure):
@@ -170,6 +197,27 @@ def lib() -> C.CDLL:
     L.nmoe_full_attn_step_batched.argtypes = [C.POINTER(FullAttnWeights), i, vp, vp, vp, vp, vp, vp, i, vp, vp, vp]
     L.nmoe_full_attn_batched_workspace_bytes.restype = sz
     L.nmoe_full_attn_batched_workspace_bytes.argtypes = [i]
+    i64, f32 = C.c_int64, C.c_float
+    L.nmoe_full_attn_append_paged.restype = i
+    L.nmoe_full_attn_append_paged.argtypes = [C.POINTER(FullAttnWeights), C.POINTER(FullAttnShape),
+                                              C.POINTER(PagedKVHost), i, i, vp, vp, vp, vp, i, i64, vp]
+    L.nmoe_full_attn_prefill_paged.restype = i
+    L.nmoe_full_attn_prefill_paged.argtypes = [C.POINTER(FullAttnWeights), C.POINTER(FullAttnShape),
+                                               C.POINTER(PagedKVHost), i, i, vp, vp, vp, i, i64, f32, vp, vp, vp]
+    L.nmoe_full_attn_prefill_paged_workspace_bytes.restype = sz
+    L.nmoe_full_attn_prefill_paged_workspace_bytes.argtypes = [C.POINTER(FullAttnShape), i, i]
+    L.nmoe_full_attn_step_paged.restype = i
+    L.nmoe_full_attn_step_paged.argtypes = [C.POINTER(FullAttnWeights), C.POINTER(FullAttnShape),
+                                            C.POINTER(PagedKVHost), i, vp, vp, i64, vp, vp, i64, i, f32, vp, i, vp, vp]
+    L.nmoe_full_attn_step_paged_workspace_bytes.restype = sz
+    L.nmoe_full_attn_step_paged_workspace_bytes.argtypes = [C.POINTER(FullAttnShape), i]
+    L.nmoe_full_attn_error.restype = C.c_char_p
+    L.nmoe_linear_attn_prefill.restype = i
+    L.nmoe_linear_attn_prefill.argtypes = [C.POINTER(LinearAttnWeights), C.POINTER(LinearAttnShape), i, i, vp, vp, i64,
+                                           vp, i64, vp, vp, i64, i, vp, vp, vp, vp, vp, i, vp, vp]
+    L.nmoe_linear_attn_prefill_workspace_bytes.restype = sz
+    L.nmoe_linear_attn_prefill_workspace_bytes.argtypes = [C.POINTER(LinearAttnShape), i, i]
+    L.nmoe_linear_attn_error.restype = C.c_char_p
     L.nmoe_decoder_create.restype = vp
     L.nmoe_decoder_create.argtypes = [vp, i, i, i, C.POINTER(i)]
     L.nmoe_decoder_destroy.argtypes = [vp]
@@ -537,6 +585,209 @@ def full_attn_step_batched(weights: dict, q, k_new, v_new, k_cache, v_cache, pos
                                            _ptr(workspace), stream)
     if rc != OK:
         raise NmoeError(rc, "nmoe_full_attn_step_batched")
+
+
+_kinds = None
+
+
+def _dtypes():
+    """torch element types by dtype code (bf16 also as raw 16-bit words); torch is imported at first use."""
+    global _kinds
+    if _kinds is None:
+        import torch
+        _kinds = {DTYPE_F32: (torch.float32,), DTYPE_BF16: (torch.bfloat16, torch.int16), "i32": torch.int32,
+                  "device": torch.cuda.current_device if torch.cuda.is_available() else lambda: None}
+    return _kinds
+
+
+def _device_tensors(*tensors):
+    """The calls below take torch tensors: on the current device, so that a kernel never meets
+    memory of another one."""
+    here = _dtypes()["device"]()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
+            raise NmoeError(EINVAL, f"a tensor is on {t.device}, not on the current CUDA device")
+
+
+def _int32(t, n, name):
+    if t.dtype != _dtypes()["i32"] or not t.is_contiguous() or t.numel() < n:
+        raise NmoeError(EINVAL, f"{name} must be a contiguous int32 tensor of at least {n} entries")
+
+
+def _rows(t, rows, width, dtype, name):
+    """Row stride in elements of a [rows][width] operand whose rows are contiguous."""
+    want = _dtypes().get(dtype)
+    if want is None or t.dtype not in want:
+        raise NmoeError(EINVAL, f"{name}: element type {t.dtype} does not match the dtype argument {dtype}")
+    shape = t.shape
+    if len(shape) == 2 and shape[0] >= rows and shape[1] == width and (t.stride(1) == 1 or width == 1):
+        return t.stride(0) if shape[0] > 1 else width
+    if rows == 0:
+        return width
+    if len(shape) < 2 or shape[0] < rows or t[0].numel() != width or not t[0].is_contiguous():
+        raise NmoeError(EINVAL, f"{name} must hold at least {rows} rows of {width} contiguous elements")
+    return t.stride(0) if shape[0] > 1 else width
+
+
+def _output(t, n, dtype, name="out"):
+    if t.dtype not in _dtypes().get(dtype, ()) or not t.is_contiguous() or t.numel() < n:
+        raise NmoeError(EINVAL, f"{name} must be a contiguous tensor of {n} elements in its dtype")
+
+
+def _states(t, n, name):
+    if t is not None and (t.dtype not in _dtypes()[DTYPE_F32] or not t.is_contiguous() or t.numel() != n):
+        raise NmoeError(EINVAL, f"{name} must be a contiguous float32 tensor of {n} elements")
+
+
+def _workspace(t, need):
+    if need and (t is None or t.numel() * t.element_size() < need):
+        raise NmoeError(EINVAL, f"workspace of at least {need} bytes needed")
+
+
+class PagedKV:
+    """nmoe_paged_kv: bf16 pages k, v [pages][page_size][kv_heads][head_dim] (any strides, the
+    same for both, the last one 1) and an int32 block table [sequences][max_pages]. Holds the
+    tensors; the cache may be used by every layer call of its layer."""
+
+    def __init__(self, k, v, block_table):
+        import torch
+        for t in (k, v):
+            if t.dim() != 4 or t.dtype not in (torch.bfloat16, torch.int16) or t.stride(3) != 1:
+                raise NmoeError(EINVAL, "pages must be bf16 [pages][page_size][kv_heads][head_dim], the last stride 1")
+        if k.shape != v.shape or k.stride() != v.stride():
+            raise NmoeError(EINVAL, "k and v pages must have one shape and one set of strides")
+        if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+            raise NmoeError(EINVAL, "block_table must be int32 [sequences][max_pages], the last stride 1")
+        _device_tensors(k, v, block_table)
+        self.k, self.v, self.block_table = k, v, block_table
+        self.host = PagedKVHost(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), k.shape[0],
+                                k.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.stride(0))
+
+    def _check(self, shape, seqs):
+        if self.k.shape[2] != shape.kv_heads or self.k.shape[3] != shape.head_dim:
+            raise NmoeError(EINVAL, f"pages of {tuple(self.k.shape[2:])} (KV heads, head dim) do not fit the shape")
+        if self.block_table.shape[0] < seqs:
+            raise NmoeError(EINVAL, "block_table has fewer rows than there are sequences")
+
+
+def _full_attn_check(rc):
+    if rc != OK:
+        raise NmoeError(rc, lib().nmoe_full_attn_error().decode())
+
+
+def _norms(weights, shape):
+    q, k = weights.get("q_norm"), weights.get("k_norm")
+    for t in (q, k):
+        if t is not None and (t.dtype not in _dtypes()[DTYPE_BF16] or not t.is_contiguous()
+                              or t.numel() != shape.head_dim):
+            raise NmoeError(EINVAL, f"q_norm and k_norm must be contiguous bf16 tensors of {shape.head_dim}")
+    _device_tensors(q, k)
+    return FullAttnWeights(_ptr(q), _ptr(k))
+
+
+def full_attn_append_paged(weights: dict, shape: FullAttnShape, cache: PagedKV, k_new, v_new, cu_rows, kv_lens,
+                           x_dtype=DTYPE_BF16, stream=0):
+    """nmoe_full_attn_append_paged: normalise and rotate the packed rows' keys and append keys
+    and values to their pages. k_new / v_new [rows][kv_heads * head_dim] (one row stride for both)."""
+    seqs, rows, width = cu_rows.numel() - 1, k_new.shape[0], shape.kv_heads * shape.head_dim
+    _device_tensors(k_new, v_new, cu_rows, kv_lens)
+    _int32(cu_rows, 1, "cu_rows")
+    _int32(kv_lens, seqs, "kv_lens")
+    cache._check(shape, seqs)
+    stride = _rows(k_new, rows, width, x_dtype, "k_new")
+    if _rows(v_new, rows, width, x_dtype, "v_new") != stride:
+        raise NmoeError(EINVAL, "k_new and v_new must have the same row stride")
+    w = _norms(weights, shape)
+    _full_attn_check(lib().nmoe_full_attn_append_paged(C.byref(w), C.byref(shape), C.byref(cache.host), seqs, rows,
+                                                       _ptr(cu_rows), _ptr(kv_lens), _ptr(k_new), _ptr(v_new), x_dtype,
+                                                       stride, stream))
+
+
+def full_attn_prefill_paged_workspace_bytes(shape: FullAttnShape, num_seqs: int, total_rows: int) -> int:
+    return int(lib().nmoe_full_attn_prefill_paged_workspace_bytes(C.byref(shape), num_seqs, total_rows))
+
+
+def full_attn_prefill_paged(weights: dict, shape: FullAttnShape, cache: PagedKV, q, cu_rows, kv_lens, out, workspace,
+                            x_dtype=DTYPE_BF16, scale=0.0, stream=0):
+    """nmoe_full_attn_prefill_paged: causal attention of packed prompts over the cache, which
+    holds their keys and values. q [rows][q_heads * head_dim (* 2 when gated)], out bf16
+    [rows][q_heads * head_dim]."""
+    seqs, rows, width = cu_rows.numel() - 1, q.shape[0], shape.q_heads * shape.head_dim
+    _device_tensors(q, cu_rows, kv_lens, out, workspace)
+    _int32(cu_rows, 1, "cu_rows")
+    _int32(kv_lens, seqs, "kv_lens")
+    cache._check(shape, seqs)
+    stride = _rows(q, rows, width * (2 if shape.gated else 1), x_dtype, "q")
+    _output(out, rows * width, DTYPE_BF16)
+    _workspace(workspace, full_attn_prefill_paged_workspace_bytes(shape, seqs, rows))
+    w = _norms(weights, shape)
+    _full_attn_check(lib().nmoe_full_attn_prefill_paged(C.byref(w), C.byref(shape), C.byref(cache.host), seqs, rows,
+                                                        _ptr(cu_rows), _ptr(kv_lens), _ptr(q), x_dtype, stride, scale,
+                                                        _ptr(out), _ptr(workspace), stream))
+
+
+def full_attn_step_paged_workspace_bytes(shape: FullAttnShape, batch: int) -> int:
+    return int(lib().nmoe_full_attn_step_paged_workspace_bytes(C.byref(shape), batch))
+
+
+def full_attn_step_paged(weights: dict, shape: FullAttnShape, cache: PagedKV, kv_lens, q, k_new, v_new, out, workspace,
+                         x_dtype=DTYPE_F32, out_dtype=DTYPE_F32, scale=0.0, stream=0):
+    """nmoe_full_attn_step_paged: one new token per sequence over the pages. kv_lens counts the
+    new token; k_new = v_new = None when the cache holds it already."""
+    batch, width, kw = q.shape[0], shape.q_heads * shape.head_dim, shape.kv_heads * shape.head_dim
+    _device_tensors(q, k_new, v_new, kv_lens, out, workspace)
+    _int32(kv_lens, batch, "kv_lens")
+    cache._check(shape, batch)
+    stride, kv_stride = _rows(q, batch, width * (2 if shape.gated else 1), x_dtype, "q"), 0
+    if (k_new is None) != (v_new is None):
+        raise NmoeError(EINVAL, "k_new and v_new go together")
+    if k_new is not None:
+        kv_stride = _rows(k_new, batch, kw, x_dtype, "k_new")
+        if _rows(v_new, batch, kw, x_dtype, "v_new") != kv_stride:
+            raise NmoeError(EINVAL, "k_new and v_new must have the same row stride")
+    _output(out, batch * width, out_dtype)
+    _workspace(workspace, full_attn_step_paged_workspace_bytes(shape, batch))
+    w = _norms(weights, shape)
+    _full_attn_check(lib().nmoe_full_attn_step_paged(C.byref(w), C.byref(shape), C.byref(cache.host), batch,
+                                                     _ptr(kv_lens), _ptr(q), stride, _ptr(k_new), _ptr(v_new),
+                                                     kv_stride, x_dtype, scale, _ptr(out), out_dtype, _ptr(workspace),
+                                                     stream))
+
+
+def linear_attn_prefill_workspace_bytes(shape: LinearAttnShape, num_seqs: int, total_rows: int) -> int:
+    return int(lib().nmoe_linear_attn_prefill_workspace_bytes(C.byref(shape), num_seqs, total_rows))
+
+
+def linear_attn_prefill(weights: dict, shape: LinearAttnShape, qkv, z, alpha, beta, cu_rows, conv_in, delta_in,
+                        conv_out, delta_out, out, workspace, x_dtype=DTYPE_BF16, out_dtype=DTYPE_BF16, stream=0):
+    """nmoe_linear_attn_prefill: the GatedDeltaNet core of packed prompts. conv_in / delta_in
+    None: new sequences; they may be conv_out / delta_out themselves."""
+    seqs, rows = cu_rows.numel() - 1, qkv.shape[0]
+    ch, vw = (2 * shape.key_heads + shape.value_heads) * 128, shape.value_heads * 128
+    _device_tensors(qkv, z, alpha, beta, cu_rows, conv_in, delta_in, conv_out, delta_out, out, workspace,
+                    *weights.values())
+    _int32(cu_rows, 1, "cu_rows")
+    strides = [_rows(t, rows, n, x_dtype, name) for t, n, name in
+               ((qkv, ch, "qkv"), (z, vw, "z"), (alpha, shape.value_heads, "alpha"), (beta, shape.value_heads, "beta"))]
+    if strides[2] != strides[3]:
+        raise NmoeError(EINVAL, "alpha and beta must have the same row stride")
+    for t, n, name in ((weights["conv_w"], ch * 4, "conv_w"), (weights["A_log"], shape.value_heads, "A_log"),
+                       (weights["dt_bias"], shape.value_heads, "dt_bias"), (weights["norm_w"], 128, "norm_w")):
+        if t.dtype not in _dtypes()[DTYPE_F32 if name == "A_log" else DTYPE_BF16] or not t.is_contiguous() or t.numel() != n:
+            raise NmoeError(EINVAL, f"{name} must be a contiguous tensor of {n} elements ({'f32' if name == 'A_log' else 'bf16'})")
+    for t, n, name in ((conv_in, seqs * 3 * ch, "conv_in"), (conv_out, seqs * 3 * ch, "conv_out"),
+                       (delta_in, seqs * vw * 128, "delta_in"), (delta_out, seqs * vw * 128, "delta_out")):
+        _states(t, n, name)
+    _output(out, rows * vw, out_dtype)
+    _workspace(workspace, linear_attn_prefill_workspace_bytes(shape, seqs, rows))
+    w = LinearAttnWeights(_ptr(weights["conv_w"]), _ptr(weights["A_log"]), _ptr(weights["dt_bias"]),
+                          _ptr(weights["norm_w"]))
+    rc = lib().nmoe_linear_attn_prefill(C.byref(w), C.byref(shape), seqs, rows, _ptr(cu_rows), _ptr(qkv), strides[0],
+                                        _ptr(z), strides[1], _ptr(alpha), _ptr(beta), strides[2], x_dtype,
+                                        _ptr(conv_in), _ptr(delta_in), _ptr(conv_out), _ptr(delta_out), _ptr(out),
+                                        out_dtype, _ptr(workspace), stream)
+    if rc != OK:
+        raise NmoeError(rc, lib().nmoe_linear_attn_error().decode())
 
 
 def _q4t(m):
