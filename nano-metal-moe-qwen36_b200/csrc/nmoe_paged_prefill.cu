@@ -1,12 +1,44 @@
 // nmoe_paged_prefill.cu -- causal attention of packed prompts over a paged bf16 cache.
+//
+// out_i = sigmoid(gate_i) * sum_{p <= pos_i} softmax_p(scale q_i . k_p) v_p, 4 head_dim flops per
+// visible pair of a query row and a position: the bound is the tensor cores, once a prompt has a
+// few hundred rows.
+//
+// Tile: a pair of CTAs (cta_group::2, M = 256) takes 256 query rows of one KV head, each CTA 128 of
+// them (a row is a token's query head; the heads of a group share the rows' keys and values), and
+// walks over the positions in tiles of 128. S = Q K^T (Q in shared memory) and O += P V (P in tensor
+// memory) are tcgen05 MMAs issued by one thread of the first CTA; each CTA holds half of every K
+// tile (64 positions) and half of every V tile (head_dim / 2 columns), so a tile crosses from L2
+// once per 256 rows. At head_dim 256, O takes half of the tensor memory and two S tiles the other
+// half; a CTA of its own with M = 128 would have to read 62 bytes a cycle from L2 and 160 a cycle
+// from shared memory to keep the tensor cores busy, the pair 31 and 95.
+//
+// Softmax: a thread per query row (warps 0-3) reads its 128 scores from tensor memory, keeps the
+// running maximum and sum in fp32, and writes P back as bf16 over the scores. O is rescaled only
+// when a row's maximum has grown by more than 2^8 since the last time: O and the sum carry the same
+// reference, so the result does not depend on which one it is. While S of tile j is in the softmax,
+// the tensor cores run S of tile j + 1 and P V of tile j - 1.
+//
+// Pages: a warp of each CTA copies boxes of page rows by TMA (the rows of a box lie in one page, as
+// a tile's 64 positions may lie in many). Positions behind a sequence's end, and pages that are
+// none, are masked in the scores, and their V rows are set to zero in shared memory before the MMA
+// reads them: 0 * NaN is NaN. Page sizes that are no multiple of 8 rows are copied by the warp
+// itself.
+#include <cooperative_groups.h>
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
+#include "nmoe_gemm.cuh"
 #include "nmoe_paged.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nmoe {
 namespace {
 
 struct PrefillArgs {
+    CUtensorMap k_map, v_map;   // pages as 4D tensors, boxes of 64 columns x box_rows
     PagedDev c;
     RotaryDev rot;
     HeadDev h;
@@ -14,57 +46,626 @@ struct PrefillArgs {
     const void *q;
     long long q_stride;
     uint16_t *out;
-    float scale;   // softmax scale
+    float scale;   // softmax scale times log2(e)
     int num_seqs, total_rows, kv_heads, group, gated, x_bf16;
+    int box_rows;    // rows of a TMA box: 8..64, or 0: no TMA
+    int rows_inner;  // the map's dims are (column, row, head, page), else (column, head, row, page)
 };
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 192;   // warps 0-3 softmax, 4 copies, 5 MMA
+constexpr int kRows = 128;      // query rows of a CTA
+constexpr int kTile = 128;      // positions of a tile
+constexpr int kInfo = 8;        // ring of tile masks
 
-// A warp per (row, query head): the positions one after another, lane l holding dims E l ..
 template <int D>
-__global__ void __launch_bounds__(kThreads) k_prefill_rows(const __grid_constant__ PrefillArgs a) {
-    constexpr int E = D / 32;
-    __shared__ float2 cs[kThreads / 32][128];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int heads = a.kv_heads * a.group;
-    const long long unit = (long long)blockIdx.x * (kThreads / 32) + warp;
-    if (unit >= (long long)a.total_rows * heads) return;
-    const int r = (int)(unit / heads), head = (int)(unit - (long long)r * heads), kvh = head / a.group;
-    const int b = find_sequence(a.cu_rows, a.num_seqs, r, lane);
-    if (b < 0) return;
-    const long long at = (long long)a.kv_lens[b] - a.cu_rows[b + 1] + r;
-    const int position = at < 0 ? -1 : (int)min(at, (long long)a.c.capacity - 1);
-    float q[E], o[E];
-    const long long src = (long long)r * a.q_stride + (long long)head * (a.gated ? 2 * D : D) + E * lane;
-    load_elems<E>(a.q, src, a.x_bf16, q);
-    for (int t = lane; t < a.rot.half; t += 32) cs[warp][t] = rotary_cs(a.rot.freq[t], (int)at);
-    __syncwarp();
-    prepare_head<E>(q, a.h.q_norm, a.h.eps, cs[warp], a.rot.half, lane);
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = 0.f;
-    for (int p = 0; p <= position; ++p) {
-        const long long row = paged_row(a.c, b, p);
-        if (row < 0) continue;
-        const long long x = row + kvh * a.c.head_stride + E * lane;
-        float k[E], v[E];
-        load_elems<E>(a.c.k, x, true, k);
-        load_elems<E>(a.c.v, x, true, v);
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) s = fmaf(q[i], k[i], s);
-        s = warp_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), c = m == -INFINITY ? 0.f : __expf(m - mn), w = __expf(s - mn);
-#pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = fmaf(o[i], c, w * v[i]);
-        l = fmaf(l, c, w);
-        m = mn;
+struct Cfg {
+    static constexpr int kQB = kRows * D * 2;
+    static constexpr int kStageB = 64 * D * 2;              // half a K or V tile
+    static constexpr int kStages = D == 256 ? 5 : 10;
+    static constexpr int kSmem = kQB + kStages * kStageB + 1024;   // + alignment
+    static constexpr uint32_t kO = 0, kS = D;               // TMEM columns: O, then two S tiles of 128
+};
+
+struct Shared {
+    uint64_t full[10], empty[10], landed, s_full[2], p_ready[2], o_done, q_ready;
+    long long row_off[kTile];         // pages without TMA: element offset of each position, -1: none
+    uint32_t info[kInfo][5];          // valid positions of a tile, then whether all are
+    long long scan[kThreads / 32];
+    long long unit_off;
+    int unit_seq;
+    uint32_t tmem;
+    int stop;                         // a bounded wait has run out
+};
+
+__device__ __forceinline__ uint32_t cluster_addr(const void *p, int rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void arrive_tx_cluster(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+// Bounded wait: a barrier that never completes sets `stop` and lets every later wait go at once.
+__device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, volatile int *stop) {
+    for (uint32_t n = 0;; ++n) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (*stop) return false;
+        if (n >= (1u << 16)) {
+            *stop = 1;
+            return false;
+        }
     }
-    float g[E];
-    if (a.gated) load_elems<E>(a.q, src + D, a.x_bf16, g);
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int col, int c1, int c2, int page,
+                                        uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(col), "r"(c1), "r"(c2), "r"(page), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// All MMAs issued so far have completed: one arrival at the barrier of both CTAs.
+__device__ __forceinline__ void commit2(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// [row][64 columns] panels, 128-byte swizzle, 8 rows apart 1024 bytes. K-major: the columns are the
+// sum's index. MN-major: the rows are, and 64-column panels lie `panel` bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) { return sw128_desc(addr); }
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t panel) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ uint32_t idesc2(int n, int b_mn) {   // bf16 x bf16 -> fp32, M = 256
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *v) {
+    tc_st16(taddr, v);
+    tc_st16(taddr + 16, v + 16);
+}
+__device__ __forceinline__ float ex2f(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The prepared, scaled queries of this CTA's 128 rows, bf16, into 128-byte-swizzled panels. A warp
+// per row; the angles of a token stay in the lanes' registers (lane t: t, t + 32, ..) for its heads.
+template <int D>
+__device__ __forceinline__ void prepare_queries(const PrefillArgs &a, uint8_t *q_smem, int row0, int rows, int pos0,
+                                                int kvh, int warp, int lane) {
+    constexpr int E = D / 32, kBatch = 4;
+    const int tokens = min(kRows / a.group, rows), half = a.rot.half;
+    float2 ang[4];
+    int cur = -1;
+    for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += kBatch) {
+        float v[kBatch][E];
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = l == 0.f ? 0.f : o[i] / l * (a.gated ? sigmoidf_(g[i]) : 1.f);
-    store_bf16<E>(a.out + (long long)r * heads * D + (long long)head * D + E * lane, o);
+        for (int x = 0; x < kBatch; ++x) {
+            const int tok = (r0 + x) / a.group, head = (r0 + x) - tok * a.group;
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[x][i] = 0.f;
+            if (tok < tokens)
+                load_elems<E>(a.q, (long long)(row0 + tok) * a.q_stride +
+                                       (long long)(kvh * a.group + head) * (a.gated ? 2 * D : D) + E * lane,
+                              a.x_bf16, v[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int r = r0 + x, tok = r / a.group;
+            if (tok < tokens) {
+                if (tok != cur && half > 0) {
+                    cur = tok;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (lane + 32 * i < half) ang[i] = rotary_cs(a.rot.freq[lane + 32 * i], pos0 + tok);
+                }
+                float *y = v[x];
+                if (a.h.q_norm != nullptr) {
+                    float ss = 0.f;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) ss = fmaf(y[i], y[i], ss);
+                    const float inv = rsqrtf(warp_sum(ss) / (float)D + a.h.eps);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) y[i] = y[i] * inv * (bf16_to_f32(a.h.q_norm[E * lane + i]) + 1.0f);
+                }
+                if (half > 0) {
+                    const int d = E * lane;
+#pragma unroll
+                    for (int i = 0; i < E; ++i) {
+                        const float other = __shfl_xor_sync(0xffffffffu, y[i], half / E);
+                        const int t = (d + i) & (half - 1);
+                        float2 k = make_float2(1.f, 0.f);
+#pragma unroll
+                        for (int s = 0; s < 4; ++s) {
+                            if (32 * s < half) {   // uniform
+                                const float c = __shfl_sync(0xffffffffu, ang[s].x, t & 31);
+                                const float n = __shfl_sync(0xffffffffu, ang[s].y, t & 31);
+                                if ((t >> 5) == s) k = make_float2(c, n);
+                            }
+                        }
+                        if (d < 2 * half) y[i] = d >= half ? fmaf(other, k.y, y[i] * k.x) : fmaf(-other, k.y, y[i] * k.x);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < E; ++i) y[i] *= a.scale;
+            }
+            const int d = E * lane;
+            uint8_t *dst = q_smem + (d >> 6) * (kRows * 128) + sw128_off(r, (d & 63) >> 3) + (d & 7) * 2;
+            store_bf16<E>(reinterpret_cast<uint16_t *>(dst), v[x]);
+        }
+    }
+}
+
+// What a warp needs to copy tiles of one unit's K and V into the ring.
+template <int D>
+struct Copier {
+    const PrefillArgs &a;
+    Shared *S;
+    uint8_t *ring;
+    int b, kvh, rank, lane, len;   // len: positions that exist
+    uint32_t it = 0;               // stages filled
+    uint32_t landed = 0;
+    int page = -1, row = 0;        // this lane's box of the current tile (TMA)
+    int v_page = -1, v_row = 0;    // and of the tile before it
+    uint32_t boxes = 0, v_boxes = 0;
+
+    __device__ __forceinline__ int lookup(int p, int *in_page) const {
+        const int slot = (unsigned)p / (unsigned)a.c.page_size;
+        *in_page = p - slot * a.c.page_size;
+        if (slot >= a.c.max_pages) return -1;
+        const int pg = a.c.table[(long long)b * a.c.table_stride + slot];
+        return pg >= 0 && pg < a.c.num_pages ? pg : -1;
+    }
+    // The tile's pages, and its mask for the softmax.
+    __device__ __forceinline__ void begin(int tile) {
+        uint32_t *info = S->info[tile % kInfo];
+        v_page = page, v_row = row, v_boxes = boxes;
+        if (a.box_rows > 0) {
+            const int n = kTile / a.box_rows;
+            page = lane < n ? lookup(tile * kTile + lane * a.box_rows, &row) : -1;
+            boxes = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane < 4) {
+                uint32_t w = 0;
+                for (int i = 0; i < 32; i += min(32, a.box_rows))
+                    if (boxes >> ((32 * lane + i) / a.box_rows) & 1u)
+                        w |= (a.box_rows >= 32 ? 0xffffffffu : ((1u << a.box_rows) - 1u) << i);
+                info[lane] = w;
+            }
+            if (lane == 4) info[4] = boxes == (n == 32 ? 0xffffffffu : (1u << n) - 1u);
+        } else {
+            uint32_t all = 0xffffffffu;
+            for (int i = 0; i < 4; ++i) {
+                int r;
+                const int p = tile * kTile + 32 * i + lane, pg = lookup(p, &r);
+                const uint32_t w = __ballot_sync(0xffffffffu, pg >= 0);
+                all &= w;
+                if (lane == 0) info[i] = w;
+            }
+            if (lane == 0) info[4] = all == 0xffffffffu;
+        }
+        __syncwarp();
+    }
+    __device__ __forceinline__ uint32_t acquire() {
+        const uint32_t s = it % Cfg<D>::kStages;
+        wait_cluster(&S->empty[s], ((it / Cfg<D>::kStages) & 1) ^ 1, &S->stop);
+        ++it;
+        return s;
+    }
+    __device__ __forceinline__ void box(bool value, uint32_t dst, int col, int r, int pg, uint32_t bar) const {
+        tma_box(dst, value ? &a.v_map : &a.k_map, col, a.rows_inner ? r : kvh, a.rows_inner ? kvh : r, pg, bar);
+    }
+    // Positions p0 .. p0 + n - 1, columns c0 .. c0 + 64 panels - 1, by the warp's own loads and stores.
+    __device__ __forceinline__ void by_hand(const uint16_t *src, uint8_t *dst, int p0, int n, int c0, int panels,
+                                            bool zero) {
+        for (int i = lane; i < n; i += 32) {
+            int r;
+            const int p = p0 + i, pg = p < len ? lookup(p, &r) : -1;
+            S->row_off[i] = pg < 0 ? -1
+                                   : (long long)pg * a.c.page_stride + (long long)r * a.c.row_stride +
+                                         (long long)kvh * a.c.head_stride;
+        }
+        __syncwarp();
+        const int per = panels * 8, total = n * per;
+#pragma unroll 4
+        for (int i = lane; i < total; i += 32) {
+            const int r = i / per, x = i - r * per, panel = x >> 3, chunk = x & 7;
+            const long long off = S->row_off[r];
+            if (off < 0 && !zero) continue;
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (off >= 0) u = *reinterpret_cast<const uint4 *>(src + off + c0 + 8 * x);
+            *reinterpret_cast<uint4 *>(dst + panel * n * 128 + sw128_off(r, chunk)) = u;
+        }
+        fence_async_smem();
+        __syncwarp();
+    }
+    // This CTA's 64 positions of the tile's K: panels of [64 rows][64 columns].
+    __device__ __forceinline__ void keys(int tile) {
+        const uint32_t s = acquire();
+        uint8_t *dst = ring + s * Cfg<D>::kStageB;
+        const uint32_t bar = cluster_addr(&S->full[s], 0);
+        if (a.box_rows > 0) {
+            const int per = 64 / a.box_rows, first = rank * per;
+            const uint32_t mine = (boxes >> first) & ((1u << per) - 1u);
+            if (lane == 0) arrive_tx_cluster(bar, __popc(mine) * a.box_rows * D * 2);
+            __syncwarp();
+            if (lane >= first && lane < first + per && page >= 0)
+                for (int p = 0; p < D / 64; ++p)
+                    box(false, smem_u32(dst) + p * 8192 + (lane - first) * a.box_rows * 128, 64 * p, row, page, bar);
+        } else {
+            by_hand(a.c.k, dst, tile * kTile + 64 * rank, 64, 0, D / 64, false);
+            if (lane == 0) arrive_cluster(bar);
+        }
+    }
+    // This CTA's half of the columns of all of the tile's V: panels of [128 rows][64 columns]. The tile
+    // is the current one (last), or the one before it.
+    __device__ __forceinline__ void values(int tile, bool last) {
+        const uint32_t s = acquire();
+        uint8_t *dst = ring + s * Cfg<D>::kStageB;
+        const uint32_t bar = cluster_addr(&S->full[s], 0);
+        constexpr int kPanels = D / 128;
+        const int c0 = rank * (D / 2);
+        if (a.box_rows == 0) {
+            by_hand(a.c.v, dst, tile * kTile, kTile, c0, kPanels, true);
+            if (lane == 0) arrive_cluster(bar);
+            return;
+        }
+        const int pg = last ? page : v_page, r = last ? row : v_row;
+        const uint32_t bx = last ? boxes : v_boxes;
+        const int n = kTile / a.box_rows;
+        const bool clean = __popc(bx) == n && (tile + 1) * kTile <= len;
+        const uint32_t bytes = __popc(bx) * a.box_rows * 128 * kPanels;
+        const uint32_t to = clean ? bar : cluster_addr(&S->landed, rank);
+        if (lane == 0) {
+            if (clean) arrive_tx_cluster(bar, bytes);
+            else arrive_tx_cluster(to, bytes);
+        }
+        __syncwarp();
+        if (pg >= 0)
+            for (int p = 0; p < kPanels; ++p)
+                box(true, smem_u32(dst) + p * 16384 + lane * a.box_rows * 128, c0 + 64 * p, r, pg, to);
+        if (!clean) {
+            wait_cluster(&S->landed, landed & 1, &S->stop);
+            ++landed;
+            for (int i = 0; i < kTile; ++i) {
+                const bool gone = tile * kTile + i >= len || !(bx >> (i / a.box_rows) & 1u);
+                if (gone && lane < 8 * kPanels)
+                    *reinterpret_cast<uint4 *>(dst + (lane >> 3) * 16384 + i * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(bar);
+        }
+    }
+};
+
+template <int D>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefill_pairs(const __grid_constant__ PrefillArgs a) {
+    using C = Cfg<D>;
+    extern __shared__ uint8_t raw[];
+    __shared__ Shared S;
+    cg::cluster_group cluster = cg::this_cluster();
+    uint8_t *q_smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    uint8_t *ring = q_smem + C::kQB;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)cluster.block_rank();
+    const int per_cta = kRows / a.group, per_unit = 2 * per_cta;   // tokens
+
+    // ---- the unit: (sequence, query tile, KV head), the last tiles (the longest) of a sequence first
+    const int unit = blockIdx.x >> 1, kvh = unit % a.kv_heads;
+    const long long want = unit / a.kv_heads;
+    if (tid == 0) {
+        S.unit_seq = -1;
+        S.stop = 0;
+    }
+    {
+        const int per = (a.num_seqs + kThreads - 1) / kThreads;
+        const int first = min(a.num_seqs, tid * per), last = min(a.num_seqs, first + per);
+        auto tiles = [&](int b) {
+            const int lo = max(0, a.cu_rows[b]), hi = min(a.total_rows, a.cu_rows[b + 1]);
+            return hi > lo ? (hi - lo + per_unit - 1) / per_unit : 0;
+        };
+        long long own = 0;
+        for (int b = first; b < last; ++b) own += tiles(b);
+        long long inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) S.scan[warp] = inc;
+        __syncthreads();
+        long long before = inc - own;
+        for (int w = 0; w < warp; ++w) before += S.scan[w];
+        if (want >= before && want < before + own)
+            for (int b = first; b < last; ++b) {
+                const int n = tiles(b);
+                if (want < before + n) {
+                    S.unit_seq = b;
+                    S.unit_off = n - 1 - (want - before);
+                    break;
+                }
+                before += n;
+            }
+        __syncthreads();
+    }
+    const int b = S.unit_seq;
+    if (b < 0) return;   // both CTAs of the pair: there are fewer units than the grid has room for
+    const int lo = max(0, a.cu_rows[b]), rows_b = min(a.total_rows, a.cu_rows[b + 1]) - lo;
+    const int tok0 = (int)S.unit_off * per_unit;          // first token of the pair in the sequence
+    const long long len64 = a.kv_lens[b];
+    const long long seq0 = len64 - rows_b;                // position of the sequence's first row
+    const int len = (int)max(0ll, min(len64, (long long)a.c.capacity));
+    const long long last_pos = min((long long)len, seq0 + min(rows_b, tok0 + per_unit)) - 1;
+    const int n_tiles = last_pos < 0 ? 0 : (int)(last_pos / kTile) + 1;   // both CTAs alike
+    const int my_tok0 = tok0 + rank * per_cta;            // this CTA's tokens
+    const int my_rows = max(0, min(per_cta, rows_b - my_tok0));
+
+    // ---- barriers and tensor memory
+    if (tid == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            mbar_init(&S.full[s], 2);    // one arrival of each CTA's copier (the first CTA's barrier is used)
+            mbar_init(&S.empty[s], 1);
+        }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&S.s_full[s], 1);
+            mbar_init(&S.p_ready[s], 8);   // the softmax warps of both CTAs
+        }
+        mbar_init(&S.landed, 1);
+        mbar_init(&S.o_done, 1);
+        mbar_init(&S.q_ready, 8);
+        mbar_fence_init();
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc_fence_before();
+    cluster.sync();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem;
+
+    if (warp == 4) {
+        if (n_tiles > 0) {
+            Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
+            for (int j = 0; j < n_tiles; ++j) {
+                cp.begin(j);
+                cp.keys(j);
+                if (j > 0) cp.values(j - 1, false);
+            }
+            cp.values(n_tiles - 1, true);
+        }
+    } else if (warp == 5) {
+        if (rank == 0 && lane == 0 && n_tiles > 0) {
+            const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
+            uint32_t used = 0;
+            const uint32_t id_s = idesc2(kTile, 0), id_o = idesc2(D, 1);
+            bool ok = wait_cluster(&S.q_ready, 0, &S.stop);
+            auto pv = [&](int j) {
+                ok = ok && wait_cluster(&S.p_ready[j & 1], (j >> 1) & 1, &S.stop);
+                const uint32_t s = used % C::kStages;
+                ok = ok && wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
+                if (!ok) return;
+                ++used;
+                tc_fence_after();
+                const uint32_t at = ring_at + s * C::kStageB, p = tmem + C::kS + (j & 1) * kTile;
+#pragma unroll
+                for (int i = 0; i < kTile / 16; ++i)
+                    mma2_ts(tmem + C::kO, p + 8 * i, desc_mn(at + 2048 * i, 16384), id_o, (j > 0 || i > 0) ? 1u : 0u);
+                commit2(&S.empty[s]);
+                commit2(&S.o_done);
+            };
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const uint32_t s = used % C::kStages;
+                ok = wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
+                if (!ok) break;
+                ++used;
+                tc_fence_after();
+                const uint32_t at = ring_at + s * C::kStageB, d = tmem + C::kS + (j & 1) * kTile;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    mma2_ss(d, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
+                            desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u);
+                commit2(&S.empty[s]);
+                commit2(&S.s_full[j & 1]);
+                if (j > 0) pv(j - 1);
+            }
+            if (ok) pv(n_tiles - 1);
+        }
+    } else {
+        // ---- queries
+        const int token = tid / a.group, head = tid - token * a.group;   // this thread's row
+        const bool live = token < my_rows;
+        const long long pos64 = seq0 + my_tok0 + token;
+        // position up to which this row sees; -1: nothing
+        const int pos = live && pos64 >= 0 ? (int)min(pos64, (long long)len - 1) : -1;
+        float m = -INFINITY, l = 0.f;
+        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        if (n_tiles > 0) {
+            prepare_queries<D>(a, q_smem, lo + my_tok0, my_rows, (int)(seq0 + my_tok0), kvh, warp, lane);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) arrive_cluster(cluster_addr(&S.q_ready, 0));
+            const uint32_t p_bar = cluster_addr(&S.p_ready[0], 0);
+            // the first position that some row of this warp does not see
+            const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
+            for (int j = 0; j < n_tiles; ++j) {
+                wait_cluster(&S.s_full[j & 1], (j >> 1) & 1, &S.stop);
+                tc_fence_after();
+                const uint32_t st = tmem + lanes + C::kS + (j & 1) * kTile;
+                float s[kTile];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tc_ld32(st + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+                tc_wait_ld();
+                const uint32_t *info = S.info[j % kInfo];
+                if ((j + 1) * kTile > seen || !info[4]) {
+                    const int n = pos - j * kTile;   // columns 0..n are seen
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int k = n - 32 * c;
+                        const uint32_t w = info[c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) s[32 * c + i] = w >> i & 1u ? s[32 * c + i] : -INFINITY;
+                    }
+                }
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < kTile; i += 4)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[i + x]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
+                const float mn = grow ? top : m;
+                const float base = mn == -INFINITY ? 0.f : mn;
+                const bool scale_o = j > 0 && __any_sync(0xffffffffu, grow);
+                const float c = grow ? ex2f(m - base) : 1.0f;
+                l *= c;
+                m = mn;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < kTile; i += 4)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        s[i + x] = ex2f(s[i + x] - base);
+                        sum[x] += s[i + x];
+                    }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                uint32_t p[kTile / 2];
+#pragma unroll
+                for (int i = 0; i < kTile / 2; ++i) p[i] = pack2_bf16(s[2 * i], s[2 * i + 1]);
+                tc_st32(st, p);
+                tc_st32(st + 32, p + 32);
+                // P V of tile j - 1 is complete: the tensor cores are at S of tile j + 1 by now
+                if (j > 0) wait_cluster(&S.o_done, (j - 1) & 1, &S.stop);
+                if (scale_o) {
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int x = 0; x < D; x += 32) {
+                        uint32_t o[32];
+                        tc_ld32(tmem + lanes + C::kO + x, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
+                        tc_st32(tmem + lanes + C::kO + x, o);
+                    }
+                }
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) arrive_cluster(p_bar + (j & 1) * 8);
+            }
+            wait_cluster(&S.o_done, (n_tiles - 1) & 1, &S.stop);
+            tc_fence_after();
+        }
+        // ---- O / l times the gate
+        const int heads = a.kv_heads * a.group;
+        const long long r = (long long)lo + my_tok0 + token;
+        uint16_t *out = a.out + (r * heads + kvh * a.group + head) * D;
+        const long long gate = r * a.q_stride + (long long)(kvh * a.group + head) * 2 * D + D;
+        const float inv = S.stop ? NAN : l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll 1
+        for (int x = 0; x < D; x += 32) {
+            uint32_t o[32];
+            if (n_tiles > 0) {
+                tc_ld32(tmem + lanes + C::kO + x, o);
+                tc_wait_ld();
+            }
+            if (live) {
+#pragma unroll
+                for (int y = 0; y < 32; y += 8) {
+                    float v[8], g[8];
+                    if (a.gated) load_elems<8>(a.q, gate + x + y, a.x_bf16, g);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        v[i] = inv == 0.f ? 0.f : __uint_as_float(o[y + i]) * inv;
+                        if (a.gated) v[i] *= sigmoidf_(g[i]);
+                    }
+                    if (l == 0.f && !S.stop)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+                    store_bf16<8>(out + x + y, v);
+                }
+            }
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (S.stop && warp == 4) {   // copies in flight land before the shared memory goes (each wait bounded)
+        int go_on = 0;
+        for (int s = 0; s < C::kStages; ++s)
+            for (int n = 0; n < 1000 && !mbar_try_wait_sleep(&S.full[s], go_on, 1000); ++n) {}
+    }
+    cluster.sync();   // neither CTA leaves while the other may still signal it
+    tc_fence_after();
+    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
+
+EncodeFn encode_fn() {
+    static EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return (EncodeFn) nullptr;
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// Pages as a 4D tensor, dims in the order of their strides; boxes of 64 columns and `rows` rows of one
+// page and head, 128-byte swizzle.
+bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, bool rows_inner) {
+    const cuuint64_t row_b = c.row_stride * 2, head_b = c.head_stride * 2, page_b = c.page_stride * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)(rows_inner ? c.page_size : heads),
+                                (cuuint64_t)(rows_inner ? heads : c.page_size), (cuuint64_t)c.num_pages};
+    const cuuint64_t strides[3] = {rows_inner ? row_b : head_b, rows_inner ? head_b : row_b, page_b};
+    const cuuint32_t box[4] = {64, (cuuint32_t)(rows_inner ? rows : 1), (cuuint32_t)(rows_inner ? 1 : rows), 1};
+    const cuuint32_t es[4] = {1, 1, 1, 1};
+    EncodeFn fn = encode_fn();
+    return fn != nullptr &&
+           fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t *>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+cudaError_t launch(const PrefillArgs &a, long long units, cudaStream_t st) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(k_prefill_pairs<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+    if (e != cudaSuccess) return e;
+    k_prefill_pairs<D><<<(unsigned)(2 * units), kThreads, Cfg<D>::kSmem, st>>>(a);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -105,7 +706,7 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.kv_lens = kv_lens;
     a.q = q;
     a.out = out;
-    a.scale = scale == 0.f ? 1.0f / sqrtf((float)shape->head_dim) : scale;
+    a.scale = (scale == 0.f ? 1.0f / sqrtf((float)shape->head_dim) : scale) * 1.4426950408889634f;
     a.num_seqs = num_seqs;
     a.total_rows = total_rows;
     a.kv_heads = shape->kv_heads;
@@ -113,14 +714,19 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.gated = shape->gated;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     (void)workspace;
-    const long long units = (long long)total_rows * shape->q_heads;
-    const long long grid = (units + kThreads / 32 - 1) / (kThreads / 32);
-    if (grid > 2147483647ll) return full_attn_fail(NMOE_EINVAL, "too many rows");
+    // boxes of the largest power of two of rows that divides a page, up to 64
+    int box = a.c.page_size & -a.c.page_size;
+    box = box > 64 ? 64 : box;
+    a.rows_inner = a.c.row_stride <= a.c.head_stride;
+    a.box_rows = box < 8 ? 0 : box;
+    if (a.box_rows > 0 &&
+        !(page_map(&a.k_map, a.c, a.c.k, shape->head_dim, a.kv_heads, box, a.rows_inner) &&
+          page_map(&a.v_map, a.c, a.c.v, shape->head_dim, a.kv_heads, box, a.rows_inner)))
+        a.box_rows = 0;   // strides that a tensor map cannot have: the warp copies
+    const int per_unit = 2 * (kRows / a.group);
+    const long long units = ((long long)total_rows / per_unit + num_seqs) * a.kv_heads;
+    if (2 * units > 2147483647ll) return full_attn_fail(NMOE_EINVAL, "too many rows");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (shape->head_dim == 256)
-        k_prefill_rows<256><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    else
-        k_prefill_rows<128><<<(unsigned)grid, kThreads, 0, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    const cudaError_t e = shape->head_dim == 256 ? launch<256>(a, units, st) : launch<128>(a, units, st);
     return e == cudaSuccess ? NMOE_OK : full_attn_fail(NMOE_ECUDA, "prefill: %s", cudaGetErrorString(e));
 }
