@@ -19,17 +19,21 @@ struct PagedDev {
     int capacity;   // max_pages * page_size positions (checked to fit an int)
 };
 
-// Rotation frequencies theta^(-2 t / rotary_dims), t < half, in 64 bits: the angle position *
-// freq has to be reduced before it is rounded (an fp32 angle at position 32768 is off by 2e-3).
+// Rotation: pair t < half turns by position * theta^(-t / half), in 64 bits, since the angle has to
+// be reduced before it is rounded (an fp32 angle at position 32768 is off by 2e-3). A thread that
+// needs a frequency computes it once: a table in the kernel's parameters, read by 32 lanes at 32
+// addresses, costs tens of microseconds of constant-cache misses.
 struct RotaryDev {
-    double freq[128];
-    int half;   // rotary_dims / 2
+    double step;   // log2(theta) / half
+    int half;      // rotary_dims / 2
 };
 
 struct HeadDev {
     const uint16_t *q_norm, *k_norm;   // bf16 [head_dim] or null
     float eps;
 };
+
+__device__ __forceinline__ double rotary_freq(const RotaryDev &r, int t) { return exp2(-r.step * t); }
 
 __device__ __forceinline__ float2 rotary_cs(double freq, int position) {
     double a = (double)position * freq;

@@ -82,8 +82,7 @@ int check_paged_kv(const nmoe_paged_kv *kv, PagedDev *d) {
 
 void fill_rotary(const nmoe_full_attn_shape *s, RotaryDev *r) {
     r->half = s->rotary_dims / 2;
-    for (int t = 0; t < 128; ++t)
-        r->freq[t] = t < r->half ? pow((double)s->rope_theta, -2.0 * t / s->rotary_dims) : 0.0;
+    r->step = r->half > 0 ? log2((double)s->rope_theta) / r->half : 0.0;
 }
 
 int check_x(const char *what, const void *p, int x_dtype, long long stride, long long width) {
@@ -131,6 +130,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = blockIdx.x * a.rows_per_cta;
     const int rows = min(a.rows_per_cta, a.total_rows - row0);
+    const double freq = a.rot.half > 0 ? rotary_freq(a.rot, tid & (a.rot.half - 1)) : 0.0;
     if (warp < rows) {
         const int r = row0 + warp;
         const int b = find_sequence(a.cu_rows, a.num_seqs, r, lane);
@@ -145,9 +145,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_co
         }
     }
     __syncthreads();
-    for (int i = tid; i < rows * a.rot.half; i += kAppendThreads) {
-        const int r = i / a.rot.half, t = i - r * a.rot.half;
-        cs[r][t] = rotary_cs(a.rot.freq[t], at[r]);
+    if (a.rot.half > 0) {   // half is a power of two that divides the threads: a thread keeps its t
+        const int t = tid & (a.rot.half - 1);
+        for (int r = tid / a.rot.half; r < rows; r += kAppendThreads / a.rot.half) cs[r][t] = rotary_cs(freq, at[r]);
     }
     __syncthreads();
     const int units = rows * a.kv_heads * 2;
@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
         for (int s = 0; s < kStages; ++s) mbar_init(&bars[warp][s], 1);
         mbar_fence_init();
     }
+    const double freq = tid < a.rot.half ? rotary_freq(a.rot, tid) : 0.0;
     const Plan plan = plan_tiles(a.kv_lens, a.batch, a.c.capacity, sm_scan);
     const long long total = plan.total * a.kv_heads;
     const long long pieces = min((long long)a.ctas, total);   // no piece is empty
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
         for (; issued < kStages && issued < steps; ++issued) issue(issued);
 
         // ---- the queries of the group, prepared, scaled and split into bf16 parts
-        if (tid < a.rot.half) cs[tid] = rotary_cs(a.rot.freq[tid], len - 1);
+        if (tid < a.rot.half) cs[tid] = rotary_cs(freq, len - 1);
         for (int i = tid; i < Cfg::q_bytes(PARTS) / 16; i += kStepThreads)
             *reinterpret_cast<uint4 *>(smem + Cfg::kQ + 16 * i) = make_uint4(0, 0, 0, 0);
         __syncthreads();

@@ -39,6 +39,9 @@ namespace {
 
 struct PrefillArgs {
     CUtensorMap k_map, v_map;   // pages as 4D tensors, boxes of 64 columns x box_rows
+    CUtensorMap q_map;          // prepared queries, boxes of 64 columns x 128 rows
+    uint16_t *q_ready;
+    int prep_rows;
     PagedDev c;
     RotaryDev rot;
     HeadDev h;
@@ -116,6 +119,13 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, in
         "l"(map), "r"(col), "r"(c1), "r"(c2), "r"(page), "r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int col, int row, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(col), "r"(row), "r"(bar)
+        : "memory");
+}
 __device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -158,71 +168,42 @@ __device__ __forceinline__ float ex2f(float x) {
     return y;
 }
 
-// The prepared, scaled queries of this CTA's 128 rows, bf16, into 128-byte-swizzled panels. A warp
-// per row; the angles of a token stay in the lanes' registers (lane t: t, t + 32, ..) for its heads.
+// The prepared, scaled queries in bf16, [KV head][row][head of the group][D], so that the rows of a
+// tile lie together: a kernel of its own (and launch), since the tiles' kernel has one warp a
+// scheduler and would spend tens of microseconds a unit on it. One (cos, sin) table a row, a warp
+// per (row, head).
+constexpr int kPrepThreads = 256, kPrepRows = 8;
+
 template <int D>
-__device__ __forceinline__ void prepare_queries(const PrefillArgs &a, uint8_t *q_smem, int row0, int rows, int pos0,
-                                                int kvh, int warp, int lane) {
-    constexpr int E = D / 32, kBatch = 4;
-    const int tokens = min(kRows / a.group, rows), half = a.rot.half;
-    float2 ang[4];
-    int cur = -1;
-    for (int r0 = warp * 32; r0 < warp * 32 + 32; r0 += kBatch) {
-        float v[kBatch][E];
-#pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            const int tok = (r0 + x) / a.group, head = (r0 + x) - tok * a.group;
-#pragma unroll
-            for (int i = 0; i < E; ++i) v[x][i] = 0.f;
-            if (tok < tokens)
-                load_elems<E>(a.q, (long long)(row0 + tok) * a.q_stride +
-                                       (long long)(kvh * a.group + head) * (a.gated ? 2 * D : D) + E * lane,
-                              a.x_bf16, v[x]);
+__global__ void __launch_bounds__(kPrepThreads) k_prefill_queries(const __grid_constant__ PrefillArgs a) {
+    constexpr int E = D / 32;
+    __shared__ float2 cs[kPrepRows][128];
+    __shared__ int at[kPrepRows], live[kPrepRows];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = a.rot.half;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int row0 = blockIdx.x * a.prep_rows, rows = min(a.prep_rows, a.total_rows - row0);
+    const double freq = half > 0 ? rotary_freq(a.rot, tid & (half - 1)) : 0.0;
+    if (warp < rows) {
+        const int r = row0 + warp, b = find_sequence(a.cu_rows, a.num_seqs, r, lane);
+        if (lane == 0) {
+            live[warp] = b >= 0;
+            at[warp] = b >= 0 ? (int)((long long)a.kv_lens[b] - a.cu_rows[b + 1] + r) : 0;
         }
+    }
+    __syncthreads();
+    if (half > 0)
+        for (int r = tid / half; r < rows; r += kPrepThreads / half) cs[r][tid & (half - 1)] = rotary_cs(freq, at[r]);
+    __syncthreads();
+    const int heads = a.kv_heads * a.group;
+    for (int u = warp; u < rows * heads; u += kPrepThreads / 32) {
+        const int r = u / heads, h = u - r * heads, kvh = h / a.group;
+        if (!live[r]) continue;
+        float v[E];
+        load_elems<E>(a.q, (long long)(row0 + r) * a.q_stride + (long long)h * (a.gated ? 2 * D : D) + E * lane, a.x_bf16, v);
+        prepare_head<E>(v, a.h.q_norm, a.h.eps, cs[r], half, lane);
 #pragma unroll
-        for (int x = 0; x < kBatch; ++x) {
-            const int r = r0 + x, tok = r / a.group;
-            if (tok < tokens) {
-                if (tok != cur && half > 0) {
-                    cur = tok;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (lane + 32 * i < half) ang[i] = rotary_cs(a.rot.freq[lane + 32 * i], pos0 + tok);
-                }
-                float *y = v[x];
-                if (a.h.q_norm != nullptr) {
-                    float ss = 0.f;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) ss = fmaf(y[i], y[i], ss);
-                    const float inv = rsqrtf(warp_sum(ss) / (float)D + a.h.eps);
-#pragma unroll
-                    for (int i = 0; i < E; ++i) y[i] = y[i] * inv * (bf16_to_f32(a.h.q_norm[E * lane + i]) + 1.0f);
-                }
-                if (half > 0) {
-                    const int d = E * lane;
-#pragma unroll
-                    for (int i = 0; i < E; ++i) {
-                        const float other = __shfl_xor_sync(0xffffffffu, y[i], half / E);
-                        const int t = (d + i) & (half - 1);
-                        float2 k = make_float2(1.f, 0.f);
-#pragma unroll
-                        for (int s = 0; s < 4; ++s) {
-                            if (32 * s < half) {   // uniform
-                                const float c = __shfl_sync(0xffffffffu, ang[s].x, t & 31);
-                                const float n = __shfl_sync(0xffffffffu, ang[s].y, t & 31);
-                                if ((t >> 5) == s) k = make_float2(c, n);
-                            }
-                        }
-                        if (d < 2 * half) y[i] = d >= half ? fmaf(other, k.y, y[i] * k.x) : fmaf(-other, k.y, y[i] * k.x);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < E; ++i) y[i] *= a.scale;
-            }
-            const int d = E * lane;
-            uint8_t *dst = q_smem + (d >> 6) * (kRows * 128) + sw128_off(r, (d & 63) >> 3) + (d & 7) * 2;
-            store_bf16<E>(reinterpret_cast<uint16_t *>(dst), v[x]);
-        }
+        for (int i = 0; i < E; ++i) v[i] *= a.scale;
+        store_bf16<E>(a.q_ready + (((long long)kvh * a.total_rows + row0 + r) * a.group + (h - kvh * a.group)) * D + E * lane, v);
     }
 }
 
@@ -356,11 +337,14 @@ struct Copier {
         if (!clean) {
             wait_cluster(&S->landed, landed & 1, &S->stop);
             ++landed;
-            for (int i = 0; i < kTile; ++i) {
-                const bool gone = tile * kTile + i >= len || !(bx >> (i / a.box_rows) & 1u);
-                if (gone && lane < 8 * kPanels)
-                    *reinterpret_cast<uint4 *>(dst + (lane >> 3) * 16384 + i * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-            }
+            // rows that are no positions: 8 kPanels lanes a row
+            constexpr int kLanes = 8 * kPanels;
+            const uint32_t *info = S->info[tile % kInfo];
+            const int exist = len - tile * kTile;   // rows from here on lie behind the sequence
+            const int part = lane % kLanes;
+            for (int i = lane / kLanes + (info[4] ? exist & ~(32 / kLanes - 1) : 0); i < kTile; i += 32 / kLanes)
+                if (i >= exist || !(info[i >> 5] >> (i & 31) & 1u))
+                    *reinterpret_cast<uint4 *>(dst + (part >> 3) * 16384 + i * 128 + (part & 7) * 16) = make_uint4(0, 0, 0, 0);
             fence_async_smem();
             __syncwarp();
             if (lane == 0) arrive_cluster(bar);
@@ -442,7 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         }
         mbar_init(&S.landed, 1);
         mbar_init(&S.o_done, 1);
-        mbar_init(&S.q_ready, 8);
+        mbar_init(&S.q_ready, 2);
         mbar_fence_init();
     }
     if (warp == 5) {
@@ -457,6 +441,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
     if (warp == 4) {
         if (n_tiles > 0) {
             Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
+            asm volatile("griddepcontrol.wait;" ::: "memory");   // the prepared queries
+            if (lane == 0) {
+                const uint32_t bar = cluster_addr(&S.q_ready, 0);
+                arrive_tx_cluster(bar, C::kQB);
+                for (int p = 0; p < D / 64; ++p)
+                    tma_rows(smem_u32(q_smem) + p * (kRows * 128), &a.q_map, 64 * p,
+                             (kvh * a.total_rows + lo + my_tok0) * a.group, bar);
+            }
+            __syncwarp();
             for (int j = 0; j < n_tiles; ++j) {
                 cp.begin(j);
                 cp.keys(j);
@@ -502,7 +495,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
             if (ok) pv(n_tiles - 1);
         }
     } else {
-        // ---- queries
         const int token = tid / a.group, head = tid - token * a.group;   // this thread's row
         const bool live = token < my_rows;
         const long long pos64 = seq0 + my_tok0 + token;
@@ -511,10 +503,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         float m = -INFINITY, l = 0.f;
         const uint32_t lanes = (uint32_t)(warp * 32) << 16;
         if (n_tiles > 0) {
-            prepare_queries<D>(a, q_smem, lo + my_tok0, my_rows, (int)(seq0 + my_tok0), kvh, warp, lane);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) arrive_cluster(cluster_addr(&S.q_ready, 0));
             const uint32_t p_bar = cluster_addr(&S.p_ready[0], 0);
             // the first position that some row of this warp does not see
             const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
@@ -595,25 +583,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
 #pragma unroll 1
         for (int x = 0; x < D; x += 32) {
             uint32_t o[32];
+            float g[32];
+            if (a.gated && live)
+#pragma unroll
+                for (int y = 0; y < 32; y += 8) load_elems<8>(a.q, gate + x + y, a.x_bf16, g + y);
             if (n_tiles > 0) {
                 tc_ld32(tmem + lanes + C::kO + x, o);
                 tc_wait_ld();
             }
             if (live) {
+                float v[32];
 #pragma unroll
-                for (int y = 0; y < 32; y += 8) {
-                    float v[8], g[8];
-                    if (a.gated) load_elems<8>(a.q, gate + x + y, a.x_bf16, g);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        v[i] = inv == 0.f ? 0.f : __uint_as_float(o[y + i]) * inv;
-                        if (a.gated) v[i] *= sigmoidf_(g[i]);
-                    }
-                    if (l == 0.f && !S.stop)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-                    store_bf16<8>(out + x + y, v);
+                for (int i = 0; i < 32; ++i) {
+                    v[i] = inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
+                    if (a.gated) v[i] *= __fdividef(1.0f, 1.0f + __expf(-g[i]));
                 }
+#pragma unroll
+                for (int y = 0; y < 32; y += 8) store_bf16<8>(out + x + y, v + y);
             }
         }
         tc_fence_before();
@@ -659,13 +645,34 @@ bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, in
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool query_map(CUtensorMap *m, const uint16_t *base, int d, long long rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d * 2};
+    const cuuint32_t box[2] = {64, kRows}, es[2] = {1, 1};
+    EncodeFn fn = encode_fn();
+    return fn != nullptr &&
+           fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D>
 cudaError_t launch(const PrefillArgs &a, long long units, cudaStream_t st) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(k_prefill_pairs<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+    cudaError_t e = cudaFuncSetAttribute(k_prefill_pairs<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
     if (e != cudaSuccess) return e;
-    k_prefill_pairs<D><<<(unsigned)(2 * units), kThreads, Cfg<D>::kSmem, st>>>(a);
-    return cudaGetLastError();
+    k_prefill_queries<D><<<(a.total_rows + a.prep_rows - 1) / a.prep_rows, kPrepThreads, 0, st>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    // the tiles' kernel sets up and reads K while the queries are prepared
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * units));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Cfg<D>::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k_prefill_pairs<D>, a);
 }
 
 }  // namespace
@@ -675,10 +682,9 @@ using namespace nmoe;
 
 extern "C" size_t nmoe_full_attn_prefill_paged_workspace_bytes(const nmoe_full_attn_shape *s, int num_seqs,
                                                                int total_rows) {
-    (void)s;
-    (void)num_seqs;
-    (void)total_rows;
-    return 0;
+    const nmoe_full_attn_weights none = {nullptr, nullptr};
+    if (num_seqs < 1 || total_rows < 1 || check_full_attn_shape(&none, s) != NMOE_OK) return 0;
+    return (size_t)total_rows * s->q_heads * s->head_dim * sizeof(uint16_t);
 }
 
 extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, const nmoe_full_attn_shape *shape,
@@ -698,7 +704,9 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.q_stride = q_stride == 0 ? qw : q_stride;
     rc = check_x("q", q, x_dtype, a.q_stride, qw);
     if (rc != NMOE_OK) return rc;
-    if (out == nullptr || !aligned_to(out, 16)) return full_attn_fail(NMOE_EINVAL, "out is NULL or not 16-byte aligned");
+    if (out == nullptr || workspace == nullptr || !aligned_to(out, 16) || !aligned_to(workspace, 16))
+        return full_attn_fail(NMOE_EINVAL, "out or workspace is NULL or not 16-byte aligned");
+    if ((long long)total_rows * shape->q_heads > 2147483647ll) return full_attn_fail(NMOE_EINVAL, "too many rows");
     if (!(scale >= 0.f && scale <= 3.0e38f)) return full_attn_fail(NMOE_EINVAL, "scale must be finite and not negative");
     fill_rotary(shape, &a.rot);
     a.h = {w->q_norm, nullptr, shape->norm_eps};
@@ -713,7 +721,13 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.group = shape->q_heads / shape->kv_heads;
     a.gated = shape->gated;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
-    (void)workspace;
+    a.q_ready = static_cast<uint16_t *>(workspace);
+    int sms = 0;
+    if ((rc = device_sm_count(&sms)) != NMOE_OK) return rc;
+    const int per = total_rows / (4 * sms);
+    a.prep_rows = per < 1 ? 1 : (per > kPrepRows ? kPrepRows : per);
+    if (!query_map(&a.q_map, a.q_ready, shape->head_dim, (long long)total_rows * shape->q_heads))
+        return full_attn_fail(NMOE_ECUDA, "cuTensorMapEncodeTiled failed");
     // boxes of the largest power of two of rows that divides a page, up to 64
     int box = a.c.page_size & -a.c.page_size;
     box = box > 64 ? 64 : box;
@@ -725,7 +739,7 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
         a.box_rows = 0;   // strides that a tensor map cannot have: the warp copies
     const int per_unit = 2 * (kRows / a.group);
     const long long units = ((long long)total_rows / per_unit + num_seqs) * a.kv_heads;
-    if (2 * units > 2147483647ll) return full_attn_fail(NMOE_EINVAL, "too many rows");
+    if (2 * units > 2147483647ll) return full_attn_fail(NMOE_EINVAL, "too many rows or sequences");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const cudaError_t e = shape->head_dim == 256 ? launch<256>(a, units, st) : launch<128>(a, units, st);
     return e == cudaSuccess ? NMOE_OK : full_attn_fail(NMOE_ECUDA, "prefill: %s", cudaGetErrorString(e));
