@@ -22,7 +22,7 @@
 // Pages: a warp of each CTA copies boxes of page rows by TMA (the rows of a box lie in one page, as
 // a tile's 64 positions may lie in many). Positions behind a sequence's end, and pages that are
 // none, are masked in the scores, and their V rows are set to zero in shared memory before the MMA
-// reads them: 0 * NaN is NaN. Page sizes that are no multiple of 8 rows are copied by the warp
+// reads them: 0 * NaN is NaN. Page sizes that are no multiple of 16 rows are copied by the warp
 // itself.
 #include <cooperative_groups.h>
 #include <cuda.h>
@@ -51,11 +51,10 @@ struct PrefillArgs {
     uint16_t *out;
     float scale;   // softmax scale times log2(e)
     int num_seqs, total_rows, kv_heads, group, gated, x_bf16;
-    int box_rows;    // rows of a TMA box: 8..64, or 0: no TMA
-    int rows_inner;  // the map's dims are (column, row, head, page), else (column, head, row, page)
+    int box_rows, box_shift;   // rows of a TMA box: 16, 32 or 64, or 0: no TMA
 };
 
-constexpr int kThreads = 192;   // warps 0-3 softmax, 4 copies, 5 MMA
+constexpr int kThreads = 224;   // warps 0-3 softmax, 4 copies Q and K, 5 MMA, 6 copies V
 constexpr int kRows = 128;      // query rows of a CTA
 constexpr int kTile = 128;      // positions of a tile
 constexpr int kInfo = 8;        // ring of tile masks
@@ -71,7 +70,7 @@ struct Cfg {
 
 struct Shared {
     uint64_t full[10], empty[10], landed, s_full[2], p_ready[2], o_done, q_ready;
-    long long row_off[kTile];         // pages without TMA: element offset of each position, -1: none
+    long long row_off[64 + kTile];    // of the two copying warps
     uint32_t info[kInfo][5];          // valid positions of a tile, then whether all are
     long long scan[kThreads / 32];
     long long unit_off;
@@ -111,12 +110,13 @@ __device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, vol
         }
     }
 }
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int col, int c1, int c2, int page,
+// A box of page rows: coordinates (column 0, row, panel of 64 columns, head, page).
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int panel, int row, int head, int page,
                                         uint32_t bar) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
-        "%3, %4, %5}], [%6];" ::"r"(dst),
-        "l"(map), "r"(col), "r"(c1), "r"(c2), "r"(page), "r"(bar)
+        "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(row), "r"(panel), "r"(head), "r"(page), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int col, int row, uint32_t bar) {
@@ -207,48 +207,57 @@ __global__ void __launch_bounds__(kPrepThreads) k_prefill_queries(const __grid_c
     }
 }
 
-// What a warp needs to copy tiles of one unit's K and V into the ring.
+// A warp that copies one unit's K tiles, or its V tiles, into the ring. The ring's stages are taken
+// in the order of the MMAs (K 0, K 1, V 0, K 2, V 1, ..), so each of the two warps knows its stages.
 template <int D>
 struct Copier {
     const PrefillArgs &a;
     Shared *S;
     uint8_t *ring;
+    long long *row_off;            // pages without TMA: element offset of each position, -1: none
     int b, kvh, rank, lane, len;   // len: positions that exist
-    uint32_t it = 0;               // stages filled
-    uint32_t landed = 0;
     int page = -1, row = 0;        // this lane's box of the current tile (TMA)
-    int v_page = -1, v_row = 0;    // and of the tile before it
-    uint32_t boxes = 0, v_boxes = 0;
+    int next_page = -1, next_row = 0;
+    uint32_t boxes = 0;
 
     __device__ __forceinline__ int lookup(int p, int *in_page) const {
         const int slot = (unsigned)p / (unsigned)a.c.page_size;
         *in_page = p - slot * a.c.page_size;
-        if (slot >= a.c.max_pages) return -1;
-        const int pg = a.c.table[(long long)b * a.c.table_stride + slot];
-        return pg >= 0 && pg < a.c.num_pages ? pg : -1;
+        return slot < a.c.max_pages ? a.c.table[(long long)b * a.c.table_stride + slot] : -1;
     }
-    // The tile's pages, and its mask for the softmax.
-    __device__ __forceinline__ void begin(int tile) {
+    __device__ __forceinline__ int checked(int page_id) const {
+        return page_id >= 0 && page_id < a.c.num_pages ? page_id : -1;
+    }
+    // The boxes of tile `tile` become current; those of the next tile are looked up meanwhile.
+    __device__ __forceinline__ void look_ahead(int tile) {
+        next_page = -1;
+        if (lane < kTile / a.box_rows && tile * kTile + lane * a.box_rows < len)
+            next_page = lookup(tile * kTile + lane * a.box_rows, &next_row);
+    }
+    __device__ __forceinline__ void begin(int tile, bool more) {
+        if (a.box_rows == 0) return;
+        page = checked(next_page), row = next_row;
+        boxes = __ballot_sync(0xffffffffu, page >= 0);
+        if (more) look_ahead(tile + 1);
+    }
+    // The mask of the tile's positions for the softmax.
+    __device__ __forceinline__ void mask(int tile) {
         uint32_t *info = S->info[tile % kInfo];
-        v_page = page, v_row = row, v_boxes = boxes;
         if (a.box_rows > 0) {
             const int n = kTile / a.box_rows;
-            page = lane < n ? lookup(tile * kTile + lane * a.box_rows, &row) : -1;
-            boxes = __ballot_sync(0xffffffffu, page >= 0);
             if (lane < 4) {
                 uint32_t w = 0;
                 for (int i = 0; i < 32; i += min(32, a.box_rows))
-                    if (boxes >> ((32 * lane + i) / a.box_rows) & 1u)
+                    if (boxes >> ((32 * lane + i) >> a.box_shift) & 1u)
                         w |= (a.box_rows >= 32 ? 0xffffffffu : ((1u << a.box_rows) - 1u) << i);
                 info[lane] = w;
             }
-            if (lane == 4) info[4] = boxes == (n == 32 ? 0xffffffffu : (1u << n) - 1u);
+            if (lane == 4) info[4] = boxes == (1u << n) - 1u;
         } else {
             uint32_t all = 0xffffffffu;
             for (int i = 0; i < 4; ++i) {
                 int r;
-                const int p = tile * kTile + 32 * i + lane, pg = lookup(p, &r);
-                const uint32_t w = __ballot_sync(0xffffffffu, pg >= 0);
+                const uint32_t w = __ballot_sync(0xffffffffu, checked(lookup(tile * kTile + 32 * i + lane, &r)) >= 0);
                 all &= w;
                 if (lane == 0) info[i] = w;
             }
@@ -256,31 +265,27 @@ struct Copier {
         }
         __syncwarp();
     }
-    __device__ __forceinline__ uint32_t acquire() {
-        const uint32_t s = it % Cfg<D>::kStages;
-        wait_cluster(&S->empty[s], ((it / Cfg<D>::kStages) & 1) ^ 1, &S->stop);
-        ++it;
+    __device__ __forceinline__ uint32_t acquire(uint32_t n) const {   // the n-th stage filled
+        const uint32_t s = n % Cfg<D>::kStages;
+        wait_cluster(&S->empty[s], ((n / Cfg<D>::kStages) & 1) ^ 1, &S->stop);
         return s;
-    }
-    __device__ __forceinline__ void box(bool value, uint32_t dst, int col, int r, int pg, uint32_t bar) const {
-        tma_box(dst, value ? &a.v_map : &a.k_map, col, a.rows_inner ? r : kvh, a.rows_inner ? kvh : r, pg, bar);
     }
     // Positions p0 .. p0 + n - 1, columns c0 .. c0 + 64 panels - 1, by the warp's own loads and stores.
     __device__ __forceinline__ void by_hand(const uint16_t *src, uint8_t *dst, int p0, int n, int c0, int panels,
-                                            bool zero) {
+                                            bool zero) const {
         for (int i = lane; i < n; i += 32) {
             int r;
-            const int p = p0 + i, pg = p < len ? lookup(p, &r) : -1;
-            S->row_off[i] = pg < 0 ? -1
-                                   : (long long)pg * a.c.page_stride + (long long)r * a.c.row_stride +
-                                         (long long)kvh * a.c.head_stride;
+            const int p = p0 + i, pg = p < len ? checked(lookup(p, &r)) : -1;
+            row_off[i] = pg < 0 ? -1
+                                : (long long)pg * a.c.page_stride + (long long)r * a.c.row_stride +
+                                      (long long)kvh * a.c.head_stride;
         }
         __syncwarp();
         const int per = panels * 8, total = n * per;
 #pragma unroll 4
         for (int i = lane; i < total; i += 32) {
             const int r = i / per, x = i - r * per, panel = x >> 3, chunk = x & 7;
-            const long long off = S->row_off[r];
+            const long long off = row_off[r];
             if (off < 0 && !zero) continue;
             uint4 u = make_uint4(0, 0, 0, 0);
             if (off >= 0) u = *reinterpret_cast<const uint4 *>(src + off + c0 + 8 * x);
@@ -290,66 +295,65 @@ struct Copier {
         __syncwarp();
     }
     // This CTA's 64 positions of the tile's K: panels of [64 rows][64 columns].
-    __device__ __forceinline__ void keys(int tile) {
-        const uint32_t s = acquire();
+    __device__ __forceinline__ void keys(int tile, uint32_t n) {
+        mask(tile);
+        const uint32_t s = acquire(n);
         uint8_t *dst = ring + s * Cfg<D>::kStageB;
         const uint32_t bar = cluster_addr(&S->full[s], 0);
-        if (a.box_rows > 0) {
-            const int per = 64 / a.box_rows, first = rank * per;
-            const uint32_t mine = (boxes >> first) & ((1u << per) - 1u);
-            if (lane == 0) arrive_tx_cluster(bar, __popc(mine) * a.box_rows * D * 2);
-            __syncwarp();
-            if (lane >= first && lane < first + per && page >= 0)
-                for (int p = 0; p < D / 64; ++p)
-                    box(false, smem_u32(dst) + p * 8192 + (lane - first) * a.box_rows * 128, 64 * p, row, page, bar);
-        } else {
-            by_hand(a.c.k, dst, tile * kTile + 64 * rank, 64, 0, D / 64, false);
-            if (lane == 0) arrive_cluster(bar);
-        }
-    }
-    // This CTA's half of the columns of all of the tile's V: panels of [128 rows][64 columns]. The tile
-    // is the current one (last), or the one before it.
-    __device__ __forceinline__ void values(int tile, bool last) {
-        const uint32_t s = acquire();
-        uint8_t *dst = ring + s * Cfg<D>::kStageB;
-        const uint32_t bar = cluster_addr(&S->full[s], 0);
-        constexpr int kPanels = D / 128;
-        const int c0 = rank * (D / 2);
         if (a.box_rows == 0) {
-            by_hand(a.c.v, dst, tile * kTile, kTile, c0, kPanels, true);
+            by_hand(a.c.k, dst, tile * kTile + 64 * rank, 64, 0, D / 64, false);
             if (lane == 0) arrive_cluster(bar);
             return;
         }
-        const int pg = last ? page : v_page, r = last ? row : v_row;
-        const uint32_t bx = last ? boxes : v_boxes;
-        const int n = kTile / a.box_rows;
-        const bool clean = __popc(bx) == n && (tile + 1) * kTile <= len;
-        const uint32_t bytes = __popc(bx) * a.box_rows * 128 * kPanels;
-        const uint32_t to = clean ? bar : cluster_addr(&S->landed, rank);
-        if (lane == 0) {
-            if (clean) arrive_tx_cluster(bar, bytes);
-            else arrive_tx_cluster(to, bytes);
-        }
+        const int per = 64 >> a.box_shift, first = rank * per;
+        const uint32_t mine = (boxes >> first) & ((1u << per) - 1u);
+        if (lane == 0) arrive_tx_cluster(bar, __popc(mine) * a.box_rows * D * 2);
         __syncwarp();
-        if (pg >= 0)
-            for (int p = 0; p < kPanels; ++p)
-                box(true, smem_u32(dst) + p * 16384 + lane * a.box_rows * 128, c0 + 64 * p, r, pg, to);
+        if (lane >= first && lane < first + per && page >= 0) {
+            const uint32_t at = smem_u32(dst) + (lane - first) * a.box_rows * 128;
+            if (a.box_rows == 64) {   // all panels in one copy
+                tma_box(at, &a.k_map, 0, row, kvh, page, bar);
+            } else {
+                for (int p = 0; p < D / 64; ++p) tma_box(at + p * 8192, &a.k_map, p, row, kvh, page, bar);
+            }
+        }
+    }
+    // This CTA's half of the columns of all of the tile's V. One copy a box: [box][panel][rows][64].
+    __device__ __forceinline__ void values(int tile, uint32_t n) {
+        const uint32_t s = acquire(n);
+        uint8_t *dst = ring + s * Cfg<D>::kStageB;
+        const uint32_t bar = cluster_addr(&S->full[s], 0);
+        constexpr int kPanels = D / 128;
+        if (a.box_rows == 0) {
+            by_hand(a.c.v, dst, tile * kTile, kTile, rank * (D / 2), kPanels, true);
+            if (lane == 0) arrive_cluster(bar);
+            return;
+        }
+        const bool clean = __popc(boxes) == kTile >> a.box_shift && (tile + 1) * kTile <= len;
+        const uint32_t bytes = __popc(boxes) * a.box_rows * 128 * kPanels;
+        const uint32_t to = clean ? bar : cluster_addr(&S->landed, rank);
+        if (lane == 0) arrive_tx_cluster(to, bytes);
+        __syncwarp();
+        if (page >= 0)
+            tma_box(smem_u32(dst) + lane * a.box_rows * 128 * kPanels, &a.v_map, rank * kPanels, row, kvh, page, to);
         if (!clean) {
             wait_cluster(&S->landed, landed & 1, &S->stop);
             ++landed;
-            // rows that are no positions: 8 kPanels lanes a row
-            constexpr int kLanes = 8 * kPanels;
-            const uint32_t *info = S->info[tile % kInfo];
-            const int exist = len - tile * kTile;   // rows from here on lie behind the sequence
-            const int part = lane % kLanes;
-            for (int i = lane / kLanes + (info[4] ? exist & ~(32 / kLanes - 1) : 0); i < kTile; i += 32 / kLanes)
-                if (i >= exist || !(info[i >> 5] >> (i & 31) & 1u))
-                    *reinterpret_cast<uint4 *>(dst + (part >> 3) * 16384 + i * 128 + (part & 7) * 16) = make_uint4(0, 0, 0, 0);
+            // rows that are no positions: a box's rows [exist, box_rows), or all of them
+            for (int i = 0; i < kTile >> a.box_shift; ++i) {
+                const int exist = (boxes >> i & 1u) ? max(0, min(a.box_rows, len - tile * kTile - i * a.box_rows)) : 0;
+                uint8_t *box = dst + i * a.box_rows * 128 * kPanels;
+                for (int x = lane; x < (a.box_rows - exist) * 8 * kPanels; x += 32) {
+                    const int panel = kPanels == 1 ? 0 : x & 1, y = x / kPanels;
+                    *reinterpret_cast<uint4 *>(box + panel * a.box_rows * 128 + exist * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+                }
+            }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) arrive_cluster(bar);
         }
     }
+    uint32_t landed = 0;
 };
 
 template <int D>
@@ -440,28 +444,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
 
     if (warp == 4) {
         if (n_tiles > 0) {
-            Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
-            asm volatile("griddepcontrol.wait;" ::: "memory");   // the prepared queries
-            if (lane == 0) {
-                const uint32_t bar = cluster_addr(&S.q_ready, 0);
-                arrive_tx_cluster(bar, C::kQB);
-                for (int p = 0; p < D / 64; ++p)
-                    tma_rows(smem_u32(q_smem) + p * (kRows * 128), &a.q_map, 64 * p,
-                             (kvh * a.total_rows + lo + my_tok0) * a.group, bar);
-            }
-            __syncwarp();
+            Copier<D> cp{a, &S, ring, S.row_off, b, kvh, rank, lane, len};
+            if (a.box_rows > 0) cp.look_ahead(0);
             for (int j = 0; j < n_tiles; ++j) {
-                cp.begin(j);
-                cp.keys(j);
-                if (j > 0) cp.values(j - 1, false);
+                cp.begin(j, j + 1 < n_tiles);
+                cp.keys(j, j == 0 ? 0 : 2 * j - 1);
+                if (j == 0) {
+                    asm volatile("griddepcontrol.wait;" ::: "memory");   // the prepared queries
+                    if (lane == 0) {
+                        const uint32_t bar = cluster_addr(&S.q_ready, 0);
+                        arrive_tx_cluster(bar, C::kQB);
+                        for (int p = 0; p < D / 64; ++p)
+                            tma_rows(smem_u32(q_smem) + p * (kRows * 128), &a.q_map, 64 * p,
+                                     (kvh * a.total_rows + lo + my_tok0) * a.group, bar);
+                    }
+                    __syncwarp();
+                }
             }
-            cp.values(n_tiles - 1, true);
+        }
+    } else if (warp == 6) {
+        Copier<D> cp{a, &S, ring, S.row_off + 64, b, kvh, rank, lane, len};
+        if (a.box_rows > 0 && n_tiles > 0) cp.look_ahead(0);
+        for (int j = 0; j < n_tiles; ++j) {
+            cp.begin(j, j + 1 < n_tiles);
+            cp.values(j, j < n_tiles - 1 ? 2 * j + 2 : 2 * n_tiles - 1);
         }
     } else if (warp == 5) {
         if (rank == 0 && lane == 0 && n_tiles > 0) {
             const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
             uint32_t used = 0;
             const uint32_t id_s = idesc2(kTile, 0), id_o = idesc2(D, 1);
+            // V in shared memory: [box][panel][rows][64], one box when the warp copies
+            const int v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
             bool ok = wait_cluster(&S.q_ready, 0, &S.stop);
             auto pv = [&](int j) {
                 ok = ok && wait_cluster(&S.p_ready[j & 1], (j >> 1) & 1, &S.stop);
@@ -473,7 +487,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 const uint32_t at = ring_at + s * C::kStageB, p = tmem + C::kS + (j & 1) * kTile;
 #pragma unroll
                 for (int i = 0; i < kTile / 16; ++i)
-                    mma2_ts(tmem + C::kO, p + 8 * i, desc_mn(at + 2048 * i, 16384), id_o, (j > 0 || i > 0) ? 1u : 0u);
+                    mma2_ts(tmem + C::kO, p + 8 * i,
+                            desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1 << v_shift) - 1)) * 2048, v_rows * 128),
+                            id_o, (j > 0 || i > 0) ? 1u : 0u);
                 commit2(&S.empty[s]);
                 commit2(&S.o_done);
             };
@@ -605,7 +621,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         tc_fence_before();
     }
     __syncthreads();
-    if (S.stop && warp == 4) {   // copies in flight land before the shared memory goes (each wait bounded)
+    if (S.stop && (warp == 4 || warp == 6)) {   // copies in flight land before the shared memory goes (each wait bounded)
         int go_on = 0;
         for (int s = 0; s < C::kStages; ++s)
             for (int n = 0; n < 1000 && !mbar_try_wait_sleep(&S.full[s], go_on, 1000); ++n) {}
@@ -629,18 +645,18 @@ EncodeFn encode_fn() {
     return fn;
 }
 
-// Pages as a 4D tensor, dims in the order of their strides; boxes of 64 columns and `rows` rows of one
-// page and head, 128-byte swizzle.
-bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, bool rows_inner) {
-    const cuuint64_t row_b = c.row_stride * 2, head_b = c.head_stride * 2, page_b = c.page_stride * 2;
-    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)(rows_inner ? c.page_size : heads),
-                                (cuuint64_t)(rows_inner ? heads : c.page_size), (cuuint64_t)c.num_pages};
-    const cuuint64_t strides[3] = {rows_inner ? row_b : head_b, rows_inner ? head_b : row_b, page_b};
-    const cuuint32_t box[4] = {64, (cuuint32_t)(rows_inner ? rows : 1), (cuuint32_t)(rows_inner ? 1 : rows), 1};
-    const cuuint32_t es[4] = {1, 1, 1, 1};
+// Pages as a 5D tensor (64 columns, page rows, panels of 64 columns, heads, pages); boxes of `rows`
+// rows and `panels` panels of one page and head, 128-byte swizzle: in shared memory [panel][row][64].
+bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, int panels) {
+    const cuuint64_t dims[5] = {64, (cuuint64_t)c.page_size, (cuuint64_t)(d / 64), (cuuint64_t)heads,
+                                (cuuint64_t)c.num_pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)c.row_stride * 2, 128, (cuuint64_t)c.head_stride * 2,
+                                   (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)panels, 1, 1};
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
     EncodeFn fn = encode_fn();
     return fn != nullptr &&
-           fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<uint16_t *>(base), dims, strides, box, es,
+           fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<uint16_t *>(base), dims, strides, box, es,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -728,14 +744,16 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.prep_rows = per < 1 ? 1 : (per > kPrepRows ? kPrepRows : per);
     if (!query_map(&a.q_map, a.q_ready, shape->head_dim, (long long)total_rows * shape->q_heads))
         return full_attn_fail(NMOE_ECUDA, "cuTensorMapEncodeTiled failed");
-    // boxes of the largest power of two of rows that divides a page, up to 64
-    int box = a.c.page_size & -a.c.page_size;
+    // boxes of the largest power of two of rows that divides a page, 16 to 64: an MMA's 16 positions lie
+    // in one box. A page's K box takes all panels at 64 rows (the tile's rows are then 128 bytes apart).
+    int box = a.c.page_size & -a.c.page_size, shift = 0;
     box = box > 64 ? 64 : box;
-    a.rows_inner = a.c.row_stride <= a.c.head_stride;
-    a.box_rows = box < 8 ? 0 : box;
-    if (a.box_rows > 0 &&
-        !(page_map(&a.k_map, a.c, a.c.k, shape->head_dim, a.kv_heads, box, a.rows_inner) &&
-          page_map(&a.v_map, a.c, a.c.v, shape->head_dim, a.kv_heads, box, a.rows_inner)))
+    while (1 << shift < box) ++shift;
+    a.box_rows = box < 16 ? 0 : box;
+    a.box_shift = shift;
+    const int d = shape->head_dim;
+    if (a.box_rows > 0 && !(page_map(&a.k_map, a.c, a.c.k, d, a.kv_heads, box, box == 64 ? d / 64 : 1) &&
+                            page_map(&a.v_map, a.c, a.c.v, d, a.kv_heads, box, d / 128)))
         a.box_rows = 0;   // strides that a tensor map cannot have: the warp copies
     const int per_unit = 2 * (kRows / a.group);
     const long long units = ((long long)total_rows / per_unit + num_seqs) * a.kv_heads;
