@@ -13,8 +13,8 @@
 // half; a CTA of its own with M = 128 would have to read 62 bytes a cycle from L2 and 160 a cycle
 // from shared memory to keep the tensor cores busy, the pair 31 and 95.
 //
-// Softmax: a thread per query row (warps 0-3) reads its 128 scores from tensor memory, keeps the
-// running maximum and sum in fp32, and writes P back as bf16 over the scores. O is rescaled only
+// Softmax: two threads per query row (warps 0-7, 64 columns each) read its 128 scores from tensor
+// memory, keep the running maximum and sum in fp32, and write P back as bf16 over the scores. O is rescaled only
 // when a row's maximum has grown by more than 2^8 since the last time: O and the sum carry the same
 // reference, so the result does not depend on which one it is. While S of tile j is in the softmax,
 // the tensor cores run S of tile j + 1 and P V of tile j - 1.
@@ -54,29 +54,36 @@ struct PrefillArgs {
     int box_rows, box_shift;   // rows of a TMA box: 16, 32 or 64, or 0: no TMA
 };
 
-constexpr int kThreads = 224;   // warps 0-3 softmax, 4 copies Q and K, 5 MMA, 6 copies V
+constexpr int kThreads = 352;   // warps 0-7 softmax, 8 copies Q and K, 9 MMA, 10 copies V
 constexpr int kRows = 128;      // query rows of a CTA
 constexpr int kTile = 128;      // positions of a tile
 constexpr int kInfo = 8;        // ring of tile masks
+
+struct Shared {
+    uint64_t full[10], empty[10], landed, s_full[2], p_ready[2], o_done, q_ready;
+    uint32_t info[kInfo][5];          // valid positions of a tile, then whether all are
+    long long scan[kThreads / 32];
+    long long unit_off;
+    int unit_seq;
+    float row_max[2][2][kRows];       // of a row's two halves, by the parity of the tile
+    uint32_t tmem;
+    int stop;                         // a bounded wait has run out
+};
 
 template <int D>
 struct Cfg {
     static constexpr int kQB = kRows * D * 2;
     static constexpr int kStageB = 64 * D * 2;              // half a K or V tile
     static constexpr int kStages = D == 256 ? 5 : 10;
-    static constexpr int kSmem = kQB + kStages * kStageB + 1024;   // + alignment
+    static constexpr int kRing = kQB, kShared = kQB + kStages * kStageB;   // offsets in shared memory
+    static constexpr int kSmem = kShared + (int)sizeof(Shared);
+    static_assert(kSmem <= 232448, "shared memory of a CTA");
     static constexpr uint32_t kO = 0, kS = D;               // TMEM columns: O, then two S tiles of 128
-};
-
-struct Shared {
-    uint64_t full[10], empty[10], landed, s_full[2], p_ready[2], o_done, q_ready;
-    long long row_off[64 + kTile];    // of the two copying warps
-    uint32_t info[kInfo][5];          // valid positions of a tile, then whether all are
-    long long scan[kThreads / 32];
-    long long unit_off;
-    int unit_seq;
-    uint32_t tmem;
-    int stop;                         // a bounded wait has run out
+    static constexpr int kOutB = D * 4 + 16;                // a row of O on its way out
+    static_assert(kRows * kOutB <= kQB + kStages * kStageB, "the output rows reuse the queries and the ring");
+    // the stage that holds K tile j, V tile j of n
+    __device__ static uint32_t k_stage(int j) { return j == 0 ? 0 : 2 * j - 1; }
+    __device__ static uint32_t v_stage(int j, int n) { return j == n - 1 ? 2 * j + 1 : 2 * j + 2; }
 };
 
 __device__ __forceinline__ uint32_t cluster_addr(const void *p, int rank) {
@@ -158,10 +165,26 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t panel) {
 __device__ __forceinline__ uint32_t idesc2(int n, int b_mn) {   // bf16 x bf16 -> fp32, M = 256
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (16u << 24);
 }
-__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t *v) {
-    tc_st16(taddr, v);
-    tc_st16(taddr + 16, v + 16);
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// The two warps of a row quarter.
+__device__ __forceinline__ void pair_sync(int quad) { asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory"); }
 __device__ __forceinline__ float ex2f(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -214,7 +237,6 @@ struct Copier {
     const PrefillArgs &a;
     Shared *S;
     uint8_t *ring;
-    long long *row_off;            // pages without TMA: element offset of each position, -1: none
     int b, kvh, rank, lane, len;   // len: positions that exist
     int page = -1, row = 0;        // this lane's box of the current tile (TMA)
     int next_page = -1, next_row = 0;
@@ -273,23 +295,22 @@ struct Copier {
     // Positions p0 .. p0 + n - 1, columns c0 .. c0 + 64 panels - 1, by the warp's own loads and stores.
     __device__ __forceinline__ void by_hand(const uint16_t *src, uint8_t *dst, int p0, int n, int c0, int panels,
                                             bool zero) const {
-        for (int i = lane; i < n; i += 32) {
-            int r;
-            const int p = p0 + i, pg = p < len ? checked(lookup(p, &r)) : -1;
-            row_off[i] = pg < 0 ? -1
-                                : (long long)pg * a.c.page_stride + (long long)r * a.c.row_stride +
-                                      (long long)kvh * a.c.head_stride;
-        }
-        __syncwarp();
-        const int per = panels * 8, total = n * per;
+        const int per = panels * 8;   // 16-byte pieces of a row
+        for (int base = 0; base < n; base += 32) {
+            int in_page;
+            const int p = p0 + base + lane, pg = p < len ? checked(lookup(p, &in_page)) : -1;
+            const long long mine = pg < 0 ? -1
+                                          : (long long)pg * a.c.page_stride + (long long)in_page * a.c.row_stride +
+                                                (long long)kvh * a.c.head_stride;
 #pragma unroll 4
-        for (int i = lane; i < total; i += 32) {
-            const int r = i / per, x = i - r * per, panel = x >> 3, chunk = x & 7;
-            const long long off = row_off[r];
-            if (off < 0 && !zero) continue;
-            uint4 u = make_uint4(0, 0, 0, 0);
-            if (off >= 0) u = *reinterpret_cast<const uint4 *>(src + off + c0 + 8 * x);
-            *reinterpret_cast<uint4 *>(dst + panel * n * 128 + sw128_off(r, chunk)) = u;
+            for (int i = lane; i < 32 * per; i += 32) {
+                const int r = i / per, x = i - r * per, panel = x >> 3, chunk = x & 7;
+                const long long off = __shfl_sync(0xffffffffu, mine, r);
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (off >= 0) u = *reinterpret_cast<const uint4 *>(src + off + c0 + 8 * x);
+                if (off >= 0 || zero) *reinterpret_cast<uint4 *>(dst + panel * n * 128 + sw128_off(base + r, chunk)) = u;
+            }
+            __syncwarp();
         }
         fence_async_smem();
         __syncwarp();
@@ -359,11 +380,10 @@ struct Copier {
 template <int D>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefill_pairs(const __grid_constant__ PrefillArgs a) {
     using C = Cfg<D>;
-    extern __shared__ uint8_t raw[];
-    __shared__ Shared S;
+    extern __shared__ __align__(1024) uint8_t raw[];   // the only shared memory: queries, ring, the rest
     cg::cluster_group cluster = cg::this_cluster();
-    uint8_t *q_smem = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
-    uint8_t *ring = q_smem + C::kQB;
+    uint8_t *q_smem = raw, *ring = raw + C::kRing;
+    Shared &S = *reinterpret_cast<Shared *>(raw + C::kShared);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)cluster.block_rank();
     const int per_cta = kRows / a.group, per_unit = 2 * per_cta;   // tokens
@@ -426,14 +446,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&S.s_full[s], 1);
-            mbar_init(&S.p_ready[s], 8);   // the softmax warps of both CTAs
+            mbar_init(&S.p_ready[s], 16);   // the softmax warps of both CTAs
         }
         mbar_init(&S.landed, 1);
         mbar_init(&S.o_done, 1);
         mbar_init(&S.q_ready, 2);
         mbar_fence_init();
     }
-    if (warp == 5) {
+    if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
@@ -442,13 +462,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
     tc_fence_after();
     const uint32_t tmem = S.tmem;
 
-    if (warp == 4) {
+    if (warp == 8) {
         if (n_tiles > 0) {
-            Copier<D> cp{a, &S, ring, S.row_off, b, kvh, rank, lane, len};
+            Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
             if (a.box_rows > 0) cp.look_ahead(0);
             for (int j = 0; j < n_tiles; ++j) {
                 cp.begin(j, j + 1 < n_tiles);
-                cp.keys(j, j == 0 ? 0 : 2 * j - 1);
+                cp.keys(j, C::k_stage(j));
                 if (j == 0) {
                     asm volatile("griddepcontrol.wait;" ::: "memory");   // the prepared queries
                     if (lane == 0) {
@@ -462,14 +482,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 }
             }
         }
-    } else if (warp == 6) {
-        Copier<D> cp{a, &S, ring, S.row_off + 64, b, kvh, rank, lane, len};
+    } else if (warp == 10) {
+        Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
         if (a.box_rows > 0 && n_tiles > 0) cp.look_ahead(0);
         for (int j = 0; j < n_tiles; ++j) {
             cp.begin(j, j + 1 < n_tiles);
-            cp.values(j, j < n_tiles - 1 ? 2 * j + 2 : 2 * n_tiles - 1);
+            cp.values(j, C::v_stage(j, n_tiles));
         }
-    } else if (warp == 5) {
+    } else if (warp == 9) {
         if (rank == 0 && lane == 0 && n_tiles > 0) {
             const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
             uint32_t used = 0;
@@ -506,18 +526,69 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                             desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u);
                 commit2(&S.empty[s]);
                 commit2(&S.s_full[j & 1]);
+                if (j > 0) pv(j - 1);   // S of tile j runs while tile j - 1 is in the softmax
+            }
+            if (ok) pv(n_tiles - 1);
+        }
+    } else if (warp == 10) {
+        Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
+        if (a.box_rows > 0 && n_tiles > 0) cp.look_ahead(0);
+        for (int j = 0; j < n_tiles; ++j) {
+            cp.begin(j, j + 1 < n_tiles);
+            cp.values(j, C::v_stage(j, n_tiles));
+        }
+    } else if (warp == 9) {
+        if (rank == 0 && lane == 0 && n_tiles > 0) {
+            const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
+            uint32_t used = 0;
+            const uint32_t id_s = idesc2(kTile, 0), id_o = idesc2(D, 1);
+            // V in shared memory: [box][panel][rows][64], one box when the warp copies
+            const int v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
+            bool ok = wait_cluster(&S.q_ready, 0, &S.stop);
+            auto pv = [&](int j) {
+                ok = ok && wait_cluster(&S.p_ready[j & 1], (j >> 1) & 1, &S.stop);
+                const uint32_t s = used % C::kStages;
+                ok = ok && wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
+                if (!ok) return;
+                ++used;
+                tc_fence_after();
+                const uint32_t at = ring_at + s * C::kStageB, p = tmem + C::kS + (j & 1) * kTile;
+#pragma unroll
+                for (int i = 0; i < kTile / 16; ++i)
+                    mma2_ts(tmem + C::kO, p + 8 * i,
+                            desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1 << v_shift) - 1)) * 2048, v_rows * 128),
+                            id_o, (j > 0 || i > 0) ? 1u : 0u);
+                commit2(&S.empty[s]);
+                commit2(&S.o_done);
+            };
+            for (int j = 0; j < n_tiles && ok; ++j) {
+                const uint32_t s = used % C::kStages;
+                ok = wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
+                if (!ok) break;
+                ++used;
+                tc_fence_after();
+                const uint32_t at = ring_at + s * C::kStageB, d = tmem + C::kS + (j & 1) * kTile;
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+                    mma2_ss(d, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
+                            desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u);
+                commit2(&S.empty[s]);
+                commit2(&S.s_full[j & 1]);
+                // two S tiles: S of tile j runs while tile j - 1 is in the softmax
                 if (j > 0) pv(j - 1);
             }
             if (ok) pv(n_tiles - 1);
         }
     } else {
-        const int token = tid / a.group, head = tid - token * a.group;   // this thread's row
+        // ---- softmax: two threads a row, 64 columns each; warps w and w + 4 hold the same 32 rows
+        const int wg = warp >> 2, quad = warp & 3, r_cta = quad * 32 + lane;
+        const int token = r_cta / a.group;
         const bool live = token < my_rows;
         const long long pos64 = seq0 + my_tok0 + token;
         // position up to which this row sees; -1: nothing
         const int pos = live && pos64 >= 0 ? (int)min(pos64, (long long)len - 1) : -1;
         float m = -INFINITY, l = 0.f;
-        const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+        const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         if (n_tiles > 0) {
             const uint32_t p_bar = cluster_addr(&S.p_ready[0], 0);
             // the first position that some row of this warp does not see
@@ -526,27 +597,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 wait_cluster(&S.s_full[j & 1], (j >> 1) & 1, &S.stop);
                 tc_fence_after();
                 const uint32_t st = tmem + lanes + C::kS + (j & 1) * kTile;
-                float s[kTile];
+                float s[64];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tc_ld32(st + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+                for (int c = 0; c < 2; ++c) tc_ld32(st + 64 * wg + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
                 tc_wait_ld();
                 const uint32_t *info = S.info[j % kInfo];
                 if ((j + 1) * kTile > seen || !info[4]) {
-                    const int n = pos - j * kTile;   // columns 0..n are seen
+                    const int n = pos - j * kTile - 64 * wg;   // columns 0..n of this half are seen
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 2; ++c) {
                         const int k = n - 32 * c;
-                        const uint32_t w = info[c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
+                        const uint32_t w = info[2 * wg + c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) s[32 * c + i] = w >> i & 1u ? s[32 * c + i] : -INFINITY;
                     }
                 }
                 float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < kTile; i += 4)
+                for (int i = 4; i < 60; i += 8)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[i + x]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                    for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[i + x], s[i + 4 + x]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[60 + x]);
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                S.row_max[j & 1][wg][r_cta] = top;
+                tc_fence_before();
+                pair_sync(quad);   // the other half's maximum; and its scores are read: P may go over them
+                tc_fence_after();
+                top = fmaxf(top, S.row_max[j & 1][wg ^ 1][r_cta]);
                 const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
                 const float mn = grow ? top : m;
                 const float base = mn == -INFINITY ? 0.f : mn;
@@ -554,32 +632,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 const float c = grow ? ex2f(m - base) : 1.0f;
                 l *= c;
                 m = mn;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint64_t neg = pack_f32x2(-base, -base);
+                uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int i = 0; i < kTile; i += 4)
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t p[16];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        s[i + x] = ex2f(s[i + x] - base);
-                        sum[x] += s[i + x];
+                    for (int i = 0; i < 16; ++i) {
+                        float e0, e1;
+                        unpack_f32x2(add_f32x2(pack_f32x2(s[32 * x + 2 * i], s[32 * x + 2 * i + 1]), neg), e0, e1);
+                        e0 = ex2f(e0), e1 = ex2f(e1);
+                        sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
+                        p[i] = pack2_bf16(e0, e1);
                     }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                uint32_t p[kTile / 2];
-#pragma unroll
-                for (int i = 0; i < kTile / 2; ++i) p[i] = pack2_bf16(s[2 * i], s[2 * i + 1]);
-                tc_st32(st, p);
-                tc_st32(st + 32, p + 32);
+                    tc_st16(st + 32 * wg + 16 * x, p);
+                }
+                float s0, s1;
+                unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
+                l += s0 + s1;
                 // P V of tile j - 1 is complete: the tensor cores are at S of tile j + 1 by now
                 if (j > 0) wait_cluster(&S.o_done, (j - 1) & 1, &S.stop);
                 if (scale_o) {
                     tc_fence_after();
 #pragma unroll 1
-                    for (int x = 0; x < D; x += 32) {
+                    for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
                         uint32_t o[32];
                         tc_ld32(tmem + lanes + C::kO + x, o);
                         tc_wait_ld();
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * c);
-                        tc_st32(tmem + lanes + C::kO + x, o);
+                        tc_st16(tmem + lanes + C::kO + x, o);
+                        tc_st16(tmem + lanes + C::kO + x + 16, o + 16);
                     }
                 }
                 tc_wait_st();
@@ -589,46 +672,75 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
             }
             wait_cluster(&S.o_done, (n_tiles - 1) & 1, &S.stop);
             tc_fence_after();
+            float(*sums)[kRows] = S.row_max[n_tiles & 1];   // the parity that the last tile left alone
+            sums[wg][r_cta] = l;
+            pair_sync(quad);
+            l += sums[wg ^ 1][r_cta];
         }
-        // ---- O / l times the gate
-        const int heads = a.kv_heads * a.group;
-        const long long r = (long long)lo + my_tok0 + token;
-        uint16_t *out = a.out + (r * heads + kvh * a.group + head) * D;
-        const long long gate = r * a.q_stride + (long long)(kvh * a.group + head) * 2 * D + D;
+        // ---- O / l through shared memory (the MMAs have read the queries and the ring for the last
+        // time), so that a warp gates and stores a row of D at a time
         const float inv = S.stop ? NAN : l == 0.f ? 0.f : 1.0f / l;
+        uint8_t *rows_out = q_smem + quad * 32 * C::kOutB;
+        if (n_tiles > 0) {
+            uint8_t *to = rows_out + lane * C::kOutB;
 #pragma unroll 1
-        for (int x = 0; x < D; x += 32) {
-            uint32_t o[32];
-            float g[32];
-            if (a.gated && live)
-#pragma unroll
-                for (int y = 0; y < 32; y += 8) load_elems<8>(a.q, gate + x + y, a.x_bf16, g + y);
-            if (n_tiles > 0) {
+            for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
+                uint32_t o[32];
                 tc_ld32(tmem + lanes + C::kO + x, o);
                 tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = inv == 0.f ? 0u : __float_as_uint(__uint_as_float(o[i]) * inv);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    *reinterpret_cast<uint4 *>(to + (x + i) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
-            if (live) {
-                float v[32];
+            pair_sync(quad);
+        }
+        constexpr int E = D / 32;
+        const int heads = a.kv_heads * a.group, first = wg * 16;   // this warp's 16 of the pair's 32 rows
+        const int mine = min(first + 16, my_rows * a.group - quad * 32);
+        constexpr int kAtOnce = 8;   // rows whose gates are on their way together
+        for (int i0 = first; i0 < mine; i0 += kAtOnce) {
+            float g[kAtOnce][E];
+            long long to[kAtOnce];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    v[i] = inv == 0.f ? 0.f : __uint_as_float(o[i]) * inv;
-                    if (a.gated) v[i] *= __fdividef(1.0f, 1.0f + __expf(-g[i]));
+            for (int y = 0; y < kAtOnce; ++y) {
+                const int rr = quad * 32 + min(i0 + y, mine - 1), tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
+                const long long r = (long long)lo + my_tok0 + tok;
+                to[y] = (r * heads + h) * D + E * lane;
+                if (a.gated) load_elems<E>(a.q, r * a.q_stride + (long long)h * 2 * D + D + E * lane, a.x_bf16, g[y]);
+            }
+#pragma unroll
+            for (int y = 0; y < kAtOnce; ++y) {
+                if (i0 + y >= mine) break;
+                float v[E];
+#pragma unroll
+                for (int x = 0; x < E; ++x) v[x] = 0.f;
+                if (n_tiles > 0) {
+                    const float4 *src = reinterpret_cast<const float4 *>(rows_out + (i0 + y) * C::kOutB + E * lane * 4);
+#pragma unroll
+                    for (int x = 0; x < E / 4; ++x) {
+                        const float4 f = src[x];
+                        v[4 * x] = f.x, v[4 * x + 1] = f.y, v[4 * x + 2] = f.z, v[4 * x + 3] = f.w;
+                    }
                 }
+                if (a.gated)
 #pragma unroll
-                for (int y = 0; y < 32; y += 8) store_bf16<8>(out + x + y, v + y);
+                    for (int x = 0; x < E; ++x) v[x] = __fdividef(v[x], 1.0f + __expf(-g[y][x]));
+                store_bf16<E>(a.out + to[y], v);
             }
         }
         tc_fence_before();
     }
     __syncthreads();
-    if (S.stop && (warp == 4 || warp == 6)) {   // copies in flight land before the shared memory goes (each wait bounded)
+    if (S.stop && (warp == 8 || warp == 10)) {   // copies in flight land before the shared memory goes (each wait bounded)
         int go_on = 0;
         for (int s = 0; s < C::kStages; ++s)
             for (int n = 0; n < 1000 && !mbar_try_wait_sleep(&S.full[s], go_on, 1000); ++n) {}
     }
     cluster.sync();   // neither CTA leaves while the other may still signal it
     tc_fence_after();
-    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
