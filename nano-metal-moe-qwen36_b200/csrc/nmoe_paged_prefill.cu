@@ -91,20 +91,27 @@ __device__ __forceinline__ uint32_t cluster_addr(const void *p, int rank) {
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
     return r;
 }
+// After writes to shared memory that the pair's MMAs read.
 __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Where no generic write has to be seen by the other CTA: P goes through tensor memory, ordered by the
+// tcgen05 fences, and copies complete on the barrier themselves. A release at cluster scope takes 1200
+// cycles here, in every tile's critical path.
+__device__ __forceinline__ void signal_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void arrive_tx_cluster(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+    asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
 // Bounded wait: a barrier that never completes sets `stop` and lets every later wait go at once.
-__device__ __forceinline__ bool wait_cluster(uint64_t *bar, uint32_t parity, volatile int *stop) {
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
     for (uint32_t n = 0;; ++n) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
             : "r"(smem_u32(bar)), "r"(parity)
@@ -133,27 +140,36 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, i
         "l"(map), "r"(col), "r"(row), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The MMAs and commits are executed by a whole warp, of which one lane (`one` != 0) issues: operands
+// that are the same in all lanes stay in uniform registers. In a branch of one lane each MMA took 85
+// cycles to issue, more than the 64 that it runs.
+__device__ __forceinline__ void mma2_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma2_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
         : "memory");
 }
 // All MMAs issued so far have completed: one arrival at the barrier of both CTAs.
-__device__ __forceinline__ void commit2(uint64_t *bar) {
+__device__ __forceinline__ void commit2(uint64_t *bar, uint32_t one) {
     asm volatile(
-        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(
             smem_u32(bar)),
-        "h"((uint16_t)3)
+        "h"((uint16_t)3), "r"(one)
         : "memory");
+}
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
 }
 // [row][64 columns] panels, 128-byte swizzle, 8 rows apart 1024 bytes. K-major: the columns are the
 // sum's index. MN-major: the rows are, and 64-column panels lie `panel` bytes apart.
@@ -289,7 +305,7 @@ struct Copier {
     }
     __device__ __forceinline__ uint32_t acquire(uint32_t n) const {   // the n-th stage filled
         const uint32_t s = n % Cfg<D>::kStages;
-        wait_cluster(&S->empty[s], ((n / Cfg<D>::kStages) & 1) ^ 1, &S->stop);
+        wait_bar(&S->empty[s], ((n / Cfg<D>::kStages) & 1) ^ 1, &S->stop);
         return s;
     }
     // Positions p0 .. p0 + n - 1, columns c0 .. c0 + 64 panels - 1, by the warp's own loads and stores.
@@ -358,7 +374,7 @@ struct Copier {
         if (page >= 0)
             tma_box(smem_u32(dst) + lane * a.box_rows * 128 * kPanels, &a.v_map, rank * kPanels, row, kvh, page, to);
         if (!clean) {
-            wait_cluster(&S->landed, landed & 1, &S->stop);
+            wait_bar(&S->landed, landed & 1, &S->stop);
             ++landed;
             // rows that are no positions: a box's rows [exist, box_rows), or all of them
             for (int i = 0; i < kTile >> a.box_shift; ++i) {
@@ -490,94 +506,51 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
             cp.values(j, C::v_stage(j, n_tiles));
         }
     } else if (warp == 9) {
-        if (rank == 0 && lane == 0 && n_tiles > 0) {
+        if (rank == 0 && n_tiles > 0) {
+            // every value below is the same in all lanes, and the compiler can see it (votes, shuffles)
+            const uint32_t one = elect_one();
             const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
-            uint32_t used = 0;
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const int n = __shfl_sync(0xffffffffu, n_tiles, 0);
             const uint32_t id_s = idesc2(kTile, 0), id_o = idesc2(D, 1);
             // V in shared memory: [box][panel][rows][64], one box when the warp copies
-            const int v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
-            bool ok = wait_cluster(&S.q_ready, 0, &S.stop);
-            auto pv = [&](int j) {
-                ok = ok && wait_cluster(&S.p_ready[j & 1], (j >> 1) & 1, &S.stop);
-                const uint32_t s = used % C::kStages;
-                ok = ok && wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
-                if (!ok) return;
-                ++used;
-                tc_fence_after();
-                const uint32_t at = ring_at + s * C::kStageB, p = tmem + C::kS + (j & 1) * kTile;
-#pragma unroll
-                for (int i = 0; i < kTile / 16; ++i)
-                    mma2_ts(tmem + C::kO, p + 8 * i,
-                            desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1 << v_shift) - 1)) * 2048, v_rows * 128),
-                            id_o, (j > 0 || i > 0) ? 1u : 0u);
-                commit2(&S.empty[s]);
-                commit2(&S.o_done);
+            const uint32_t v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop));
             };
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                const uint32_t s = used % C::kStages;
-                ok = wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
-                if (!ok) break;
-                ++used;
-                tc_fence_after();
-                const uint32_t at = ring_at + s * C::kStageB, d = tmem + C::kS + (j & 1) * kTile;
-#pragma unroll
-                for (int i = 0; i < D / 16; ++i)
-                    mma2_ss(d, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
-                            desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u);
-                commit2(&S.empty[s]);
-                commit2(&S.s_full[j & 1]);
-                if (j > 0) pv(j - 1);   // S of tile j runs while tile j - 1 is in the softmax
-            }
-            if (ok) pv(n_tiles - 1);
-        }
-    } else if (warp == 10) {
-        Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
-        if (a.box_rows > 0 && n_tiles > 0) cp.look_ahead(0);
-        for (int j = 0; j < n_tiles; ++j) {
-            cp.begin(j, j + 1 < n_tiles);
-            cp.values(j, C::v_stage(j, n_tiles));
-        }
-    } else if (warp == 9) {
-        if (rank == 0 && lane == 0 && n_tiles > 0) {
-            const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
-            uint32_t used = 0;
-            const uint32_t id_s = idesc2(kTile, 0), id_o = idesc2(D, 1);
-            // V in shared memory: [box][panel][rows][64], one box when the warp copies
-            const int v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
-            bool ok = wait_cluster(&S.q_ready, 0, &S.stop);
-            auto pv = [&](int j) {
-                ok = ok && wait_cluster(&S.p_ready[j & 1], (j >> 1) & 1, &S.stop);
-                const uint32_t s = used % C::kStages;
-                ok = ok && wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
-                if (!ok) return;
-                ++used;
-                tc_fence_after();
-                const uint32_t at = ring_at + s * C::kStageB, p = tmem + C::kS + (j & 1) * kTile;
-#pragma unroll
-                for (int i = 0; i < kTile / 16; ++i)
-                    mma2_ts(tmem + C::kO, p + 8 * i,
-                            desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1 << v_shift) - 1)) * 2048, v_rows * 128),
-                            id_o, (j > 0 || i > 0) ? 1u : 0u);
-                commit2(&S.empty[s]);
-                commit2(&S.o_done);
+            uint32_t s = 0, round = 0;   // the stage that the next MMAs read, and the parity of its use
+            auto next = [&] {
+                if (++s == C::kStages) s = 0, round ^= 1;
             };
-            for (int j = 0; j < n_tiles && ok; ++j) {
-                const uint32_t s = used % C::kStages;
-                ok = wait_cluster(&S.full[s], (used / C::kStages) & 1, &S.stop);
-                if (!ok) break;
-                ++used;
+            auto pv = [&](int j) {
+                if (!wait(&S.p_ready[j & 1], (j >> 1) & 1) || !wait(&S.full[s], round)) return false;
                 tc_fence_after();
-                const uint32_t at = ring_at + s * C::kStageB, d = tmem + C::kS + (j & 1) * kTile;
+                const uint32_t at = ring_at + s * C::kStageB, p = tm + C::kS + (j & 1) * kTile;
 #pragma unroll
-                for (int i = 0; i < D / 16; ++i)
+                for (uint32_t i = 0; i < kTile / 16; ++i)
+                    mma2_ts(tm + C::kO, p + 8 * i,
+                            desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1u << v_shift) - 1)) * 2048, v_rows * 128),
+                            id_o, (j > 0 || i > 0) ? 1u : 0u, one);
+                commit2(&S.empty[s], one);
+                commit2(&S.o_done, one);
+                next();
+                return true;
+            };
+            bool ok = wait(&S.q_ready, 0);
+            for (int j = 0; j < n && ok; ++j) {
+                if (!(ok = wait(&S.full[s], round))) break;
+                tc_fence_after();
+                const uint32_t at = ring_at + s * C::kStageB, d = tm + C::kS + (j & 1) * kTile;
+#pragma unroll
+                for (uint32_t i = 0; i < D / 16; ++i)
                     mma2_ss(d, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
-                            desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u);
-                commit2(&S.empty[s]);
-                commit2(&S.s_full[j & 1]);
-                // two S tiles: S of tile j runs while tile j - 1 is in the softmax
-                if (j > 0) pv(j - 1);
+                            desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u, one);
+                commit2(&S.empty[s], one);
+                commit2(&S.s_full[j & 1], one);
+                next();
+                if (j > 0) ok = pv(j - 1);   // S of tile j runs while tile j - 1 is in the softmax
             }
-            if (ok) pv(n_tiles - 1);
+            if (ok) pv(n - 1);
         }
     } else {
         // ---- softmax: two threads a row, 64 columns each; warps w and w + 4 hold the same 32 rows
@@ -594,7 +567,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
             // the first position that some row of this warp does not see
             const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
             for (int j = 0; j < n_tiles; ++j) {
-                wait_cluster(&S.s_full[j & 1], (j >> 1) & 1, &S.stop);
+                wait_bar(&S.s_full[j & 1], (j >> 1) & 1, &S.stop);
                 tc_fence_after();
                 const uint32_t st = tmem + lanes + C::kS + (j & 1) * kTile;
                 float s[64];
@@ -651,7 +624,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
                 // P V of tile j - 1 is complete: the tensor cores are at S of tile j + 1 by now
-                if (j > 0) wait_cluster(&S.o_done, (j - 1) & 1, &S.stop);
+                if (j > 0) wait_bar(&S.o_done, (j - 1) & 1, &S.stop);
                 if (scale_o) {
                     tc_fence_after();
 #pragma unroll 1
@@ -668,9 +641,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) arrive_cluster(p_bar + (j & 1) * 8);
+                if (lane == 0) signal_cluster(p_bar + (j & 1) * 8);
             }
-            wait_cluster(&S.o_done, (n_tiles - 1) & 1, &S.stop);
+            wait_bar(&S.o_done, (n_tiles - 1) & 1, &S.stop);
             tc_fence_after();
             float(*sums)[kRows] = S.row_max[n_tiles & 1];   // the parity that the last tile left alone
             sums[wg][r_cta] = l;
