@@ -60,7 +60,7 @@ constexpr int kTile = 128;      // positions of a tile
 constexpr int kInfo = 8;        // ring of tile masks
 
 struct Shared {
-    uint64_t full[10], empty[10], landed, s_full[2], p_ready[2], o_done, q_ready;
+    uint64_t full[10], empty[10], landed, s_full[2], p_ready[2][2], o_done, done, q_ready;
     uint32_t info[kInfo][5];          // valid positions of a tile, then whether all are
     long long scan[kThreads / 32];
     long long unit_off;
@@ -462,10 +462,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         }
         for (int s = 0; s < 2; ++s) {
             mbar_init(&S.s_full[s], 1);
-            mbar_init(&S.p_ready[s], 16);   // the softmax warps of both CTAs
+            mbar_init(&S.p_ready[s][0], 16);   // the softmax warps of both CTAs
+            mbar_init(&S.p_ready[s][1], 16);
         }
         mbar_init(&S.landed, 1);
         mbar_init(&S.o_done, 1);
+        mbar_init(&S.done, 1);
         mbar_init(&S.q_ready, 2);
         mbar_fence_init();
     }
@@ -522,24 +524,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
             auto next = [&] {
                 if (++s == C::kStages) s = 0, round ^= 1;
             };
-            auto pv = [&](int j) {
-                if (!wait(&S.p_ready[j & 1], (j >> 1) & 1) || !wait(&S.full[s], round)) return false;
-                tc_fence_after();
-                const uint32_t at = ring_at + s * C::kStageB, p = tm + C::kS + (j & 1) * kTile;
-#pragma unroll
-                for (uint32_t i = 0; i < kTile / 16; ++i)
-                    mma2_ts(tm + C::kO, p + 8 * i,
-                            desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1u << v_shift) - 1)) * 2048, v_rows * 128),
-                            id_o, (j > 0 || i > 0) ? 1u : 0u, one);
-                commit2(&S.empty[s], one);
-                commit2(&S.o_done, one);
-                next();
-                return true;
+            auto full = [&](uint32_t ahead) {   // the stage `ahead` of the next one has been filled
+                const uint32_t x = s + ahead;
+                return x < C::kStages ? wait(&S.full[x], round) : wait(&S.full[x - C::kStages], round ^ 1);
             };
-            bool ok = wait(&S.q_ready, 0);
-            for (int j = 0; j < n && ok; ++j) {
-                if (!(ok = wait(&S.full[s], round))) break;
-                tc_fence_after();
+            auto qk = [&](int j) {
                 const uint32_t at = ring_at + s * C::kStageB, d = tm + C::kS + (j & 1) * kTile;
 #pragma unroll
                 for (uint32_t i = 0; i < D / 16; ++i)
@@ -548,9 +537,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 commit2(&S.empty[s], one);
                 commit2(&S.s_full[j & 1], one);
                 next();
-                if (j > 0) ok = pv(j - 1);   // S of tile j runs while tile j - 1 is in the softmax
+            };
+            // P V of tile j, the two quarters of P that the softmax hands over first, then the others
+            auto pv = [&](int j) {
+                const uint32_t at = ring_at + s * C::kStageB, p = tm + C::kS + (j & 1) * kTile;
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x) {
+                    if (!wait(&S.p_ready[j & 1][x], (j >> 1) & 1)) return false;
+                    tc_fence_after();
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) {
+                        const uint32_t i = 2 * x + (y & 1) + 4 * (y >> 1);
+                        mma2_ts(tm + C::kO, p + 8 * i,
+                                desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1u << v_shift) - 1)) * 2048, v_rows * 128),
+                                id_o, (j > 0 || x + y > 0) ? 1u : 0u, one);
+                    }
+                }
+                commit2(&S.empty[s], one);
+                commit2(&S.o_done, one);
+                next();
+                return true;
+            };
+            // S 0, S 1, P V 0, S 2, P V 1, ..: S of tile j + 1 runs while tile j is in the softmax. What was
+            // copied is waited for ahead of P, so that P V j and S j + 2 follow it at once.
+            bool ok = wait(&S.q_ready, 0) && full(0);
+            tc_fence_after();
+            if (ok) qk(0);
+            if (ok && n > 1 && (ok = full(0))) {
+                tc_fence_after();
+                qk(1);
             }
-            if (ok) pv(n - 1);
+            for (int j = 0; j < n && ok; ++j) {
+                ok = full(0) && (j + 2 >= n || full(1)) && pv(j);
+                if (ok && j + 2 < n) qk(j + 2);
+            }
+            if (ok) commit2(&S.done, one);
         }
     } else {
         // ---- softmax: two threads a row, 64 columns each; warps w and w + 4 hold the same 32 rows
@@ -563,7 +584,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         float m = -INFINITY, l = 0.f;
         const uint32_t lanes = (uint32_t)(quad * 32) << 16;
         if (n_tiles > 0) {
-            const uint32_t p_bar = cluster_addr(&S.p_ready[0], 0);
+            const uint32_t p_bar = cluster_addr(&S.p_ready[0][0], 0);
             // the first position that some row of this warp does not see
             const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
             for (int j = 0; j < n_tiles; ++j) {
@@ -605,27 +626,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 const float c = grow ? ex2f(m - base) : 1.0f;
                 l *= c;
                 m = mn;
-                const uint64_t neg = pack_f32x2(-base, -base);
-                uint64_t sum[2] = {0, 0};
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    uint32_t p[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float e0, e1;
-                        unpack_f32x2(add_f32x2(pack_f32x2(s[32 * x + 2 * i], s[32 * x + 2 * i + 1]), neg), e0, e1);
-                        e0 = ex2f(e0), e1 = ex2f(e1);
-                        sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
-                        p[i] = pack2_bf16(e0, e1);
-                    }
-                    tc_st16(st + 32 * wg + 16 * x, p);
-                }
-                float s0, s1;
-                unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
-                l += s0 + s1;
-                // P V of tile j - 1 is complete: the tensor cores are at S of tile j + 1 by now
-                if (j > 0) wait_bar(&S.o_done, (j - 1) & 1, &S.stop);
                 if (scale_o) {
+                    // P V of tile j - 1 is the last that added to O; that of tile j - 2 is complete, since S of
+                    // tile j, issued after it, is
+                    wait_bar(&S.o_done, (j - 1) & 1, &S.stop);
                     tc_fence_after();
 #pragma unroll 1
                     for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
@@ -638,12 +642,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                         tc_st16(tmem + lanes + C::kO + x + 16, o + 16);
                     }
                 }
-                tc_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) signal_cluster(p_bar + (j & 1) * 8);
+                const uint64_t neg = pack_f32x2(-base, -base);
+                uint64_t sum[2] = {0, 0};
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {   // 32 columns at a time into the MMAs' hands
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float e0, e1;
+                        unpack_f32x2(add_f32x2(pack_f32x2(s[32 * x + 2 * i], s[32 * x + 2 * i + 1]), neg), e0, e1);
+                        e0 = ex2f(e0), e1 = ex2f(e1);
+                        sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
+                        p[i] = pack2_bf16(e0, e1);
+                    }
+                    tc_st16(st + 32 * wg + 16 * x, p);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) signal_cluster(p_bar + (j & 1) * 16 + x * 8);
+                }
+                float s0, s1;
+                unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
+                l += s0 + s1;
             }
-            wait_bar(&S.o_done, (n_tiles - 1) & 1, &S.stop);
+            wait_bar(&S.done, 0, &S.stop);
             tc_fence_after();
             float(*sums)[kRows] = S.row_max[n_tiles & 1];   // the parity that the last tile left alone
             sums[wg][r_cta] = l;
