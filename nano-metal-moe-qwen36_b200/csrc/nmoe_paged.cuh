@@ -67,9 +67,11 @@ __device__ __forceinline__ int find_sequence(const int *cu, int n, int r, int la
     return lo < n && cu[0] <= r ? lo : -1;
 }
 
-template <int E>
-__device__ __forceinline__ void load_elems(const void *base, long long at, bool bf16, float *v) {
-    if (bf16) {
+// E elements of x_dtype as floats. The type is a template argument wherever several loads are on their
+// way together: a branch per load makes each wait for the one before it.
+template <int E, bool kBf16>
+__device__ __forceinline__ void load_typed(const void *base, long long at, float *v) {
+    if constexpr (kBf16) {
         const uint16_t *p = static_cast<const uint16_t *>(base) + at;
         uint32_t w[E / 2];
         if constexpr (E == 8) {
@@ -89,6 +91,13 @@ __device__ __forceinline__ void load_elems(const void *base, long long at, bool 
             v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
         }
     }
+}
+template <int E>
+__device__ __forceinline__ void load_elems(const void *base, long long at, bool bf16, float *v) {
+    if (bf16)
+        load_typed<E, true>(base, at, v);
+    else
+        load_typed<E, false>(base, at, v);
 }
 
 __device__ __forceinline__ uint32_t pack2_bf16(float lo, float hi) {

@@ -121,7 +121,7 @@ constexpr int kAppendThreads = 256, kAppendRows = 8;
 
 // A CTA takes rows_per_cta rows (1 when there are few, so that they spread over the SMs): one
 // (cos, sin) table per row for all its heads, then a warp per (row, head, k or v).
-template <int D>
+template <int D, bool kBf16>
 __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_constant__ AppendArgs a) {
     constexpr int E = D / 32;
     __shared__ float2 cs[kAppendRows][128];
@@ -151,20 +151,21 @@ __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_co
     }
     __syncthreads();
     const int units = rows * a.kv_heads * 2;
-    for (int u = warp; u < units; u += kAppendThreads / 32) {
-        const int r = u / (2 * a.kv_heads), hv = u - r * 2 * a.kv_heads, head = hv >> 1;
-        const long long w = where[r];
-        if (w < 0) continue;
-        const long long src = (long long)(row0 + r) * a.kv_stride + head * D + E * lane;
-        const long long dst = w + head * a.c.head_stride + E * lane;
-        float v[E];
-        if (hv & 1) {
-            load_elems<E>(a.v_new, src, a.x_bf16, v);
-            store_bf16<E>(a.c.v + dst, v);
-        } else {
-            load_elems<E>(a.k_new, src, a.x_bf16, v);
-            prepare_head<E>(v, a.h.k_norm, a.h.eps, cs[r], a.rot.half, lane);
-            store_bf16<E>(a.c.k + dst, v);
+    constexpr int kAtOnce = 4, kWarps = kAppendThreads / 32;   // loads of a warp on their way together
+    for (int u0 = warp; u0 < units; u0 += kWarps * kAtOnce) {
+        float v[kAtOnce][E];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int u = min(u0 + x * kWarps, units - 1), r = u / (2 * a.kv_heads), hv = u - r * 2 * a.kv_heads;
+            load_typed<E, kBf16>(hv & 1 ? a.v_new : a.k_new,
+                                 (long long)(row0 + r) * a.kv_stride + (hv >> 1) * D + E * lane, v[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int u = u0 + x * kWarps, r = u / (2 * a.kv_heads), hv = u - r * 2 * a.kv_heads;
+            if (u >= units || where[r] < 0) continue;
+            if (!(hv & 1)) prepare_head<E>(v[x], a.h.k_norm, a.h.eps, cs[r], a.rot.half, lane);
+            store_bf16<E>((hv & 1 ? a.c.v : a.c.k) + where[r] + (hv >> 1) * a.c.head_stride + E * lane, v[x]);
         }
     }
 }
@@ -697,9 +698,9 @@ extern "C" int nmoe_full_attn_append_paged(const nmoe_full_attn_weights *w, cons
     const int grid = (total_rows + a.rows_per_cta - 1) / a.rows_per_cta;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (shape->head_dim == 256)
-        k_append_paged<256><<<grid, kAppendThreads, 0, st>>>(a);
+        (a.x_bf16 ? k_append_paged<256, true> : k_append_paged<256, false>)<<<grid, kAppendThreads, 0, st>>>(a);
     else
-        k_append_paged<128><<<grid, kAppendThreads, 0, st>>>(a);
+        (a.x_bf16 ? k_append_paged<128, true> : k_append_paged<128, false>)<<<grid, kAppendThreads, 0, st>>>(a);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? NMOE_OK : full_attn_fail(NMOE_ECUDA, "append: %s", cudaGetErrorString(e));
 }

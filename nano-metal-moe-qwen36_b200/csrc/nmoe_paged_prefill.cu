@@ -29,6 +29,8 @@
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "nmoe_gemm.cuh"
 #include "nmoe_paged.cuh"
 
@@ -213,7 +215,7 @@ __device__ __forceinline__ float ex2f(float x) {
 // per (row, head).
 constexpr int kPrepThreads = 256, kPrepRows = 8;
 
-template <int D>
+template <int D, bool kBf16>
 __global__ void __launch_bounds__(kPrepThreads) k_prefill_queries(const __grid_constant__ PrefillArgs a) {
     constexpr int E = D / 32;
     __shared__ float2 cs[kPrepRows][128];
@@ -233,16 +235,25 @@ __global__ void __launch_bounds__(kPrepThreads) k_prefill_queries(const __grid_c
     if (half > 0)
         for (int r = tid / half; r < rows; r += kPrepThreads / half) cs[r][tid & (half - 1)] = rotary_cs(freq, at[r]);
     __syncthreads();
-    const int heads = a.kv_heads * a.group;
-    for (int u = warp; u < rows * heads; u += kPrepThreads / 32) {
-        const int r = u / heads, h = u - r * heads, kvh = h / a.group;
-        if (!live[r]) continue;
-        float v[E];
-        load_elems<E>(a.q, (long long)(row0 + r) * a.q_stride + (long long)h * (a.gated ? 2 * D : D) + E * lane, a.x_bf16, v);
-        prepare_head<E>(v, a.h.q_norm, a.h.eps, cs[r], half, lane);
+    const int heads = a.kv_heads * a.group, units = rows * heads;
+    constexpr int kAtOnce = 4, kWarps = kPrepThreads / 32;   // loads of a warp on their way together
+    for (int u0 = warp; u0 < units; u0 += kWarps * kAtOnce) {
+        float v[kAtOnce][E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] *= a.scale;
-        store_bf16<E>(a.q_ready + (((long long)kvh * a.total_rows + row0 + r) * a.group + (h - kvh * a.group)) * D + E * lane, v);
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int u = min(u0 + x * kWarps, units - 1), r = u / heads, h = u - r * heads;
+            load_typed<E, kBf16>(a.q, (long long)(row0 + r) * a.q_stride + (long long)h * (a.gated ? 2 * D : D) + E * lane, v[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int u = u0 + x * kWarps, r = u / heads, h = u - r * heads, kvh = h / a.group;
+            if (u >= units || !live[r]) continue;
+            prepare_head<E>(v[x], a.h.q_norm, a.h.eps, cs[r], half, lane);
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[x][i] *= a.scale;
+            store_bf16<E>(a.q_ready + (((long long)kvh * a.total_rows + row0 + r) * a.group + (h - kvh * a.group)) * D + E * lane,
+                          v[x]);
+        }
     }
 }
 
@@ -695,36 +706,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         const int heads = a.kv_heads * a.group, first = wg * 16;   // this warp's 16 of the pair's 32 rows
         const int mine = min(first + 16, my_rows * a.group - quad * 32);
         constexpr int kAtOnce = 8;   // rows whose gates are on their way together
-        for (int i0 = first; i0 < mine; i0 += kAtOnce) {
-            float g[kAtOnce][E];
-            long long to[kAtOnce];
+        auto store_rows = [&](auto bf16) {
+            for (int i0 = first; i0 < mine; i0 += kAtOnce) {
+                float g[kAtOnce][E];
+                long long at[kAtOnce];
 #pragma unroll
-            for (int y = 0; y < kAtOnce; ++y) {
-                const int rr = quad * 32 + min(i0 + y, mine - 1), tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
-                const long long r = (long long)lo + my_tok0 + tok;
-                to[y] = (r * heads + h) * D + E * lane;
-                if (a.gated) load_elems<E>(a.q, r * a.q_stride + (long long)h * 2 * D + D + E * lane, a.x_bf16, g[y]);
-            }
-#pragma unroll
-            for (int y = 0; y < kAtOnce; ++y) {
-                if (i0 + y >= mine) break;
-                float v[E];
-#pragma unroll
-                for (int x = 0; x < E; ++x) v[x] = 0.f;
-                if (n_tiles > 0) {
-                    const float4 *src = reinterpret_cast<const float4 *>(rows_out + (i0 + y) * C::kOutB + E * lane * 4);
-#pragma unroll
-                    for (int x = 0; x < E / 4; ++x) {
-                        const float4 f = src[x];
-                        v[4 * x] = f.x, v[4 * x + 1] = f.y, v[4 * x + 2] = f.z, v[4 * x + 3] = f.w;
-                    }
+                for (int y = 0; y < kAtOnce; ++y) {
+                    const int rr = quad * 32 + min(i0 + y, mine - 1), tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
+                    const long long r = (long long)lo + my_tok0 + tok;
+                    at[y] = (r * heads + h) * D + E * lane;
+                    if (a.gated) load_typed<E, decltype(bf16)::value>(a.q, r * a.q_stride + (long long)h * 2 * D + D + E * lane, g[y]);
                 }
-                if (a.gated)
 #pragma unroll
-                    for (int x = 0; x < E; ++x) v[x] = __fdividef(v[x], 1.0f + __expf(-g[y][x]));
-                store_bf16<E>(a.out + to[y], v);
+                for (int y = 0; y < kAtOnce; ++y) {
+                    if (i0 + y >= mine) break;
+                    float v[E];
+#pragma unroll
+                    for (int x = 0; x < E; ++x) v[x] = 0.f;
+                    if (n_tiles > 0) {
+                        const float4 *src = reinterpret_cast<const float4 *>(rows_out + (i0 + y) * C::kOutB + E * lane * 4);
+#pragma unroll
+                        for (int x = 0; x < E / 4; ++x) {
+                            const float4 f = src[x];
+                            v[4 * x] = f.x, v[4 * x + 1] = f.y, v[4 * x + 2] = f.z, v[4 * x + 3] = f.w;
+                        }
+                    }
+                    if (a.gated)
+#pragma unroll
+                        for (int x = 0; x < E; ++x) v[x] = __fdividef(v[x], 1.0f + __expf(-g[y][x]));
+                    store_bf16<E>(a.out + at[y], v);
+                }
             }
-        }
+        };
+        if (a.x_bf16)
+            store_rows(std::true_type{});
+        else
+            store_rows(std::false_type{});
         tc_fence_before();
     }
     __syncthreads();
@@ -782,7 +799,8 @@ template <int D>
 cudaError_t launch(const PrefillArgs &a, long long units, cudaStream_t st) {
     cudaError_t e = cudaFuncSetAttribute(k_prefill_pairs<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
     if (e != cudaSuccess) return e;
-    k_prefill_queries<D><<<(a.total_rows + a.prep_rows - 1) / a.prep_rows, kPrepThreads, 0, st>>>(a);
+    (a.x_bf16 ? k_prefill_queries<D, true> : k_prefill_queries<D, false>)
+        <<<(a.total_rows + a.prep_rows - 1) / a.prep_rows, kPrepThreads, 0, st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     // the tiles' kernel sets up and reads K while the queries are prepared
     cudaLaunchConfig_t cfg = {};
