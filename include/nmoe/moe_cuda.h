@@ -451,7 +451,8 @@ size_t nmoe_full_attn_step_paged_workspace_bytes(const nmoe_full_attn_shape *sha
  * nmoe_linear_attn_step goes on from. Head dim 128, conv width 4; conv channels (2 key_heads +
  * value_heads) * 128: q, then k, then v; value head h reads key head h / (value_heads /
  * key_heads). All weights as in nmoe_linear_attn_weights for that many heads.
- * DEVICE pointers, 16-byte aligned: qkv [total_rows][channels], z [total_rows][value_heads *
+ * DEVICE pointers, 16-byte aligned (conv_w and norm_w 8, alpha and beta as their elements): qkv
+ * [total_rows][channels], z [total_rows][value_heads *
  * 128], alpha / beta [total_rows][value_heads], all in x_dtype, row r at r * its stride in
  * elements (0: packed; qkv and z rows 16-byte aligned). conv_in / conv_out f32
  * [num_seqs][3][channels], delta_in / delta_out f32 [num_seqs][value_heads][128][128] (in and

@@ -1,11 +1,33 @@
-// nmoe_gdn_prefill.cu -- the GatedDeltaNet core of packed prompts.
-#include <cuda_bf16.h>
+// nmoe_gdn_prefill.cu -- the GatedDeltaNet core of packed prompts, 64 tokens of a sequence at a time.
+//
+// Per value head, with k, q of unit length times a constant, g_t the decay and b_t the step:
+//     S_t = g_t S_{t-1} + b_t (v_t - g_t S_{t-1} k_t) k_t^T,   o_t = S_t q_t
+// Inside a chunk (G_t: the sum of log g up to t, S the state before it) the rank-one updates are
+//     u_t = b_t (v_t - e^{G_t} S k_t - sum_{s<t} e^{G_t-G_s} (k_t . k_s) u_s)
+// a unit lower triangular system: U = T b (V - e^G K S^T), T = (I + M)^{-1},
+// M_ts = b_t e^{G_t-G_s} k_t . k_s (s < t). Then, with P_ts = e^{G_t-G_s} q_t . k_s (s <= t),
+//     O = e^G Q S^T + P U,   S' = e^{G_63} S + sum_t (e^{G_63-G_t} u_t) k_t^T
+//
+// Three launches. k_gdn_chunks, a CTA per (chunk, key head): convolution and norms of q and k, K K^T and
+// Q K^T, T b and P of its value heads; nothing here depends on the state. k_gdn_scan, a CTA per
+// (sequence, value head, 32 of the 128 value columns): the recurrence over the chunks; the columns of
+// the state never mix, so four CTAs a head share nothing. k_gdn_finish: gated norm and conv states.
+//
+// Arithmetic: products run on the warp tensor instructions (m16n8k16, fp16 operands, fp32 sums) with
+// every operand split into two fp16 parts, x = hi + lo (22 bits), and the three products hi hi, hi lo,
+// lo hi, so that states are as exact as with fp32 operands (1e-7 of their norm). fp16 has the range of
+// 2^40 only: k, q and P are scaled by constants, the state and U by a power of two that follows a bound
+// on them (|u| <= max |v| + |S|, |S'|^2 <= |S|^2 + sum v^2, row by row, since |k| <= 1 and b <= 1). The
+// products that reach nothing but a bf16 output (Q S^T, P U) take the hi parts alone: 2^-12 against
+// its 2^-9. What bounds it: on one sequence the scan's chain of three dependent products a chunk; on
+// many, the warp tensor rate (1024 products a cycle and SM).
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
 
 #include "nmoe/moe_cuda.h"
-#include "nmoe_common.cuh"
+#include "nmoe_sm100.cuh"
 
 namespace nmoe {
 namespace {
@@ -20,7 +42,16 @@ int fail(int status, const char *fmt, ...) {
     return status;
 }
 
-constexpr int kD = 128;
+constexpr int kD = 128, kC = 64;      // head dim, tokens of a chunk
+constexpr int kSplit = 4, kN = kD / kSplit;   // value columns of a scan CTA: 32
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about 1 / 11 and 1 / 128
+
+// Tile images, the same in the workspace and in shared memory: rows of fp16 in 16-byte pieces, piece
+// p of row r at p ^ (r & 7), so that an ldmatrix of 8 rows meets 8 bank groups.
+constexpr int kTileX = kC * kD * 2;   // K or Q, one part: 16 KB
+constexpr int kTileT = kC * kC * 2;   // T b or P, one part: 8 KB
+constexpr int kGates = 2 * kC * 4;    // e^{G_t}, e^{G_63 - G_t}
 
 struct GdnArgs {
     const int *cu_rows;
@@ -32,6 +63,9 @@ struct GdnArgs {
     float *conv_out, *delta_out;
     void *out;
     int num_seqs, total_rows, key_heads, value_heads, channels, x_bf16, out_bf16;
+    // workspace, per chunk and head: K hi | K lo | Q hi | Q lo; T hi | T lo | P hi | P lo; gates; and O
+    uint8_t *kq, *tp, *gates;
+    float *o;
 };
 
 __device__ __forceinline__ float load_x(const void *p, long long at, int bf16) {
@@ -40,92 +74,731 @@ __device__ __forceinline__ float load_x(const void *p, long long at, int bf16) {
 // log(1 + exp(x)) without overflow
 __device__ __forceinline__ float softplus(float x) { return fmaxf(x, 0.f) + log1pf(expf(-fabsf(x))); }
 
-__device__ __forceinline__ float block_sum(float v, float *red, int warp, int lane) {
-    v = warp_sum(v);
-    __syncthreads();
-    if (lane == 0) red[warp] = v;
-    __syncthreads();
-    return (red[0] + red[1]) + (red[2] + red[3]);
+__device__ __forceinline__ int seq_first(const GdnArgs &a, int b) { return max(0, min(a.cu_rows[b], a.total_rows)); }
+__device__ __forceinline__ int seq_rows(const GdnArgs &a, int b) {
+    return max(0, min(a.cu_rows[b + 1], a.total_rows) - seq_first(a, b));
 }
+__device__ __forceinline__ int seq_chunks(const GdnArgs &a, int b) { return (seq_rows(a, b) + kC - 1) / kC; }
 
-// A CTA per (value head, sequence), token by token; thread t holds row t of the state and
-// convolves channel t of the head's q, k and v.
-__global__ void __launch_bounds__(kD) k_gdn_rows(const __grid_constant__ GdnArgs a) {
-    __shared__ __align__(16) float qs[kD], ks[kD];
-    __shared__ float red[4];
-    const int t = threadIdx.x, warp = t >> 5, lane = t & 31;
-    const int vh = blockIdx.x, b = blockIdx.y, kh = vh / (a.value_heads / a.key_heads);
-    const int r0 = max(0, min(a.cu_rows[b], a.total_rows)), r1 = min(a.cu_rows[b + 1], a.total_rows);
-    float S[kD];
-    const long long so = (((long long)b * a.value_heads + vh) * kD + t) * kD;
+// x = hi + lo in fp16, two values at a time
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = *reinterpret_cast<const uint32_t *>(&l);
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t *r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t *r) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void stsm4t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
+                 "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// byte offset of 16-byte piece p of row r: rows of 256, 128 and 64 bytes
+__device__ __forceinline__ uint32_t at256(int r, int p) { return r * 256 + ((p ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t at128(int r, int p) { return r * 128 + ((p ^ (r & 7)) << 4); }
+__device__ __forceinline__ uint32_t at64(int r, int p) { return r * 64 + ((p ^ ((r >> 1) & 3)) << 4); }
+
+// ---- chunks ---------------------------------------------------------------------------------------
+
+constexpr int kLd = 66;    // K K^T, Q K^T rows
+constexpr int kLdT = 68;   // T rows
+struct ChunkSmem {
+    static constexpr int kK = 0, kQ = 2 * kTileX;                       // hi, lo
+    static constexpr int kT = kQ;                                       // two heads' T over Q, once it is read
+    static constexpr int kQT = 2 * kC * kLdT * 4 > 2 * kTileX ? 2 * kC * kLdT * 4 : 2 * kTileX;
+    static constexpr int kKK = kQ + kQT, kQK = kKK + kC * kLd * 4;
+    static constexpr int kScratch = kQK + kC * kLd * 4;                 // 16 x 16 a warp
+    static constexpr int kBytes = kScratch + kWarps * 256 * 4;
+};
+
+template <bool kBf16, bool kFull>
+__global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constant__ GdnArgs a) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ double G[2][kC];   // sums down to -1000 and beyond, whose differences matter
+    __shared__ float beta[2][kC];
+    __shared__ int scan[kWarps], found[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int chunk = blockIdx.x, kh = blockIdx.y;
+
+    // ---- the chunk's sequence
+    if (tid == 0) found[0] = -1;
+    {
+        const int per = (a.num_seqs + kThreads - 1) / kThreads;
+        const int first = min(a.num_seqs, tid * per), last = min(a.num_seqs, first + per);
+        int own = 0;
+        for (int b = first; b < last; ++b) own += seq_chunks(a, b);
+        int inc = own;
 #pragma unroll
-    for (int i = 0; i < kD; ++i) S[i] = a.delta_in ? a.delta_in[so + i] : 0.f;
-    const int ch[3] = {kh * kD + t, (a.key_heads + kh) * kD + t, (2 * a.key_heads + vh) * kD + t};
-    float w[3][4], x[3][3];
-#pragma unroll
-    for (int c = 0; c < 3; ++c) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[c][j] = bf16_to_f32(a.conv_w[4 * ch[c] + j]);
-#pragma unroll
-        for (int j = 0; j < 3; ++j) x[c][j] = a.conv_in ? a.conv_in[((long long)b * 3 + j) * a.channels + ch[c]] : 0.f;
-    }
-    const float rate = -expf(a.A_log[vh]), dt = bf16_to_f32(a.dt_bias[vh]), nw = bf16_to_f32(a.norm_w[t]);
-    for (long long r = r0; r < r1; ++r) {
-        float y[3];
-#pragma unroll
-        for (int c = 0; c < 3; ++c) {
-            const float n = load_x(a.qkv, r * a.qkv_stride + ch[c], a.x_bf16);
-            const float s = x[c][0] * w[c][0] + x[c][1] * w[c][1] + x[c][2] * w[c][2] + n * w[c][3];
-            y[c] = siluf_(s);
-            x[c][0] = x[c][1], x[c][1] = x[c][2], x[c][2] = n;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
         }
-        const float qq = block_sum(y[0] * y[0], red, warp, lane), kk = block_sum(y[1] * y[1], red, warp, lane);
-        qs[t] = y[0] * rsqrtf(qq / kD + 1e-12f) * (1.0f / kD);
-        ks[t] = y[1] * rsqrtf(kk / kD + 1e-12f) * rsqrtf((float)kD);
+        if (lane == 31) scan[warp] = inc;
         __syncthreads();
-        const float g = expf(rate * softplus(load_x(a.alpha, r * a.ab_stride + vh, a.x_bf16) + dt));
-        const float beta = sigmoidf_(load_x(a.beta, r * a.ab_stride + vh, a.x_bf16));
-        float kv = 0.f;
-#pragma unroll
-        for (int i = 0; i < kD; ++i) {
-            S[i] *= g;
-            kv = fmaf(S[i], ks[i], kv);
-        }
-        const float d = (y[2] - kv) * beta;
-        float o = 0.f;
-#pragma unroll
-        for (int i = 0; i < kD; ++i) {
-            S[i] = fmaf(ks[i], d, S[i]);
-            o = fmaf(S[i], qs[i], o);
-        }
-        const float oo = block_sum(o * o, red, warp, lane);
-        const float zz = load_x(a.z, r * a.z_stride + vh * kD + t, a.x_bf16);
-        const float v = o * rsqrtf(oo / kD + 1e-6f) * nw * siluf_(zz);
-        const long long at = (r * a.value_heads + vh) * kD + t;
-        if (a.out_bf16)
-            static_cast<uint16_t *>(a.out)[at] = __bfloat16_as_ushort(__float2bfloat16(v));
-        else
-            static_cast<float *>(a.out)[at] = v;
+        int before = inc - own;
+        for (int w = 0; w < warp; ++w) before += scan[w];
+        if (chunk >= before && chunk < before + own)
+            for (int b = first; b < last; ++b) {
+                const int n = seq_chunks(a, b);
+                if (chunk < before + n) {
+                    found[0] = b;
+                    found[1] = chunk - before;
+                    break;
+                }
+                before += n;
+            }
+        __syncthreads();
     }
+    const int b = found[0];
+    if (b < 0) return;   // fewer chunks than the grid has room for
+    const int row0 = seq_first(a, b), in_seq = found[1] * kC, n = min(kC, seq_rows(a, b) - in_seq);
+    const uint32_t sm = smem_u32(smem);
+
+    // ---- convolution, SiLU and norm of q and k: a warp takes 8 tokens, a lane 4 channels of each
+    {
+        const int t0 = 8 * warp, cq = kh * kD + 4 * lane, ck = (a.key_heads + kh) * kD + 4 * lane;
+        float x[11][8];
 #pragma unroll
-    for (int i = 0; i < kD; ++i) a.delta_out[so + i] = S[i];
+        for (int i = 0; i < 11; ++i) {
+            const int t = t0 + i - 3, r = in_seq + t;   // token of the chunk, row of the sequence
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
+            if (r >= 0 && t < n) {
+                const long long at = (long long)(row0 + r) * a.qkv_stride;
+                if constexpr (kBf16) {
+                    const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.qkv) + at + cq);
+                    const uint2 k = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.qkv) + at + ck);
+                    x[i][0] = bf16_lo(q.x), x[i][1] = bf16_hi(q.x), x[i][2] = bf16_lo(q.y), x[i][3] = bf16_hi(q.y);
+                    x[i][4] = bf16_lo(k.x), x[i][5] = bf16_hi(k.x), x[i][6] = bf16_lo(k.y), x[i][7] = bf16_hi(k.y);
+                } else {
+                    const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.qkv) + at + cq);
+                    const float4 k = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.qkv) + at + ck);
+                    x[i][0] = q.x, x[i][1] = q.y, x[i][2] = q.z, x[i][3] = q.w;
+                    x[i][4] = k.x, x[i][5] = k.y, x[i][6] = k.z, x[i][7] = k.w;
+                }
+            } else if (r < 0 && a.conv_in != nullptr) {
+                const float *c = a.conv_in + ((long long)b * 3 + 3 + r) * a.channels;
+                const float4 q = *reinterpret_cast<const float4 *>(c + cq), k = *reinterpret_cast<const float4 *>(c + ck);
+                x[i][0] = q.x, x[i][1] = q.y, x[i][2] = q.z, x[i][3] = q.w;
+                x[i][4] = k.x, x[i][5] = k.y, x[i][6] = k.z, x[i][7] = k.w;
+            }
+        }
+        uint2 w[8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            w[j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (cq + j));
+            w[4 + j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ck + j));
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = t0 + i;
+            float y[8];
+            float qq = 0.f, kk = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float s = x[i][j] * bf16_lo(w[j].x) + x[i + 1][j] * bf16_hi(w[j].x) + x[i + 2][j] * bf16_lo(w[j].y) +
+                                x[i + 3][j] * bf16_hi(w[j].y);
+                y[j] = t < n ? siluf_(s) : 0.f;
+                if (j < 4)
+                    qq = fmaf(y[j], y[j], qq);
+                else
+                    kk = fmaf(y[j], y[j], kk);
+            }
+            const float iq = rsqrtf(warp_sum(qq) / kD + 1e-12f) * (kScaleQ / kD);
+            const float ik = rsqrtf(warp_sum(kk) / kD + 1e-12f) * (kScaleK * 0.08838834764831845f);
+            uint32_t h0, l0, h1, l1;
+            const uint32_t at = at256(t, lane >> 1) + (lane & 1) * 8;
+            split2(y[0] * iq, y[1] * iq, h0, l0);
+            split2(y[2] * iq, y[3] * iq, h1, l1);
+            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kQ + at) = make_uint2(h0, h1);
+            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kQ + kTileX + at) = make_uint2(l0, l1);
+            split2(y[4] * ik, y[5] * ik, h0, l0);
+            split2(y[6] * ik, y[7] * ik, h1, l1);
+            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kK + at) = make_uint2(h0, h1);
+            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kK + kTileX + at) = make_uint2(l0, l1);
+        }
+    }
+    __syncthreads();
+    {   // the tile images into the workspace
+        uint4 *dst = reinterpret_cast<uint4 *>(a.kq + ((long long)chunk * a.key_heads + kh) * 4 * kTileX);
+        constexpr int kParts = kFull ? 4 : 3;   // Q lo only where it is read
+        for (int i = tid; i < kParts * kTileX / 16; i += kThreads) dst[i] = reinterpret_cast<const uint4 *>(smem)[i];
+    }
+    // ---- K K^T and Q K^T, the 16 x 16 blocks on and below the diagonal: 20 of them over the warps
+    for (int u = warp; u < 20; u += kWarps) {
+        const int v = u % 10, i = v < 1 ? 0 : v < 3 ? 1 : v < 6 ? 2 : 3, j = v - i * (i + 1) / 2;
+        const uint32_t ka = sm + (u < 10 ? ChunkSmem::kK : ChunkSmem::kQ), kb = sm + ChunkSmem::kK;
+        float c[2][4] = {};
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+            uint32_t ah[4], al[4], bh[4], bl[4];
+            const uint32_t pa = at256(16 * i + (lane & 15), 2 * kk + (lane >> 4));
+            const uint32_t pb = at256(16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1));
+            ldsm4(ka + pa, ah);
+            ldsm4(ka + kTileX + pa, al);
+            ldsm4(kb + pb, bh);
+            ldsm4(kb + kTileX + pb, bl);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                mma_f16(c[x], al, bh[2 * x], bh[2 * x + 1]);
+                mma_f16(c[x], ah, bl[2 * x], bl[2 * x + 1]);
+                mma_f16(c[x], ah, bh[2 * x], bh[2 * x + 1]);
+            }
+        }
+        float *to = reinterpret_cast<float *>(smem + (u < 10 ? ChunkSmem::kKK : ChunkSmem::kQK));
+        const float s = u < 10 ? 1.f / (kScaleK * kScaleK) : 1.f / kScaleK;   // Q K^T keeps the scale of q: P does
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            float *p = to + (16 * i + (lane >> 2)) * kLd + 16 * j + 8 * x + 2 * (lane & 3);
+            *reinterpret_cast<float2 *>(p) = make_float2(c[x][0] * s, c[x][1] * s);
+            *reinterpret_cast<float2 *>(p + 8 * kLd) = make_float2(c[x][2] * s, c[x][3] * s);
+        }
+    }
+    const float *kkt = reinterpret_cast<const float *>(smem + ChunkSmem::kKK);
+    const float *qkt = reinterpret_cast<const float *>(smem + ChunkSmem::kQK);
+
+    // ---- the value heads of the key head, two at a time: four warps each
+    const int ratio = a.value_heads / a.key_heads;
+    const int half = warp >> 2, q4 = warp & 3, t128 = tid & 127;
+    for (int v0 = 0; v0 < ratio; v0 += 2) {
+        const bool on = v0 + half < ratio;
+        const int vh = kh * ratio + v0 + half;
+        float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT) + half * kC * kLdT;
+        float *scratch = reinterpret_cast<float *>(smem + ChunkSmem::kScratch) + warp * 256;
+        if (on && q4 == 0) {   // G: the running sum of log g
+            const float rate = -expf(a.A_log[vh]), dt = bf16_to_f32(a.dt_bias[vh]);
+            float g[2], bt[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int t = 2 * lane + j;
+                const long long at = (long long)(row0 + in_seq + t) * a.ab_stride + vh;
+                g[j] = t < n ? rate * softplus(load_x(a.alpha, at, kBf16) + dt) : 0.f;
+                bt[j] = t < n ? sigmoidf_(load_x(a.beta, at, kBf16)) : 0.f;
+            }
+            double inc = (double)g[0] + g[1];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            G[half][2 * lane] = inc - g[1];
+            G[half][2 * lane + 1] = inc;
+            beta[half][2 * lane] = bt[0];
+            beta[half][2 * lane + 1] = bt[1];
+        }
+        __syncthreads();   // also: K K^T, Q K^T are complete, and Q is read
+        if (on) {
+            float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
+            if (t128 < kC) {
+                gates[t128] = expf((float)G[half][t128]);
+                gates[kC + t128] = expf((float)(G[half][kC - 1] - G[half][t128]));
+            }
+            // M below the diagonal; P with its diagonal, straight into its tile
+            uint8_t *P = a.tp + (((long long)chunk * a.value_heads + vh) * 4 + 2) * kTileT;
+            for (int i = t128; i < kC * kC / 8; i += 128) {
+                const int t = i >> 3, s0 = (i & 7) * 8;
+                float p[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int s = s0 + j;
+                    const float e = s <= t ? expf((float)(G[half][t] - G[half][s])) : 0.f;
+                    p[j] = s <= t ? e * qkt[t * kLd + s] : 0.f;
+                    T[t * kLdT + s] = s < t ? beta[half][t] * e * kkt[t * kLd + s] : 0.f;
+                }
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split2(p[2 * j], p[2 * j + 1], h[j], l[j]);
+                *reinterpret_cast<uint4 *>(P + at128(t, i & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+                if (kFull) *reinterpret_cast<uint4 *>(P + kTileT + at128(t, i & 7)) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+        }
+        __syncthreads();
+        // (I + M)^-1 by 16 x 16 blocks: the diagonal ones by substitution, a lane per column, ..
+        if (on && lane < 16) {
+            const float *m = T + 16 * q4 * kLdT + 16 * q4;
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float s = i == lane ? 1.f : 0.f;
+#pragma unroll
+                for (int k = 0; k < i; ++k) s = fmaf(-m[i * kLdT + k], x[k], s);
+                x[i] = s;
+            }
+            __syncwarp(0xffffu);
+            float *to = T + 16 * q4 * kLdT + 16 * q4 + lane;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) to[i * kLdT] = x[i];
+        }
+        __syncthreads();
+        // .. then block row i: T_ij = -T_ii sum_{j<=k<i} M_ik T_kj, a warp per j; a lane holds 8 columns of a row
+        for (int i = 1; i < 4; ++i) {
+            const int j = q4, r = lane & 15, c = (lane >> 4) * 8;
+            float acc[8] = {};
+            if (on && j < i) {
+                for (int k = 16 * j; k < 16 * i; ++k) {
+                    const float m = T[(16 * i + r) * kLdT + k];
+                    const float4 u = *reinterpret_cast<const float4 *>(T + k * kLdT + 16 * j + c);
+                    const float4 w = *reinterpret_cast<const float4 *>(T + k * kLdT + 16 * j + c + 4);
+                    acc[0] = fmaf(m, u.x, acc[0]), acc[1] = fmaf(m, u.y, acc[1]), acc[2] = fmaf(m, u.z, acc[2]);
+                    acc[3] = fmaf(m, u.w, acc[3]), acc[4] = fmaf(m, w.x, acc[4]), acc[5] = fmaf(m, w.y, acc[5]);
+                    acc[6] = fmaf(m, w.z, acc[6]), acc[7] = fmaf(m, w.w, acc[7]);
+                }
+                *reinterpret_cast<float4 *>(scratch + r * 16 + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                *reinterpret_cast<float4 *>(scratch + r * 16 + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+                for (int k = 0; k < 16; ++k) {
+                    const float m = -T[(16 * i + r) * kLdT + 16 * i + k];
+                    const float4 u = *reinterpret_cast<const float4 *>(scratch + k * 16 + c);
+                    const float4 w = *reinterpret_cast<const float4 *>(scratch + k * 16 + c + 4);
+                    acc[0] = fmaf(m, u.x, acc[0]), acc[1] = fmaf(m, u.y, acc[1]), acc[2] = fmaf(m, u.z, acc[2]);
+                    acc[3] = fmaf(m, u.w, acc[3]), acc[4] = fmaf(m, w.x, acc[4]), acc[5] = fmaf(m, w.y, acc[5]);
+                    acc[6] = fmaf(m, w.z, acc[6]), acc[7] = fmaf(m, w.w, acc[7]);
+                }
+            }
+            __syncthreads();   // every M of the block row is read
+            if (on && j < i) {
+                float *to = T + (16 * i + r) * kLdT + 16 * j + c;
+                *reinterpret_cast<float4 *>(to) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+                *reinterpret_cast<float4 *>(to + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
+            }
+            __syncthreads();
+        }
+        if (on) {   // T b
+            uint8_t *to = a.tp + ((long long)chunk * a.value_heads + vh) * 4 * kTileT;
+            for (int i = t128; i < kC * kC / 8; i += 128) {
+                const int t = i >> 3, s0 = (i & 7) * 8;
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int s = s0 + 2 * j;
+                    split2(T[t * kLdT + s] * beta[half][s], T[t * kLdT + s + 1] * beta[half][s + 1], h[j], l[j]);
+                }
+                *reinterpret_cast<uint4 *>(to + at128(t, i & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(to + kTileT + at128(t, i & 7)) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+        }
+        __syncthreads();
+    }
 }
 
-// The last three inputs of every channel. After the rows: the states may be updated in place.
-__global__ void k_gdn_conv_state(const __grid_constant__ GdnArgs a) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x, b = blockIdx.y;
-    if (c >= a.channels) return;
-    const int r0 = max(0, min(a.cu_rows[b], a.total_rows)), r1 = min(a.cu_rows[b + 1], a.total_rows);
-    const int n = max(0, r1 - r0);
-    float v[3];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-        const int i = n + j - 3;   // row of the sequence, negative: of the state before it
-        v[j] = i >= 0 ? load_x(a.qkv, (long long)(r0 + i) * a.qkv_stride + c, a.x_bf16)
-                      : (a.conv_in ? a.conv_in[((long long)b * 3 + 3 + i) * a.channels + c] : 0.f);
+// ---- scan -------------------------------------------------------------------------------------------
+
+template <bool kFull>
+struct ScanSmem {
+    static constexpr int kQParts = kFull ? 2 : 1;
+    static constexpr int kStage = (2 + kQParts) * kTileX + 2 * kTileT + kGates;   // K hi, lo, Q, T hi, lo, gates
+    static constexpr int kT = (2 + kQParts) * kTileX, kGate = kT + 2 * kTileT;
+    static constexpr int kP = 2 * kStage, kS = kP + kQParts * kTileT;             // P of the current chunk; S hi, lo
+    static constexpr int kV = kS + 2 * kN * kD * 2, kR = kV + kC * kN * 4;        // V fp32; R hi, lo
+    static constexpr int kU = kR + 2 * kC * kN * 2, kW = kU + 2 * kC * kN * 2;    // U, e^{G_63 - G} U: hi, lo
+    static constexpr int kBytes = kW + 2 * kC * kN * 2;
+    static constexpr int kTileU = kC * kN * 2;
+};
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
+// e with bound * 2^-e in [2^12, 2^13), so that fp16 holds what the bound bounds and its parts reach 2^-37 of it
+__device__ __forceinline__ int exponent_of(float bound) {
+    const int e = (__float_as_int(bound) >> 23) - 127 - 12;
+    return min(100, max(-100, e));
+}
+
+template <bool kBf16, bool kFull>
+__global__ void __launch_bounds__(kThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
+    using L = ScanSmem<kFull>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t full[2], p_full;
+    __shared__ int vmax[2], first_chunk;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x, vh = blockIdx.y, b = blockIdx.z, kh = vh / (a.value_heads / a.key_heads);
+    const uint32_t sm = smem_u32(smem);
+    if (tid == 0) {
+        mbar_init(&full[0], 1);
+        mbar_init(&full[1], 1);
+        mbar_init(&p_full, 1);
+        mbar_fence_init();
+        vmax[0] = vmax[1] = 0;
+        first_chunk = 0;
     }
+    __syncthreads();
+    {
+        int before = 0;
+        for (int i = tid; i < b; i += kThreads) before += seq_chunks(a, i);
+        if (before) atomicAdd(&first_chunk, before);   // integers: the order does not matter
+    }
+    const int row0 = seq_first(a, b), rows = seq_rows(a, b), chunks = (rows + kC - 1) / kC;
+    __syncthreads();
+    const long long chunk0 = first_chunk;
+
+    // ---- the state: S^T, rows (dims) 16 warp + lane / 4 (+ 8), columns 8 j + 2 (lane % 4) (+ 1) of 32
+    float S[4][4];
+    float bound2 = 0.f;   // of |S|^2, per value row
+    const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN) * kD;
+    const int dim = 16 * warp + (lane >> 2), col = 2 * (lane & 3);
 #pragma unroll
-    for (int j = 0; j < 3; ++j) a.conv_out[((long long)b * 3 + j) * a.channels + c] = v[j];
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            S[j][e] = a.delta_in ? a.delta_in[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] : 0.f;
+            bound2 = fmaxf(bound2, fabsf(S[j][e]));
+        }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) bound2 = fmaxf(bound2, __shfl_xor_sync(0xffffffffu, bound2, o));
+    if (lane == 0) atomicMax(&vmax[1], __float_as_int(bound2));   // not negative: ordered as integers
+    __syncthreads();
+    bound2 = __int_as_float(vmax[1]);
+    bound2 = bound2 * bound2 * kD;
+    __syncthreads();
+    if (tid == 0) vmax[1] = 0;
+
+    // S, scaled, as the B operand of the next chunk: [column][dim]
+    auto store_state = [&](int e) {
+        const float s = pow2(-e);
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                split2(S[j + x][0] * s, S[j + x][1] * s, h[2 * x], l[2 * x]);
+                split2(S[j + x][2] * s, S[j + x][3] * s, h[2 * x + 1], l[2 * x + 1]);
+            }
+            const int c = 8 * (j + (lane >> 4)) + (lane & 7);
+            const uint32_t at = sm + L::kS + at256(c, 2 * warp + ((lane >> 3) & 1));
+            stsm4t(at, h[0], h[1], h[2], h[3]);
+            stsm4t(at + kN * kD * 2, l[0], l[1], l[2], l[3]);
+        }
+    };
+    // ---- copies: K, Q, T and the gates of chunk c into stage c % 2; P of chunk c
+    auto copy_stage = [&](int c) {
+        uint8_t *st = smem + (c & 1) * L::kStage;
+        const uint8_t *kq = a.kq + ((chunk0 + c) * a.key_heads + kh) * 4 * kTileX;
+        const uint8_t *tp = a.tp + ((chunk0 + c) * a.value_heads + vh) * 4 * kTileT;
+        const uint64_t keep = policy_evict_normal();
+        mbar_arrive_expect_tx(&full[c & 1], L::kStage);
+        bulk_g2s(st, kq, (2 + L::kQParts) * kTileX, &full[c & 1], keep);
+        bulk_g2s(st + L::kT, tp, 2 * kTileT, &full[c & 1], keep);
+        bulk_g2s(st + L::kGate, a.gates + ((chunk0 + c) * a.value_heads + vh) * kGates, kGates, &full[c & 1], keep);
+    };
+    auto copy_p = [&](int c) {
+        const uint8_t *tp = a.tp + (((chunk0 + c) * a.value_heads + vh) * 4 + 2) * kTileT;
+        mbar_arrive_expect_tx(&p_full, L::kQParts * kTileT);
+        bulk_g2s(smem + L::kP, tp, L::kQParts * kTileT, &p_full, policy_evict_normal());
+    };
+    // ---- V: channel `lane`, tokens 8 warp .. + 7 of a chunk; the inputs are loaded a chunk ahead
+    const int ch = (2 * a.key_heads + vh) * kD + split * kN + lane;
+    const uint2 cw = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * ch);
+    float raw[11];
+    auto load_raw = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 11; ++i) {
+            const int r = c * kC + 8 * warp + i - 3;
+            raw[i] = 0.f;
+            if (r >= 0 && r < rows)
+                raw[i] = load_x(a.qkv, (long long)(row0 + r) * a.qkv_stride + ch, kBf16);
+            else if (r < 0 && a.conv_in != nullptr)
+                raw[i] = a.conv_in[((long long)b * 3 + 3 + r) * a.channels + ch];
+        }
+    };
+    auto v_at = [&](int t, int c) { return reinterpret_cast<float *>(smem + L::kV) + t * kN + (((c >> 3) ^ (t & 3)) << 3) + (c & 7); };
+    auto store_values = [&](int c) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = 8 * warp + i;
+            const float s = raw[i] * bf16_lo(cw.x) + raw[i + 1] * bf16_hi(cw.x) + raw[i + 2] * bf16_lo(cw.y) +
+                            raw[i + 3] * bf16_hi(cw.y);
+            const float v = c * kC + t < rows ? siluf_(s) : 0.f;
+            *v_at(t, lane) = v;
+            m = fmaxf(m, fabsf(v));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) atomicMax(&vmax[c & 1], __float_as_int(m));
+    };
+
+    bool ok = true;
+    int es = exponent_of(sqrtf(bound2));
+    if (chunks > 0) {
+        if (tid == 0) copy_stage(0);
+        load_raw(0);
+        store_state(es);
+        __syncthreads();   // vmax[1] is clear
+        store_values(0);
+        __syncthreads();
+    }
+    for (int c = 0; c < chunks; ++c) {
+        if (tid == 0) {
+            copy_p(c);
+            if (c + 1 < chunks) copy_stage(c + 1);
+        }
+        if (c + 1 < chunks) load_raw(c + 1);
+        const float vm = __int_as_float(vmax[c & 1]);
+        bound2 += kC * vm * vm;   // of the states of this chunk, and of the one it leaves
+        const int eu = exponent_of(vm + sqrtf(bound2));
+        const uint32_t st = sm + (c & 1) * L::kStage;
+        const float *eg = reinterpret_cast<const float *>(smem + (c & 1) * L::kStage + L::kGate), *el = eg + kC;
+        ok &= mbar_wait_spin(&full[c & 1], (c >> 1) & 1);
+
+        // ---- 1: K S^T (warps 0-3) and Q S^T (warps 4-7), 16 tokens a warp, all 32 columns
+        const int mt = warp & 3;
+        const bool is_q = warp >= 4;
+        float acc[4][4] = {};
+        {
+            const uint32_t A = st + (is_q ? 2 * kTileX : 0), B = sm + L::kS;
+#pragma unroll
+            for (int kk = 0; kk < kD / 16; ++kk) {
+                uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+                const uint32_t pa = at256(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
+                ldsm4(A + pa, ah);
+#pragma unroll
+                for (int p = 0; p < 2; ++p)
+                    ldsm4(B + at256(16 * p + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), bh[p]);
+                if (kFull || !is_q) {
+                    ldsm4(A + kTileX + pa, al);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        ldsm4(B + kN * kD * 2 + at256(16 * p + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), bl[p]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+            }
+        }
+        const int t0 = 16 * mt + (lane >> 2);   // this lane's tokens t0, t0 + 8
+        const float g0 = eg[t0], g1 = eg[t0 + 8];
+        if (!is_q) {   // R = V - e^G K S^T, scaled
+            const float s = pow2(-eu), k0 = g0 * pow2(es) * (1.f / kScaleK), k1 = g1 * pow2(es) * (1.f / kScaleK);
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float2 v0 = *reinterpret_cast<const float2 *>(v_at(t0, 8 * (j + x) + col));
+                    const float2 v1 = *reinterpret_cast<const float2 *>(v_at(t0 + 8, 8 * (j + x) + col));
+                    split2((v0.x - k0 * acc[j + x][0]) * s, (v0.y - k0 * acc[j + x][1]) * s, h[2 * x], l[2 * x]);
+                    split2((v1.x - k1 * acc[j + x][2]) * s, (v1.y - k1 * acc[j + x][3]) * s, h[2 * x + 1], l[2 * x + 1]);
+                }
+                const uint32_t at = sm + L::kR + at64(16 * mt + (lane & 15), j + (lane >> 4));
+                stsm4(at, h[0], h[1], h[2], h[3]);
+                stsm4(at + L::kTileU, l[0], l[1], l[2], l[3]);
+            }
+        } else {       // e^G Q S^T on the scale of P U
+            const float k0 = g0 * pow2(es) * pow2(-eu), k1 = g1 * pow2(es) * pow2(-eu);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][0] *= k0, acc[j][1] *= k0, acc[j][2] *= k1, acc[j][3] *= k1;
+        }
+        __syncthreads();
+        // ---- 2: U = T b R: 16 tokens x 16 columns a warp, long rows beside short ones
+        {
+            const int i = is_q ? 3 - mt : mt, h2 = is_q ? 1 : 0;
+            float u[2][4] = {};
+            for (int kk = 0; kk <= i; ++kk) {
+                uint32_t ah[4], al[4], bh[4], bl[4];
+                const uint32_t pa = at128(16 * i + (lane & 15), 2 * kk + (lane >> 4));
+                const uint32_t pb = at64(16 * kk + (lane & 15), 2 * h2 + (lane >> 4));
+                ldsm4(st + L::kT + pa, ah);
+                ldsm4(st + L::kT + kTileT + pa, al);
+                ldsm4t(sm + L::kR + pb, bh);
+                ldsm4t(sm + L::kR + L::kTileU + pb, bl);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) mma_f16(u[x], al, bh[2 * x], bh[2 * x + 1]);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) mma_f16(u[x], ah, bl[2 * x], bl[2 * x + 1]);
+#pragma unroll
+                for (int x = 0; x < 2; ++x) mma_f16(u[x], ah, bh[2 * x], bh[2 * x + 1]);
+            }
+            const int t = 16 * i + (lane >> 2);
+            const float e0 = el[t], e1 = el[t + 8];
+            uint32_t h[4], l[4], wh[4], wl[4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                split2(u[x][0], u[x][1], h[2 * x], l[2 * x]);
+                split2(u[x][2], u[x][3], h[2 * x + 1], l[2 * x + 1]);
+                split2(u[x][0] * e0, u[x][1] * e0, wh[2 * x], wl[2 * x]);
+                split2(u[x][2] * e1, u[x][3] * e1, wh[2 * x + 1], wl[2 * x + 1]);
+            }
+            const uint32_t at = at64(16 * i + (lane & 15), 2 * h2 + (lane >> 4));
+            stsm4(sm + L::kU + at, h[0], h[1], h[2], h[3]);
+            if (kFull) stsm4(sm + L::kU + L::kTileU + at, l[0], l[1], l[2], l[3]);
+            stsm4(sm + L::kW + at, wh[0], wh[1], wh[2], wh[3]);
+            stsm4(sm + L::kW + L::kTileU + at, wl[0], wl[1], wl[2], wl[3]);
+        }
+        __syncthreads();
+        // ---- 3: S' = e^{G_63} S + K^T (e^{G_63 - G} U), 16 dims a warp; P U on top of e^G Q S^T (warps 4-7)
+        {
+            float up[4][4] = {};
+#pragma unroll
+            for (int kk = 0; kk < kC / 16; ++kk) {
+                uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+                const uint32_t pa = at256(16 * kk + (lane & 7) + ((lane >> 4) << 3), 2 * warp + ((lane >> 3) & 1));
+                ldsm4t(st + pa, ah);
+                ldsm4t(st + kTileX + pa, al);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const uint32_t pb = at64(16 * kk + (lane & 15), 2 * p + (lane >> 4));
+                    ldsm4t(sm + L::kW + pb, bh[p]);
+                    ldsm4t(sm + L::kW + L::kTileU + pb, bl[p]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_f16(up[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+            }
+            const float keep = eg[kC - 1], add = pow2(eu) * (1.f / kScaleK);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) S[j][e] = fmaf(S[j][e], keep, up[j][e] * add);
+        }
+        es = exponent_of(sqrtf(bound2));
+        if (is_q) {
+            ok &= mbar_wait_spin(&p_full, c & 1);
+            for (int kk = 0; kk <= mt; ++kk) {
+                uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+                const uint32_t pa = at128(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
+                ldsm4(sm + L::kP + pa, ah);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) ldsm4t(sm + L::kU + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bh[p]);
+                if (kFull) {
+                    ldsm4(sm + L::kP + kTileT + pa, al);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        ldsm4t(sm + L::kU + L::kTileU + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bl[p]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+            }
+            const float s = pow2(eu) * (1.f / kScaleQ);
+            const int r = c * kC + t0;
+            float *o = a.o + ((long long)(row0 + r) * a.value_heads + vh) * kD + split * kN + col;
+            const long long step = 8ll * a.value_heads * kD;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (r < rows) *reinterpret_cast<float2 *>(o + 8 * j) = make_float2(acc[j][0] * s, acc[j][1] * s);
+                if (r + 8 < rows) *reinterpret_cast<float2 *>(o + step + 8 * j) = make_float2(acc[j][2] * s, acc[j][3] * s);
+            }
+        }
+        if (c + 1 < chunks) {
+            store_state(es);   // every warp has read the old one (two barriers ago)
+            store_values(c + 1);
+        }
+        __syncthreads();
+        if (tid == 0) vmax[c & 1] = 0;   // read at the head of this chunk; next added to in the next one
+    }
+    if (!ok)   // a copy that never landed must not pass for an answer
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[j][e] = NAN;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            a.delta_out[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] = S[j][e];
+}
+
+// ---- finish -------------------------------------------------------------------------------------------
+
+// Gated RMS norm of every (row, value head), a warp each; then (the last blocks) the last three inputs
+// of every channel: after the other launches, so that the states may be updated in place.
+template <bool kBf16>
+__global__ void __launch_bounds__(kThreads) k_gdn_finish(const __grid_constant__ GdnArgs a, int norm_blocks) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if ((int)blockIdx.x >= norm_blocks) {
+        const long long i = (long long)(blockIdx.x - norm_blocks) * kThreads + tid;
+        if (i >= (long long)a.num_seqs * a.channels) return;
+        const int b = (int)(i / a.channels), c = (int)(i - (long long)b * a.channels);
+        const int r0 = seq_first(a, b), n = seq_rows(a, b);
+        float v[3];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+            const int r = n + j - 3;   // row of the sequence, negative: of the state before it
+            v[j] = r >= 0 ? load_x(a.qkv, (long long)(r0 + r) * a.qkv_stride + c, kBf16)
+                          : (a.conv_in ? a.conv_in[((long long)b * 3 + 3 + r) * a.channels + c] : 0.f);
+        }
+#pragma unroll
+        for (int j = 0; j < 3; ++j) a.conv_out[((long long)b * 3 + j) * a.channels + c] = v[j];
+        return;
+    }
+    const int first = max(0, min(a.cu_rows[0], a.total_rows)), end = min(a.cu_rows[a.num_seqs], a.total_rows);
+    const long long units = (long long)max(0, end - first) * a.value_heads;
+    const uint2 wv = *reinterpret_cast<const uint2 *>(a.norm_w + 4 * lane);
+    for (long long u = (long long)blockIdx.x * kWarps + warp; u < units; u += (long long)norm_blocks * kWarps) {
+        const long long r = first + u / a.value_heads;
+        const int vh = (int)(u % a.value_heads);
+        const float4 o = *reinterpret_cast<const float4 *>(a.o + (r * a.value_heads + vh) * kD + 4 * lane);
+        float z[4];
+        const long long za = r * a.z_stride + vh * kD + 4 * lane;
+        if constexpr (kBf16) {
+            const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.z) + za);
+            z[0] = bf16_lo(q.x), z[1] = bf16_hi(q.x), z[2] = bf16_lo(q.y), z[3] = bf16_hi(q.y);
+        } else {
+            const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.z) + za);
+            z[0] = q.x, z[1] = q.y, z[2] = q.z, z[3] = q.w;
+        }
+        const float inv = rsqrtf(warp_sum(o.x * o.x + o.y * o.y + o.z * o.z + o.w * o.w) / kD + 1e-6f);
+        const float v0 = o.x * inv * bf16_lo(wv.x) * siluf_(z[0]), v1 = o.y * inv * bf16_hi(wv.x) * siluf_(z[1]);
+        const float v2 = o.z * inv * bf16_lo(wv.y) * siluf_(z[2]), v3 = o.w * inv * bf16_hi(wv.y) * siluf_(z[3]);
+        const long long at = (r * a.value_heads + vh) * kD + 4 * lane;
+        if (a.out_bf16)
+            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+        else
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v0, v1, v2, v3);
+    }
+}
+
+long long max_chunks(int num_seqs, int total_rows) { return (long long)total_rows / kC + num_seqs; }
+
+template <bool kBf16, bool kFull>
+cudaError_t launch(const GdnArgs &a, cudaStream_t st) {
+    cudaError_t e = cudaSuccess;
+    if (a.total_rows > 0) {
+        e = cudaFuncSetAttribute(k_gdn_chunks<kBf16, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem::kBytes);
+        if (e != cudaSuccess) return e;
+        const dim3 grid((unsigned)max_chunks(a.num_seqs, a.total_rows), a.key_heads);
+        k_gdn_chunks<kBf16, kFull><<<grid, kThreads, ChunkSmem::kBytes, st>>>(a);
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    }
+    e = cudaFuncSetAttribute(k_gdn_scan<kBf16, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<kFull>::kBytes);
+    if (e != cudaSuccess) return e;
+    k_gdn_scan<kBf16, kFull><<<dim3(kSplit, a.value_heads, a.num_seqs), kThreads, ScanSmem<kFull>::kBytes, st>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    const long long units = (long long)a.total_rows * a.value_heads, want = (units + kWarps - 1) / kWarps;
+    const int norm_blocks = (int)(want < 8 * 148 ? want : 8 * 148);   // 8 CTAs an SM
+    const long long conv_blocks = ((long long)a.num_seqs * a.channels + kThreads - 1) / kThreads;
+    k_gdn_finish<kBf16><<<(unsigned)(norm_blocks + conv_blocks), kThreads, 0, st>>>(a, norm_blocks);
+    return cudaGetLastError();
 }
 
 int check_shape(const nmoe_linear_attn_shape *s) {
@@ -135,6 +808,26 @@ int check_shape(const nmoe_linear_attn_shape *s) {
         return fail(NMOE_EINVAL, "value_heads %d must be a multiple of key_heads %d (at most 1024; 8192 value heads)",
                     s->value_heads, s->key_heads);
     return NMOE_OK;
+}
+
+// The parts of the workspace, 256-byte aligned, from `base`; returns their size.
+size_t carve(const nmoe_linear_attn_shape &s, int num_seqs, int total_rows, uint8_t *base, GdnArgs *a) {
+    const size_t chunks = (size_t)max_chunks(num_seqs, total_rows);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        uint8_t *p = base + at;
+        at += (n + 255) & ~(size_t)255;
+        return p;
+    };
+    uint8_t *kq = take(chunks * s.key_heads * 4 * kTileX), *tp = take(chunks * s.value_heads * 4 * kTileT);
+    uint8_t *gates = take(chunks * s.value_heads * kGates), *o = take((size_t)total_rows * s.value_heads * kD * 4);
+    if (a != nullptr) {
+        a->kq = kq;
+        a->tp = tp;
+        a->gates = gates;
+        a->o = reinterpret_cast<float *>(o);
+    }
+    return at;
 }
 
 bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
@@ -148,10 +841,8 @@ extern "C" const char *nmoe_linear_attn_error(void) { return g_err; }
 
 extern "C" size_t nmoe_linear_attn_prefill_workspace_bytes(const nmoe_linear_attn_shape *s, int num_seqs,
                                                            int total_rows) {
-    (void)s;
-    (void)num_seqs;
-    (void)total_rows;
-    return 0;
+    if (check_shape(s) != NMOE_OK || num_seqs < 1 || total_rows < 0) return 0;
+    return carve(*s, num_seqs, total_rows, nullptr, nullptr);
 }
 
 extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const nmoe_linear_attn_shape *shape,
@@ -181,10 +872,10 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
     a.ab_stride = ab_stride == 0 ? shape->value_heads : ab_stride;
     const int unit = x_dtype == NMOE_DTYPE_BF16 ? 8 : 4;
     if (a.qkv_stride < ch || a.z_stride < vw || a.ab_stride < shape->value_heads || a.qkv_stride % unit != 0 ||
-        a.z_stride % unit != 0 || !aligned_to(qkv, 16) || !aligned_to(z, 16) || !aligned_to(alpha, 4) ||
-        !aligned_to(beta, 4))
+        a.z_stride % unit != 0 || !aligned_to(qkv, 16) || !aligned_to(z, 16) || !aligned_to(alpha, 16 / unit) ||
+        !aligned_to(beta, 16 / unit))
         return fail(NMOE_EINVAL, "a row stride is too small, or qkv or z rows are not 16-byte aligned");
-    if (!aligned_to(w->conv_w, 8) || !aligned_to(w->A_log, 4) || !aligned_to(conv_in, 16) || !aligned_to(conv_out, 16) ||
+    if (!aligned_to(w->conv_w, 8) || !aligned_to(w->A_log, 4) || !aligned_to(w->norm_w, 8) || !aligned_to(w->dt_bias, 2) || !aligned_to(conv_in, 16) || !aligned_to(conv_out, 16) ||
         !aligned_to(delta_in, 16) || !aligned_to(delta_out, 16) || !aligned_to(out, 16))
         return fail(NMOE_EINVAL, "a state, weight or output is not aligned");
     a.cu_rows = cu_rows;
@@ -208,10 +899,13 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
     a.channels = (int)ch;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     a.out_bf16 = out_dtype == NMOE_DTYPE_BF16;
-    (void)workspace;
+    if (workspace == nullptr || !aligned_to(workspace, 16)) return fail(NMOE_EINVAL, "workspace is NULL or not aligned");
+    if (max_chunks(num_seqs, total_rows) > 2147483647ll || a.value_heads > 65535)
+        return fail(NMOE_EINVAL, "too many rows or sequences");
+    carve(*shape, num_seqs, total_rows, static_cast<uint8_t *>(workspace), &a);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    k_gdn_rows<<<dim3(shape->value_heads, num_seqs), kD, 0, st>>>(a);
-    k_gdn_conv_state<<<dim3((unsigned)((ch + 255) / 256), num_seqs), 256, 0, st>>>(a);
-    const cudaError_t e = cudaGetLastError();
+    // an fp32 output takes the lo parts of Q and P too
+    const cudaError_t e = a.x_bf16 ? (a.out_bf16 ? launch<true, false>(a, st) : launch<true, true>(a, st))
+                                   : (a.out_bf16 ? launch<false, false>(a, st) : launch<false, true>(a, st));
     return e == cudaSuccess ? NMOE_OK : fail(NMOE_ECUDA, "prefill: %s", cudaGetErrorString(e));
 }

@@ -261,13 +261,6 @@ __device__ __forceinline__ void copy_row(uint32_t dst, const void *src, uint32_t
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// A wait for this warp's own copies, bounded by its number of tries.
-__device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity) {
-    for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n)
-        if (n >= kMaxSpins) return false;
-    return true;
-}
-
 // out[b][head][d .. d + 3] = weighted values / sum, times the gate; nothing seen: zeros.
 template <int D>
 __device__ __forceinline__ void write_out(const StepArgs &a, int b, int head, int d, float4 A, float L) {
