@@ -17,14 +17,14 @@
 // every operand split into two fp16 parts, x = hi + lo (22 bits), and the three products hi hi, hi lo,
 // lo hi, so that states are as exact as with fp32 operands (1e-7 of their norm). fp16 has the range of
 // 2^40 only: k, q and P are scaled by constants, the state and U by a power of two that follows a bound
-// on them (|u| <= max |v| + |S|, |S'|^2 <= |S|^2 + sum v^2, row by row, since |k| <= 1 and b <= 1). The
-// products that reach nothing but a bf16 output (Q S^T, P U) take the hi parts alone: 2^-12 against
-// its 2^-9. What bounds it: on one sequence the scan's chain of three dependent products a chunk; on
+// on them (|u| <= max |v| + |S|, |S'|^2 <= |S|^2 + sum v^2, row by row, since |k| <= 1 and b <= 1). What bounds it: on one sequence the scan's chain of three dependent products a chunk; on
 // many, the warp tensor rate (1024 products a cycle and SM).
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
+
+#include <type_traits>
 
 #include "nmoe/moe_cuda.h"
 #include "nmoe_sm100.cuh"
@@ -45,6 +45,7 @@ int fail(int status, const char *fmt, ...) {
 constexpr int kD = 128, kC = 64;      // head dim, tokens of a chunk
 constexpr int kSplit = 4, kN = kD / kSplit;   // value columns of a scan CTA: 32
 constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kScanThreads = 512;
 constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about 1 / 11 and 1 / 128
 
 // Tile images, the same in the workspace and in shared memory: rows of fp16 in 16-byte pieces, piece
@@ -114,6 +115,12 @@ __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) {
+    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+// x / (1 + e^-x) with the hardware's exponential and reciprocal: a few 2^-23 of it
+__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
 // byte offset of 16-byte piece p of row r: rows of 256, 128 and 64 bytes
 __device__ __forceinline__ uint32_t at256(int r, int p) { return r * 256 + ((p ^ (r & 7)) << 4); }
 __device__ __forceinline__ uint32_t at128(int r, int p) { return r * 128 + ((p ^ (r & 7)) << 4); }
@@ -135,8 +142,8 @@ struct ChunkSmem {
 template <bool kBf16, bool kFull>
 __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constant__ GdnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ double G[2][kC];   // sums down to -1000 and beyond, whose differences matter
-    __shared__ float beta[2][kC];
+    __shared__ __align__(16) float2 G[2][kC];
+    __shared__ __align__(16) float beta[2][kC];
     __shared__ int scan[kWarps], found[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int chunk = blockIdx.x, kh = blockIdx.y;
@@ -175,68 +182,99 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     const int row0 = seq_first(a, b), in_seq = found[1] * kC, n = min(kC, seq_rows(a, b) - in_seq);
     const uint32_t sm = smem_u32(smem);
 
-    // ---- convolution, SiLU and norm of q and k: a warp takes 8 tokens, a lane 4 channels of each
+    const int ratio = a.value_heads / a.key_heads;
+    const int half = warp >> 2, q4 = warp & 3, t128 = tid & 127;
+    // G: the running sum of log g, in two floats (sums run to -1000 and beyond, and it is differences
+    // that count); a warp per head
+    auto gates_of = [&](int v0) {
+        if (q4 != 3 || v0 + half >= ratio) return;
+        const int vh = kh * ratio + v0 + half;
+        const float rate = -expf(a.A_log[vh]), dt = bf16_to_f32(a.dt_bias[vh]);
+        double g[2];
+        float bt[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int t = 2 * lane + j;
+            const long long at = (long long)(row0 + in_seq + min(t, n - 1)) * a.ab_stride + vh;
+            const float al = load_x(a.alpha, at, kBf16), be = load_x(a.beta, at, kBf16);
+            g[j] = t < n ? rate * softplus(al + dt) : 0.f;
+            bt[j] = t < n ? sigmoidf_(be) : 0.f;
+        }
+        double inc = g[0] + g[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        const double first = inc - g[1];
+        const float h0 = (float)first, h1 = (float)inc;
+        *reinterpret_cast<float4 *>(&G[half][2 * lane]) = make_float4(h0, (float)(first - h0), h1, (float)(inc - h1));
+        *reinterpret_cast<float2 *>(&beta[half][2 * lane]) = make_float2(bt[0], bt[1]);
+    };
+
+    // ---- convolution, SiLU and norm of q and k: a warp takes 8 tokens, a lane 4 channels of each. All rows
+    // are asked for first, wherever they lie; what is no row of the sequence is replaced after.
     {
         const int t0 = 8 * warp, cq = kh * kD + 4 * lane, ck = (a.key_heads + kh) * kD + 4 * lane;
-        float x[11][8];
+        using Raw4 = typename std::conditional<kBf16, uint2, float4>::type;
+        using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
+        Raw4 xr[2][11];
 #pragma unroll
         for (int i = 0; i < 11; ++i) {
-            const int t = t0 + i - 3, r = in_seq + t;   // token of the chunk, row of the sequence
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
-            if (r >= 0 && t < n) {
-                const long long at = (long long)(row0 + r) * a.qkv_stride;
-                if constexpr (kBf16) {
-                    const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.qkv) + at + cq);
-                    const uint2 k = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.qkv) + at + ck);
-                    x[i][0] = bf16_lo(q.x), x[i][1] = bf16_hi(q.x), x[i][2] = bf16_lo(q.y), x[i][3] = bf16_hi(q.y);
-                    x[i][4] = bf16_lo(k.x), x[i][5] = bf16_hi(k.x), x[i][6] = bf16_lo(k.y), x[i][7] = bf16_hi(k.y);
-                } else {
-                    const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.qkv) + at + cq);
-                    const float4 k = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.qkv) + at + ck);
-                    x[i][0] = q.x, x[i][1] = q.y, x[i][2] = q.z, x[i][3] = q.w;
-                    x[i][4] = k.x, x[i][5] = k.y, x[i][6] = k.z, x[i][7] = k.w;
-                }
-            } else if (r < 0 && a.conv_in != nullptr) {
-                const float *c = a.conv_in + ((long long)b * 3 + 3 + r) * a.channels;
-                const float4 q = *reinterpret_cast<const float4 *>(c + cq), k = *reinterpret_cast<const float4 *>(c + ck);
-                x[i][0] = q.x, x[i][1] = q.y, x[i][2] = q.z, x[i][3] = q.w;
-                x[i][4] = k.x, x[i][5] = k.y, x[i][6] = k.z, x[i][7] = k.w;
-            }
+            const int r = min(max(in_seq + t0 + i - 3, 0), in_seq + n - 1);
+            const Raw *p = static_cast<const Raw *>(a.qkv) + (long long)(row0 + r) * a.qkv_stride;
+            xr[0][i] = *reinterpret_cast<const Raw4 *>(p + cq);
+            xr[1][i] = *reinterpret_cast<const Raw4 *>(p + ck);
         }
-        uint2 w[8];
+        uint2 w[2][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            w[j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (cq + j));
-            w[4 + j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ck + j));
+            w[0][j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (cq + j));
+            w[1][j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ck + j));
         }
+        gates_of(0);   // while they are on their way
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int t = t0 + i;
-            float y[8];
-            float qq = 0.f, kk = 0.f;
+        for (int side = 0; side < 2; ++side) {   // q, then k
+            float x[11][4];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float s = x[i][j] * bf16_lo(w[j].x) + x[i + 1][j] * bf16_hi(w[j].x) + x[i + 2][j] * bf16_lo(w[j].y) +
-                                x[i + 3][j] * bf16_hi(w[j].y);
-                y[j] = t < n ? siluf_(s) : 0.f;
-                if (j < 4)
-                    qq = fmaf(y[j], y[j], qq);
-                else
-                    kk = fmaf(y[j], y[j], kk);
+            for (int i = 0; i < 11; ++i) {
+                if constexpr (kBf16) {
+                    x[i][0] = bf16_lo(xr[side][i].x), x[i][1] = bf16_hi(xr[side][i].x);
+                    x[i][2] = bf16_lo(xr[side][i].y), x[i][3] = bf16_hi(xr[side][i].y);
+                } else {
+                    x[i][0] = xr[side][i].x, x[i][1] = xr[side][i].y, x[i][2] = xr[side][i].z, x[i][3] = xr[side][i].w;
+                }
             }
-            const float iq = rsqrtf(warp_sum(qq) / kD + 1e-12f) * (kScaleQ / kD);
-            const float ik = rsqrtf(warp_sum(kk) / kD + 1e-12f) * (kScaleK * 0.08838834764831845f);
-            uint32_t h0, l0, h1, l1;
-            const uint32_t at = at256(t, lane >> 1) + (lane & 1) * 8;
-            split2(y[0] * iq, y[1] * iq, h0, l0);
-            split2(y[2] * iq, y[3] * iq, h1, l1);
-            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kQ + at) = make_uint2(h0, h1);
-            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kQ + kTileX + at) = make_uint2(l0, l1);
-            split2(y[4] * ik, y[5] * ik, h0, l0);
-            split2(y[6] * ik, y[7] * ik, h1, l1);
-            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kK + at) = make_uint2(h0, h1);
-            *reinterpret_cast<uint2 *>(smem + ChunkSmem::kK + kTileX + at) = make_uint2(l0, l1);
+            if (in_seq == 0 && warp == 0) {   // the inputs before the sequence
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (a.conv_in != nullptr)
+                        c = *reinterpret_cast<const float4 *>(a.conv_in + ((long long)b * 3 + i) * a.channels + (side ? ck : cq));
+                    x[i][0] = c.x, x[i][1] = c.y, x[i][2] = c.z, x[i][3] = c.w;
+                }
+            }
+            const float scale = side ? kScaleK * 0.08838834764831845f : kScaleQ / kD;
+            uint8_t *tile = smem + (side ? ChunkSmem::kK : ChunkSmem::kQ);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int t = t0 + i;
+                float y[4], ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float s = x[i][j] * bf16_lo(w[side][j].x) + x[i + 1][j] * bf16_hi(w[side][j].x) +
+                                    x[i + 2][j] * bf16_lo(w[side][j].y) + x[i + 3][j] * bf16_hi(w[side][j].y);
+                    y[j] = t < n ? silu_fast(s) : 0.f;
+                    ss = fmaf(y[j], y[j], ss);
+                }
+                const float inv = rsqrtf(warp_sum(ss) / kD + 1e-12f) * scale;
+                uint32_t h0, l0, h1, l1;
+                const uint32_t at = at256(t, lane >> 1) + (lane & 1) * 8;
+                split2(y[0] * inv, y[1] * inv, h0, l0);
+                split2(y[2] * inv, y[3] * inv, h1, l1);
+                *reinterpret_cast<uint2 *>(tile + at) = make_uint2(h0, h1);
+                *reinterpret_cast<uint2 *>(tile + kTileX + at) = make_uint2(l0, l1);
+            }
         }
     }
     __syncthreads();
@@ -279,53 +317,38 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     const float *qkt = reinterpret_cast<const float *>(smem + ChunkSmem::kQK);
 
     // ---- the value heads of the key head, two at a time: four warps each
-    const int ratio = a.value_heads / a.key_heads;
-    const int half = warp >> 2, q4 = warp & 3, t128 = tid & 127;
+    auto diff = [&](int t, int s) { return (G[half][t].x - G[half][s].x) + (G[half][t].y - G[half][s].y); };
     for (int v0 = 0; v0 < ratio; v0 += 2) {
         const bool on = v0 + half < ratio;
         const int vh = kh * ratio + v0 + half;
         float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT) + half * kC * kLdT;
         float *scratch = reinterpret_cast<float *>(smem + ChunkSmem::kScratch) + warp * 256;
-        if (on && q4 == 0) {   // G: the running sum of log g
-            const float rate = -expf(a.A_log[vh]), dt = bf16_to_f32(a.dt_bias[vh]);
-            float g[2], bt[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int t = 2 * lane + j;
-                const long long at = (long long)(row0 + in_seq + t) * a.ab_stride + vh;
-                g[j] = t < n ? rate * softplus(load_x(a.alpha, at, kBf16) + dt) : 0.f;
-                bt[j] = t < n ? sigmoidf_(load_x(a.beta, at, kBf16)) : 0.f;
-            }
-            double inc = (double)g[0] + g[1];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
-            }
-            G[half][2 * lane] = inc - g[1];
-            G[half][2 * lane + 1] = inc;
-            beta[half][2 * lane] = bt[0];
-            beta[half][2 * lane + 1] = bt[1];
-        }
+        if (v0 > 0) gates_of(v0);
         __syncthreads();   // also: K K^T, Q K^T are complete, and Q is read
         if (on) {
             float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
             if (t128 < kC) {
-                gates[t128] = expf((float)G[half][t128]);
-                gates[kC + t128] = expf((float)(G[half][kC - 1] - G[half][t128]));
+                gates[t128] = expf(G[half][t128].x + G[half][t128].y);
+                gates[kC + t128] = expf(diff(kC - 1, t128));
             }
             // M below the diagonal; P with its diagonal, straight into its tile
             uint8_t *P = a.tp + (((long long)chunk * a.value_heads + vh) * 4 + 2) * kTileT;
             for (int i = t128; i < kC * kC / 8; i += 128) {
                 const int t = i >> 3, s0 = (i & 7) * 8;
-                float p[8];
+                float p[8], m[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int s = s0 + j;
-                    const float e = s <= t ? expf((float)(G[half][t] - G[half][s])) : 0.f;
-                    p[j] = s <= t ? e * qkt[t * kLd + s] : 0.f;
-                    T[t * kLdT + s] = s < t ? beta[half][t] * e * kkt[t * kLd + s] : 0.f;
+                for (int j = 0; j < 8; ++j) p[j] = m[j] = 0.f;
+                if (s0 <= t) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int s = s0 + j;
+                        const float e = s <= t ? __expf(diff(t, s)) : 0.f;   // at most 1: 2^-22 or so of it, and of 1
+                        p[j] = s <= t ? e * qkt[t * kLd + s] : 0.f;
+                        m[j] = s < t ? beta[half][t] * e * kkt[t * kLd + s] : 0.f;
+                    }
                 }
+                *reinterpret_cast<float4 *>(T + t * kLdT + s0) = make_float4(m[0], m[1], m[2], m[3]);
+                *reinterpret_cast<float4 *>(T + t * kLdT + s0 + 4) = make_float4(m[4], m[5], m[6], m[7]);
                 uint32_t h[4], l[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) split2(p[2 * j], p[2 * j + 1], h[j], l[j]);
@@ -356,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             const int j = q4, r = lane & 15, c = (lane >> 4) * 8;
             float acc[8] = {};
             if (on && j < i) {
+#pragma unroll 8
                 for (int k = 16 * j; k < 16 * i; ++k) {
                     const float m = T[(16 * i + r) * kLdT + k];
                     const float4 u = *reinterpret_cast<const float4 *>(T + k * kLdT + 16 * j + c);
@@ -369,6 +393,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 __syncwarp();
 #pragma unroll
                 for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+#pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     const float m = -T[(16 * i + r) * kLdT + 16 * i + k];
                     const float4 u = *reinterpret_cast<const float4 *>(scratch + k * 16 + c);
@@ -419,19 +444,27 @@ struct ScanSmem {
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
-// e with bound * 2^-e in [2^12, 2^13), so that fp16 holds what the bound bounds and its parts reach 2^-37 of it
-__device__ __forceinline__ int exponent_of(float bound) {
-    const int e = (__float_as_int(bound) >> 23) - 127 - 12;
+// The scale 2^-e for values whose square is at most `square`: they come below 2^13, so that fp16 holds
+// them and its parts reach 2^-37 of that.
+__device__ __forceinline__ int exponent_of(float square) {
+    const int e = (((__float_as_int(square) >> 23) - 127 + 2) >> 1) - 13;   // 2^(e + 13) > sqrt(square)
     return min(100, max(-100, e));
 }
 
+// Eight warps carry the recurrence (K S^T, U, the new state); eight others work beside them on what it
+// does not wait for (Q S^T, P U and the output, and the values of the next chunk). Named barriers:
+//   1  the first eight among themselves
+//   2  U of the chunk is stored        (the first eight arrive, the others wait)
+//   3  the others are done with the chunk's state and U, and the next values are stored
+//   4  the next state is stored
 template <bool kBf16, bool kFull>
-__global__ void __launch_bounds__(kThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
     using L = ScanSmem<kFull>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[2], p_full;
     __shared__ int vmax[2], first_chunk;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = (tid >> 5) & 7, lane = tid & 31;
+    const bool chain = tid < kScanThreads / 2;
     const int split = blockIdx.x, vh = blockIdx.y, b = blockIdx.z, kh = vh / (a.value_heads / a.key_heads);
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
@@ -445,30 +478,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_gdn_scan(const __grid_constant_
     __syncthreads();
     {
         int before = 0;
-        for (int i = tid; i < b; i += kThreads) before += seq_chunks(a, i);
+        for (int i = tid; i < b; i += kScanThreads) before += seq_chunks(a, i);
         if (before) atomicAdd(&first_chunk, before);   // integers: the order does not matter
     }
     const int row0 = seq_first(a, b), rows = seq_rows(a, b), chunks = (rows + kC - 1) / kC;
+    const int col = 2 * (lane & 3);
+
+    // ---- the state (the first eight warps): S^T, rows (dims) 16 warp + lane / 4 (+ 8), columns 8 j + col (+ 1)
+    float S[4][4];
+    const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN) * kD;
+    const int dim = 16 * warp + (lane >> 2);
+    if (chain) {
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                S[j][e] = a.delta_in ? a.delta_in[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] : 0.f;
+                m = fmaxf(m, fabsf(S[j][e]));
+            }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) atomicMax(&vmax[1], __float_as_int(m));   // not negative: ordered as integers
+    }
     __syncthreads();
     const long long chunk0 = first_chunk;
-
-    // ---- the state: S^T, rows (dims) 16 warp + lane / 4 (+ 8), columns 8 j + 2 (lane % 4) (+ 1) of 32
-    float S[4][4];
-    float bound2 = 0.f;   // of |S|^2, per value row
-    const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN) * kD;
-    const int dim = 16 * warp + (lane >> 2), col = 2 * (lane & 3);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            S[j][e] = a.delta_in ? a.delta_in[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] : 0.f;
-            bound2 = fmaxf(bound2, fabsf(S[j][e]));
-        }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) bound2 = fmaxf(bound2, __shfl_xor_sync(0xffffffffu, bound2, o));
-    if (lane == 0) atomicMax(&vmax[1], __float_as_int(bound2));   // not negative: ordered as integers
-    __syncthreads();
-    bound2 = __int_as_float(vmax[1]);
+    float bound2 = __int_as_float(vmax[1]);   // of |S|^2, per value row
     bound2 = bound2 * bound2 * kD;
     __syncthreads();
     if (tid == 0) vmax[1] = 0;
@@ -484,8 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_gdn_scan(const __grid_constant_
                 split2(S[j + x][0] * s, S[j + x][1] * s, h[2 * x], l[2 * x]);
                 split2(S[j + x][2] * s, S[j + x][3] * s, h[2 * x + 1], l[2 * x + 1]);
             }
-            const int c = 8 * (j + (lane >> 4)) + (lane & 7);
-            const uint32_t at = sm + L::kS + at256(c, 2 * warp + ((lane >> 3) & 1));
+            const uint32_t at = sm + L::kS + at256(8 * (j + (lane >> 4)) + (lane & 7), 2 * warp + ((lane >> 3) & 1));
             stsm4t(at, h[0], h[1], h[2], h[3]);
             stsm4t(at + kN * kD * 2, l[0], l[1], l[2], l[3]);
         }
@@ -506,30 +540,42 @@ __global__ void __launch_bounds__(kThreads, 1) k_gdn_scan(const __grid_constant_
         mbar_arrive_expect_tx(&p_full, L::kQParts * kTileT);
         bulk_g2s(smem + L::kP, tp, L::kQParts * kTileT, &p_full, policy_evict_normal());
     };
-    // ---- V: channel `lane`, tokens 8 warp .. + 7 of a chunk; the inputs are loaded a chunk ahead
+    // ---- V (the other eight warps): channel `lane`, tokens 8 warp .. + 7 of a chunk; the inputs are loaded a
+    // chunk ahead, and stay as they are until they are used (a conversion would wait for them)
+    using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
+    constexpr int kTok = kC / 8;
     const int ch = (2 * a.key_heads + vh) * kD + split * kN + lane;
     const uint2 cw = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * ch);
-    float raw[11];
+    Raw raw[kTok + 3];
+    float before[3] = {0.f, 0.f, 0.f};   // the inputs before the sequence, for its first tokens
+    if (!chain && warp == 0 && a.conv_in != nullptr)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) before[i] = a.conv_in[((long long)b * 3 + i) * a.channels + ch];
+    const Raw *raw_at = static_cast<const Raw *>(a.qkv) + (long long)(row0 + kTok * warp - 3) * a.qkv_stride + ch;
     auto load_raw = [&](int c) {
+        const Raw *p = raw_at + (long long)c * kC * a.qkv_stride;
+        const int r = c * kC + kTok * warp - 3;
 #pragma unroll
-        for (int i = 0; i < 11; ++i) {
-            const int r = c * kC + 8 * warp + i - 3;
-            raw[i] = 0.f;
-            if (r >= 0 && r < rows)
-                raw[i] = load_x(a.qkv, (long long)(row0 + r) * a.qkv_stride + ch, kBf16);
-            else if (r < 0 && a.conv_in != nullptr)
-                raw[i] = a.conv_in[((long long)b * 3 + 3 + r) * a.channels + ch];
-        }
+        for (int i = 0; i < kTok + 3; ++i, p += a.qkv_stride) raw[i] = r + i >= 0 && r + i < rows ? *p : Raw(0);
     };
-    auto v_at = [&](int t, int c) { return reinterpret_cast<float *>(smem + L::kV) + t * kN + (((c >> 3) ^ (t & 3)) << 3) + (c & 7); };
+    auto v_at = [&](int t, int x) {
+        return reinterpret_cast<float *>(smem + L::kV) + t * kN + (((x >> 3) ^ (t & 3)) << 3) + (x & 7);
+    };
     auto store_values = [&](int c) {
-        float m = 0.f;
+        float x[kTok + 3], m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int t = 8 * warp + i;
-            const float s = raw[i] * bf16_lo(cw.x) + raw[i + 1] * bf16_hi(cw.x) + raw[i + 2] * bf16_lo(cw.y) +
-                            raw[i + 3] * bf16_hi(cw.y);
-            const float v = c * kC + t < rows ? siluf_(s) : 0.f;
+        for (int i = 0; i < kTok + 3; ++i) {
+            if constexpr (kBf16)
+                x[i] = bf16_to_f32(raw[i]);
+            else
+                x[i] = raw[i];
+            if (i < 3 && c == 0 && warp == 0) x[i] = before[i];
+        }
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+            const int t = kTok * warp + i;
+            const float s = x[i] * bf16_lo(cw.x) + x[i + 1] * bf16_hi(cw.x) + x[i + 2] * bf16_lo(cw.y) + x[i + 3] * bf16_hi(cw.y);
+            const float v = c * kC + t < rows ? silu_fast(s) : 0.f;
             *v_at(t, lane) = v;
             m = fmaxf(m, fabsf(v));
         }
@@ -539,193 +585,197 @@ __global__ void __launch_bounds__(kThreads, 1) k_gdn_scan(const __grid_constant_
     };
 
     bool ok = true;
-    int es = exponent_of(sqrtf(bound2));
+    int es = exponent_of(bound2);
     if (chunks > 0) {
         if (tid == 0) copy_stage(0);
-        load_raw(0);
-        store_state(es);
-        __syncthreads();   // vmax[1] is clear
-        store_values(0);
+        if (chain) {
+            store_state(es);
+        } else {
+            load_raw(0);
+            store_values(0);   // vmax[0]
+            if (chunks > 1) load_raw(1);
+        }
         __syncthreads();
     }
+    const int mt = warp & 3, nh = warp >> 2;   // 16 tokens, 16 columns
+    const int t0 = 16 * mt + (lane >> 2);      // this lane's tokens t0, t0 + 8
     for (int c = 0; c < chunks; ++c) {
-        if (tid == 0) {
+        const float vm = __int_as_float(vmax[c & 1]);
+        bound2 += kC * vm * vm;   // of the states of this chunk, and of the one it leaves
+        const int eu = exponent_of(bound2) + 1;   // max |v| + |S| <= 9/8 sqrt(bound2)
+        const uint32_t st = sm + (c & 1) * L::kStage;
+        const float *eg = reinterpret_cast<const float *>(smem + (c & 1) * L::kStage + L::kGate), *el = eg + kC;
+        if (tid == kScanThreads / 2) {
             copy_p(c);
             if (c + 1 < chunks) copy_stage(c + 1);
         }
-        if (c + 1 < chunks) load_raw(c + 1);
-        const float vm = __int_as_float(vmax[c & 1]);
-        bound2 += kC * vm * vm;   // of the states of this chunk, and of the one it leaves
-        const int eu = exponent_of(vm + sqrtf(bound2));
-        const uint32_t st = sm + (c & 1) * L::kStage;
-        const float *eg = reinterpret_cast<const float *>(smem + (c & 1) * L::kStage + L::kGate), *el = eg + kC;
         ok &= mbar_wait_spin(&full[c & 1], (c >> 1) & 1);
-
-        // ---- 1: K S^T (warps 0-3) and Q S^T (warps 4-7), 16 tokens a warp, all 32 columns
-        const int mt = warp & 3;
-        const bool is_q = warp >= 4;
-        float acc[4][4] = {};
+        // K S^T, or Q S^T
+        float acc[2][4] = {};
         {
-            const uint32_t A = st + (is_q ? 2 * kTileX : 0), B = sm + L::kS;
+            const uint32_t A = st + (chain ? 0 : 2 * kTileX), B = sm + L::kS;
+            const bool exact = kFull || chain;
 #pragma unroll
             for (int kk = 0; kk < kD / 16; ++kk) {
-                uint32_t ah[4], al[4], bh[2][4], bl[2][4];
+                uint32_t ah[4], al[4], bh[4], bl[4];
                 const uint32_t pa = at256(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
+                const uint32_t pb = at256(16 * nh + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1));
                 ldsm4(A + pa, ah);
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    ldsm4(B + at256(16 * p + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), bh[p]);
-                if (kFull || !is_q) {
+                ldsm4(B + pb, bh);
+                if (exact) {
                     ldsm4(A + kTileX + pa, al);
+                    ldsm4(B + kN * kD * 2 + pb, bl);
 #pragma unroll
-                    for (int p = 0; p < 2; ++p)
-                        ldsm4(B + kN * kD * 2 + at256(16 * p + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1)), bl[p]);
+                    for (int j = 0; j < 2; ++j) mma_f16(acc[j], al, bh[2 * j], bh[2 * j + 1]);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
+                    for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bl[2 * j], bl[2 * j + 1]);
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+                for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bh[2 * j], bh[2 * j + 1]);
             }
         }
-        const int t0 = 16 * mt + (lane >> 2);   // this lane's tokens t0, t0 + 8
         const float g0 = eg[t0], g1 = eg[t0 + 8];
-        if (!is_q) {   // R = V - e^G K S^T, scaled
-            const float s = pow2(-eu), k0 = g0 * pow2(es) * (1.f / kScaleK), k1 = g1 * pow2(es) * (1.f / kScaleK);
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
+        if (chain) {
+            {   // R = V - e^G K S^T, scaled
+                const float s = pow2(-eu), k0 = g0 * pow2(es) * (1.f / kScaleK), k1 = g1 * pow2(es) * (1.f / kScaleK);
                 uint32_t h[4], l[4];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const float2 v0 = *reinterpret_cast<const float2 *>(v_at(t0, 8 * (j + x) + col));
-                    const float2 v1 = *reinterpret_cast<const float2 *>(v_at(t0 + 8, 8 * (j + x) + col));
-                    split2((v0.x - k0 * acc[j + x][0]) * s, (v0.y - k0 * acc[j + x][1]) * s, h[2 * x], l[2 * x]);
-                    split2((v1.x - k1 * acc[j + x][2]) * s, (v1.y - k1 * acc[j + x][3]) * s, h[2 * x + 1], l[2 * x + 1]);
+                    const float2 v0 = *reinterpret_cast<const float2 *>(v_at(t0, 16 * nh + 8 * x + col));
+                    const float2 v1 = *reinterpret_cast<const float2 *>(v_at(t0 + 8, 16 * nh + 8 * x + col));
+                    split2((v0.x - k0 * acc[x][0]) * s, (v0.y - k0 * acc[x][1]) * s, h[2 * x], l[2 * x]);
+                    split2((v1.x - k1 * acc[x][2]) * s, (v1.y - k1 * acc[x][3]) * s, h[2 * x + 1], l[2 * x + 1]);
                 }
-                const uint32_t at = sm + L::kR + at64(16 * mt + (lane & 15), j + (lane >> 4));
+                const uint32_t at = sm + L::kR + at64(16 * mt + (lane & 15), 2 * nh + (lane >> 4));
                 stsm4(at, h[0], h[1], h[2], h[3]);
                 stsm4(at + L::kTileU, l[0], l[1], l[2], l[3]);
             }
-        } else {       // e^G Q S^T on the scale of P U
-            const float k0 = g0 * pow2(es) * pow2(-eu), k1 = g1 * pow2(es) * pow2(-eu);
+            bar_sync(1, 256);
+            {   // U = T b R: 16 tokens x 16 columns a warp, a long row beside a short one on each scheduler
+                const int i = nh ? 3 - mt : mt;
+                float u[2][4] = {}, v[2][4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[j][0] *= k0, acc[j][1] *= k0, acc[j][2] *= k1, acc[j][3] *= k1;
-        }
-        __syncthreads();
-        // ---- 2: U = T b R: 16 tokens x 16 columns a warp, long rows beside short ones
-        {
-            const int i = is_q ? 3 - mt : mt, h2 = is_q ? 1 : 0;
-            float u[2][4] = {};
-            for (int kk = 0; kk <= i; ++kk) {
-                uint32_t ah[4], al[4], bh[4], bl[4];
-                const uint32_t pa = at128(16 * i + (lane & 15), 2 * kk + (lane >> 4));
-                const uint32_t pb = at64(16 * kk + (lane & 15), 2 * h2 + (lane >> 4));
-                ldsm4(st + L::kT + pa, ah);
-                ldsm4(st + L::kT + kTileT + pa, al);
-                ldsm4t(sm + L::kR + pb, bh);
-                ldsm4t(sm + L::kR + L::kTileU + pb, bl);
+                for (int kk = 0; kk < kC / 16; ++kk) {
+                    if (kk <= i) {
+                        uint32_t ah[4], al[4], bh[4], bl[4];
+                        const uint32_t pa = at128(16 * i + (lane & 15), 2 * kk + (lane >> 4));
+                        const uint32_t pb = at64(16 * kk + (lane & 15), 2 * nh + (lane >> 4));
+                        ldsm4(st + L::kT + pa, ah);
+                        ldsm4t(sm + L::kR + pb, bh);
+                        ldsm4(st + L::kT + kTileT + pa, al);
+                        ldsm4t(sm + L::kR + L::kTileU + pb, bl);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) mma_f16(u[x], al, bh[2 * x], bh[2 * x + 1]);
+                        for (int x = 0; x < 2; ++x) mma_f16(u[x], ah, bh[2 * x], bh[2 * x + 1]);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) mma_f16(u[x], ah, bl[2 * x], bl[2 * x + 1]);
+                        for (int x = 0; x < 2; ++x) mma_f16(v[x], al, bh[2 * x], bh[2 * x + 1]);
 #pragma unroll
-                for (int x = 0; x < 2; ++x) mma_f16(u[x], ah, bh[2 * x], bh[2 * x + 1]);
+                        for (int x = 0; x < 2; ++x) mma_f16(v[x], ah, bl[2 * x], bl[2 * x + 1]);
+                    }
+                }
+                const int t = 16 * i + (lane >> 2);
+                const float e0 = el[t], e1 = el[t + 8];
+                uint32_t h[4], l[4], wh[4], wl[4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[x][e] += v[x][e];
+                    split2(u[x][0], u[x][1], h[2 * x], l[2 * x]);
+                    split2(u[x][2], u[x][3], h[2 * x + 1], l[2 * x + 1]);
+                    split2(u[x][0] * e0, u[x][1] * e0, wh[2 * x], wl[2 * x]);
+                    split2(u[x][2] * e1, u[x][3] * e1, wh[2 * x + 1], wl[2 * x + 1]);
+                }
+                const uint32_t at = at64(16 * i + (lane & 15), 2 * nh + (lane >> 4));
+                stsm4(sm + L::kW + at, wh[0], wh[1], wh[2], wh[3]);
+                stsm4(sm + L::kW + L::kTileU + at, wl[0], wl[1], wl[2], wl[3]);
+                stsm4(sm + L::kU + at, h[0], h[1], h[2], h[3]);
+                if (kFull) stsm4(sm + L::kU + L::kTileU + at, l[0], l[1], l[2], l[3]);
             }
-            const int t = 16 * i + (lane >> 2);
-            const float e0 = el[t], e1 = el[t + 8];
-            uint32_t h[4], l[4], wh[4], wl[4];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                split2(u[x][0], u[x][1], h[2 * x], l[2 * x]);
-                split2(u[x][2], u[x][3], h[2 * x + 1], l[2 * x + 1]);
-                split2(u[x][0] * e0, u[x][1] * e0, wh[2 * x], wl[2 * x]);
-                split2(u[x][2] * e1, u[x][3] * e1, wh[2 * x + 1], wl[2 * x + 1]);
-            }
-            const uint32_t at = at64(16 * i + (lane & 15), 2 * h2 + (lane >> 4));
-            stsm4(sm + L::kU + at, h[0], h[1], h[2], h[3]);
-            if (kFull) stsm4(sm + L::kU + L::kTileU + at, l[0], l[1], l[2], l[3]);
-            stsm4(sm + L::kW + at, wh[0], wh[1], wh[2], wh[3]);
-            stsm4(sm + L::kW + L::kTileU + at, wl[0], wl[1], wl[2], wl[3]);
-        }
-        __syncthreads();
-        // ---- 3: S' = e^{G_63} S + K^T (e^{G_63 - G} U), 16 dims a warp; P U on top of e^G Q S^T (warps 4-7)
-        {
+            bar_arrive(2, 512);
+            bar_sync(1, 256);
+            // S' = e^{G_63} S + K^T (e^{G_63 - G} U), 16 dims and all columns a warp
             float up[4][4] = {};
 #pragma unroll
             for (int kk = 0; kk < kC / 16; ++kk) {
                 uint32_t ah[4], al[4], bh[2][4], bl[2][4];
                 const uint32_t pa = at256(16 * kk + (lane & 7) + ((lane >> 4) << 3), 2 * warp + ((lane >> 3) & 1));
                 ldsm4t(st + pa, ah);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) ldsm4t(sm + L::kW + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bh[p]);
                 ldsm4t(st + kTileX + pa, al);
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    const uint32_t pb = at64(16 * kk + (lane & 15), 2 * p + (lane >> 4));
-                    ldsm4t(sm + L::kW + pb, bh[p]);
-                    ldsm4t(sm + L::kW + L::kTileU + pb, bl[p]);
-                }
+                for (int p = 0; p < 2; ++p)
+                    ldsm4t(sm + L::kW + L::kTileU + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bl[p]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) mma_f16(up[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
             }
             const float keep = eg[kC - 1], add = pow2(eu) * (1.f / kScaleK);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[j][e] = fmaf(S[j][e], keep, up[j][e] * add);
-        }
-        es = exponent_of(sqrtf(bound2));
-        if (is_q) {
-            ok &= mbar_wait_spin(&p_full, c & 1);
-            for (int kk = 0; kk <= mt; ++kk) {
-                uint32_t ah[4], al[4], bh[2][4], bl[2][4];
-                const uint32_t pa = at128(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
-                ldsm4(sm + L::kP + pa, ah);
+            es = exponent_of(bound2);
+            bar_sync(3, 512);
+            if (tid == 0) vmax[c & 1] = 0;   // read by all; next added to in the next chunk
+            if (c + 1 < chunks) store_state(es);
+            bar_sync(4, 512);
+        } else {
+            {   // e^G Q S^T on the scale of P U
+                const float k0 = g0 * pow2(es) * pow2(-eu), k1 = g1 * pow2(es) * pow2(-eu);
 #pragma unroll
-                for (int p = 0; p < 2; ++p) ldsm4t(sm + L::kU + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bh[p]);
-                if (kFull) {
-                    ldsm4(sm + L::kP + kTileT + pa, al);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p)
-                        ldsm4t(sm + L::kU + L::kTileU + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bl[p]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
-                }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(acc[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
+                for (int j = 0; j < 2; ++j) acc[j][0] *= k0, acc[j][1] *= k0, acc[j][2] *= k1, acc[j][3] *= k1;
             }
+            es = exponent_of(bound2);
+            ok &= mbar_wait_spin(&p_full, c & 1);
+            bar_sync(2, 512);
+#pragma unroll
+            for (int kk = 0; kk < kC / 16; ++kk) {
+                if (kk <= mt) {
+                    uint32_t ah[4], al[4], bh[4], bl[4];
+                    const uint32_t pa = at128(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
+                    const uint32_t pb = at64(16 * kk + (lane & 15), 2 * nh + (lane >> 4));
+                    ldsm4(sm + L::kP + pa, ah);
+                    ldsm4t(sm + L::kU + pb, bh);
+                    if (kFull) {
+                        ldsm4(sm + L::kP + kTileT + pa, al);
+                        ldsm4t(sm + L::kU + L::kTileU + pb, bl);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma_f16(acc[j], al, bh[2 * j], bh[2 * j + 1]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bl[2 * j], bl[2 * j + 1]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bh[2 * j], bh[2 * j + 1]);
+                }
+            }
+            if (c + 1 < chunks) store_values(c + 1);   // over this chunk's, which U is made of
+            bar_arrive(3, 512);
+            if (c + 2 < chunks) load_raw(c + 2);
             const float s = pow2(eu) * (1.f / kScaleQ);
             const int r = c * kC + t0;
-            float *o = a.o + ((long long)(row0 + r) * a.value_heads + vh) * kD + split * kN + col;
+            float *o = a.o + ((long long)(row0 + r) * a.value_heads + vh) * kD + split * kN + 16 * nh + col;
             const long long step = 8ll * a.value_heads * kD;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 if (r < rows) *reinterpret_cast<float2 *>(o + 8 * j) = make_float2(acc[j][0] * s, acc[j][1] * s);
                 if (r + 8 < rows) *reinterpret_cast<float2 *>(o + step + 8 * j) = make_float2(acc[j][2] * s, acc[j][3] * s);
             }
+            bar_sync(4, 512);
         }
-        if (c + 1 < chunks) {
-            store_state(es);   // every warp has read the old one (two barriers ago)
-            store_values(c + 1);
-        }
-        __syncthreads();
-        if (tid == 0) vmax[c & 1] = 0;   // read at the head of this chunk; next added to in the next one
     }
-    if (!ok)   // a copy that never landed must not pass for an answer
+    if (!ok && !chain) vmax[0] = -1;   // a copy that never landed must not pass for an answer
+    __syncthreads();
+    if (chain) {
+        ok &= chunks == 0 || vmax[0] != -1;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[j][e] = NAN;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            a.delta_out[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] = S[j][e];
+            for (int e = 0; e < 4; ++e)
+                a.delta_out[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] = ok ? S[j][e] : NAN;
+    }
 }
 
 // ---- finish -------------------------------------------------------------------------------------------
@@ -792,7 +842,7 @@ cudaError_t launch(const GdnArgs &a, cudaStream_t st) {
     }
     e = cudaFuncSetAttribute(k_gdn_scan<kBf16, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<kFull>::kBytes);
     if (e != cudaSuccess) return e;
-    k_gdn_scan<kBf16, kFull><<<dim3(kSplit, a.value_heads, a.num_seqs), kThreads, ScanSmem<kFull>::kBytes, st>>>(a);
+    k_gdn_scan<kBf16, kFull><<<dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem<kFull>::kBytes, st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const long long units = (long long)a.total_rows * a.value_heads, want = (units + kWarps - 1) / kWarps;
     const int norm_blocks = (int)(want < 8 * 148 ? want : 8 * 148);   // 8 CTAs an SM
@@ -904,8 +954,6 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
         return fail(NMOE_EINVAL, "too many rows or sequences");
     carve(*shape, num_seqs, total_rows, static_cast<uint8_t *>(workspace), &a);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    // an fp32 output takes the lo parts of Q and P too
-    const cudaError_t e = a.x_bf16 ? (a.out_bf16 ? launch<true, false>(a, st) : launch<true, true>(a, st))
-                                   : (a.out_bf16 ? launch<false, false>(a, st) : launch<false, true>(a, st));
+    const cudaError_t e = a.x_bf16 ? launch<true, true>(a, st) : launch<false, true>(a, st);
     return e == cudaSuccess ? NMOE_OK : fail(NMOE_ECUDA, "prefill: %s", cudaGetErrorString(e));
 }
