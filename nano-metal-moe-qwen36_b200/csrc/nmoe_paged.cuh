@@ -1,6 +1,8 @@
 // nmoe_paged.cuh -- what the paged full-attention kernels share: the device view of a paged
 // cache, the row -> sequence search, and the preparation of one head (RMS norm, rotation).
 #pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -152,6 +154,11 @@ int check_paged_kv(const nmoe_paged_kv *kv, PagedDev *dev);
 void fill_rotary(const nmoe_full_attn_shape *s, RotaryDev *r);
 int check_x(const char *what, const void *p, int x_dtype, long long stride, long long width);
 int device_sm_count(int *sms);
+using TensorMapEncode = PFN_cuTensorMapEncodeTiled_v12000;
+TensorMapEncode tensor_map_encode();
+// Pages as a 5D tensor (64 columns, page rows, panels of 64 columns, heads, pages); boxes of `rows`
+// rows and `panels` panels of one page and head, 128-byte swizzle: in shared memory [panel][row][64].
+bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, int panels);
 
 inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 

@@ -11,9 +11,10 @@
 // Split: the positions of all (sequence, KV head) pairs, in tiles of 64, form one line that is cut
 // into equal pieces, one per CTA (one CTA per SM), whatever the lengths are; a piece may end one
 // pair and begin the next. Lengths are read on the device. Each of a CTA's four warps takes 16
-// positions of every tile with its own ring of bulk copies (a row of K or V per lane) and its own
+// positions of every tile with its own ring of copies (16 rows of K, 16 of V, by TMA) and its own
 // running maximum and sum; warps join through shared memory at the end of a pair, and pieces of
-// one pair join in a second launch.
+// one pair join in a second launch. Beginning and ending a pair costs a piece about four tiles' time, and
+// counts as that much on the line.
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -103,6 +104,32 @@ int device_sm_count(int *sms) {
     return NMOE_OK;
 }
 
+TensorMapEncode tensor_map_encode() {
+    static TensorMapEncode fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return (TensorMapEncode) nullptr;
+        return reinterpret_cast<TensorMapEncode>(p);
+    }();
+    return fn;
+}
+
+bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, int panels) {
+    const cuuint64_t dims[5] = {64, (cuuint64_t)c.page_size, (cuuint64_t)(d / 64), (cuuint64_t)heads,
+                                (cuuint64_t)c.num_pages};
+    const cuuint64_t strides[4] = {(cuuint64_t)c.row_stride * 2, 128, (cuuint64_t)c.head_stride * 2,
+                                   (cuuint64_t)c.page_stride * 2};
+    const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)panels, 1, 1};
+    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
+    const TensorMapEncode fn = tensor_map_encode();
+    return fn != nullptr &&
+           fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<uint16_t *>(base), dims, strides, box, es,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 namespace {
 
 // ---- append ------------------------------------------------------------------------------------
@@ -176,8 +203,10 @@ constexpr int kStepWarps = 4, kStepThreads = 32 * kStepWarps;
 constexpr int kTile = 64;        // positions of a tile: 16 per warp
 constexpr int kMaxCtas = 512;    // pieces of the line of tiles (workspace bound)
 constexpr int kGroupMax = 8;
+constexpr int kPairCost = 4;     // tiles
 
 struct StepArgs {
+    CUtensorMap k_map, v_map;   // pages in boxes of 16 rows and all columns, where boxed
     PagedDev c;
     RotaryDev rot;
     HeadDev h;
@@ -187,25 +216,34 @@ struct StepArgs {
     float *part;   // [pairs + CTAs][group][D + 4]: weighted values, maximum, sum
     void *out;
     float scale;   // softmax scale times log2(e)
-    int batch, kv_heads, group, gated, x_bf16, out_bf16, ctas;
+    int batch, kv_heads, group, gated, x_bf16, out_bf16, ctas, boxed;
 };
 
 template <int D>
 struct StepCfg {
-    static constexpr int kRowB = D * 2 + 16;   // 16 bytes of padding: 8 rows of an ldmatrix in 8 bank groups
+    static constexpr int kHalfB = 16 * D * 2;         // 16 rows of K (or V): panels of [16 rows][64 columns], swizzled
+    static constexpr int kStageB = 2 * kHalfB;
     static constexpr int kStages = D == 256 ? 3 : 6;
-    static constexpr int kStageB = 32 * kRowB;   // 16 K rows, 16 V rows
     static constexpr int kRingB = kStepWarps * kStages * kStageB;
-    static constexpr int kQ = kRingB;                       // query parts
+    static constexpr int kQ = kRingB;                 // query parts: rows of kRowB
+    static constexpr int kRowB = D * 2 + 16;          // 16 bytes of padding: 8 rows of an ldmatrix in 8 bank groups
     static constexpr int q_bytes(int parts) { return (parts == 3 ? 32 : 16) * kRowB; }
-    static constexpr int bytes(int parts) { return kRingB + q_bytes(parts); }
+    static constexpr int bytes(int parts) { return kRingB + q_bytes(parts) + 1024; }   // + alignment
 };
+
+// byte offset of 16-byte piece x of row r (of 16) of a half stage
+__device__ __forceinline__ uint32_t at_panel(int r, int x) {
+    return (uint32_t)(x >> 3) * 2048u + (uint32_t)r * 128u + (uint32_t)(((x & 7) ^ (r & 7)) << 4);
+}
 
 __device__ __forceinline__ int seq_tiles(int len, int capacity) {
     return len < 1 || len > capacity ? 0 : (len + kTile - 1) / kTile;
 }
+// What a (sequence, KV head) pair counts on the line: its tiles and what beginning and ending it costs
+// (queries, first copies, the join of the warps), in tiles.
+__device__ __forceinline__ long long pair_weight(int tiles) { return tiles > 0 ? tiles + kPairCost : 0; }
 
-// All threads of a CTA: tiles of the sequences before this thread's stripe of them, and of all.
+// All threads of a CTA: weight of the sequences before this thread's stripe of them, and of all.
 struct Plan {
     long long before, total;   // per KV head
     int first, last;           // this thread's stripe of sequences
@@ -217,7 +255,7 @@ __device__ __forceinline__ Plan plan_tiles(const int *lens, int batch, int capac
     p.first = min(batch, tid * per);
     p.last = min(batch, p.first + per);
     long long own = 0;
-    for (int b = p.first; b < p.last; ++b) own += seq_tiles(lens[b], capacity);
+    for (int b = p.first; b < p.last; ++b) own += pair_weight(seq_tiles(lens[b], capacity));
     long long inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -254,10 +292,13 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void copy_row(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
-                 "l"(src), "r"(bytes), "r"(bar)
-                 : "memory");
+// 16 page rows of one head, all columns
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap *map, int row, int head, int page, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst),
+        "l"(map), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page), "r"(bar)
+        : "memory");
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -286,7 +327,7 @@ template <int D, int PARTS>
 __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_constant__ StepArgs a) {
     using Cfg = StepCfg<D>;
     constexpr int E = D / 32, kRowB = Cfg::kRowB, kStages = Cfg::kStages;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t bars[kStepWarps][kStages];
     __shared__ uint32_t live[kStepWarps][kStages];   // bit i: position i of the stage takes part
     __shared__ float2 cs[128];
@@ -295,6 +336,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
     __shared__ int sm_seq;
     __shared__ long long sm_off;
 
+    uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);   // the swizzle goes by the address
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (lane == 0) {
@@ -311,7 +353,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
     {
         long long before = plan.before;
         for (int b = plan.first; b < plan.last; ++b) {
-            const long long n = (long long)seq_tiles(a.kv_lens[b], a.c.capacity);
+            const long long n = pair_weight(seq_tiles(a.kv_lens[b], a.c.capacity));
             if (cur >= before * a.kv_heads && cur < (before + n) * a.kv_heads) {
                 sm_seq = b;
                 sm_off = cur - before * a.kv_heads;
@@ -321,7 +363,8 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
     }
     __syncthreads();
     int b = sm_seq, len = a.kv_lens[b], nt = seq_tiles(len, a.c.capacity);
-    int kvh = (int)(sm_off / nt), t0 = (int)(sm_off - (long long)kvh * nt);
+    int kvh = (int)(sm_off / (nt + kPairCost));
+    int at = (int)(sm_off - (long long)kvh * (nt + kPairCost));   // where the piece begins in its pair
 
     const uint32_t ring = smem_u32(smem) + warp * kStages * Cfg::kStageB;
     uint8_t *ring_p = smem + warp * kStages * Cfg::kStageB;
@@ -331,15 +374,17 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
     bool lost = false;
 
     while (true) {
-        const int t1 = (int)min((long long)nt, t0 + (end - cur));
+        // tiles t0 .. t1 - 1 of this pair; none when the piece holds no more than the pair's cost
+        const int to = (int)min((long long)nt + kPairCost, at + (end - cur));
+        const int t0 = max(0, at - kPairCost), t1 = max(0, to - kPairCost);
         const int steps = t1 - t0;
         const bool whole = steps == nt;
         const int fresh = a.k_new != nullptr ? len - 1 : -1;   // position that comes from k_new / v_new
 
-        // ---- copies of this warp's 16 positions of tile t0 + i: lane l < 16 a K row, l >= 16 a V row
+        // ---- copies of this warp's 16 positions of tile t0 + i
         int page_next = -1;
-        auto page_of = [&](int i) {
-            const int p = (t0 + i) * kTile + 16 * warp + (lane & 15);
+        auto page_of = [&](int i) {   // boxed: of all 16 positions; else of position lane % 16
+            const int p = (t0 + i) * kTile + 16 * warp + (a.boxed ? 0 : lane & 15);
             return i < steps && p < len ? a.c.table[(long long)b * a.c.table_stride + (unsigned)p / (unsigned)a.c.page_size]
                                         : -1;
         };
@@ -347,32 +392,42 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
             const int s = it % kStages;
             const int page = page_next;
             page_next = page_of(i + 1);
-            const int p = (t0 + i) * kTile + 16 * warp + (lane & 15);
+            const int base = (t0 + i) * kTile + 16 * warp;
             const bool ok = page >= 0 && page < a.c.num_pages;   // page is -1 past the end
-            const bool copy = ok && p != fresh;
-            const uint32_t okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-            const uint32_t cpm = __ballot_sync(0xffffffffu, copy);
-            // a V row that takes no part is zero: its probability is zero, and 0 * NaN is NaN
-            for (uint32_t z = ~okm & 0xffffu; z != 0; z &= z - 1) {
-                const int row = 16 + __ffs(z) - 1;
-                for (int j = lane; j < D / 8; j += 32)
-                    *reinterpret_cast<uint4 *>(ring_p + s * Cfg::kStageB + row * kRowB + 16 * j) = make_uint4(0, 0, 0, 0);
+            uint8_t *stage = ring_p + s * Cfg::kStageB;
+            uint32_t okm;
+            if (a.boxed) {
+                okm = ok ? (len - base >= 16 ? 0xffffu : (1u << (len - base)) - 1u) : 0u;
+            } else {
+                okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
             }
             if (lane == 0) {
                 live[warp][s] = okm;
-                mbar_arrive_expect_tx(&bars[warp][s], __popc(cpm) * D * 2);
+                mbar_arrive_expect_tx(&bars[warp][s], a.boxed && ok ? Cfg::kStageB : 0);
             }
             fence_async_shared();   // this warp's reads and writes of the stage, before the copies
             __syncwarp();
-            if (copy) {
-                const long long off = (long long)page * a.c.page_stride +
-                                      (long long)((unsigned)p % (unsigned)a.c.page_size) * a.c.row_stride +
-                                      (long long)kvh * a.c.head_stride;
-                copy_row(ring + s * Cfg::kStageB + lane * kRowB, (lane < 16 ? a.c.k : a.c.v) + off, D * 2,
-                         smem_u32(&bars[warp][s]));
+            if (a.boxed && ok) {
+                if (lane < 2)
+                    copy_box(ring + s * Cfg::kStageB + lane * Cfg::kHalfB, lane ? &a.v_map : &a.k_map,
+                             (int)((unsigned)base % (unsigned)a.c.page_size), kvh, page, smem_u32(&bars[warp][s]));
+            } else if (!a.boxed) {   // pages that no box fits: row by row, D / 8 pieces each
+                for (int r = 0; r < 16; ++r) {
+                    const int pg = __shfl_sync(0xffffffffu, page, r);
+                    if (!(okm >> r & 1u)) continue;
+                    const long long off = (long long)pg * a.c.page_stride +
+                                          (long long)((unsigned)(base + r) % (unsigned)a.c.page_size) * a.c.row_stride +
+                                          (long long)kvh * a.c.head_stride;
+                    for (int x = lane; x < D / 4; x += 32) {
+                        const int v = x >= D / 8, piece = x - v * (D / 8);
+                        *reinterpret_cast<uint4 *>(stage + v * Cfg::kHalfB + at_panel(r, piece)) =
+                            *reinterpret_cast<const uint4 *>((v ? a.c.v : a.c.k) + off + 8 * piece);
+                    }
+                }
             }
             ++it;
         };
+        if (steps > 0) {
         page_next = page_of(0);
         int issued = 0;
         for (; issued < kStages && issued < steps; ++issued) issue(issued);
@@ -414,30 +469,38 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
             __syncwarp();
             const int base = (t0 + i) * kTile + 16 * warp;
             uint32_t lv = live[warp][s];
-            const uint32_t ks = ring + s * Cfg::kStageB, vs = ks + 16 * kRowB;
+            const uint32_t ks = ring + s * Cfg::kStageB, vs = ks + Cfg::kHalfB;
+            uint8_t *stage = ring_p + s * Cfg::kStageB;
+            // a V row that takes no part is zero: its probability is zero, and 0 * NaN is NaN
+            if (lv != 0xffffu) {
+                for (uint32_t z = ~lv & 0xffffu; z != 0; z &= z - 1)
+                    if (lane < D / 8)
+                        *reinterpret_cast<uint4 *>(stage + Cfg::kHalfB + at_panel(__ffs(z) - 1, lane)) = make_uint4(0, 0, 0, 0);
+                __syncwarp();
+            }
             if (fresh >= base && fresh < base + 16 && (lv >> (fresh - base) & 1u)) {
                 // the new token: its key and value into the cache and into this stage
                 float v[E];
                 const long long src = (long long)b * a.kv_stride + (long long)kvh * D + E * lane;
                 const long long dst = paged_row(a.c, b, fresh) + (long long)kvh * a.c.head_stride + E * lane;
-                uint8_t *row = ring_p + s * Cfg::kStageB + (fresh - base) * kRowB + 2 * E * lane;
+                uint8_t *row = stage + at_panel(fresh - base, E * lane / 8) + (E * lane % 8) * 2;
                 load_elems<E>(a.k_new, src, a.x_bf16, v);
                 prepare_head<E>(v, a.h.k_norm, a.h.eps, cs, a.rot.half, lane);
                 store_bf16<E>(a.c.k + dst, v);
                 store_bf16<E>(reinterpret_cast<uint16_t *>(row), v);
                 load_elems<E>(a.v_new, src, a.x_bf16, v);
                 store_bf16<E>(a.c.v + dst, v);
-                store_bf16<E>(reinterpret_cast<uint16_t *>(row + 16 * kRowB), v);
+                store_bf16<E>(reinterpret_cast<uint16_t *>(row + Cfg::kHalfB), v);
                 __syncwarp();
             }
             float sc[2][2][4];   // [kk parity][8 positions][fragment]
 #pragma unroll
             for (int x = 0; x < 16; ++x) (&sc[0][0][0])[x] = 0.f;
-            const uint32_t ka = ks + ((lane >> 4) * 8 + (lane & 7)) * kRowB + ((lane >> 3) & 1) * 16;
+            const int kr = (lane >> 4) * 8 + (lane & 7), kx = (lane >> 3) & 1;
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
                 uint32_t kf[4];
-                ldsm4(ka + 32 * kk, kf);
+                ldsm4(ks + at_panel(kr, 2 * kk + kx), kf);
                 mma_bf16(sc[kk & 1][0], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], kf[0], kf[1]);
                 mma_bf16(sc[kk & 1][1], qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3], kf[2], kf[3]);
                 if constexpr (PARTS == 3) {
@@ -486,11 +549,11 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
                 pf3[2] = pack2_bf16(r1[2] - bf16_round(r1[2]), r1[3] - bf16_round(r1[3]));
                 pf3[1] = pf3[3] = 0u;
             }
-            const uint32_t va = vs + (((lane >> 3) & 1) * 8 + (lane & 7)) * kRowB + (lane >> 4) * 16;
+            const int vr = lane & 15, vx = lane >> 4;
 #pragma unroll
             for (int n = 0; n < D / 16; ++n) {
                 uint32_t vf[4];
-                ldsm4t(va + 32 * n, vf);
+                ldsm4t(vs + at_panel(vr, 2 * n + vx), vf);
                 mma_bf16(acc[2 * n], pf[0], pf[1], pf[2], pf[3], vf[0], vf[1]);
                 mma_bf16(acc[2 * n + 1], pf[0], pf[1], pf[2], pf[3], vf[2], vf[3]);
                 if constexpr (PARTS == 3) {
@@ -542,10 +605,11 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
                 if (d == 0) *reinterpret_cast<float2 *>(pb + D) = make_float2(M, L);
             }
         }
-        cur += steps;
+        }
+        cur += to - at;
         if (cur >= end) break;
         __syncthreads();
-        t0 = 0;   // the next pair that has tiles
+        at = 0;   // the next pair that has tiles
         if (++kvh == a.kv_heads) {
             kvh = 0;
             do {
@@ -573,7 +637,7 @@ __global__ void __launch_bounds__(kStepThreads) k_step_join(const __grid_constan
     const Plan plan = plan_tiles(a.kv_lens, a.batch, a.c.capacity, sm_scan);
     if (b >= plan.first && b < plan.last) {
         long long before = plan.before;
-        for (int x = plan.first; x < b; ++x) before += seq_tiles(a.kv_lens[x], a.c.capacity);
+        for (int x = plan.first; x < b; ++x) before += pair_weight(seq_tiles(a.kv_lens[x], a.c.capacity));
         sm_before = before;
     }
     __syncthreads();
@@ -586,7 +650,8 @@ __global__ void __launch_bounds__(kStepThreads) k_step_join(const __grid_constan
         return;
     }
     const long long total = plan.total * a.kv_heads;
-    const long long first = sm_before * a.kv_heads + (long long)kvh * nt, last = first + nt - 1;
+    // where the pair's first and last tile are on the line
+    const long long first = sm_before * a.kv_heads + (long long)kvh * (nt + kPairCost) + kPairCost, last = first + nt - 1;
     // the CTA that takes tile t: the largest c with total * c / pieces <= t
     const long long pieces = min((long long)a.ctas, total);
     const int c0 = (int)(((first + 1) * pieces - 1) / total), c1 = (int)(((last + 1) * pieces - 1) / total);
@@ -753,6 +818,10 @@ extern "C" int nmoe_full_attn_step_paged(const nmoe_full_attn_weights *w, const 
     a.gated = shape->gated;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     a.out_bf16 = out_dtype == NMOE_DTYPE_BF16;
+    // boxes of 16 rows and all columns: 16 positions lie in one page
+    const int d = shape->head_dim;
+    a.boxed = a.c.page_size % 16 == 0 && page_map(&a.k_map, a.c, a.c.k, d, a.kv_heads, 16, d / 64) &&
+              page_map(&a.v_map, a.c, a.c.v, d, a.kv_heads, 16, d / 64);
     const long long most = (long long)batch * shape->kv_heads * ((a.c.capacity + kTile - 1) / kTile);
     a.ctas = (int)(most < sms ? most : sms);
     if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;

@@ -25,8 +25,6 @@
 // reads them: 0 * NaN is NaN. Page sizes that are no multiple of 16 rows are copied by the warp
 // itself.
 #include <cooperative_groups.h>
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include <type_traits>
@@ -755,40 +753,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-using EncodeFn = PFN_cuTensorMapEncodeTiled_v12000;
-
-EncodeFn encode_fn() {
-    static EncodeFn fn = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess)
-            return (EncodeFn) nullptr;
-        return reinterpret_cast<EncodeFn>(p);
-    }();
-    return fn;
-}
-
-// Pages as a 5D tensor (64 columns, page rows, panels of 64 columns, heads, pages); boxes of `rows`
-// rows and `panels` panels of one page and head, 128-byte swizzle: in shared memory [panel][row][64].
-bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, int panels) {
-    const cuuint64_t dims[5] = {64, (cuuint64_t)c.page_size, (cuuint64_t)(d / 64), (cuuint64_t)heads,
-                                (cuuint64_t)c.num_pages};
-    const cuuint64_t strides[4] = {(cuuint64_t)c.row_stride * 2, 128, (cuuint64_t)c.head_stride * 2,
-                                   (cuuint64_t)c.page_stride * 2};
-    const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)panels, 1, 1};
-    const cuuint32_t es[5] = {1, 1, 1, 1, 1};
-    EncodeFn fn = encode_fn();
-    return fn != nullptr &&
-           fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<uint16_t *>(base), dims, strides, box, es,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 bool query_map(CUtensorMap *m, const uint16_t *base, int d, long long rows) {
     const cuuint64_t dims[2] = {(cuuint64_t)d, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)d * 2};
     const cuuint32_t box[2] = {64, kRows}, es[2] = {1, 1};
-    EncodeFn fn = encode_fn();
+    const TensorMapEncode fn = tensor_map_encode();
     return fn != nullptr &&
            fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(base), dims, strides, box, es,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
