@@ -8,9 +8,9 @@
 // the 8 query heads' upper and lower bf16 parts, so q and p lose nothing against fp32 sums but the
 // parts' own residue (2^-17), and K and V are the B operands straight from shared memory.
 //
-// Split: the positions of all (sequence, KV head) pairs, in tiles of 64, form one line that is cut
+// Split: the positions of all (sequence, KV head) pairs, in tiles of 64 or 128, form one line that is cut
 // into equal pieces, one per CTA (one CTA per SM), whatever the lengths are; a piece may end one
-// pair and begin the next. Lengths are read on the device. Each of a CTA's four warps takes 16
+// pair and begin the next. Lengths are read on the device. Each of a CTA's four or eight warps takes 16
 // positions of every tile with its own ring of copies (16 rows of K, 16 of V, by TMA) and its own
 // running maximum and sum; warps join through shared memory at the end of a pair, and pieces of
 // one pair join in a second launch. Beginning and ending a pair costs a piece about four tiles' time, and
@@ -199,8 +199,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_co
 
 // ---- step ----------------------------------------------------------------------------------------
 
-constexpr int kStepWarps = 4, kStepThreads = 32 * kStepWarps;
-constexpr int kTile = 64;        // positions of a tile: 16 per warp
+constexpr int kJoinThreads = 128;
 constexpr int kMaxCtas = 512;    // pieces of the line of tiles (workspace bound)
 constexpr int kGroupMax = 8;
 constexpr int kPairCost = 4;     // tiles
@@ -219,12 +218,17 @@ struct StepArgs {
     int batch, kv_heads, group, gated, x_bf16, out_bf16, ctas, boxed;
 };
 
+// Warps a CTA: what a scheduler needs to hide a step's chain of products behind another warp's, as far as
+// the registers allow. head_dim 128: 8 (a ragged fp32 batch 95 us with 4); 256: 4, whose
+// sums take 128 registers a thread (64 sequences of 32768: 99% of the copy rate).
 template <int D>
 struct StepCfg {
+    static constexpr int kWarps = D == 256 ? 4 : 8, kThreads = 32 * kWarps;
+    static constexpr int kTile = 16 * kWarps;         // positions of a tile: 16 per warp
     static constexpr int kHalfB = 16 * D * 2;         // 16 rows of K (or V): panels of [16 rows][64 columns], swizzled
     static constexpr int kStageB = 2 * kHalfB;
-    static constexpr int kStages = D == 256 ? 3 : 6;
-    static constexpr int kRingB = kStepWarps * kStages * kStageB;
+    static constexpr int kStages = 3;
+    static constexpr int kRingB = kWarps * kStages * kStageB;
     static constexpr int kQ = kRingB;                 // query parts: rows of kRowB
     static constexpr int kRowB = D * 2 + 16;          // 16 bytes of padding: 8 rows of an ldmatrix in 8 bank groups
     static constexpr int q_bytes(int parts) { return (parts == 3 ? 32 : 16) * kRowB; }
@@ -236,7 +240,9 @@ __device__ __forceinline__ uint32_t at_panel(int r, int x) {
     return (uint32_t)(x >> 3) * 2048u + (uint32_t)r * 128u + (uint32_t)(((x & 7) ^ (r & 7)) << 4);
 }
 
+template <int D>
 __device__ __forceinline__ int seq_tiles(int len, int capacity) {
+    constexpr int kTile = StepCfg<D>::kTile;
     return len < 1 || len > capacity ? 0 : (len + kTile - 1) / kTile;
 }
 // What a (sequence, KV head) pair counts on the line: its tiles and what beginning and ending it costs
@@ -248,14 +254,15 @@ struct Plan {
     long long before, total;   // per KV head
     int first, last;           // this thread's stripe of sequences
 };
+template <int D, int kThreads>
 __device__ __forceinline__ Plan plan_tiles(const int *lens, int batch, int capacity, long long *sm) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int per = (batch + kStepThreads - 1) / kStepThreads;
+    const int per = (batch + kThreads - 1) / kThreads;
     Plan p;
     p.first = min(batch, tid * per);
     p.last = min(batch, p.first + per);
     long long own = 0;
-    for (int b = p.first; b < p.last; ++b) own += pair_weight(seq_tiles(lens[b], capacity));
+    for (int b = p.first; b < p.last; ++b) own += pair_weight(seq_tiles<D>(lens[b], capacity));
     long long inc = own;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -266,7 +273,7 @@ __device__ __forceinline__ Plan plan_tiles(const int *lens, int batch, int capac
     __syncthreads();
     long long pre = 0, tot = 0;
 #pragma unroll
-    for (int w = 0; w < kStepWarps; ++w) {
+    for (int w = 0; w < kThreads / 32; ++w) {
         if (w < warp) pre += sm[w];
         tot += sm[w];
     }
@@ -324,15 +331,16 @@ __device__ __forceinline__ void write_out(const StepArgs &a, int b, int head, in
 
 // PARTS: bf16 parts of q and p: 2 (residue 2^-17) for a bf16 output, 3 (fp32) for an fp32 one.
 template <int D, int PARTS>
-__global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_constant__ StepArgs a) {
+__global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __grid_constant__ StepArgs a) {
     using Cfg = StepCfg<D>;
     constexpr int E = D / 32, kRowB = Cfg::kRowB, kStages = Cfg::kStages;
+    constexpr int kWarps = Cfg::kWarps, kThreads = Cfg::kThreads, kTile = Cfg::kTile;
     extern __shared__ uint8_t raw_smem[];
-    __shared__ uint64_t bars[kStepWarps][kStages];
-    __shared__ uint32_t live[kStepWarps][kStages];   // bit i: position i of the stage takes part
+    __shared__ uint64_t bars[kWarps][kStages];
+    __shared__ uint32_t live[kWarps][kStages];   // bit i: position i of the stage takes part
     __shared__ float2 cs[128];
-    __shared__ float sm_m[kStepWarps][kGroupMax], sm_l[kStepWarps][kGroupMax];
-    __shared__ long long sm_scan[kStepWarps];
+    __shared__ float sm_m[kWarps][kGroupMax], sm_l[kWarps][kGroupMax];
+    __shared__ long long sm_scan[kWarps];
     __shared__ int sm_seq;
     __shared__ long long sm_off;
 
@@ -344,7 +352,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
         mbar_fence_init();
     }
     const double freq = tid < a.rot.half ? rotary_freq(a.rot, tid) : 0.0;
-    const Plan plan = plan_tiles(a.kv_lens, a.batch, a.c.capacity, sm_scan);
+    const Plan plan = plan_tiles<D, kThreads>(a.kv_lens, a.batch, a.c.capacity, sm_scan);
     const long long total = plan.total * a.kv_heads;
     const long long pieces = min((long long)a.ctas, total);   // no piece is empty
     if (blockIdx.x >= pieces) return;
@@ -353,7 +361,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
     {
         long long before = plan.before;
         for (int b = plan.first; b < plan.last; ++b) {
-            const long long n = pair_weight(seq_tiles(a.kv_lens[b], a.c.capacity));
+            const long long n = pair_weight(seq_tiles<D>(a.kv_lens[b], a.c.capacity));
             if (cur >= before * a.kv_heads && cur < (before + n) * a.kv_heads) {
                 sm_seq = b;
                 sm_off = cur - before * a.kv_heads;
@@ -362,7 +370,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
         }
     }
     __syncthreads();
-    int b = sm_seq, len = a.kv_lens[b], nt = seq_tiles(len, a.c.capacity);
+    int b = sm_seq, len = a.kv_lens[b], nt = seq_tiles<D>(len, a.c.capacity);
     int kvh = (int)(sm_off / (nt + kPairCost));
     int at = (int)(sm_off - (long long)kvh * (nt + kPairCost));   // where the piece begins in its pair
 
@@ -434,10 +442,10 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
 
         // ---- the queries of the group, prepared, scaled and split into bf16 parts
         if (tid < a.rot.half) cs[tid] = rotary_cs(freq, len - 1);
-        for (int i = tid; i < Cfg::q_bytes(PARTS) / 16; i += kStepThreads)
+        for (int i = tid; i < Cfg::q_bytes(PARTS) / 16; i += kThreads)
             *reinterpret_cast<uint4 *>(smem + Cfg::kQ + 16 * i) = make_uint4(0, 0, 0, 0);
         __syncthreads();
-        for (int g = warp; g < a.group; g += kStepWarps) {
+        for (int g = warp; g < a.group; g += kWarps) {
             float v[E];
             load_elems<E>(a.q, (long long)b * a.q_stride + (long long)(kvh * a.group + g) * (a.gated ? 2 * D : D) + E * lane,
                           a.x_bf16, v);
@@ -581,16 +589,16 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
         }
         __syncthreads();
         const long long pair = (long long)b * a.kv_heads + kvh;
-        for (int u = tid; u < a.group * (D / 4); u += kStepThreads) {
+        for (int u = tid; u < a.group * (D / 4); u += kThreads) {
             const int g = u / (D / 4), d = 4 * (u - g * (D / 4));
             float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) M = fmaxf(M, sm_m[w][g]);
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm_m[w][g]);
             const float ms = M == -INFINITY ? 0.f : M;
             float L = 0.f;
             float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < kStepWarps; ++w) {
+            for (int w = 0; w < kWarps; ++w) {
                 const float e = ex2(sm_m[w][g] - ms);
                 const float4 o = *reinterpret_cast<const float4 *>(reinterpret_cast<float *>(smem) +
                                                                    (w * kGroupMax + g) * D + d);
@@ -615,7 +623,7 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
             do {
                 ++b;
                 len = a.kv_lens[b];
-                nt = seq_tiles(len, a.c.capacity);
+                nt = seq_tiles<D>(len, a.c.capacity);
             } while (nt == 0 && b < a.batch - 1);   // tiles are left (cur < end): a later sequence has some
             if (nt == 0) break;
         }
@@ -625,23 +633,23 @@ __global__ void __launch_bounds__(kStepThreads, 1) k_step_paged(const __grid_con
 // The pieces of one (pair, query head), or zeros for a sequence without positions. The plan is
 // recomputed while the step kernel runs (it reads only the lengths).
 template <int D>
-__global__ void __launch_bounds__(kStepThreads) k_step_join(const __grid_constant__ StepArgs a) {
-    constexpr int kLanes = D / 4, kSets = kStepThreads / kLanes;
-    __shared__ long long sm_scan[kStepWarps];
+__global__ void __launch_bounds__(kJoinThreads) k_step_join(const __grid_constant__ StepArgs a) {
+    constexpr int kLanes = D / 4, kSets = kJoinThreads / kLanes;
+    __shared__ long long sm_scan[kJoinThreads / 32];
     __shared__ long long sm_before;
     __shared__ float sm_m[kMaxCtas], sm_l[kMaxCtas];
-    __shared__ float4 sm_a[kStepThreads];
+    __shared__ float4 sm_a[kJoinThreads];
     __shared__ float sm_s[kSets];
     const int tid = threadIdx.x;
     const int pair = blockIdx.x, b = pair / a.kv_heads, kvh = pair - b * a.kv_heads, g = blockIdx.y;
-    const Plan plan = plan_tiles(a.kv_lens, a.batch, a.c.capacity, sm_scan);
+    const Plan plan = plan_tiles<D, kJoinThreads>(a.kv_lens, a.batch, a.c.capacity, sm_scan);
     if (b >= plan.first && b < plan.last) {
         long long before = plan.before;
-        for (int x = plan.first; x < b; ++x) before += pair_weight(seq_tiles(a.kv_lens[x], a.c.capacity));
+        for (int x = plan.first; x < b; ++x) before += pair_weight(seq_tiles<D>(a.kv_lens[x], a.c.capacity));
         sm_before = before;
     }
     __syncthreads();
-    const int nt = seq_tiles(a.kv_lens[b], a.c.capacity);
+    const int nt = seq_tiles<D>(a.kv_lens[b], a.c.capacity);
     // every CTA waits for the step kernel, so that this launch never ends before it
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int d = 4 * (tid % kLanes), set = tid / kLanes;
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(kStepThreads) k_step_join(const __grid_constan
     const int n = c1 - c0 + 1;
     const float *pb = a.part + (((long long)pair + c0) * a.group + g) * (D + 4);
     const long long step = (long long)a.group * (D + 4);
-    for (int i = tid; i < n; i += kStepThreads) {
+    for (int i = tid; i < n; i += kJoinThreads) {
         const float2 ml = *reinterpret_cast<const float2 *>(pb + i * step + D);
         sm_m[i] = ml.x;
         sm_l[i] = ml.y;
@@ -697,13 +705,13 @@ int launch_step(const StepArgs &a, cudaStream_t st) {
     constexpr int smem = StepCfg<D>::bytes(PARTS);
     cudaError_t e = cudaFuncSetAttribute(k_step_paged<D, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e == cudaSuccess) {
-        k_step_paged<D, PARTS><<<a.ctas, kStepThreads, smem, st>>>(a);
+        k_step_paged<D, PARTS><<<a.ctas, StepCfg<D>::kThreads, smem, st>>>(a);
         e = cudaGetLastError();
     }
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(a.batch * a.kv_heads, a.group);
-        cfg.blockDim = dim3(kStepThreads);
+        cfg.blockDim = dim3(kJoinThreads);
         cfg.stream = st;
         cudaLaunchAttribute at[1];
         at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -822,7 +830,7 @@ extern "C" int nmoe_full_attn_step_paged(const nmoe_full_attn_weights *w, const 
     const int d = shape->head_dim;
     a.boxed = a.c.page_size % 16 == 0 && page_map(&a.k_map, a.c, a.c.k, d, a.kv_heads, 16, d / 64) &&
               page_map(&a.v_map, a.c, a.c.v, d, a.kv_heads, 16, d / 64);
-    const long long most = (long long)batch * shape->kv_heads * ((a.c.capacity + kTile - 1) / kTile);
+    const long long most = (long long)batch * shape->kv_heads * ((a.c.capacity + 63) / 64);
     a.ctas = (int)(most < sms ? most : sms);
     if (a.ctas > kMaxCtas) a.ctas = kMaxCtas;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
