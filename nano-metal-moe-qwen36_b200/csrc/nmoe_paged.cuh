@@ -7,6 +7,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "nmoe/moe_cuda.h"
 #include "nmoe_common.cuh"
 
@@ -159,6 +161,22 @@ TensorMapEncode tensor_map_encode();
 // Pages as a 5D tensor (64 columns, page rows, panels of 64 columns, heads, pages); boxes of `rows`
 // rows and `panels` panels of one page and head, 128-byte swizzle: in shared memory [panel][row][64].
 bool page_map(CUtensorMap *m, const PagedDev &c, const uint16_t *base, int d, int heads, int rows, int panels);
+
+// The dynamic shared memory of a kernel: a property of the function on each device, set at its first call there.
+struct SmemOnce {
+    std::atomic<uint64_t> done{0};   // a bit per device
+    template <class K>
+    cudaError_t set(K kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+        if (bit != 0 && (done.load(std::memory_order_acquire) & bit)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+        return e;
+    }
+};
 
 inline bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 

@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_co
 
 // ---- step ----------------------------------------------------------------------------------------
 
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 512;   // sets of D / 4 threads, each taking every n-th piece
 constexpr int kMaxCtas = 512;    // pieces of the line of tiles (workspace bound)
 constexpr int kGroupMax = 8;
 constexpr int kPairCost = 4;     // tiles
@@ -674,11 +674,13 @@ __global__ void __launch_bounds__(kJoinThreads) k_step_join(const __grid_constan
     }
     __syncthreads();
     float M = -INFINITY;
-    for (int i = 0; i < n; ++i) M = fmaxf(M, sm_m[i]);
+    for (int i = tid & 31; i < n; i += 32) M = fmaxf(M, sm_m[i]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     const float ms = M == -INFINITY ? 0.f : M;
     float L = 0.f;
     float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = set; i < n; i += kSets) {
         const float e = ex2(sm_m[i] - ms);
         const float4 o = *reinterpret_cast<const float4 *>(pb + i * step + d);
@@ -703,7 +705,8 @@ __global__ void __launch_bounds__(kJoinThreads) k_step_join(const __grid_constan
 template <int D, int PARTS>
 int launch_step(const StepArgs &a, cudaStream_t st) {
     constexpr int smem = StepCfg<D>::bytes(PARTS);
-    cudaError_t e = cudaFuncSetAttribute(k_step_paged<D, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static SmemOnce once;
+    cudaError_t e = once.set(k_step_paged<D, PARTS>, smem);
     if (e == cudaSuccess) {
         k_step_paged<D, PARTS><<<a.ctas, StepCfg<D>::kThreads, smem, st>>>(a);
         e = cudaGetLastError();

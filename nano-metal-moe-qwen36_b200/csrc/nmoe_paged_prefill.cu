@@ -765,7 +765,8 @@ bool query_map(CUtensorMap *m, const uint16_t *base, int d, long long rows) {
 
 template <int D>
 cudaError_t launch(const PrefillArgs &a, long long units, cudaStream_t st) {
-    cudaError_t e = cudaFuncSetAttribute(k_prefill_pairs<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::kSmem);
+    static SmemOnce once;
+    cudaError_t e = once.set(k_prefill_pairs<D>, Cfg<D>::kSmem);
     if (e != cudaSuccess) return e;
     (a.x_bf16 ? k_prefill_queries<D, true> : k_prefill_queries<D, false>)
         <<<(a.total_rows + a.prep_rows - 1) / a.prep_rows, kPrepThreads, 0, st>>>(a);

@@ -600,7 +600,7 @@ def _dtypes():
     return _kinds
 
 
-def _device_tensors(*tensors):
+def _on_device(tensors):
     """The calls below take torch tensors: on the current device, so that a kernel never meets
     memory of another one."""
     here = _dtypes()["device"]()
@@ -610,23 +610,24 @@ def _device_tensors(*tensors):
 
 
 def _int32(t, n, name):
-    if t.dtype != _dtypes()["i32"] or not t.is_contiguous() or t.numel() < n:
+    if t.dtype is not _dtypes()["i32"] or not t.is_contiguous() or t.numel() < n:
         raise NmoeError(EINVAL, f"{name} must be a contiguous int32 tensor of at least {n} entries")
 
 
 def _rows(t, rows, width, dtype, name):
     """Row stride in elements of a [rows][width] operand whose rows are contiguous."""
-    want = _dtypes().get(dtype)
-    if want is None or t.dtype not in want:
+    if t.dtype not in _dtypes().get(dtype, ()):
         raise NmoeError(EINVAL, f"{name}: element type {t.dtype} does not match the dtype argument {dtype}")
-    shape = t.shape
-    if len(shape) == 2 and shape[0] >= rows and shape[1] == width and (t.stride(1) == 1 or width == 1):
-        return t.stride(0) if shape[0] > 1 else width
+    if t.dim() == 2:
+        n, w = t.shape
+        stride, inner = t.stride()
+        if n >= rows and w == width and (inner == 1 or width == 1):
+            return stride if n > 1 else width
     if rows == 0:
         return width
-    if len(shape) < 2 or shape[0] < rows or t[0].numel() != width or not t[0].is_contiguous():
+    if t.dim() < 2 or t.shape[0] < rows or t[0].numel() != width or not t[0].is_contiguous():
         raise NmoeError(EINVAL, f"{name} must hold at least {rows} rows of {width} contiguous elements")
-    return t.stride(0) if shape[0] > 1 else width
+    return t.stride(0) if t.shape[0] > 1 else width
 
 
 def _output(t, n, dtype, name="out"):
@@ -635,7 +636,7 @@ def _output(t, n, dtype, name="out"):
 
 
 def _states(t, n, name):
-    if t is not None and (t.dtype not in _dtypes()[DTYPE_F32] or not t.is_contiguous() or t.numel() != n):
+    if t is not None and (t.dtype not in _dtypes()[DTYPE_F32] or t.numel() != n or not t.is_contiguous()):
         raise NmoeError(EINVAL, f"{name} must be a contiguous float32 tensor of {n} elements")
 
 
@@ -658,15 +659,17 @@ class PagedKV:
             raise NmoeError(EINVAL, "k and v pages must have one shape and one set of strides")
         if block_table.dim() != 2 or block_table.dtype != torch.int32 or block_table.stride(1) != 1:
             raise NmoeError(EINVAL, "block_table must be int32 [sequences][max_pages], the last stride 1")
-        _device_tensors(k, v, block_table)
+        _on_device((k, v, block_table))
         self.k, self.v, self.block_table = k, v, block_table
+        self._fits = (k.shape[2], k.shape[3], block_table.shape[0])
         self.host = PagedKVHost(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), k.shape[0],
                                 k.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.stride(0))
 
     def _check(self, shape, seqs):
-        if self.k.shape[2] != shape.kv_heads or self.k.shape[3] != shape.head_dim:
-            raise NmoeError(EINVAL, f"pages of {tuple(self.k.shape[2:])} (KV heads, head dim) do not fit the shape")
-        if self.block_table.shape[0] < seqs:
+        heads, dim, rows = self._fits
+        if heads != shape.kv_heads or dim != shape.head_dim:
+            raise NmoeError(EINVAL, f"pages of {heads} KV heads of {dim} do not fit the shape")
+        if rows < seqs:
             raise NmoeError(EINVAL, "block_table has fewer rows than there are sequences")
 
 
@@ -677,11 +680,11 @@ def _full_attn_check(rc):
 
 def _norms(weights, shape):
     q, k = weights.get("q_norm"), weights.get("k_norm")
+    kinds, d = _dtypes()[DTYPE_BF16], shape.head_dim
     for t in (q, k):
-        if t is not None and (t.dtype not in _dtypes()[DTYPE_BF16] or not t.is_contiguous()
-                              or t.numel() != shape.head_dim):
-            raise NmoeError(EINVAL, f"q_norm and k_norm must be contiguous bf16 tensors of {shape.head_dim}")
-    _device_tensors(q, k)
+        if t is not None and (t.dtype not in kinds or t.numel() != d or not t.is_contiguous()):
+            raise NmoeError(EINVAL, f"q_norm and k_norm must be contiguous bf16 tensors of {d}")
+    _on_device((q, k))
     return FullAttnWeights(_ptr(q), _ptr(k))
 
 
@@ -690,7 +693,7 @@ def full_attn_append_paged(weights: dict, shape: FullAttnShape, cache: PagedKV, 
     """nmoe_full_attn_append_paged: normalise and rotate the packed rows' keys and append keys
     and values to their pages. k_new / v_new [rows][kv_heads * head_dim] (one row stride for both)."""
     seqs, rows, width = cu_rows.numel() - 1, k_new.shape[0], shape.kv_heads * shape.head_dim
-    _device_tensors(k_new, v_new, cu_rows, kv_lens)
+    _on_device((k_new, v_new, cu_rows, kv_lens))
     _int32(cu_rows, 1, "cu_rows")
     _int32(kv_lens, seqs, "kv_lens")
     cache._check(shape, seqs)
@@ -713,7 +716,7 @@ def full_attn_prefill_paged(weights: dict, shape: FullAttnShape, cache: PagedKV,
     holds their keys and values. q [rows][q_heads * head_dim (* 2 when gated)], out bf16
     [rows][q_heads * head_dim]."""
     seqs, rows, width = cu_rows.numel() - 1, q.shape[0], shape.q_heads * shape.head_dim
-    _device_tensors(q, cu_rows, kv_lens, out, workspace)
+    _on_device((q, cu_rows, kv_lens, out, workspace))
     _int32(cu_rows, 1, "cu_rows")
     _int32(kv_lens, seqs, "kv_lens")
     cache._check(shape, seqs)
@@ -735,7 +738,7 @@ def full_attn_step_paged(weights: dict, shape: FullAttnShape, cache: PagedKV, kv
     """nmoe_full_attn_step_paged: one new token per sequence over the pages. kv_lens counts the
     new token; k_new = v_new = None when the cache holds it already."""
     batch, width, kw = q.shape[0], shape.q_heads * shape.head_dim, shape.kv_heads * shape.head_dim
-    _device_tensors(q, k_new, v_new, kv_lens, out, workspace)
+    _on_device((q, k_new, v_new, kv_lens, out, workspace))
     _int32(kv_lens, batch, "kv_lens")
     cache._check(shape, batch)
     stride, kv_stride = _rows(q, batch, width * (2 if shape.gated else 1), x_dtype, "q"), 0
@@ -762,30 +765,31 @@ def linear_attn_prefill(weights: dict, shape: LinearAttnShape, qkv, z, alpha, be
                         conv_out, delta_out, out, workspace, x_dtype=DTYPE_BF16, out_dtype=DTYPE_BF16, stream=0):
     """nmoe_linear_attn_prefill: the GatedDeltaNet core of packed prompts. conv_in / delta_in
     None: new sequences; they may be conv_out / delta_out themselves."""
-    seqs, rows = cu_rows.numel() - 1, qkv.shape[0]
-    ch, vw = (2 * shape.key_heads + shape.value_heads) * 128, shape.value_heads * 128
-    _device_tensors(qkv, z, alpha, beta, cu_rows, conv_in, delta_in, conv_out, delta_out, out, workspace,
-                    *weights.values())
+    seqs, rows, heads = cu_rows.numel() - 1, qkv.shape[0], shape.value_heads
+    ch, vw = (2 * shape.key_heads + heads) * 128, heads * 128
+    _on_device((qkv, z, alpha, beta, cu_rows, conv_in, delta_in, conv_out, delta_out, out, workspace))
+    conv_w, A_log, dt_bias, norm_w = (weights[k] for k in ("conv_w", "A_log", "dt_bias", "norm_w"))
+    _on_device((conv_w, A_log, dt_bias, norm_w))
     _int32(cu_rows, 1, "cu_rows")
-    strides = [_rows(t, rows, n, x_dtype, name) for t, n, name in
-               ((qkv, ch, "qkv"), (z, vw, "z"), (alpha, shape.value_heads, "alpha"), (beta, shape.value_heads, "beta"))]
-    if strides[2] != strides[3]:
+    qkv_stride, z_stride = _rows(qkv, rows, ch, x_dtype, "qkv"), _rows(z, rows, vw, x_dtype, "z")
+    ab_stride = _rows(alpha, rows, heads, x_dtype, "alpha")
+    if _rows(beta, rows, heads, x_dtype, "beta") != ab_stride:
         raise NmoeError(EINVAL, "alpha and beta must have the same row stride")
-    for t, n, name in ((weights["conv_w"], ch * 4, "conv_w"), (weights["A_log"], shape.value_heads, "A_log"),
-                       (weights["dt_bias"], shape.value_heads, "dt_bias"), (weights["norm_w"], 128, "norm_w")):
-        if t.dtype not in _dtypes()[DTYPE_F32 if name == "A_log" else DTYPE_BF16] or not t.is_contiguous() or t.numel() != n:
-            raise NmoeError(EINVAL, f"{name} must be a contiguous tensor of {n} elements ({'f32' if name == 'A_log' else 'bf16'})")
-    for t, n, name in ((conv_in, seqs * 3 * ch, "conv_in"), (conv_out, seqs * 3 * ch, "conv_out"),
-                       (delta_in, seqs * vw * 128, "delta_in"), (delta_out, seqs * vw * 128, "delta_out")):
-        _states(t, n, name)
+    bf16, f32 = _dtypes()[DTYPE_BF16], _dtypes()[DTYPE_F32]
+    for t, n, kinds in ((conv_w, ch * 4, bf16), (A_log, heads, f32), (dt_bias, heads, bf16), (norm_w, 128, bf16)):
+        if t.dtype not in kinds or t.numel() != n or not t.is_contiguous():
+            raise NmoeError(EINVAL, f"a weight must be a contiguous {kinds[0]} tensor of {n} elements")
+    _states(conv_in, seqs * 3 * ch, "conv_in")
+    _states(conv_out, seqs * 3 * ch, "conv_out")
+    _states(delta_in, seqs * vw * 128, "delta_in")
+    _states(delta_out, seqs * vw * 128, "delta_out")
     _output(out, rows * vw, out_dtype)
     _workspace(workspace, linear_attn_prefill_workspace_bytes(shape, seqs, rows))
-    w = LinearAttnWeights(_ptr(weights["conv_w"]), _ptr(weights["A_log"]), _ptr(weights["dt_bias"]),
-                          _ptr(weights["norm_w"]))
-    rc = lib().nmoe_linear_attn_prefill(C.byref(w), C.byref(shape), seqs, rows, _ptr(cu_rows), _ptr(qkv), strides[0],
-                                        _ptr(z), strides[1], _ptr(alpha), _ptr(beta), strides[2], x_dtype,
-                                        _ptr(conv_in), _ptr(delta_in), _ptr(conv_out), _ptr(delta_out), _ptr(out),
-                                        out_dtype, _ptr(workspace), stream)
+    w = LinearAttnWeights(conv_w.data_ptr(), A_log.data_ptr(), dt_bias.data_ptr(), norm_w.data_ptr())
+    rc = lib().nmoe_linear_attn_prefill(C.byref(w), C.byref(shape), seqs, rows, _ptr(cu_rows), _ptr(qkv), qkv_stride,
+                                        _ptr(z), z_stride, _ptr(alpha), _ptr(beta), ab_stride, x_dtype, _ptr(conv_in),
+                                        _ptr(delta_in), _ptr(conv_out), _ptr(delta_out), _ptr(out), out_dtype,
+                                        _ptr(workspace), stream)
     if rc != OK:
         raise NmoeError(rc, lib().nmoe_linear_attn_error().decode())
 
