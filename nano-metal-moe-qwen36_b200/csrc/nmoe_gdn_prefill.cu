@@ -8,17 +8,25 @@
 // M_ts = b_t e^{G_t-G_s} k_t . k_s (s < t). Then, with P_ts = e^{G_t-G_s} q_t . k_s (s <= t),
 //     O = e^G Q S^T + P U,   S' = e^{G_63} S + sum_t (e^{G_63-G_t} u_t) k_t^T
 //
-// Three launches. k_gdn_chunks, a CTA per (chunk, key head): convolution and norms of q and k, K K^T and
-// Q K^T, T b and P of its value heads; nothing here depends on the state. k_gdn_scan, a CTA per
-// (sequence, value head, 32 of the 128 value columns): the recurrence over the chunks; the columns of
-// the state never mix, so four CTAs a head share nothing. k_gdn_finish: gated norm and conv states.
+// Since P U = (P T b) (V - e^G K S^T), U and P U come out of one product.
 //
-// Arithmetic: products run on the warp tensor instructions (m16n8k16, fp16 operands, fp32 sums) with
-// every operand split into two fp16 parts, x = hi + lo (22 bits), and the three products hi hi, hi lo,
-// lo hi, so that states are as exact as with fp32 operands (1e-7 of their norm). fp16 has the range of
-// 2^40 only: k, q and P are scaled by constants, the state and U by a power of two that follows a bound
-// on them (|u| <= max |v| + |S|, |S'|^2 <= |S|^2 + sum v^2, row by row, since |k| <= 1 and b <= 1). What bounds it: on one sequence the scan's chain of three dependent products a chunk; on
-// many, the warp tensor rate (1024 products a cycle and SM).
+// Three launches. k_gdn_chunks, a CTA per (chunk, key head): convolution and norms of q and k, K K^T and
+// Q K^T, T b and P T b of its value heads; nothing here depends on the state. k_gdn_scan, a CTA per
+// (sequence, value head, 64 of the 128 value columns): the recurrence over the chunks; the columns of
+// the state never mix, so the CTAs of a head share nothing. k_gdn_finish: gated norm and conv states.
+//
+// Arithmetic: every product's operands are split into two fp16 parts, x = hi + lo (22 bits), and the
+// products hi hi, hi lo, lo hi summed in fp32, so that states are as exact as with fp32 operands (1e-7 of
+// their norm). fp16 has the range of 2^40 only: k, q and P are scaled by constants, the state and U by a
+// power of two that follows a bound on them (|u| <= max |v| + |S|, |S'|^2 <= |S|^2 + sum v^2, row by row,
+// since |k| <= 1 and b <= 1).
+//
+// The scan is a chain of three products a chunk, 128 rows high, on tcgen05: [K; Q] S^T (128 x 64 x 128),
+// [T b; P T b] R (128 x 64 x 64), K^T W (128 x 64 x 64), W = e^{G_63 - G} U; between them eight warps
+// read the sums from tensor memory, a thread per row and 32 columns, and write the next operand as rows
+// of 128 bytes, which the MMA takes as they are (MN-major). The warp tensor instructions needed the
+// fragments through registers, 3 KB of shared memory traffic a cycle's worth of products, and ran
+// 3.4 us a chunk for half the columns. What bounds it: the chain's latency.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -27,7 +35,7 @@
 #include <type_traits>
 
 #include "nmoe/moe_cuda.h"
-#include "nmoe_sm100.cuh"
+#include "nmoe_gemm.cuh"
 
 namespace nmoe {
 namespace {
@@ -43,15 +51,16 @@ int fail(int status, const char *fmt, ...) {
 }
 
 constexpr int kD = 128, kC = 64;      // head dim, tokens of a chunk
-constexpr int kSplit = 4, kN = kD / kSplit;   // value columns of a scan CTA: 32
+constexpr int kSplit = 2, kN = kD / kSplit;   // value columns of a scan CTA: 64
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kScanThreads = 512;
+constexpr int kScanThreads = 288;     // eight warps on the rows, one that copies and issues the MMAs
 constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about 1 / 11 and 1 / 128
 
-// Tile images, the same in the workspace and in shared memory: rows of fp16 in 16-byte pieces, piece
-// p of row r at p ^ (r & 7), so that an ldmatrix of 8 rows meets 8 bank groups.
-constexpr int kTileX = kC * kD * 2;   // K or Q, one part: 16 KB
-constexpr int kTileT = kC * kC * 2;   // T b or P, one part: 8 KB
+// Tile images, the same in the workspace and in shared memory: rows of 128 bytes (64 fp16) in 16-byte
+// pieces, piece p of row r at p ^ (r & 7): the MMA's 128-byte swizzle, and 8 bank groups for an ldmatrix.
+constexpr int kPanel = 128 * 128;     // 128 rows: K over Q, T b over P T b
+constexpr int kTileX = 2 * kPanel;    // K over Q, one part (hi or lo): two panels of 64 dims
+constexpr int kTileT = kPanel;        // T b over P T b, one part
 constexpr int kGates = 2 * kC * 4;    // e^{G_t}, e^{G_63 - G_t}
 
 struct GdnArgs {
@@ -64,7 +73,7 @@ struct GdnArgs {
     float *conv_out, *delta_out;
     void *out;
     int num_seqs, total_rows, key_heads, value_heads, channels, x_bf16, out_bf16;
-    // workspace, per chunk and head: K hi | K lo | Q hi | Q lo; T hi | T lo | P hi | P lo; gates; and O
+    // workspace, per chunk and head: K over Q, hi and lo; T b over P T b, hi and lo; gates; and O
     uint8_t *kq, *tp, *gates;
     float *o;
 };
@@ -105,41 +114,38 @@ __device__ __forceinline__ void stsm4(uint32_t addr, uint32_t a, uint32_t b, uin
     asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
 }
-__device__ __forceinline__ void stsm4t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
-                 "r"(d)
-                 : "memory");
-}
 __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-__device__ __forceinline__ void bar_arrive(int id, int threads) {
-    asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory");
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
 }
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // x / (1 + e^-x) with the hardware's exponential and reciprocal: a few 2^-23 of it
 __device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
-// byte offset of 16-byte piece p of row r: rows of 256, 128 and 64 bytes
-__device__ __forceinline__ uint32_t at256(int r, int p) { return r * 256 + ((p ^ (r & 7)) << 4); }
+// byte offset of 16-byte piece p of row r: in a 128-byte row; in two panels of 128 rows
 __device__ __forceinline__ uint32_t at128(int r, int p) { return r * 128 + ((p ^ (r & 7)) << 4); }
-__device__ __forceinline__ uint32_t at64(int r, int p) { return r * 64 + ((p ^ ((r >> 1) & 3)) << 4); }
+__device__ __forceinline__ uint32_t at_kq(int r, int p) { return (p >> 3) * kPanel + at128(r, p & 7); }
 
 // ---- chunks ---------------------------------------------------------------------------------------
 
 constexpr int kLd = 66;    // K K^T, Q K^T rows
 constexpr int kLdT = 68;   // T rows
 struct ChunkSmem {
-    static constexpr int kK = 0, kQ = 2 * kTileX;                       // hi, lo
-    static constexpr int kT = kQ;                                       // two heads' T over Q, once it is read
-    static constexpr int kQT = 2 * kC * kLdT * 4 > 2 * kTileX ? 2 * kC * kLdT * 4 : 2 * kTileX;
-    static constexpr int kKK = kQ + kQT, kQK = kKK + kC * kLd * 4;
-    static constexpr int kScratch = kQK + kC * kLd * 4;                 // 16 x 16 a warp
-    static constexpr int kBytes = kScratch + kWarps * 256 * 4;
+    // K over Q, hi and lo; then, over them, the two heads' T (fp32, later T b's hi and lo in its place) and P's
+    // (later P T b's) hi and lo
+    static constexpr int kT = 0, kTBytes = kC * kLdT * 4, kP = 2 * kTBytes, kPBytes = 2 * kC * 128;
+    static constexpr int kScratch = kP + 2 * kPBytes;            // 16 x 16 a warp
+    static constexpr int kKK = kScratch + kWarps * 256 * 4, kQK = kKK + kC * kLd * 4;
+    static constexpr int kBytes = kQK + kC * kLd * 4;
+    static_assert(2 * kTileX <= kScratch, "K and Q end before what is used beside them");
 };
 
-template <bool kBf16, bool kFull>
+template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constant__ GdnArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(16) float2 G[2][kC];
@@ -255,7 +261,6 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 }
             }
             const float scale = side ? kScaleK * 0.08838834764831845f : kScaleQ / kD;
-            uint8_t *tile = smem + (side ? ChunkSmem::kK : ChunkSmem::kQ);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int t = t0 + i;
@@ -269,34 +274,34 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 }
                 const float inv = rsqrtf(warp_sum(ss) / kD + 1e-12f) * scale;
                 uint32_t h0, l0, h1, l1;
-                const uint32_t at = at256(t, lane >> 1) + (lane & 1) * 8;
+                const uint32_t at = at_kq(side ? t : kC + t, lane >> 1) + (lane & 1) * 8;
                 split2(y[0] * inv, y[1] * inv, h0, l0);
                 split2(y[2] * inv, y[3] * inv, h1, l1);
-                *reinterpret_cast<uint2 *>(tile + at) = make_uint2(h0, h1);
-                *reinterpret_cast<uint2 *>(tile + kTileX + at) = make_uint2(l0, l1);
+                *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h0, h1);
+                *reinterpret_cast<uint2 *>(smem + kTileX + at) = make_uint2(l0, l1);
             }
         }
     }
     __syncthreads();
     {   // the tile images into the workspace
-        uint4 *dst = reinterpret_cast<uint4 *>(a.kq + ((long long)chunk * a.key_heads + kh) * 4 * kTileX);
-        constexpr int kParts = kFull ? 4 : 3;   // Q lo only where it is read
-        for (int i = tid; i < kParts * kTileX / 16; i += kThreads) dst[i] = reinterpret_cast<const uint4 *>(smem)[i];
+        uint4 *dst = reinterpret_cast<uint4 *>(a.kq + ((long long)chunk * a.key_heads + kh) * 2 * kTileX);
+#pragma unroll 4
+        for (int i = tid; i < 2 * kTileX / 16; i += kThreads) dst[i] = reinterpret_cast<const uint4 *>(smem)[i];
     }
     // ---- K K^T and Q K^T, the 16 x 16 blocks on and below the diagonal: 20 of them over the warps
     for (int u = warp; u < 20; u += kWarps) {
         const int v = u % 10, i = v < 1 ? 0 : v < 3 ? 1 : v < 6 ? 2 : 3, j = v - i * (i + 1) / 2;
-        const uint32_t ka = sm + (u < 10 ? ChunkSmem::kK : ChunkSmem::kQ), kb = sm + ChunkSmem::kK;
+        const int ra = u < 10 ? 0 : kC;   // K's rows, or Q's
         float c[2][4] = {};
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk) {
             uint32_t ah[4], al[4], bh[4], bl[4];
-            const uint32_t pa = at256(16 * i + (lane & 15), 2 * kk + (lane >> 4));
-            const uint32_t pb = at256(16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1));
-            ldsm4(ka + pa, ah);
-            ldsm4(ka + kTileX + pa, al);
-            ldsm4(kb + pb, bh);
-            ldsm4(kb + kTileX + pb, bl);
+            const uint32_t pa = at_kq(ra + 16 * i + (lane & 15), 2 * kk + (lane >> 4));
+            const uint32_t pb = at_kq(16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1));
+            ldsm4(sm + pa, ah);
+            ldsm4(sm + kTileX + pa, al);
+            ldsm4(sm + pb, bh);
+            ldsm4(sm + kTileX + pb, bl);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 mma_f16(c[x], al, bh[2 * x], bh[2 * x + 1]);
@@ -321,18 +326,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     for (int v0 = 0; v0 < ratio; v0 += 2) {
         const bool on = v0 + half < ratio;
         const int vh = kh * ratio + v0 + half;
-        float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT) + half * kC * kLdT;
+        float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT + half * ChunkSmem::kTBytes);
+        uint8_t *P = smem + ChunkSmem::kP + half * ChunkSmem::kPBytes;
         float *scratch = reinterpret_cast<float *>(smem + ChunkSmem::kScratch) + warp * 256;
         if (v0 > 0) gates_of(v0);
-        __syncthreads();   // also: K K^T, Q K^T are complete, and Q is read
+        __syncthreads();   // also: K K^T, Q K^T are complete, and K and Q are read
         if (on) {
             float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
             if (t128 < kC) {
                 gates[t128] = expf(G[half][t128].x + G[half][t128].y);
                 gates[kC + t128] = expf(diff(kC - 1, t128));
             }
-            // M below the diagonal; P with its diagonal, straight into its tile
-            uint8_t *P = a.tp + (((long long)chunk * a.value_heads + vh) * 4 + 2) * kTileT;
+            // M below the diagonal; P with its diagonal
             for (int i = t128; i < kC * kC / 8; i += 128) {
                 const int t = i >> 3, s0 = (i & 7) * 8;
                 float p[8], m[8];
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
 #pragma unroll
                 for (int j = 0; j < 4; ++j) split2(p[2 * j], p[2 * j + 1], h[j], l[j]);
                 *reinterpret_cast<uint4 *>(P + at128(t, i & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-                if (kFull) *reinterpret_cast<uint4 *>(P + kTileT + at128(t, i & 7)) = make_uint4(l[0], l[1], l[2], l[3]);
+                *reinterpret_cast<uint4 *>(P + kC * 128 + at128(t, i & 7)) = make_uint4(l[0], l[1], l[2], l[3]);
             }
         }
         __syncthreads();
@@ -411,18 +416,72 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             }
             __syncthreads();
         }
-        if (on) {   // T b
-            uint8_t *to = a.tp + ((long long)chunk * a.value_heads + vh) * 4 * kTileT;
-            for (int i = t128; i < kC * kC / 8; i += 128) {
-                const int t = i >> 3, s0 = (i & 7) * 8;
-                uint32_t h[4], l[4];
+        // T b, in T's place: a thread holds four 16-byte pieces of it
+        uint32_t th[4][4], tl[4][4];
+        if (on)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int i = t128 + 128 * x, t = i >> 3, s0 = (i & 7) * 8;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int s = s0 + 2 * j;
-                    split2(T[t * kLdT + s] * beta[half][s], T[t * kLdT + s + 1] * beta[half][s + 1], h[j], l[j]);
+                    split2(T[t * kLdT + s] * beta[half][s], T[t * kLdT + s + 1] * beta[half][s + 1], th[x][j], tl[x][j]);
                 }
-                *reinterpret_cast<uint4 *>(to + at128(t, i & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(to + kTileT + at128(t, i & 7)) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+        __syncthreads();
+        uint8_t *TB = reinterpret_cast<uint8_t *>(T);
+        if (on)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int i = t128 + 128 * x, at = at128(i >> 3, i & 7);
+                *reinterpret_cast<uint4 *>(TB + at) = make_uint4(th[x][0], th[x][1], th[x][2], th[x][3]);
+                *reinterpret_cast<uint4 *>(TB + kC * 128 + at) = make_uint4(tl[x][0], tl[x][1], tl[x][2], tl[x][3]);
+            }
+        __syncthreads();
+        // P T b: 16 rows a warp, the columns in pairs of 8; lower triangular as both are
+        float c[4][2][4] = {};
+        if (on)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int k = j; k < 4; ++k)
+                    if (k <= q4) {
+                        uint32_t ah[4], al[4], bh[4], bl[4];
+                        const uint32_t pa = smem_u32(P) + at128(16 * q4 + (lane & 15), 2 * k + (lane >> 4));
+                        const uint32_t pb = smem_u32(TB) + at128(16 * k + (lane & 15), 2 * j + (lane >> 4));
+                        ldsm4(pa, ah);
+                        ldsm4(pa + kC * 128, al);
+                        ldsm4t(pb, bh);
+                        ldsm4t(pb + kC * 128, bl);
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            mma_f16(c[j][x], al, bh[2 * x], bh[2 * x + 1]);
+                            mma_f16(c[j][x], ah, bl[2 * x], bl[2 * x + 1]);
+                            mma_f16(c[j][x], ah, bh[2 * x], bh[2 * x + 1]);
+                        }
+                    }
+        __syncwarp();   // a warp reads and writes its own rows of P
+        if (on)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    split2(c[j][x][0], c[j][x][1], h[2 * x], l[2 * x]);
+                    split2(c[j][x][2], c[j][x][3], h[2 * x + 1], l[2 * x + 1]);
+                }
+                const uint32_t at = smem_u32(P) + at128(16 * q4 + (lane & 15), 2 * j + (lane >> 4));
+                stsm4(at, h[0], h[1], h[2], h[3]);
+                stsm4(at + kC * 128, l[0], l[1], l[2], l[3]);
+            }
+        __syncthreads();
+        if (on) {
+            uint4 *to = reinterpret_cast<uint4 *>(a.tp + ((long long)chunk * a.value_heads + vh) * 2 * kTileT);
+            constexpr int kHalf = kC * 128 / 16;   // 16-byte pieces of 64 rows: T b hi, P T b hi, T b lo, P T b lo
+#pragma unroll 4
+            for (int i = t128; i < 4 * kHalf; i += 128) {
+                const int part = i / kHalf, x = i - part * kHalf;
+                to[i] = reinterpret_cast<const uint4 *>((part & 1 ? P : TB) + (part >> 1) * kC * 128)[x];
             }
         }
         __syncthreads();
@@ -431,17 +490,56 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
 
 // ---- scan -------------------------------------------------------------------------------------------
 
-template <bool kFull>
 struct ScanSmem {
-    static constexpr int kQParts = kFull ? 2 : 1;
-    static constexpr int kStage = (2 + kQParts) * kTileX + 2 * kTileT + kGates;   // K hi, lo, Q, T hi, lo, gates
-    static constexpr int kT = (2 + kQParts) * kTileX, kGate = kT + 2 * kTileT;
-    static constexpr int kP = 2 * kStage, kS = kP + kQParts * kTileT;             // P of the current chunk; S hi, lo
-    static constexpr int kV = kS + 2 * kN * kD * 2, kR = kV + kC * kN * 4;        // V fp32; R hi, lo
-    static constexpr int kU = kR + 2 * kC * kN * 2, kW = kU + 2 * kC * kN * 2;    // U, e^{G_63 - G} U: hi, lo
-    static constexpr int kBytes = kW + 2 * kC * kN * 2;
-    static constexpr int kTileU = kC * kN * 2;
+    static constexpr int kStage = 2 * kTileX;                       // K over Q of a chunk, hi and lo; two of them
+    static constexpr int kTP = 2 * kStage;                          // T b over P T b, hi and lo
+    static constexpr int kS = kTP + 2 * kTileT, kTileS = kD * 128;  // the state: [dim][64 columns], hi and lo
+    static constexpr int kR = kS + 2 * kTileS, kTileR = kC * 128;   // R, then W: [token][64 columns], hi and lo
+    static constexpr int kV = kR + 2 * kTileR;                      // V: [token][64 columns] fp32
+    static constexpr int kGate = kV + kC * kN * 4;                  // gates of two chunks
+    static constexpr int kBytes = kGate + 2 * kGates;
 };
+
+struct ScanShared {
+    uint64_t kq_full[2], tp_full, d[3], r_ready, w_ready, s_ready;
+    int vmax[3], first_chunk, stop;
+    uint32_t tmem;
+};
+
+// One thread of a converged warp issues (`one` != 0): M = 128, N = 64, fp16, fp32 sums.
+__device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t *bar, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t idesc_f16(int a_mn, int b_mn) {
+    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(kN >> 3) << 17) | (8u << 24);
+}
+// rows are the sum's index, 64 columns a row; further columns `panel` bytes away
+__device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t panel) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Bounded: a barrier that never completes sets `stop`, and every later wait goes at once.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
+    for (uint32_t n = 0; !mbar_try_wait_sleep(bar, parity, 20000u); ++n) {
+        if (*stop) return false;
+        if (n >= (1u << 16)) {
+            *stop = 1;
+            return false;
+        }
+    }
+    return true;
+}
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 // The scale 2^-e for values whose square is at most `square`: they come below 2^13, so that fp16 holds
@@ -451,331 +549,294 @@ __device__ __forceinline__ int exponent_of(float square) {
     return min(100, max(-100, e));
 }
 
-// Eight warps carry the recurrence (K S^T, U, the new state); eight others work beside them on what it
-// does not wait for (Q S^T, P U and the output, and the values of the next chunk). Named barriers:
-//   1  the first eight among themselves
-//   2  U of the chunk is stored        (the first eight arrive, the others wait)
-//   3  the others are done with the chunk's state and U, and the next values are stored
-//   4  the next state is stored
-template <bool kBf16, bool kFull>
+// Threads 0-255: row r = 32 (warp % 4) + lane of the 128, columns 32 (warp / 4) .. + 31 of the CTA's 64.
+// Rows 0-63 are tokens (K's rows: R and W), rows 64-127 are tokens too (Q's rows: the output, and V of the
+// next chunk), and all of them are dims of the state. Warp 8 copies and issues the MMAs.
+template <bool kBf16>
 __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
-    using L = ScanSmem<kFull>;
-    extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint64_t full[2], p_full;
-    __shared__ int vmax[2], first_chunk;
-    const int tid = threadIdx.x, warp = (tid >> 5) & 7, lane = tid & 31;
-    const bool chain = tid < kScanThreads / 2;
+    using L = ScanSmem;
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ ScanShared S;
+    uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, vh = blockIdx.y, b = blockIdx.z, kh = vh / (a.value_heads / a.key_heads);
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
-        mbar_init(&full[0], 1);
-        mbar_init(&full[1], 1);
-        mbar_init(&p_full, 1);
+        for (int i = 0; i < 2; ++i) mbar_init(&S.kq_full[i], 1);
+        for (int i = 0; i < 3; ++i) mbar_init(&S.d[i], 1), S.vmax[i] = 0;
+        mbar_init(&S.tp_full, 1);
+        mbar_init(&S.r_ready, 4);   // the warps of rows 0-63
+        mbar_init(&S.w_ready, 4);
+        mbar_init(&S.s_ready, 8);
         mbar_fence_init();
-        vmax[0] = vmax[1] = 0;
-        first_chunk = 0;
+        S.first_chunk = S.stop = 0;
     }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&S.tmem)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = S.tmem;
     {
         int before = 0;
         for (int i = tid; i < b; i += kScanThreads) before += seq_chunks(a, i);
-        if (before) atomicAdd(&first_chunk, before);   // integers: the order does not matter
+        if (before) atomicAdd(&S.first_chunk, before);   // integers: the order does not matter
     }
     const int row0 = seq_first(a, b), rows = seq_rows(a, b), chunks = (rows + kC - 1) / kC;
-    const int col = 2 * (lane & 3);
+    const int wg = warp >> 2, r = 32 * (warp & 3) + lane, c0 = 32 * wg;
+    const bool is_q = warp < 8 && (warp & 3) >= 2;
 
-    // ---- the state (the first eight warps): S^T, rows (dims) 16 warp + lane / 4 (+ 8), columns 8 j + col (+ 1)
-    float S[4][4];
-    const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN) * kD;
-    const int dim = 16 * warp + (lane >> 2);
-    if (chain) {
+    // ---- the state: dim r, columns c0 .. c0 + 31
+    float St[32];
+    const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN + c0) * kD + r;
+    if (warp < 8) {
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                S[j][e] = a.delta_in ? a.delta_in[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] : 0.f;
-                m = fmaxf(m, fabsf(S[j][e]));
-            }
+        for (int j = 0; j < 32; ++j) {
+            St[j] = a.delta_in ? a.delta_in[s_at + (long long)j * kD] : 0.f;
+            m = fmaxf(m, fabsf(St[j]));
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) atomicMax(&vmax[1], __float_as_int(m));   // not negative: ordered as integers
+        if (lane == 0) atomicMax(&S.vmax[2], __float_as_int(m));   // not negative: ordered as integers
     }
     __syncthreads();
-    const long long chunk0 = first_chunk;
-    float bound2 = __int_as_float(vmax[1]);   // of |S|^2, per value row
+    const long long chunk0 = S.first_chunk;
+    float bound2 = __int_as_float(S.vmax[2]);   // of |S|^2, per value row
     bound2 = bound2 * bound2 * kD;
     __syncthreads();
-    if (tid == 0) vmax[1] = 0;
+    if (tid == 0) S.vmax[2] = 0;
 
-    // S, scaled, as the B operand of the next chunk: [column][dim]
-    auto store_state = [&](int e) {
-        const float s = pow2(-e);
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            uint32_t h[4], l[4];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                split2(S[j + x][0] * s, S[j + x][1] * s, h[2 * x], l[2 * x]);
-                split2(S[j + x][2] * s, S[j + x][3] * s, h[2 * x + 1], l[2 * x + 1]);
-            }
-            const uint32_t at = sm + L::kS + at256(8 * (j + (lane >> 4)) + (lane & 7), 2 * warp + ((lane >> 3) & 1));
-            stsm4t(at, h[0], h[1], h[2], h[3]);
-            stsm4t(at + kN * kD * 2, l[0], l[1], l[2], l[3]);
-        }
-    };
-    // ---- copies: K, Q, T and the gates of chunk c into stage c % 2; P of chunk c
-    auto copy_stage = [&](int c) {
-        uint8_t *st = smem + (c & 1) * L::kStage;
-        const uint8_t *kq = a.kq + ((chunk0 + c) * a.key_heads + kh) * 4 * kTileX;
-        const uint8_t *tp = a.tp + ((chunk0 + c) * a.value_heads + vh) * 4 * kTileT;
+    if (warp == 8) {
+        // ---- copies and MMAs; every value is the same in all lanes
+        const uint32_t one = elect_lane();
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int n = __shfl_sync(0xffffffffu, chunks, 0);
         const uint64_t keep = policy_evict_normal();
-        mbar_arrive_expect_tx(&full[c & 1], L::kStage);
-        bulk_g2s(st, kq, (2 + L::kQParts) * kTileX, &full[c & 1], keep);
-        bulk_g2s(st + L::kT, tp, 2 * kTileT, &full[c & 1], keep);
-        bulk_g2s(st + L::kGate, a.gates + ((chunk0 + c) * a.value_heads + vh) * kGates, kGates, &full[c & 1], keep);
-    };
-    auto copy_p = [&](int c) {
-        const uint8_t *tp = a.tp + (((chunk0 + c) * a.value_heads + vh) * 4 + 2) * kTileT;
-        mbar_arrive_expect_tx(&p_full, L::kQParts * kTileT);
-        bulk_g2s(smem + L::kP, tp, L::kQParts * kTileT, &p_full, policy_evict_normal());
-    };
-    // ---- V (the other eight warps): channel `lane`, tokens 8 warp .. + 7 of a chunk; the inputs are loaded a
-    // chunk ahead, and stay as they are until they are used (a conversion would wait for them)
-    using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
-    constexpr int kTok = kC / 8;
-    const int ch = (2 * a.key_heads + vh) * kD + split * kN + lane;
-    const uint2 cw = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * ch);
-    Raw raw[kTok + 3];
-    float before[3] = {0.f, 0.f, 0.f};   // the inputs before the sequence, for its first tokens
-    if (!chain && warp == 0 && a.conv_in != nullptr)
-#pragma unroll
-        for (int i = 0; i < 3; ++i) before[i] = a.conv_in[((long long)b * 3 + i) * a.channels + ch];
-    const Raw *raw_at = static_cast<const Raw *>(a.qkv) + (long long)(row0 + kTok * warp - 3) * a.qkv_stride + ch;
-    auto load_raw = [&](int c) {
-        const Raw *p = raw_at + (long long)c * kC * a.qkv_stride;
-        const int r = c * kC + kTok * warp - 3;
-#pragma unroll
-        for (int i = 0; i < kTok + 3; ++i, p += a.qkv_stride) raw[i] = r + i >= 0 && r + i < rows ? *p : Raw(0);
-    };
-    auto v_at = [&](int t, int x) {
-        return reinterpret_cast<float *>(smem + L::kV) + t * kN + (((x >> 3) ^ (t & 3)) << 3) + (x & 7);
-    };
-    auto store_values = [&](int c) {
-        float x[kTok + 3], m = 0.f;
-#pragma unroll
-        for (int i = 0; i < kTok + 3; ++i) {
-            if constexpr (kBf16)
-                x[i] = bf16_to_f32(raw[i]);
-            else
-                x[i] = raw[i];
-            if (i < 3 && c == 0 && warp == 0) x[i] = before[i];
+        auto copy_kq = [&](int c) {
+            if (!one) return;
+            uint64_t *bar = &S.kq_full[c & 1];
+            mbar_arrive_expect_tx(bar, L::kStage + kGates);
+            bulk_g2s(smem + (c & 1) * L::kStage, a.kq + ((chunk0 + c) * a.key_heads + kh) * 2 * kTileX, L::kStage, bar, keep);
+            bulk_g2s(smem + L::kGate + (c & 1) * kGates, a.gates + ((chunk0 + c) * a.value_heads + vh) * kGates, kGates, bar, keep);
+        };
+        auto copy_tp = [&](int c) {
+            if (!one) return;
+            mbar_arrive_expect_tx(&S.tp_full, 2 * kTileT);
+            bulk_g2s(smem + L::kTP, a.tp + ((chunk0 + c) * a.value_heads + vh) * 2 * kTileT, 2 * kTileT, &S.tp_full, keep);
+        };
+        auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop)); };
+        if (n > 0) {
+            copy_kq(0);
+            copy_tp(0);
+            if (n > 1) copy_kq(1);
         }
+        for (int c = 0; c < n; ++c) {
+            const uint32_t st = sm + (c & 1) * L::kStage;
+            if (!wait(&S.kq_full[c & 1], (c >> 1) & 1) || !wait(&S.s_ready, c & 1)) break;
+            tc_fence_after();
+            // the state of chunk c is stored, so K^T W of chunk c - 1, the last that read its stage, is complete
+            if (c > 0 && c + 1 < n) copy_kq(c + 1);
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-            const int t = kTok * warp + i;
-            const float s = x[i] * bf16_lo(cw.x) + x[i + 1] * bf16_hi(cw.x) + x[i + 2] * bf16_lo(cw.y) + x[i + 3] * bf16_hi(cw.y);
-            const float v = c * kC + t < rows ? silu_fast(s) : 0.f;
-            *v_at(t, lane) = v;
-            m = fmaxf(m, fabsf(v));
+            for (int pass = 0; pass < 3; ++pass)   // lo hi, hi lo, hi hi
+#pragma unroll
+                for (int k = 0; k < kD / 16; ++k)
+                    mma_one(tm, sw128_desc(st + (pass == 0 ? kTileX : 0) + (k >> 2) * kPanel + (k & 3) * 32),
+                            desc_rows(sm + L::kS + (pass == 1 ? L::kTileS : 0) + k * 2048, 0), idesc_f16(0, 1),
+                            pass + k > 0 ? 1u : 0u, one);
+            commit_one(&S.d[0], one);
+            if (!wait(&S.tp_full, c & 1) || !wait(&S.r_ready, c & 1)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int pass = 0; pass < 3; ++pass)
+#pragma unroll
+                for (int k = 0; k < kC / 16; ++k)
+                    mma_one(tm + kN, sw128_desc(sm + L::kTP + (pass == 0 ? kTileT : 0) + k * 32),
+                            desc_rows(sm + L::kR + (pass == 1 ? L::kTileR : 0) + k * 2048, 0), idesc_f16(0, 1),
+                            pass + k > 0 ? 1u : 0u, one);
+            commit_one(&S.d[1], one);
+            if (!wait(&S.w_ready, c & 1)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int pass = 0; pass < 3; ++pass)
+#pragma unroll
+                for (int k = 0; k < kC / 16; ++k)
+                    mma_one(tm + 2 * kN, desc_rows(st + (pass == 0 ? kTileX : 0) + k * 2048, kPanel),
+                            desc_rows(sm + L::kR + (pass == 1 ? L::kTileR : 0) + k * 2048, 0), idesc_f16(1, 1),
+                            pass + k > 0 ? 1u : 0u, one);
+            commit_one(&S.d[2], one);
+            if (c + 1 < n) copy_tp(c + 1);   // W is stored, so the product with T b is complete
         }
+    } else {
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        // 32 columns of row `row` of an operand image, hi and lo `part` bytes apart
+        auto store_row = [&](uint32_t image, int part, int row, const float *v) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) atomicMax(&vmax[c & 1], __float_as_int(m));
-    };
-
-    bool ok = true;
-    int es = exponent_of(bound2);
-    if (chunks > 0) {
-        if (tid == 0) copy_stage(0);
-        if (chain) {
-            store_state(es);
-        } else {
-            load_raw(0);
-            store_values(0);   // vmax[0]
-            if (chunks > 1) load_raw(1);
-        }
-        __syncthreads();
-    }
-    const int mt = warp & 3, nh = warp >> 2;   // 16 tokens, 16 columns
-    const int t0 = 16 * mt + (lane >> 2);      // this lane's tokens t0, t0 + 8
-    for (int c = 0; c < chunks; ++c) {
-        const float vm = __int_as_float(vmax[c & 1]);
-        bound2 += kC * vm * vm;   // of the states of this chunk, and of the one it leaves
-        const int eu = exponent_of(bound2) + 1;   // max |v| + |S| <= 9/8 sqrt(bound2)
-        const uint32_t st = sm + (c & 1) * L::kStage;
-        const float *eg = reinterpret_cast<const float *>(smem + (c & 1) * L::kStage + L::kGate), *el = eg + kC;
-        if (tid == kScanThreads / 2) {
-            copy_p(c);
-            if (c + 1 < chunks) copy_stage(c + 1);
-        }
-        ok &= mbar_wait_spin(&full[c & 1], (c >> 1) & 1);
-        // K S^T, or Q S^T
-        float acc[2][4] = {};
-        {
-            const uint32_t A = st + (chain ? 0 : 2 * kTileX), B = sm + L::kS;
-            const bool exact = kFull || chain;
-#pragma unroll
-            for (int kk = 0; kk < kD / 16; ++kk) {
-                uint32_t ah[4], al[4], bh[4], bl[4];
-                const uint32_t pa = at256(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
-                const uint32_t pb = at256(16 * nh + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1));
-                ldsm4(A + pa, ah);
-                ldsm4(B + pb, bh);
-                if (exact) {
-                    ldsm4(A + kTileX + pa, al);
-                    ldsm4(B + kN * kD * 2 + pb, bl);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) mma_f16(acc[j], al, bh[2 * j], bh[2 * j + 1]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bl[2 * j], bl[2 * j + 1]);
-                }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bh[2 * j], bh[2 * j + 1]);
-            }
-        }
-        const float g0 = eg[t0], g1 = eg[t0 + 8];
-        if (chain) {
-            {   // R = V - e^G K S^T, scaled
-                const float s = pow2(-eu), k0 = g0 * pow2(es) * (1.f / kScaleK), k1 = g1 * pow2(es) * (1.f / kScaleK);
+            for (int x = 0; x < 4; ++x) {
                 uint32_t h[4], l[4];
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const float2 v0 = *reinterpret_cast<const float2 *>(v_at(t0, 16 * nh + 8 * x + col));
-                    const float2 v1 = *reinterpret_cast<const float2 *>(v_at(t0 + 8, 16 * nh + 8 * x + col));
-                    split2((v0.x - k0 * acc[x][0]) * s, (v0.y - k0 * acc[x][1]) * s, h[2 * x], l[2 * x]);
-                    split2((v1.x - k1 * acc[x][2]) * s, (v1.y - k1 * acc[x][3]) * s, h[2 * x + 1], l[2 * x + 1]);
-                }
-                const uint32_t at = sm + L::kR + at64(16 * mt + (lane & 15), 2 * nh + (lane >> 4));
-                stsm4(at, h[0], h[1], h[2], h[3]);
-                stsm4(at + L::kTileU, l[0], l[1], l[2], l[3]);
+                for (int y = 0; y < 4; ++y) split2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
+                uint8_t *to = smem + image + at128(row, 4 * wg + x);
+                *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(to + part) = make_uint4(l[0], l[1], l[2], l[3]);
             }
-            bar_sync(1, 256);
-            {   // U = T b R: 16 tokens x 16 columns a warp, a long row beside a short one on each scheduler
-                const int i = nh ? 3 - mt : mt;
-                float u[2][4] = {}, v[2][4] = {};
+        };
+        auto signal = [&](uint64_t *bar) {   // this warp's operand rows are written, and its sums are read
+            fence_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto read_sums = [&](int which, float *v) {
+            tc_ld32(tmem + lanes + which * kN + c0, reinterpret_cast<uint32_t *>(v));
+            tc_wait_ld();
+        };
+        auto store_state = [&](int e) {
+            const float s = pow2(-e);
+            float v[32];
 #pragma unroll
-                for (int kk = 0; kk < kC / 16; ++kk) {
-                    if (kk <= i) {
-                        uint32_t ah[4], al[4], bh[4], bl[4];
-                        const uint32_t pa = at128(16 * i + (lane & 15), 2 * kk + (lane >> 4));
-                        const uint32_t pb = at64(16 * kk + (lane & 15), 2 * nh + (lane >> 4));
-                        ldsm4(st + L::kT + pa, ah);
-                        ldsm4t(sm + L::kR + pb, bh);
-                        ldsm4(st + L::kT + kTileT + pa, al);
-                        ldsm4t(sm + L::kR + L::kTileU + pb, bl);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) mma_f16(u[x], ah, bh[2 * x], bh[2 * x + 1]);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) mma_f16(v[x], al, bh[2 * x], bh[2 * x + 1]);
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) mma_f16(v[x], ah, bl[2 * x], bl[2 * x + 1]);
-                    }
-                }
-                const int t = 16 * i + (lane >> 2);
-                const float e0 = el[t], e1 = el[t + 8];
-                uint32_t h[4], l[4], wh[4], wl[4];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) u[x][e] += v[x][e];
-                    split2(u[x][0], u[x][1], h[2 * x], l[2 * x]);
-                    split2(u[x][2], u[x][3], h[2 * x + 1], l[2 * x + 1]);
-                    split2(u[x][0] * e0, u[x][1] * e0, wh[2 * x], wl[2 * x]);
-                    split2(u[x][2] * e1, u[x][3] * e1, wh[2 * x + 1], wl[2 * x + 1]);
-                }
-                const uint32_t at = at64(16 * i + (lane & 15), 2 * nh + (lane >> 4));
-                stsm4(sm + L::kW + at, wh[0], wh[1], wh[2], wh[3]);
-                stsm4(sm + L::kW + L::kTileU + at, wl[0], wl[1], wl[2], wl[3]);
-                stsm4(sm + L::kU + at, h[0], h[1], h[2], h[3]);
-                if (kFull) stsm4(sm + L::kU + L::kTileU + at, l[0], l[1], l[2], l[3]);
-            }
-            bar_arrive(2, 512);
-            bar_sync(1, 256);
-            // S' = e^{G_63} S + K^T (e^{G_63 - G} U), 16 dims and all columns a warp
-            float up[4][4] = {};
-#pragma unroll
-            for (int kk = 0; kk < kC / 16; ++kk) {
-                uint32_t ah[4], al[4], bh[2][4], bl[2][4];
-                const uint32_t pa = at256(16 * kk + (lane & 7) + ((lane >> 4) << 3), 2 * warp + ((lane >> 3) & 1));
-                ldsm4t(st + pa, ah);
-#pragma unroll
-                for (int p = 0; p < 2; ++p) ldsm4t(sm + L::kW + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bh[p]);
-                ldsm4t(st + kTileX + pa, al);
-#pragma unroll
-                for (int p = 0; p < 2; ++p)
-                    ldsm4t(sm + L::kW + L::kTileU + at64(16 * kk + (lane & 15), 2 * p + (lane >> 4)), bl[p]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(up[j], al, bh[j >> 1][2 * (j & 1)], bh[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) mma_f16(up[j], ah, bl[j >> 1][2 * (j & 1)], bl[j >> 1][2 * (j & 1) + 1]);
-            }
-            const float keep = eg[kC - 1], add = pow2(eu) * (1.f / kScaleK);
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) S[j][e] = fmaf(S[j][e], keep, up[j][e] * add);
-            es = exponent_of(bound2);
-            bar_sync(3, 512);
-            if (tid == 0) vmax[c & 1] = 0;   // read by all; next added to in the next chunk
-            if (c + 1 < chunks) store_state(es);
-            bar_sync(4, 512);
-        } else {
-            {   // e^G Q S^T on the scale of P U
-                const float k0 = g0 * pow2(es) * pow2(-eu), k1 = g1 * pow2(es) * pow2(-eu);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[j][0] *= k0, acc[j][1] *= k0, acc[j][2] *= k1, acc[j][3] *= k1;
-            }
-            es = exponent_of(bound2);
-            ok &= mbar_wait_spin(&p_full, c & 1);
-            bar_sync(2, 512);
-#pragma unroll
-            for (int kk = 0; kk < kC / 16; ++kk) {
-                if (kk <= mt) {
-                    uint32_t ah[4], al[4], bh[4], bl[4];
-                    const uint32_t pa = at128(16 * mt + (lane & 15), 2 * kk + (lane >> 4));
-                    const uint32_t pb = at64(16 * kk + (lane & 15), 2 * nh + (lane >> 4));
-                    ldsm4(sm + L::kP + pa, ah);
-                    ldsm4t(sm + L::kU + pb, bh);
-                    if (kFull) {
-                        ldsm4(sm + L::kP + kTileT + pa, al);
-                        ldsm4t(sm + L::kU + L::kTileU + pb, bl);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) mma_f16(acc[j], al, bh[2 * j], bh[2 * j + 1]);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bl[2 * j], bl[2 * j + 1]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) mma_f16(acc[j], ah, bh[2 * j], bh[2 * j + 1]);
-                }
-            }
-            if (c + 1 < chunks) store_values(c + 1);   // over this chunk's, which U is made of
-            bar_arrive(3, 512);
-            if (c + 2 < chunks) load_raw(c + 2);
-            const float s = pow2(eu) * (1.f / kScaleQ);
-            const int r = c * kC + t0;
-            float *o = a.o + ((long long)(row0 + r) * a.value_heads + vh) * kD + split * kN + 16 * nh + col;
-            const long long step = 8ll * a.value_heads * kD;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                if (r < rows) *reinterpret_cast<float2 *>(o + 8 * j) = make_float2(acc[j][0] * s, acc[j][1] * s);
-                if (r + 8 < rows) *reinterpret_cast<float2 *>(o + step + 8 * j) = make_float2(acc[j][2] * s, acc[j][3] * s);
-            }
-            bar_sync(4, 512);
+            for (int j = 0; j < 32; ++j) v[j] = St[j] * s;
+            store_row(L::kS, L::kTileS, r, v);
+            signal(&S.s_ready);
+        };
+        // V of a chunk, by the warps of rows 64-127: a lane two of the warp's 32 channels and 16 tokens (lanes
+        // 0-15 the first 16 of the warp's 32, lanes 16-31 the others). The inputs are loaded a chunk ahead and
+        // stay as they are until they are used (a conversion would wait for them).
+        using Raw2 = typename std::conditional<kBf16, uint32_t, float2>::type;
+        using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
+        const int vt = 32 * ((warp & 3) - 2) + 16 * (lane >> 4), vc = c0 + 2 * (lane & 15);   // first token, channel
+        const int ch = (2 * a.key_heads + vh) * kD + split * kN + vc;
+        Raw2 raw[19];
+        float w0[4], w1[4];
+        if (is_q) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * ch);
+            const uint2 v = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ch + 1));
+            w0[0] = bf16_lo(u.x), w0[1] = bf16_hi(u.x), w0[2] = bf16_lo(u.y), w0[3] = bf16_hi(u.y);
+            w1[0] = bf16_lo(v.x), w1[1] = bf16_hi(v.x), w1[2] = bf16_lo(v.y), w1[3] = bf16_hi(v.y);
         }
+        auto load_raw = [&](int c) {   // rows beyond the sequence's ends are asked for at its ends
+            const Raw *p = static_cast<const Raw *>(a.qkv) + ch;
+#pragma unroll
+            for (int i = 0; i < 19; ++i) {
+                const int x = min(max(c * kC + vt + i - 3, 0), rows - 1);
+                raw[i] = *reinterpret_cast<const Raw2 *>(p + (long long)(row0 + x) * a.qkv_stride);
+            }
+        };
+        auto store_values = [&](int c) {
+            float x0[19], x1[19], m = 0.f;
+#pragma unroll
+            for (int i = 0; i < 19; ++i) {
+                if constexpr (kBf16)
+                    x0[i] = bf16_lo(raw[i]), x1[i] = bf16_hi(raw[i]);
+                else
+                    x0[i] = raw[i].x, x1[i] = raw[i].y;
+            }
+            if (c == 0 && vt == 0)   // the inputs before the sequence
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    float2 f = make_float2(0.f, 0.f);
+                    if (a.conv_in != nullptr)
+                        f = *reinterpret_cast<const float2 *>(a.conv_in + ((long long)b * 3 + i) * a.channels + ch);
+                    x0[i] = f.x, x1[i] = f.y;
+                }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = vt + i;
+                float v0 = x0[i] * w0[0] + x0[i + 1] * w0[1] + x0[i + 2] * w0[2] + x0[i + 3] * w0[3];
+                float v1 = x1[i] * w1[0] + x1[i + 1] * w1[1] + x1[i + 2] * w1[2] + x1[i + 3] * w1[3];
+                v0 = c * kC + t < rows ? silu_fast(v0) : 0.f;
+                v1 = c * kC + t < rows ? silu_fast(v1) : 0.f;
+                *reinterpret_cast<float2 *>(smem + L::kV + t * 256 + (((vc >> 2) ^ (t & 15)) << 4) + (vc & 3) * 4) = make_float2(v0, v1);
+                m = fmaxf(m, fmaxf(fabsf(v0), fabsf(v1)));
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            if (lane == 0) atomicMax(&S.vmax[c % 3], __float_as_int(m));
+        };
+
+        int es = exponent_of(bound2);
+        if (chunks > 0) {
+            store_state(es);
+            if (is_q) {
+                load_raw(0);
+                store_values(0);
+                if (chunks > 1) load_raw(1);
+            }
+            bar_sync(1, 256);
+        }
+        const int t = r & 63;   // this row's token
+        for (int c = 0; c < chunks; ++c) {
+            if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to in the next chunk
+            const float vm = __int_as_float(S.vmax[c % 3]);
+            bound2 += kC * vm * vm;                  // of the states of this chunk, and of the one it leaves
+            const int eu = exponent_of(bound2) + 1;  // max |v| + |S| <= 9/8 sqrt(bound2)
+            const float *eg = reinterpret_cast<const float *>(smem + L::kGate + (c & 1) * kGates);
+            wait_bar(&S.kq_full[c & 1], (c >> 1) & 1, &S.stop);
+            const float g = eg[t], left = eg[kC + t], keep = eg[kC - 1];
+            float x[32], y[32];
+            wait_bar(&S.d[0], c & 1, &S.stop);
+            tc_fence_after();
+            read_sums(0, x);
+            if (!is_q) {
+                // R = V - e^G K S^T, scaled
+                const float k0 = g * pow2(es) * (1.f / kScaleK), s = pow2(-eu);
+#pragma unroll
+                for (int j = 0; j < 32; j += 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(smem + L::kV + t * 256 + ((((c0 + j) >> 2) ^ (t & 15)) << 4));
+                    y[j] = (v.x - k0 * x[j]) * s, y[j + 1] = (v.y - k0 * x[j + 1]) * s;
+                    y[j + 2] = (v.z - k0 * x[j + 2]) * s, y[j + 3] = (v.w - k0 * x[j + 3]) * s;
+                }
+                store_row(L::kR, L::kTileR, t, y);
+                signal(&S.r_ready);
+                wait_bar(&S.d[1], c & 1, &S.stop);
+                tc_fence_after();
+                read_sums(1, x);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) x[j] *= left;
+                store_row(L::kR, L::kTileR, t, x);   // W over R, which has been read
+                signal(&S.w_ready);
+            } else {
+                wait_bar(&S.d[1], c & 1, &S.stop);
+                tc_fence_after();
+                read_sums(1, y);
+                const float k0 = g * pow2(es) * pow2(-eu), s = pow2(eu) * (1.f / kScaleQ);
+                const int row = c * kC + t;
+                if (row < rows) {
+                    float4 *o = reinterpret_cast<float4 *>(a.o + ((long long)(row0 + row) * a.value_heads + vh) * kD + split * kN + c0);
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        o[j / 4] = make_float4(fmaf(k0, x[j], y[j]) * s, fmaf(k0, x[j + 1], y[j + 1]) * s,
+                                               fmaf(k0, x[j + 2], y[j + 2]) * s, fmaf(k0, x[j + 3], y[j + 3]) * s);
+                }
+                if (c + 1 < chunks) store_values(c + 1);   // over this chunk's, which R is made of
+                if (c + 2 < chunks) load_raw(c + 2);
+            }
+            es = exponent_of(bound2);
+            wait_bar(&S.d[2], c & 1, &S.stop);
+            tc_fence_after();
+            read_sums(2, x);
+            const float add = pow2(eu) * (1.f / kScaleK);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) St[j] = fmaf(St[j], keep, x[j] * add);
+            if (c + 1 < chunks) store_state(es);
+            bar_sync(1, 256);
+        }
+        const bool lost = S.stop;   // a copy or product that never came must not pass for an answer
+#pragma unroll
+        for (int j = 0; j < 32; ++j) a.delta_out[s_at + (long long)j * kD] = lost ? NAN : St[j];
+        tc_fence_before();
     }
-    if (!ok && !chain) vmax[0] = -1;   // a copy that never landed must not pass for an answer
     __syncthreads();
-    if (chain) {
-        ok &= chunks == 0 || vmax[0] != -1;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                a.delta_out[s_at + (long long)(8 * j + col + (e & 1)) * kD + dim + 8 * (e >> 1)] = ok ? S[j][e] : NAN;
+    if (S.stop && warp == 8) {   // copies in flight land before the shared memory goes (each wait bounded)
+        for (int i = 0; i < 2; ++i)
+            for (int p = 0; p < 2; ++p)
+                for (int k = 0; k < 1000 && !mbar_try_wait_sleep(&S.kq_full[i], p, 1000); ++k) {}
     }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
 }
 
 // ---- finish -------------------------------------------------------------------------------------------
@@ -830,19 +891,19 @@ __global__ void __launch_bounds__(kThreads) k_gdn_finish(const __grid_constant__
 
 long long max_chunks(int num_seqs, int total_rows) { return (long long)total_rows / kC + num_seqs; }
 
-template <bool kBf16, bool kFull>
+template <bool kBf16>
 cudaError_t launch(const GdnArgs &a, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
     if (a.total_rows > 0) {
-        e = cudaFuncSetAttribute(k_gdn_chunks<kBf16, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem::kBytes);
+        e = cudaFuncSetAttribute(k_gdn_chunks<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem::kBytes);
         if (e != cudaSuccess) return e;
         const dim3 grid((unsigned)max_chunks(a.num_seqs, a.total_rows), a.key_heads);
-        k_gdn_chunks<kBf16, kFull><<<grid, kThreads, ChunkSmem::kBytes, st>>>(a);
+        k_gdn_chunks<kBf16><<<grid, kThreads, ChunkSmem::kBytes, st>>>(a);
         if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
-    e = cudaFuncSetAttribute(k_gdn_scan<kBf16, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<kFull>::kBytes);
+    e = cudaFuncSetAttribute(k_gdn_scan<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem::kBytes + 1024);
     if (e != cudaSuccess) return e;
-    k_gdn_scan<kBf16, kFull><<<dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem<kFull>::kBytes, st>>>(a);
+    k_gdn_scan<kBf16><<<dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem::kBytes + 1024, st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     const long long units = (long long)a.total_rows * a.value_heads, want = (units + kWarps - 1) / kWarps;
     const int norm_blocks = (int)(want < 8 * 148 ? want : 8 * 148);   // 8 CTAs an SM
@@ -869,7 +930,7 @@ size_t carve(const nmoe_linear_attn_shape &s, int num_seqs, int total_rows, uint
         at += (n + 255) & ~(size_t)255;
         return p;
     };
-    uint8_t *kq = take(chunks * s.key_heads * 4 * kTileX), *tp = take(chunks * s.value_heads * 4 * kTileT);
+    uint8_t *kq = take(chunks * s.key_heads * 2 * kTileX), *tp = take(chunks * s.value_heads * 2 * kTileT);
     uint8_t *gates = take(chunks * s.value_heads * kGates), *o = take((size_t)total_rows * s.value_heads * kD * 4);
     if (a != nullptr) {
         a->kq = kq;
@@ -954,6 +1015,6 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
         return fail(NMOE_EINVAL, "too many rows or sequences");
     carve(*shape, num_seqs, total_rows, static_cast<uint8_t *>(workspace), &a);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = a.x_bf16 ? launch<true, true>(a, st) : launch<false, true>(a, st);
+    const cudaError_t e = a.x_bf16 ? launch<true>(a, st) : launch<false>(a, st);
     return e == cudaSuccess ? NMOE_OK : fail(NMOE_ECUDA, "prefill: %s", cudaGetErrorString(e));
 }
