@@ -22,7 +22,8 @@
 // since |k| <= 1 and b <= 1).
 //
 // The scan is a chain of three products a chunk, 128 rows high, on tcgen05: [K; Q] S^T (128 x 64 x 128),
-// [T b; P T b] R (128 x 64 x 64), K^T W (128 x 64 x 64), W = e^{G_63 - G} U; between them eight warps
+// [e^{G_63 - G} T b; P T b] R (128 x 64 x 64), whose upper half is W = e^{G_63 - G} U, and K^T W
+// (128 x 64 x 64); between them eight warps
 // read the sums from tensor memory, a thread per row and 32 columns, and write the next operand as rows
 // of 128 bytes, which the MMA takes as they are (MN-major). The warp tensor instructions needed the
 // fragments through registers, 3 KB of shared memory traffic a cycle's worth of products, and ran
@@ -53,7 +54,7 @@ int fail(int status, const char *fmt, ...) {
 constexpr int kD = 128, kC = 64;      // head dim, tokens of a chunk
 constexpr int kSplit = 2, kN = kD / kSplit;   // value columns of a scan CTA: 64
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kScanThreads = 288;     // eight warps on the rows, one that copies and issues the MMAs
+constexpr int kScanThreads = 448;     // warps 0-7: the rows, 8 and 13: MMAs (8 also the copies), 9-12: V
 constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about 1 / 11 and 1 / 128
 
 // Tile images, the same in the workspace and in shared memory: rows of 128 bytes (64 fp16) in 16-byte
@@ -61,7 +62,7 @@ constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about
 constexpr int kPanel = 128 * 128;     // 128 rows: K over Q, T b over P T b
 constexpr int kTileX = 2 * kPanel;    // K over Q, one part (hi or lo): two panels of 64 dims
 constexpr int kTileT = kPanel;        // T b over P T b, one part
-constexpr int kGates = 2 * kC * 4;    // e^{G_t}, e^{G_63 - G_t}
+constexpr int kGates = kC * 4;        // e^{G_t}
 
 struct GdnArgs {
     const int *cu_rows;
@@ -90,13 +91,14 @@ __device__ __forceinline__ int seq_rows(const GdnArgs &a, int b) {
 }
 __device__ __forceinline__ int seq_chunks(const GdnArgs &a, int b) { return (seq_rows(a, b) + kC - 1) / kC; }
 
-// x = hi + lo in fp16, two values at a time
+// x = hi + lo in fp16, two values at a time: hi is x rounded to 11 bits by an integer addition, which fp16
+// holds as it is, so that lo comes out of one subtraction (unpacking a converted hi goes through the slow
+// conversion unit)
 __device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const __half2 h = __floats2half2_rn(x, y);
-    const float2 f = __half22float2(h);
-    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
-    hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = *reinterpret_cast<const uint32_t *>(&l);
+    const float hx = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+    const float hy = __uint_as_float((__float_as_uint(y) + 0x1000u) & 0xffffe000u);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(hy), "f"(hx));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
 }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t *r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -333,10 +335,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         __syncthreads();   // also: K K^T, Q K^T are complete, and K and Q are read
         if (on) {
             float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
-            if (t128 < kC) {
-                gates[t128] = expf(G[half][t128].x + G[half][t128].y);
-                gates[kC + t128] = expf(diff(kC - 1, t128));
-            }
+            if (t128 < kC) gates[t128] = expf(G[half][t128].x + G[half][t128].y);
             // M below the diagonal; P with its diagonal
             for (int i = t128; i < kC * kC / 8; i += 128) {
                 const int t = i >> 3, s0 = (i & 7) * 8;
@@ -416,17 +415,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             }
             __syncthreads();
         }
-        // T b, in T's place: a thread holds four 16-byte pieces of it
+        // e^{G_63 - G} T b, whose product with R is W, into the workspace; T b itself in T's place, for P T b (a
+        // thread holds four 16-byte pieces of it meanwhile)
+        uint4 *to = reinterpret_cast<uint4 *>(a.tp + ((long long)chunk * a.value_heads + vh) * 2 * kTileT);
         uint32_t th[4][4], tl[4][4];
         if (on)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int i = t128 + 128 * x, t = i >> 3, s0 = (i & 7) * 8;
+                const float left = __expf(diff(kC - 1, t));
+                uint32_t wh[4], wl[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int s = s0 + 2 * j;
-                    split2(T[t * kLdT + s] * beta[half][s], T[t * kLdT + s + 1] * beta[half][s + 1], th[x][j], tl[x][j]);
+                    const float t0 = T[t * kLdT + s] * beta[half][s], t1 = T[t * kLdT + s + 1] * beta[half][s + 1];
+                    split2(t0, t1, th[x][j], tl[x][j]);
+                    split2(t0 * left, t1 * left, wh[j], wl[j]);
                 }
+                const int at = at128(t, i & 7) / 16;
+                to[at] = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+                to[kTileT / 16 + at] = make_uint4(wl[0], wl[1], wl[2], wl[3]);
             }
         __syncthreads();
         uint8_t *TB = reinterpret_cast<uint8_t *>(T);
@@ -476,12 +484,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             }
         __syncthreads();
         if (on) {
-            uint4 *to = reinterpret_cast<uint4 *>(a.tp + ((long long)chunk * a.value_heads + vh) * 2 * kTileT);
-            constexpr int kHalf = kC * 128 / 16;   // 16-byte pieces of 64 rows: T b hi, P T b hi, T b lo, P T b lo
+            constexpr int kHalf = kC * 128 / 16;   // 16-byte pieces of 64 rows
 #pragma unroll 4
-            for (int i = t128; i < 4 * kHalf; i += 128) {
+            for (int i = t128; i < 2 * kHalf; i += 128) {   // P T b below it, hi and lo
                 const int part = i / kHalf, x = i - part * kHalf;
-                to[i] = reinterpret_cast<const uint4 *>((part & 1 ? P : TB) + (part >> 1) * kC * 128)[x];
+                to[(2 * part + 1) * kHalf + x] = reinterpret_cast<const uint4 *>(P + part * kC * 128)[x];
             }
         }
         __syncthreads();
@@ -529,16 +536,31 @@ __device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t panel) {
     return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
-// Bounded: a barrier that never completes sets `stop`, and every later wait goes at once.
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Polls (a suspended wait wakes some hundred cycles later, five times a chunk). Bounded: a barrier that
+// never completes sets `stop`, and every later wait goes at once.
 __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    for (uint32_t n = 0; !mbar_try_wait_sleep(bar, parity, 20000u); ++n) {
-        if (*stop) return false;
-        if (n >= (1u << 16)) {
+    for (uint32_t n = 0;; ++n) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((n & 1023) == 1023 && *stop) return false;
+        if (n >= kMaxSpins) {
             *stop = 1;
             return false;
         }
     }
-    return true;
 }
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
@@ -550,8 +572,9 @@ __device__ __forceinline__ int exponent_of(float square) {
 }
 
 // Threads 0-255: row r = 32 (warp % 4) + lane of the 128, columns 32 (warp / 4) .. + 31 of the CTA's 64.
-// Rows 0-63 are tokens (K's rows: R and W), rows 64-127 are tokens too (Q's rows: the output, and V of the
-// next chunk), and all of them are dims of the state. Warp 8 copies and issues the MMAs.
+// Rows 0-63 are tokens (K's rows: R and W), rows 64-127 are tokens too (Q's rows: the output), and all of
+// them are dims of the state. Warps 9-12 convolve V a chunk ahead. Warps 8 and 13 issue half of the MMAs
+// each, into sums of their own: one thread issues one MMA in about 50 cycles, and these run 32.
 template <bool kBf16>
 __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
     using L = ScanSmem;
@@ -563,7 +586,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&S.kq_full[i], 1);
-        for (int i = 0; i < 3; ++i) mbar_init(&S.d[i], 1), S.vmax[i] = 0;
+        for (int i = 0; i < 3; ++i) mbar_init(&S.d[i], 2), S.vmax[i] = 0;   // a commit of either issuer
         mbar_init(&S.tp_full, 1);
         mbar_init(&S.r_ready, 4);   // the warps of rows 0-63
         mbar_init(&S.w_ready, 4);
@@ -572,7 +595,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         S.first_chunk = S.stop = 0;
     }
     if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&S.tmem)));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tc_fence_before();
@@ -609,25 +632,36 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     __syncthreads();
     if (tid == 0) S.vmax[2] = 0;
 
-    if (warp == 8) {
+    if (warp == 8 || warp == 13) {
         // ---- copies and MMAs; every value is the same in all lanes
         const uint32_t one = elect_lane();
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const int n = __shfl_sync(0xffffffffu, chunks, 0);
+        const int second = __shfl_sync(0xffffffffu, warp == 13, 0), n = __shfl_sync(0xffffffffu, chunks, 0);
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + second * 3 * kN;
         const uint64_t keep = policy_evict_normal();
         auto copy_kq = [&](int c) {
-            if (!one) return;
+            if (!one || second) return;
             uint64_t *bar = &S.kq_full[c & 1];
             mbar_arrive_expect_tx(bar, L::kStage + kGates);
             bulk_g2s(smem + (c & 1) * L::kStage, a.kq + ((chunk0 + c) * a.key_heads + kh) * 2 * kTileX, L::kStage, bar, keep);
             bulk_g2s(smem + L::kGate + (c & 1) * kGates, a.gates + ((chunk0 + c) * a.value_heads + vh) * kGates, kGates, bar, keep);
         };
         auto copy_tp = [&](int c) {
-            if (!one) return;
+            if (!one || second) return;
             mbar_arrive_expect_tx(&S.tp_full, 2 * kTileT);
             bulk_g2s(smem + L::kTP, a.tp + ((chunk0 + c) * a.value_heads + vh) * 2 * kTileT, 2 * kTileT, &S.tp_full, keep);
         };
         auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop)); };
+        // The products of `steps` k-steps: the first issuer takes hi hi and half of lo hi, the second hi lo and
+        // the other half. A's and B's address of k-step k, part (0 hi, 1 lo).
+        auto issue = [&](uint32_t d, uint32_t idesc, auto steps, auto at_a, auto at_b) {
+            constexpr int kSteps = decltype(steps)::value;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k)
+                mma_one(d, at_a(k, 0), at_b(k, second), idesc, k > 0 ? 1u : 0u, one);
+#pragma unroll
+            for (int k = 0; k < kSteps / 2; ++k)
+                mma_one(d, at_a(k + second * (kSteps / 2), 1), at_b(k + second * (kSteps / 2), 0), idesc, 1u, one);
+        };
         if (n > 0) {
             copy_kq(0);
             copy_tp(0);
@@ -635,82 +669,38 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         }
         for (int c = 0; c < n; ++c) {
             const uint32_t st = sm + (c & 1) * L::kStage;
+            auto state_rows = [&](int k, int part) { return desc_rows(sm + L::kS + part * L::kTileS + k * 2048, 0); };
+            auto token_rows = [&](int k, int part) { return desc_rows(sm + L::kR + part * L::kTileR + k * 2048, 0); };
             if (!wait(&S.kq_full[c & 1], (c >> 1) & 1) || !wait(&S.s_ready, c & 1)) break;
             tc_fence_after();
-            // the state of chunk c is stored, so K^T W of chunk c - 1, the last that read its stage, is complete
-            if (c > 0 && c + 1 < n) copy_kq(c + 1);
-#pragma unroll
-            for (int pass = 0; pass < 3; ++pass)   // lo hi, hi lo, hi hi
-#pragma unroll
-                for (int k = 0; k < kD / 16; ++k)
-                    mma_one(tm, sw128_desc(st + (pass == 0 ? kTileX : 0) + (k >> 2) * kPanel + (k & 3) * 32),
-                            desc_rows(sm + L::kS + (pass == 1 ? L::kTileS : 0) + k * 2048, 0), idesc_f16(0, 1),
-                            pass + k > 0 ? 1u : 0u, one);
+            issue(tm, idesc_f16(0, 1), std::integral_constant<int, kD / 16>{},
+                  [&](int k, int part) { return sw128_desc(st + part * kTileX + (k >> 2) * kPanel + (k & 3) * 32); }, state_rows);
             commit_one(&S.d[0], one);
+            // the state of chunk c was stored, so K^T W of chunk c - 1, the last that read its stage, is complete
+            if (c > 0 && c + 1 < n) copy_kq(c + 1);
             if (!wait(&S.tp_full, c & 1) || !wait(&S.r_ready, c & 1)) break;
             tc_fence_after();
-#pragma unroll
-            for (int pass = 0; pass < 3; ++pass)
-#pragma unroll
-                for (int k = 0; k < kC / 16; ++k)
-                    mma_one(tm + kN, sw128_desc(sm + L::kTP + (pass == 0 ? kTileT : 0) + k * 32),
-                            desc_rows(sm + L::kR + (pass == 1 ? L::kTileR : 0) + k * 2048, 0), idesc_f16(0, 1),
-                            pass + k > 0 ? 1u : 0u, one);
+            issue(tm + kN, idesc_f16(0, 1), std::integral_constant<int, kC / 16>{},
+                  [&](int k, int part) { return sw128_desc(sm + L::kTP + part * kTileT + k * 32); }, token_rows);
             commit_one(&S.d[1], one);
             if (!wait(&S.w_ready, c & 1)) break;
             tc_fence_after();
-#pragma unroll
-            for (int pass = 0; pass < 3; ++pass)
-#pragma unroll
-                for (int k = 0; k < kC / 16; ++k)
-                    mma_one(tm + 2 * kN, desc_rows(st + (pass == 0 ? kTileX : 0) + k * 2048, kPanel),
-                            desc_rows(sm + L::kR + (pass == 1 ? L::kTileR : 0) + k * 2048, 0), idesc_f16(1, 1),
-                            pass + k > 0 ? 1u : 0u, one);
+            issue(tm + 2 * kN, idesc_f16(1, 1), std::integral_constant<int, kC / 16>{},
+                  [&](int k, int part) { return desc_rows(st + part * kTileX + k * 2048, kPanel); }, token_rows);
             commit_one(&S.d[2], one);
-            if (c + 1 < n) copy_tp(c + 1);   // W is stored, so the product with T b is complete
+            if (c + 1 < n) copy_tp(c + 1);   // W is stored, so the products with T b are complete
         }
-    } else {
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        // 32 columns of row `row` of an operand image, hi and lo `part` bytes apart
-        auto store_row = [&](uint32_t image, int part, int row, const float *v) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int y = 0; y < 4; ++y) split2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
-                uint8_t *to = smem + image + at128(row, 4 * wg + x);
-                *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(to + part) = make_uint4(l[0], l[1], l[2], l[3]);
-            }
-        };
-        auto signal = [&](uint64_t *bar) {   // this warp's operand rows are written, and its sums are read
-            fence_async_smem();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        auto read_sums = [&](int which, float *v) {
-            tc_ld32(tmem + lanes + which * kN + c0, reinterpret_cast<uint32_t *>(v));
-            tc_wait_ld();
-        };
-        auto store_state = [&](int e) {
-            const float s = pow2(-e);
-            float v[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = St[j] * s;
-            store_row(L::kS, L::kTileS, r, v);
-            signal(&S.s_ready);
-        };
-        // V of a chunk, by the warps of rows 64-127: a lane two of the warp's 32 channels and 16 tokens (lanes
-        // 0-15 the first 16 of the warp's 32, lanes 16-31 the others). The inputs are loaded a chunk ahead and
-        // stay as they are until they are used (a conversion would wait for them).
+    } else if (warp >= 9) {
+        // ---- V of a chunk: a lane two of 32 channels (warps 9, 10: the first 32) and 16 tokens (lanes 0-15 the
+        // first 16 of the warp's 32, lanes 16-31 the others). The inputs are loaded a chunk ahead and stay as they
+        // are until they are used (a conversion would wait for them).
         using Raw2 = typename std::conditional<kBf16, uint32_t, float2>::type;
         using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
-        const int vt = 32 * ((warp & 3) - 2) + 16 * (lane >> 4), vc = c0 + 2 * (lane & 15);   // first token, channel
+        const int vt = 32 * ((warp - 9) & 1) + 16 * (lane >> 4), vc = 32 * ((warp - 9) >> 1) + 2 * (lane & 15);
         const int ch = (2 * a.key_heads + vh) * kD + split * kN + vc;
         Raw2 raw[19];
         float w0[4], w1[4];
-        if (is_q) {
+        {
             const uint2 u = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * ch);
             const uint2 v = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ch + 1));
             w0[0] = bf16_lo(u.x), w0[1] = bf16_hi(u.x), w0[2] = bf16_lo(u.y), w0[3] = bf16_hi(u.y);
@@ -724,8 +714,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 raw[i] = *reinterpret_cast<const Raw2 *>(p + (long long)(row0 + x) * a.qkv_stride);
             }
         };
-        auto store_values = [&](int c) {
-            float x0[19], x1[19], m = 0.f;
+        if (chunks > 0) load_raw(0);
+        for (int c = 0; c < chunks; ++c) {
+            float x0[19], x1[19];
+            float2 v[16];
+            float m = 0.f;
 #pragma unroll
             for (int i = 0; i < 19; ++i) {
                 if constexpr (kBf16)
@@ -733,6 +726,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 else
                     x0[i] = raw[i].x, x1[i] = raw[i].y;
             }
+            if (c + 1 < chunks) load_raw(c + 1);
             if (c == 0 && vt == 0)   // the inputs before the sequence
 #pragma unroll
                 for (int i = 0; i < 3; ++i) {
@@ -743,85 +737,135 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const int t = vt + i;
-                float v0 = x0[i] * w0[0] + x0[i + 1] * w0[1] + x0[i + 2] * w0[2] + x0[i + 3] * w0[3];
-                float v1 = x1[i] * w1[0] + x1[i + 1] * w1[1] + x1[i + 2] * w1[2] + x1[i + 3] * w1[3];
-                v0 = c * kC + t < rows ? silu_fast(v0) : 0.f;
-                v1 = c * kC + t < rows ? silu_fast(v1) : 0.f;
-                *reinterpret_cast<float2 *>(smem + L::kV + t * 256 + (((vc >> 2) ^ (t & 15)) << 4) + (vc & 3) * 4) = make_float2(v0, v1);
-                m = fmaxf(m, fmaxf(fabsf(v0), fabsf(v1)));
+                const float y0 = x0[i] * w0[0] + x0[i + 1] * w0[1] + x0[i + 2] * w0[2] + x0[i + 3] * w0[3];
+                const float y1 = x1[i] * w1[0] + x1[i + 1] * w1[1] + x1[i + 2] * w1[2] + x1[i + 3] * w1[3];
+                const bool in = c * kC + vt + i < rows;
+                v[i] = make_float2(in ? silu_fast(y0) : 0.f, in ? silu_fast(y1) : 0.f);
+                m = fmaxf(m, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            // over the values of the chunk before, once R is made of them
+            if (c > 0) wait_bar(&S.d[1], (c - 1) & 1, &S.stop);
             if (lane == 0) atomicMax(&S.vmax[c % 3], __float_as_int(m));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = vt + i;
+                *reinterpret_cast<float2 *>(smem + L::kV + t * 256 + (((vc >> 2) ^ (t & 15)) << 4) + (vc & 3) * 4) = v[i];
+            }
+            bar_sync(1, 384);   // before chunk c
+        }
+    } else {
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        // 16 columns (half hf of the thread's 32) of row `row` of an operand image, hi and lo `part` bytes apart
+        auto store_half = [&](uint32_t image, int part, int row, int hf, const float *v) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int y = 0; y < 4; ++y) split2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
+                uint8_t *to = smem + image + at128(row, 4 * wg + 2 * hf + x);
+                *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(to + part) = make_uint4(l[0], l[1], l[2], l[3]);
+            }
+        };
+        auto signal = [&](uint64_t *bar) {   // this warp's operand rows are written, and its sums are read
+            fence_async_smem();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto read_half = [&](int which, int hf, float *v) {   // 16 sums, of both issuers
+            float u[16];
+            tc_ld16(tmem + lanes + which * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(v));
+            tc_ld16(tmem + lanes + (3 + which) * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(u));
+            tc_wait_ld();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] += u[j];
+        };
+        auto store_state = [&](int e) {
+            const float s = pow2(-e);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) v[j] = St[16 * hf + j] * s;
+                store_half(L::kS, L::kTileS, r, hf, v);
+            }
+            signal(&S.s_ready);
         };
 
         int es = exponent_of(bound2);
-        if (chunks > 0) {
-            store_state(es);
-            if (is_q) {
-                load_raw(0);
-                store_values(0);
-                if (chunks > 1) load_raw(1);
-            }
-            bar_sync(1, 256);
-        }
+        if (chunks > 0) store_state(es);
         const int t = r & 63;   // this row's token
         for (int c = 0; c < chunks; ++c) {
-            if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to in the next chunk
+            bar_sync(1, 384);                        // V of the chunk is stored
+            if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to for chunk c + 2
             const float vm = __int_as_float(S.vmax[c % 3]);
             bound2 += kC * vm * vm;                  // of the states of this chunk, and of the one it leaves
             const int eu = exponent_of(bound2) + 1;  // max |v| + |S| <= 9/8 sqrt(bound2)
             const float *eg = reinterpret_cast<const float *>(smem + L::kGate + (c & 1) * kGates);
             wait_bar(&S.kq_full[c & 1], (c >> 1) & 1, &S.stop);
-            const float g = eg[t], left = eg[kC + t], keep = eg[kC - 1];
-            float x[32], y[32];
-            wait_bar(&S.d[0], c & 1, &S.stop);
-            tc_fence_after();
-            read_sums(0, x);
+            const float g = eg[t], keep = eg[kC - 1];
             if (!is_q) {
                 // R = V - e^G K S^T, scaled
                 const float k0 = g * pow2(es) * (1.f / kScaleK), s = pow2(-eu);
+                wait_bar(&S.d[0], c & 1, &S.stop);
+                tc_fence_after();
 #pragma unroll
-                for (int j = 0; j < 32; j += 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(smem + L::kV + t * 256 + ((((c0 + j) >> 2) ^ (t & 15)) << 4));
-                    y[j] = (v.x - k0 * x[j]) * s, y[j + 1] = (v.y - k0 * x[j + 1]) * s;
-                    y[j + 2] = (v.z - k0 * x[j + 2]) * s, y[j + 3] = (v.w - k0 * x[j + 3]) * s;
+                for (int hf = 0; hf < 2; ++hf) {
+                    float x[16], y[16];
+                    read_half(0, hf, x);
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const int piece = (c0 + 16 * hf + j) >> 2;
+                        const float4 v = *reinterpret_cast<const float4 *>(smem + L::kV + t * 256 + ((piece ^ (t & 15)) << 4));
+                        y[j] = (v.x - k0 * x[j]) * s, y[j + 1] = (v.y - k0 * x[j + 1]) * s;
+                        y[j + 2] = (v.z - k0 * x[j + 2]) * s, y[j + 3] = (v.w - k0 * x[j + 3]) * s;
+                    }
+                    store_half(L::kR, L::kTileR, t, hf, y);
                 }
-                store_row(L::kR, L::kTileR, t, y);
                 signal(&S.r_ready);
                 wait_bar(&S.d[1], c & 1, &S.stop);
                 tc_fence_after();
-                read_sums(1, x);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) x[j] *= left;
-                store_row(L::kR, L::kTileR, t, x);   // W over R, which has been read
+                for (int hf = 0; hf < 2; ++hf) {
+                    float x[16];
+                    read_half(1, hf, x);
+                    store_half(L::kR, L::kTileR, t, hf, x);   // W over R, which has been read
+                }
                 signal(&S.w_ready);
             } else {
-                wait_bar(&S.d[1], c & 1, &S.stop);
+                // the output before its norm: e^G Q S^T + P U
+                wait_bar(&S.d[1], c & 1, &S.stop);   // and with it the product before it
                 tc_fence_after();
-                read_sums(1, y);
                 const float k0 = g * pow2(es) * pow2(-eu), s = pow2(eu) * (1.f / kScaleQ);
                 const int row = c * kC + t;
-                if (row < rows) {
-                    float4 *o = reinterpret_cast<float4 *>(a.o + ((long long)(row0 + row) * a.value_heads + vh) * kD + split * kN + c0);
+                float4 *o = reinterpret_cast<float4 *>(a.o + ((long long)(row0 + row) * a.value_heads + vh) * kD + split * kN + c0);
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        o[j / 4] = make_float4(fmaf(k0, x[j], y[j]) * s, fmaf(k0, x[j + 1], y[j + 1]) * s,
-                                               fmaf(k0, x[j + 2], y[j + 2]) * s, fmaf(k0, x[j + 3], y[j + 3]) * s);
+                for (int hf = 0; hf < 2; ++hf) {
+                    float x[16], y[16];
+                    read_half(0, hf, x);
+                    read_half(1, hf, y);
+                    if (row < rows)
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            o[4 * hf + j / 4] = make_float4(fmaf(k0, x[j], y[j]) * s, fmaf(k0, x[j + 1], y[j + 1]) * s,
+                                                            fmaf(k0, x[j + 2], y[j + 2]) * s, fmaf(k0, x[j + 3], y[j + 3]) * s);
                 }
-                if (c + 1 < chunks) store_values(c + 1);   // over this chunk's, which R is made of
-                if (c + 2 < chunks) load_raw(c + 2);
             }
             es = exponent_of(bound2);
             wait_bar(&S.d[2], c & 1, &S.stop);
             tc_fence_after();
-            read_sums(2, x);
             const float add = pow2(eu) * (1.f / kScaleK);
 #pragma unroll
-            for (int j = 0; j < 32; ++j) St[j] = fmaf(St[j], keep, x[j] * add);
+            for (int hf = 0; hf < 2; ++hf) {
+                float x[16];
+                read_half(2, hf, x);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) St[16 * hf + j] = fmaf(St[16 * hf + j], keep, x[j] * add);
+            }
             if (c + 1 < chunks) store_state(es);
-            bar_sync(1, 256);
         }
         const bool lost = S.stop;   // a copy or product that never came must not pass for an answer
 #pragma unroll
@@ -836,7 +880,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     }
     __syncthreads();
     tc_fence_after();
-    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
+    if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 // ---- finish -------------------------------------------------------------------------------------------
