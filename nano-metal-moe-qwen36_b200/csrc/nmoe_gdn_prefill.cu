@@ -128,7 +128,12 @@ __device__ __forceinline__ uint32_t elect_lane() {
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // x / (1 + e^-x) with the hardware's exponential and reciprocal: a few 2^-23 of it
-__device__ __forceinline__ float silu_fast(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+__device__ __forceinline__ float silu_fast(float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return x * r;
+}
 // byte offset of 16-byte piece p of row r: in a 128-byte row; in two panels of 128 rows
 __device__ __forceinline__ uint32_t at128(int r, int p) { return r * 128 + ((p ^ (r & 7)) << 4); }
 __device__ __forceinline__ uint32_t at_kq(int r, int p) { return (p >> 3) * kPanel + at128(r, p & 7); }
@@ -909,27 +914,37 @@ __global__ void __launch_bounds__(kThreads) k_gdn_finish(const __grid_constant__
     const int first = max(0, min(a.cu_rows[0], a.total_rows)), end = min(a.cu_rows[a.num_seqs], a.total_rows);
     const long long units = (long long)max(0, end - first) * a.value_heads;
     const uint2 wv = *reinterpret_cast<const uint2 *>(a.norm_w + 4 * lane);
-    for (long long u = (long long)blockIdx.x * kWarps + warp; u < units; u += (long long)norm_blocks * kWarps) {
-        const long long r = first + u / a.value_heads;
-        const int vh = (int)(u % a.value_heads);
-        const float4 o = *reinterpret_cast<const float4 *>(a.o + (r * a.value_heads + vh) * kD + 4 * lane);
-        float z[4];
-        const long long za = r * a.z_stride + vh * kD + 4 * lane;
-        if constexpr (kBf16) {
-            const uint2 q = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(a.z) + za);
-            z[0] = bf16_lo(q.x), z[1] = bf16_hi(q.x), z[2] = bf16_lo(q.y), z[3] = bf16_hi(q.y);
-        } else {
-            const float4 q = *reinterpret_cast<const float4 *>(static_cast<const float *>(a.z) + za);
-            z[0] = q.x, z[1] = q.y, z[2] = q.z, z[3] = q.w;
+    const float w[4] = {bf16_lo(wv.x), bf16_hi(wv.x), bf16_lo(wv.y), bf16_hi(wv.y)};
+    constexpr int kAtOnce = 4;   // (row, head) pairs of a warp, one beside the other, on their way together
+    using Raw4 = typename std::conditional<kBf16, uint2, float4>::type;
+    using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
+    for (long long u0 = ((long long)blockIdx.x * kWarps + warp) * kAtOnce; u0 < units; u0 += (long long)norm_blocks * kWarps * kAtOnce) {
+        float4 o[kAtOnce];
+        Raw4 zr[kAtOnce];
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const long long u = min(u0 + x, units - 1), r = first + u / a.value_heads;
+            const int vh = (int)(u % a.value_heads);
+            o[x] = *reinterpret_cast<const float4 *>(a.o + (r * a.value_heads + vh) * kD + 4 * lane);
+            zr[x] = *reinterpret_cast<const Raw4 *>(static_cast<const Raw *>(a.z) + r * a.z_stride + vh * kD + 4 * lane);
         }
-        const float inv = rsqrtf(warp_sum(o.x * o.x + o.y * o.y + o.z * o.z + o.w * o.w) / kD + 1e-6f);
-        const float v0 = o.x * inv * bf16_lo(wv.x) * siluf_(z[0]), v1 = o.y * inv * bf16_hi(wv.x) * siluf_(z[1]);
-        const float v2 = o.z * inv * bf16_lo(wv.y) * siluf_(z[2]), v3 = o.w * inv * bf16_hi(wv.y) * siluf_(z[3]);
-        const long long at = (r * a.value_heads + vh) * kD + 4 * lane;
-        if (a.out_bf16)
-            *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
-        else
-            *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v0, v1, v2, v3);
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            if (u0 + x >= units) break;
+            float z[4];
+            if constexpr (kBf16)
+                z[0] = bf16_lo(zr[x].x), z[1] = bf16_hi(zr[x].x), z[2] = bf16_lo(zr[x].y), z[3] = bf16_hi(zr[x].y);
+            else
+                z[0] = zr[x].x, z[1] = zr[x].y, z[2] = zr[x].z, z[3] = zr[x].w;
+            const float inv = rsqrtf(warp_sum(o[x].x * o[x].x + o[x].y * o[x].y + o[x].z * o[x].z + o[x].w * o[x].w) / kD + 1e-6f);
+            const float v0 = o[x].x * inv * w[0] * silu_fast(z[0]), v1 = o[x].y * inv * w[1] * silu_fast(z[1]);
+            const float v2 = o[x].z * inv * w[2] * silu_fast(z[2]), v3 = o[x].w * inv * w[3] * silu_fast(z[3]);
+            const long long at = ((first + (u0 + x) / a.value_heads) * a.value_heads + (u0 + x) % a.value_heads) * kD + 4 * lane;
+            if (a.out_bf16)
+                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+            else
+                *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v0, v1, v2, v3);
+        }
     }
 }
 
@@ -949,7 +964,7 @@ cudaError_t launch(const GdnArgs &a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     k_gdn_scan<kBf16><<<dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem::kBytes + 1024, st>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const long long units = (long long)a.total_rows * a.value_heads, want = (units + kWarps - 1) / kWarps;
+    const long long units = (long long)a.total_rows * a.value_heads, want = (units + 4 * kWarps - 1) / (4 * kWarps);
     const int norm_blocks = (int)(want < 8 * 148 ? want : 8 * 148);   // 8 CTAs an SM
     const long long conv_blocks = ((long long)a.num_seqs * a.channels + kThreads - 1) / kThreads;
     k_gdn_finish<kBf16><<<(unsigned)(norm_blocks + conv_blocks), kThreads, 0, st>>>(a, norm_blocks);

@@ -25,11 +25,12 @@ struct PagedDev {
 
 // Rotation: pair t < half turns by position * theta^(-t / half), in 64 bits, since the angle has to
 // be reduced before it is rounded (an fp32 angle at position 32768 is off by 2e-3). A thread that
-// needs a frequency computes it once: a table in the kernel's parameters, read by 32 lanes at 32
-// addresses, costs tens of microseconds of constant-cache misses.
+// needs a frequency makes it once, of the powers for t's bits: a table of all of them in the kernel's
+// parameters, read by 32 lanes at 32 addresses, costs tens of microseconds of constant-cache misses,
+// and exp2 in 64 bits as much as the rest of a head's work.
 struct RotaryDev {
-    double step;   // log2(theta) / half
-    int half;      // rotary_dims / 2
+    double bit[7];   // theta^(-2^k / half)
+    int half;        // rotary_dims / 2
 };
 
 struct HeadDev {
@@ -37,13 +38,19 @@ struct HeadDev {
     float eps;
 };
 
-__device__ __forceinline__ double rotary_freq(const RotaryDev &r, int t) { return exp2(-r.step * t); }
+// theta^(-t / half) / pi: half turns per position
+__device__ __forceinline__ double rotary_freq(const RotaryDev &r, int t) {
+    double f = 0.31830988618379067;
+#pragma unroll
+    for (int k = 0; k < 7; ++k) f *= (t >> k & 1) ? r.bit[k] : 1.0;
+    return f;
+}
 
 __device__ __forceinline__ float2 rotary_cs(double freq, int position) {
     double a = (double)position * freq;
-    a -= rint(a * 0.15915494309189535) * 6.283185307179586;
+    a -= 2.0 * rint(0.5 * a);   // half turns in [-1, 1]
     float s, c;
-    sincosf((float)a, &s, &c);
+    sincospif((float)a, &s, &c);
     return make_float2(c, s);
 }
 
@@ -56,17 +63,16 @@ __device__ __forceinline__ long long paged_row(const PagedDev &c, int seq, int p
     return (long long)page * c.page_stride + (long long)(position - slot * c.page_size) * c.row_stride;
 }
 
-// One warp: the sequence that holds packed row r (cu[b] <= r < cu[b + 1]), or -1 for a row
-// behind the last sequence. 32-ary search: log32(n) dependent loads.
-__device__ __forceinline__ int find_sequence(const int *cu, int n, int r, int lane) {
-    int lo = 0, len = n;   // the answer, the number of i in 1..n with cu[i] <= r, is in [lo, lo + len]
-    while (len > 0) {
-        const int step = (len + 31) / 32;
-        const int i = lo + (lane + 1) * step;
-        const bool below = (lane + 1) * step <= len && cu[i] <= r;
-        const int full = __popc(__ballot_sync(0xffffffffu, below));
-        lo += full * step;
-        len = min(step - 1, len - full * step);
+// The sequence that holds packed row r (cu[b] <= r < cu[b + 1]), or -1 for a row behind the last
+// sequence or before the first: the number of i in 1..n with cu[i] <= r.
+__device__ __forceinline__ int find_sequence(const int *cu, int n, int r) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = lo + ((hi - lo) >> 1);
+        if (cu[mid + 1] <= r)
+            lo = mid + 1;
+        else
+            hi = mid;
     }
     return lo < n && cu[0] <= r ? lo : -1;
 }
@@ -119,30 +125,44 @@ __device__ __forceinline__ void store_bf16(uint16_t *p, const float *v) {
         *reinterpret_cast<uint2 *>(p) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
 }
 
-// One warp prepares one head of 32 E dims, lane l holding dims E l .. E l + E - 1: RMS norm by
-// (weight + 1), then the rotation of dims 0 .. 2 half - 1 with the row's (cos, sin) table cs[half].
+// This lane's norm weights + 1 (dims E lane ..): ones without a norm.
+template <int E>
+__device__ __forceinline__ void load_weight(const uint16_t *weight, int lane, float *w) {
+    if (weight != nullptr) {
+        load_typed<E, true>(weight, E * lane, w);
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i] += 1.0f;
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i] = 1.0f;
+    }
+}
+
+// One warp prepares one head of 32 E dims, lane l holding dims E l .. E l + E - 1: RMS norm by the weights
+// w (where `norm`), then the rotation of dims 0 .. 2 half - 1 with the row's (cos, sin) table cs[half].
 // half is a power of two of at least 8 >= E, so a pair's other dim is in lane ^ (half / E).
 template <int E>
-__device__ __forceinline__ void prepare_head(float *v, const uint16_t *weight, float eps, const float2 *cs, int half,
+__device__ __forceinline__ void prepare_head(float *v, const float *w, bool norm, float eps, const float2 *cs, int half,
                                              int lane) {
-    if (weight != nullptr) {
+    if (norm) {
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
         const float inv = rsqrtf(warp_sum(ss) / (float)(32 * E) + eps);
 #pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = v[i] * inv * (bf16_to_f32(weight[E * lane + i]) + 1.0f);
+        for (int i = 0; i < E; ++i) v[i] = v[i] * inv * w[i];
     }
     if (half > 0) {
         const int d = E * lane;
-        const bool second = d >= half;
-        const float2 *t = cs + (d & (half - 1));
+        const uint32_t flip = d >= half ? 0u : 0x80000000u;   // the sine's sign in a pair's first dim
+        const float4 *t = reinterpret_cast<const float4 *>(cs + (d & (half - 1)));
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float other = __shfl_xor_sync(0xffffffffu, v[i], half / E);
+        for (int i = 0; i < E; i += 2) {
+            const float o0 = __shfl_xor_sync(0xffffffffu, v[i], half / E), o1 = __shfl_xor_sync(0xffffffffu, v[i + 1], half / E);
             if (d < 2 * half) {
-                const float2 k = t[i];
-                v[i] = second ? fmaf(other, k.y, v[i] * k.x) : fmaf(-other, k.y, v[i] * k.x);
+                const float4 k = t[i / 2];
+                v[i] = fmaf(o0, __uint_as_float(__float_as_uint(k.y) ^ flip), v[i] * k.x);
+                v[i + 1] = fmaf(o1, __uint_as_float(__float_as_uint(k.w) ^ flip), v[i + 1] * k.z);
             }
         }
     }
@@ -155,6 +175,9 @@ int check_full_attn_shape(const nmoe_full_attn_weights *w, const nmoe_full_attn_
 int check_paged_kv(const nmoe_paged_kv *kv, PagedDev *dev);
 void fill_rotary(const nmoe_full_attn_shape *s, RotaryDev *r);
 int check_x(const char *what, const void *p, int x_dtype, long long stride, long long width);
+// Rows of a CTA of eight warps that prepares rows: the largest power of two up to `want` (and 8, and from 1
+// on), and the logarithm of the warps that share a row.
+void rows_a_cta(int want, int *rows, int *share_log);
 int device_sm_count(int *sms);
 using TensorMapEncode = PFN_cuTensorMapEncodeTiled_v12000;
 TensorMapEncode tensor_map_encode();

@@ -49,6 +49,8 @@ int check_full_attn_shape(const nmoe_full_attn_weights *w, const nmoe_full_attn_
         return full_attn_fail(NMOE_EINVAL, "rotary_dims %d: 0 or a power of two from 16 to head_dim", r);
     if (r != 0 && !(s->rope_theta > 0.f && s->rope_theta <= 3.0e38f))
         return full_attn_fail(NMOE_EINVAL, "rope_theta must be positive and finite");
+    if (!aligned_to(w->q_norm, 16) || !aligned_to(w->k_norm, 16))
+        return full_attn_fail(NMOE_EINVAL, "q_norm and k_norm must be 16-byte aligned");
     if ((w->q_norm != nullptr || w->k_norm != nullptr) && !(s->norm_eps > 0.f))
         return full_attn_fail(NMOE_EINVAL, "norm_eps must be positive");
     if (s->gated != 0 && s->gated != 1) return full_attn_fail(NMOE_EINVAL, "gated %d: 0 or 1", s->gated);
@@ -83,7 +85,7 @@ int check_paged_kv(const nmoe_paged_kv *kv, PagedDev *d) {
 
 void fill_rotary(const nmoe_full_attn_shape *s, RotaryDev *r) {
     r->half = s->rotary_dims / 2;
-    r->step = r->half > 0 ? log2((double)s->rope_theta) / r->half : 0.0;
+    for (int k = 0; k < 7; ++k) r->bit[k] = r->half > 0 ? pow((double)s->rope_theta, -(double)(1 << k) / r->half) : 1.0;
 }
 
 int check_x(const char *what, const void *p, int x_dtype, long long stride, long long width) {
@@ -94,6 +96,11 @@ int check_x(const char *what, const void *p, int x_dtype, long long stride, long
     if (!aligned_to(p, 16) || stride % unit != 0 || stride < width)
         return full_attn_fail(NMOE_EINVAL, "%s rows must be 16-byte aligned and at least %lld elements apart", what, width);
     return NMOE_OK;
+}
+
+void rows_a_cta(int want, int *rows, int *share_log) {
+    *rows = 8, *share_log = 0;
+    while (*rows > 1 && *rows > want) *rows >>= 1, ++*share_log;
 }
 
 int device_sm_count(int *sms) {
@@ -141,35 +148,47 @@ struct AppendArgs {
     const int *cu_rows, *kv_lens;
     const void *k_new, *v_new;
     long long kv_stride;
-    int num_seqs, total_rows, kv_heads, rows_per_cta, x_bf16;
+    int num_seqs, total_rows, kv_heads, rows_per_cta, share_log, x_bf16;
 };
 
 constexpr int kAppendThreads = 256, kAppendRows = 8;
 
-// A CTA takes rows_per_cta rows (1 when there are few, so that they spread over the SMs): one
-// (cos, sin) table per row for all its heads, then a warp per (row, head, k or v).
+// A CTA takes rows_per_cta rows (1 when there are few, so that they spread over the SMs): one (cos, sin)
+// table per row for all its heads, then a warp per (row, head, k or v). HBM bound: the operands of a
+// warp's first units are asked for before the rows' sequences, positions and angles are found, which
+// takes three dependent reads.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_constant__ AppendArgs a) {
-    constexpr int E = D / 32;
-    __shared__ float2 cs[kAppendRows][128];
+    constexpr int E = D / 32, kAtOnce = 4;
+    __shared__ __align__(16) float2 cs[kAppendRows][128];
     __shared__ long long where[kAppendRows];
     __shared__ int at[kAppendRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = blockIdx.x * a.rows_per_cta;
-    const int rows = min(a.rows_per_cta, a.total_rows - row0);
-    const double freq = a.rot.half > 0 ? rotary_freq(a.rot, tid & (a.rot.half - 1)) : 0.0;
-    if (warp < rows) {
-        const int r = row0 + warp;
-        const int b = find_sequence(a.cu_rows, a.num_seqs, r, lane);
-        if (lane == 0) {
-            long long w = -1, p = -1;
-            if (b >= 0) {
-                p = (long long)a.kv_lens[b] - a.cu_rows[b + 1] + r;
-                if (p >= 0 && p < a.c.capacity) w = paged_row(a.c, b, (int)p);
-            }
-            where[warp] = w;
-            at[warp] = w >= 0 ? (int)p : 0;
+    const int rows = min(a.rows_per_cta, a.total_rows - row0), units = 2 * a.kv_heads;   // k and v of a head
+    // 8 / rows_per_cta (a power of two) warps share a row
+    const int share_log = a.share_log, share = 1 << share_log, mine = warp >> share_log, first = warp & (share - 1);
+    float v[kAtOnce][E], w[E];
+    const long long src = (long long)(row0 + min(mine, rows - 1)) * a.kv_stride + E * lane;
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x) {
+            const int u = min(u0 + (x << share_log), units - 1);
+            load_typed<E, kBf16>(u & 1 ? a.v_new : a.k_new, src + (u >> 1) * D, v[x]);
         }
+    };
+    load(first);
+    load_weight<E>(a.h.k_norm, lane, w);
+    const double freq = a.rot.half > 0 ? rotary_freq(a.rot, tid & (a.rot.half - 1)) : 0.0;
+    if (tid < rows) {
+        const int r = row0 + tid, b = find_sequence(a.cu_rows, a.num_seqs, r);
+        long long to = -1, p = -1;
+        if (b >= 0) {
+            p = (long long)a.kv_lens[b] - a.cu_rows[b + 1] + r;
+            if (p >= 0 && p < a.c.capacity) to = paged_row(a.c, b, (int)p);
+        }
+        where[tid] = to;
+        at[tid] = to >= 0 ? (int)p : 0;
     }
     __syncthreads();
     if (a.rot.half > 0) {   // half is a power of two that divides the threads: a thread keeps its t
@@ -177,22 +196,16 @@ __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_co
         for (int r = tid / a.rot.half; r < rows; r += kAppendThreads / a.rot.half) cs[r][t] = rotary_cs(freq, at[r]);
     }
     __syncthreads();
-    const int units = rows * a.kv_heads * 2;
-    constexpr int kAtOnce = 4, kWarps = kAppendThreads / 32;   // loads of a warp on their way together
-    for (int u0 = warp; u0 < units; u0 += kWarps * kAtOnce) {
-        float v[kAtOnce][E];
+    if (mine >= rows || where[mine] < 0) return;
+    const long long dst = where[mine] + E * lane;
+    for (int u0 = first; u0 < units; u0 += kAtOnce << share_log) {
+        if (u0 != first) load(u0);
 #pragma unroll
         for (int x = 0; x < kAtOnce; ++x) {
-            const int u = min(u0 + x * kWarps, units - 1), r = u / (2 * a.kv_heads), hv = u - r * 2 * a.kv_heads;
-            load_typed<E, kBf16>(hv & 1 ? a.v_new : a.k_new,
-                                 (long long)(row0 + r) * a.kv_stride + (hv >> 1) * D + E * lane, v[x]);
-        }
-#pragma unroll
-        for (int x = 0; x < kAtOnce; ++x) {
-            const int u = u0 + x * kWarps, r = u / (2 * a.kv_heads), hv = u - r * 2 * a.kv_heads;
-            if (u >= units || where[r] < 0) continue;
-            if (!(hv & 1)) prepare_head<E>(v[x], a.h.k_norm, a.h.eps, cs[r], a.rot.half, lane);
-            store_bf16<E>((hv & 1 ? a.c.v : a.c.k) + where[r] + (hv >> 1) * a.c.head_stride + E * lane, v[x]);
+            const int u = u0 + (x << share_log);
+            if (u >= units) break;
+            if (!(u & 1)) prepare_head<E>(v[x], w, a.h.k_norm != nullptr, a.h.eps, cs[mine], a.rot.half, lane);
+            store_bf16<E>((u & 1 ? a.c.v : a.c.k) + dst + (u >> 1) * a.c.head_stride, v[x]);
         }
     }
 }
@@ -338,7 +351,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
     extern __shared__ uint8_t raw_smem[];
     __shared__ uint64_t bars[kWarps][kStages];
     __shared__ uint32_t live[kWarps][kStages];   // bit i: position i of the stage takes part
-    __shared__ float2 cs[128];
+    __shared__ __align__(16) float2 cs[128];
     __shared__ float sm_m[kWarps][kGroupMax], sm_l[kWarps][kGroupMax];
     __shared__ long long sm_scan[kWarps];
     __shared__ int sm_seq;
@@ -449,7 +462,9 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
             float v[E];
             load_elems<E>(a.q, (long long)b * a.q_stride + (long long)(kvh * a.group + g) * (a.gated ? 2 * D : D) + E * lane,
                           a.x_bf16, v);
-            prepare_head<E>(v, a.h.q_norm, a.h.eps, cs, a.rot.half, lane);
+            float w[E];
+            load_weight<E>(a.h.q_norm, lane, w);
+            prepare_head<E>(v, w, a.h.q_norm != nullptr, a.h.eps, cs, a.rot.half, lane);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[i] *= a.scale;
 #pragma unroll
@@ -493,7 +508,9 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
                 const long long dst = paged_row(a.c, b, fresh) + (long long)kvh * a.c.head_stride + E * lane;
                 uint8_t *row = stage + at_panel(fresh - base, E * lane / 8) + (E * lane % 8) * 2;
                 load_elems<E>(a.k_new, src, a.x_bf16, v);
-                prepare_head<E>(v, a.h.k_norm, a.h.eps, cs, a.rot.half, lane);
+                float w[E];
+                load_weight<E>(a.h.k_norm, lane, w);
+                prepare_head<E>(v, w, a.h.k_norm != nullptr, a.h.eps, cs, a.rot.half, lane);
                 store_bf16<E>(a.c.k + dst, v);
                 store_bf16<E>(reinterpret_cast<uint16_t *>(row), v);
                 load_elems<E>(a.v_new, src, a.x_bf16, v);
@@ -762,8 +779,7 @@ extern "C" int nmoe_full_attn_append_paged(const nmoe_full_attn_weights *w, cons
     a.total_rows = total_rows;
     a.kv_heads = shape->kv_heads;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
-    const int per = total_rows / (8 * sms);
-    a.rows_per_cta = per < 1 ? 1 : (per > kAppendRows ? kAppendRows : per);
+    rows_a_cta(total_rows / (8 * sms), &a.rows_per_cta, &a.share_log);
     const int grid = (total_rows + a.rows_per_cta - 1) / a.rows_per_cta;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (shape->head_dim == 256)

@@ -41,7 +41,7 @@ struct PrefillArgs {
     CUtensorMap k_map, v_map;   // pages as 4D tensors, boxes of 64 columns x box_rows
     CUtensorMap q_map;          // prepared queries, boxes of 64 columns x 128 rows
     uint16_t *q_ready;
-    int prep_rows;
+    int prep_rows, share_log;
     PagedDev c;
     RotaryDev rot;
     HeadDev h;
@@ -215,41 +215,52 @@ constexpr int kPrepThreads = 256, kPrepRows = 8;
 
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kPrepThreads) k_prefill_queries(const __grid_constant__ PrefillArgs a) {
-    constexpr int E = D / 32;
-    __shared__ float2 cs[kPrepRows][128];
+    constexpr int E = D / 32, kAtOnce = 4;
+    __shared__ __align__(16) float2 cs[kPrepRows][128];
     __shared__ int at[kPrepRows], live[kPrepRows];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, half = a.rot.half;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int row0 = blockIdx.x * a.prep_rows, rows = min(a.prep_rows, a.total_rows - row0);
+    const int heads = a.kv_heads * a.group;
+    // 8 / prep_rows (a power of two) warps share a row
+    const int share_log = a.share_log, share = 1 << share_log, mine = warp >> share_log, first = warp & (share - 1);
+    float next[kAtOnce][E], w[E];
+    const long long src = (long long)(row0 + min(mine, rows - 1)) * a.q_stride + E * lane;
+    const int step = a.gated ? 2 * D : D;
+    auto load = [&](int h0) {   // a warp's next heads, on their way together
+#pragma unroll
+        for (int x = 0; x < kAtOnce; ++x)
+            load_typed<E, kBf16>(a.q, src + (long long)min(h0 + (x << share_log), heads - 1) * step, next[x]);
+    };
+    load(first);
+    load_weight<E>(a.h.q_norm, lane, w);
     const double freq = half > 0 ? rotary_freq(a.rot, tid & (half - 1)) : 0.0;
-    if (warp < rows) {
-        const int r = row0 + warp, b = find_sequence(a.cu_rows, a.num_seqs, r, lane);
-        if (lane == 0) {
-            live[warp] = b >= 0;
-            at[warp] = b >= 0 ? (int)((long long)a.kv_lens[b] - a.cu_rows[b + 1] + r) : 0;
-        }
+    if (tid < rows) {
+        const int r = row0 + tid, b = find_sequence(a.cu_rows, a.num_seqs, r);
+        live[tid] = b >= 0;
+        at[tid] = b >= 0 ? (int)((long long)a.kv_lens[b] - a.cu_rows[b + 1] + r) : 0;
     }
     __syncthreads();
     if (half > 0)
         for (int r = tid / half; r < rows; r += kPrepThreads / half) cs[r][tid & (half - 1)] = rotary_cs(freq, at[r]);
     __syncthreads();
-    const int heads = a.kv_heads * a.group, units = rows * heads;
-    constexpr int kAtOnce = 4, kWarps = kPrepThreads / 32;   // loads of a warp on their way together
-    for (int u0 = warp; u0 < units; u0 += kWarps * kAtOnce) {
+    if (mine >= rows || !live[mine]) return;
+    for (int h0 = first; h0 < heads; h0 += kAtOnce << share_log) {
         float v[kAtOnce][E];
 #pragma unroll
-        for (int x = 0; x < kAtOnce; ++x) {
-            const int u = min(u0 + x * kWarps, units - 1), r = u / heads, h = u - r * heads;
-            load_typed<E, kBf16>(a.q, (long long)(row0 + r) * a.q_stride + (long long)h * (a.gated ? 2 * D : D) + E * lane, v[x]);
-        }
+        for (int x = 0; x < kAtOnce; ++x)
+#pragma unroll
+            for (int i = 0; i < E; ++i) v[x][i] = next[x][i];
+        if (h0 + (kAtOnce << share_log) < heads) load(h0 + (kAtOnce << share_log));
 #pragma unroll
         for (int x = 0; x < kAtOnce; ++x) {
-            const int u = u0 + x * kWarps, r = u / heads, h = u - r * heads, kvh = h / a.group;
-            if (u >= units || !live[r]) continue;
-            prepare_head<E>(v[x], a.h.q_norm, a.h.eps, cs[r], half, lane);
+            const int h = h0 + (x << share_log);
+            if (h >= heads) break;
+            prepare_head<E>(v[x], w, a.h.q_norm != nullptr, a.h.eps, cs[mine], half, lane);
 #pragma unroll
             for (int i = 0; i < E; ++i) v[x][i] *= a.scale;
-            store_bf16<E>(a.q_ready + (((long long)kvh * a.total_rows + row0 + r) * a.group + (h - kvh * a.group)) * D + E * lane,
+            const int kvh = h / a.group;
+            store_bf16<E>(a.q_ready + (((long long)kvh * a.total_rows + row0 + mine) * a.group + (h - kvh * a.group)) * D + E * lane,
                           v[x]);
         }
     }
@@ -834,8 +845,7 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.q_ready = static_cast<uint16_t *>(workspace);
     int sms = 0;
     if ((rc = device_sm_count(&sms)) != NMOE_OK) return rc;
-    const int per = total_rows / (4 * sms);
-    a.prep_rows = per < 1 ? 1 : (per > kPrepRows ? kPrepRows : per);
+    rows_a_cta(total_rows / (4 * sms), &a.prep_rows, &a.share_log);
     if (!query_map(&a.q_map, a.q_ready, shape->head_dim, (long long)total_rows * shape->q_heads))
         return full_attn_fail(NMOE_ECUDA, "cuTensorMapEncodeTiled failed");
     // boxes of the largest power of two of rows that divides a page, 16 to 64: an MMA's 16 positions lie
