@@ -37,6 +37,7 @@
 
 #include "nmoe/moe_cuda.h"
 #include "nmoe_gemm.cuh"
+#include "nmoe_paged.cuh"
 
 namespace nmoe {
 namespace {
@@ -74,6 +75,7 @@ struct GdnArgs {
     float *conv_out, *delta_out;
     void *out;
     int num_seqs, total_rows, key_heads, value_heads, channels, x_bf16, out_bf16;
+    int part, parts;   // of every sequence's chunks: those that a launch takes
     // workspace, per chunk and head: K over Q, hi and lo; T b over P T b, hi and lo; gates; and O
     uint8_t *kq, *tp, *gates;
     float *o;
@@ -90,6 +92,8 @@ __device__ __forceinline__ int seq_rows(const GdnArgs &a, int b) {
     return max(0, min(a.cu_rows[b + 1], a.total_rows) - seq_first(a, b));
 }
 __device__ __forceinline__ int seq_chunks(const GdnArgs &a, int b) { return (seq_rows(a, b) + kC - 1) / kC; }
+// first of the `chunks` chunks of a sequence that belongs to part p
+__device__ __forceinline__ int part_first(const GdnArgs &a, int chunks, int p) { return (int)((long long)chunks * p / a.parts); }
 
 // x = hi + lo in fp16, two values at a time: hi is x rounded to 11 bits by an integer addition, which fp16
 // holds as it is, so that lo comes out of one subtraction (unpacking a converted hi goes through the slow
@@ -121,6 +125,12 @@ __device__ __forceinline__ void mma_f16(float *d, const uint32_t *a, uint32_t b0
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// A copy out of shared memory, one group; what it reads was fenced for it.
+__device__ __forceinline__ void bulk_s2g(void *to, const void *from, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(smem_u32(from)), "r"(bytes) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ uint32_t elect_lane() {
     uint32_t one;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
@@ -138,9 +148,88 @@ __device__ __forceinline__ float silu_fast(float x) {
 __device__ __forceinline__ uint32_t at128(int r, int p) { return r * 128 + ((p ^ (r & 7)) << 4); }
 __device__ __forceinline__ uint32_t at_kq(int r, int p) { return (p >> 3) * kPanel + at128(r, p & 7); }
 
+// O in the workspace: 8 rows of the batch, a head, 4 columns, then the row of the 8. The scan has a row in a thread,
+// so its stores are 128 bytes in a row (row by row they were 16 bytes each, and kept shared memory from the
+// other warps for 900 of a chunk's 6400 cycles); the norm reads whole sectors.
+__device__ __forceinline__ long long o_at(const GdnArgs &a, long long row, int vh, int col) {
+    return (((row >> 3) * a.value_heads + vh) * (kD / 4) + (col >> 2)) * 32 + (row & 7) * 4;
+}
+
+// Gated RMS norm of every value head of rows first .. end - 1, 8 rows of a head a warp, a quarter of a row a lane;
+// by warp `warp` of `warps`. O comes from an earlier launch that this one may have run beside: past the L1.
+template <bool kBf16>
+__device__ __forceinline__ void gate_rows(const GdnArgs &a, long long first, long long end, int warp, int warps) {
+    const int lane = threadIdx.x & 31, g = lane >> 3;
+    const long long eight0 = first >> 3, units = first < end ? (((end + 7) >> 3) - eight0) * a.value_heads : 0;
+    using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
+    constexpr int kZ = kBf16 ? 1 : 2;   // 16-byte loads of 8 columns
+    uint2 w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const uint2 *>(a.norm_w + 8 * (4 * (i >> 1) + g) + 4 * (i & 1));
+    for (long long u = warp; u < units; u += warps) {
+        const int vh = (int)(u % a.value_heads);
+        const long long row = ((eight0 + u / a.value_heads) << 3) + (lane & 7);
+        const bool in = row >= first && row < end;
+        const long long src = in ? row : row < first ? first : end - 1;
+        const Raw *zp = static_cast<const Raw *>(a.z) + src * a.z_stride + vh * kD;
+        float4 o[8];
+        uint4 zr[4 * kZ];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = 8 * (4 * i + g);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) o[2 * i + x] = __ldcg(reinterpret_cast<const float4 *>(a.o + o_at(a, src, vh, c + 4 * x)));
+#pragma unroll
+            for (int x = 0; x < kZ; ++x) zr[kZ * i + x] = *reinterpret_cast<const uint4 *>(zp + c + 4 * x);
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += o[i].x * o[i].x + o[i].y * o[i].y + o[i].z * o[i].z + o[i].w * o[i].w;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const float inv = rsqrtf(sum / kD + 1e-6f);
+        const long long at = (row * a.value_heads + vh) * kD;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float z[8], v[8];
+            if constexpr (kBf16) {
+                const uint32_t r[4] = {zr[i].x, zr[i].y, zr[i].z, zr[i].w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) z[2 * j] = bf16_lo(r[j]), z[2 * j + 1] = bf16_hi(r[j]);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint4 r = zr[2 * i + x];
+                    z[4 * x] = __uint_as_float(r.x), z[4 * x + 1] = __uint_as_float(r.y);
+                    z[4 * x + 2] = __uint_as_float(r.z), z[4 * x + 3] = __uint_as_float(r.w);
+                }
+            }
+            const uint32_t wr[4] = {w[2 * i].x, w[2 * i].y, w[2 * i + 1].x, w[2 * i + 1].y};
+            const float ov[8] = {o[2 * i].x,     o[2 * i].y,     o[2 * i].z,     o[2 * i].w,
+                                 o[2 * i + 1].x, o[2 * i + 1].y, o[2 * i + 1].z, o[2 * i + 1].w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = ov[j] * inv * (j & 1 ? bf16_hi(wr[j / 2]) : bf16_lo(wr[j / 2])) * silu_fast(z[j]);
+            if (!in) continue;
+            const long long to = at + 8 * (4 * i + g);
+            if (a.out_bf16) {
+                *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + to) =
+                    make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+            } else {
+                float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + to);
+                p[0] = make_float4(v[0], v[1], v[2], v[3]);
+                p[1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- chunks ---------------------------------------------------------------------------------------
 
-constexpr int kLd = 66;    // K K^T, Q K^T rows
+constexpr int kGateRows = 4;   // rows of the grid that norm the heads of an earlier part
+constexpr int kLd = 68;    // K K^T, Q K^T rows
 constexpr int kLdT = 68;   // T rows
 struct ChunkSmem {
     // K over Q, hi and lo; then, over them, the two heads' T (fp32, later T b's hi and lo in its place) and P's
@@ -159,15 +248,26 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     __shared__ __align__(16) float beta[2][kC];
     __shared__ int scan[kWarps], found[2];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int chunk = blockIdx.x, kh = blockIdx.y;
+    // Rows of the grid: the value heads' norm of part - 2, whose scan is complete, a quarter of a chunk each;
+    // then the key heads. The last CTA returns when the scan of part - 1 has ended, and so does the launch:
+    // what waits for it has all of the parts before.
+    const int gating = a.part >= 2 ? kGateRows : 0;
+    const int kh = (int)blockIdx.y - gating, part = kh < 0 ? a.part - 2 : a.part;
+    const bool last_cta = a.part > 0 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+    pdl_trigger();
 
-    // ---- the chunk's sequence
+    // ---- the chunk's sequence, and its place in it
     if (tid == 0) found[0] = -1;
     {
+        const int chunk = blockIdx.x;
+        auto part_chunks = [&](int b) {
+            const int n = seq_chunks(a, b);
+            return part_first(a, n, part + 1) - part_first(a, n, part);
+        };
         const int per = (a.num_seqs + kThreads - 1) / kThreads;
         const int first = min(a.num_seqs, tid * per), last = min(a.num_seqs, first + per);
         int own = 0;
-        for (int b = first; b < last; ++b) own += seq_chunks(a, b);
+        for (int b = first; b < last; ++b) own += part_chunks(b);
         int inc = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -180,10 +280,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         for (int w = 0; w < warp; ++w) before += scan[w];
         if (chunk >= before && chunk < before + own)
             for (int b = first; b < last; ++b) {
-                const int n = seq_chunks(a, b);
+                const int n = part_chunks(b);
                 if (chunk < before + n) {
                     found[0] = b;
-                    found[1] = chunk - before;
+                    found[1] = chunk - before + part_first(a, seq_chunks(a, b), part);
                     break;
                 }
                 before += n;
@@ -191,8 +291,21 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         __syncthreads();
     }
     const int b = found[0];
-    if (b < 0) return;   // fewer chunks than the grid has room for
+    if (b < 0) {   // fewer chunks than the grid has room for
+        if (last_cta) pdl_wait();
+        return;
+    }
     const int row0 = seq_first(a, b), in_seq = found[1] * kC, n = min(kC, seq_rows(a, b) - in_seq);
+    if (kh < 0) {
+        gate_rows<kBf16>(a, row0 + in_seq, row0 + in_seq + n, (kh + kGateRows) * kWarps + warp, kGateRows * kWarps);
+        return;
+    }
+    // number in the workspace: over all chunks of all sequences
+    int chunk = blockIdx.x;
+    if (a.parts > 1) {
+        chunk = found[1];
+        for (int i = 0; i < b; ++i) chunk += seq_chunks(a, i);
+    }
     const uint32_t sm = smem_u32(smem);
 
     const int ratio = a.value_heads / a.key_heads;
@@ -269,37 +382,51 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             }
             const float scale = side ? kScaleK * 0.08838834764831845f : kScaleQ / kD;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int t = t0 + i;
-                float y[4], ss = 0.f;
+            for (int i0 = 0; i0 < 8; i0 += 4) {
+                float y[4][4], ss[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float s = x[i][j] * bf16_lo(w[side][j].x) + x[i + 1][j] * bf16_hi(w[side][j].x) +
-                                    x[i + 2][j] * bf16_lo(w[side][j].y) + x[i + 3][j] * bf16_hi(w[side][j].y);
-                    y[j] = t < n ? silu_fast(s) : 0.f;
-                    ss = fmaf(y[j], y[j], ss);
+                for (int i = 0; i < 4; ++i) {
+                    ss[i] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float s = x[i0 + i][j] * bf16_lo(w[side][j].x) + x[i0 + i + 1][j] * bf16_hi(w[side][j].x) +
+                                        x[i0 + i + 2][j] * bf16_lo(w[side][j].y) + x[i0 + i + 3][j] * bf16_hi(w[side][j].y);
+                        y[i][j] = t0 + i0 + i < n ? silu_fast(s) : 0.f;
+                        ss[i] = fmaf(y[i][j], y[i][j], ss[i]);
+                    }
                 }
-                const float inv = rsqrtf(warp_sum(ss) / kD + 1e-12f) * scale;
-                uint32_t h0, l0, h1, l1;
-                const uint32_t at = at_kq(side ? t : kC + t, lane >> 1) + (lane & 1) * 8;
-                split2(y[0] * inv, y[1] * inv, h0, l0);
-                split2(y[2] * inv, y[3] * inv, h1, l1);
-                *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h0, h1);
-                *reinterpret_cast<uint2 *>(smem + kTileX + at) = make_uint2(l0, l1);
+                // the four sums over the warp together: a lane keeps half of them in each of two exchanges, so
+                // that lane l ends with that of token l & 3 and takes its root
+                const bool odd = lane & 1, upper = lane & 2;
+                const float a0 = (odd ? ss[1] : ss[0]) + __shfl_xor_sync(0xffffffffu, odd ? ss[0] : ss[1], 1);
+                const float a1 = (odd ? ss[3] : ss[2]) + __shfl_xor_sync(0xffffffffu, odd ? ss[2] : ss[3], 1);
+                float sum = (upper ? a1 : a0) + __shfl_xor_sync(0xffffffffu, upper ? a0 : a1, 2);
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                const float root = rsqrtf(sum / kD + 1e-12f) * scale;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + i0 + i;
+                    const float inv = __shfl_sync(0xffffffffu, root, i);
+                    uint32_t h0, l0, h1, l1;
+                    const uint32_t at = at_kq(side ? t : kC + t, lane >> 1) + (lane & 1) * 8;
+                    split2(y[i][0] * inv, y[i][1] * inv, h0, l0);
+                    split2(y[i][2] * inv, y[i][3] * inv, h1, l1);
+                    *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h0, h1);
+                    *reinterpret_cast<uint2 *>(smem + kTileX + at) = make_uint2(l0, l1);
+                }
             }
         }
     }
+    fence_async_smem();
     __syncthreads();
-    {   // the tile images into the workspace
-        uint4 *dst = reinterpret_cast<uint4 *>(a.kq + ((long long)chunk * a.key_heads + kh) * 2 * kTileX);
-#pragma unroll 4
-        for (int i = tid; i < 2 * kTileX / 16; i += kThreads) dst[i] = reinterpret_cast<const uint4 *>(smem)[i];
-    }
+    if (tid == 0)   // the tile images into the workspace, while K K^T is made of them
+        bulk_s2g(a.kq + ((long long)chunk * a.key_heads + kh) * 2 * kTileX, smem, 2 * kTileX);
     // ---- K K^T and Q K^T, the 16 x 16 blocks on and below the diagonal: 20 of them over the warps
     for (int u = warp; u < 20; u += kWarps) {
         const int v = u % 10, i = v < 1 ? 0 : v < 3 ? 1 : v < 6 ? 2 : 3, j = v - i * (i + 1) / 2;
         const int ra = u < 10 ? 0 : kC;   // K's rows, or Q's
-        float c[2][4] = {};
+        float c[2][3][4] = {};   // hi hi, lo hi, hi lo: chains of their own
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk) {
             uint32_t ah[4], al[4], bh[4], bl[4];
@@ -311,18 +438,22 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             ldsm4(sm + kTileX + pb, bl);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                mma_f16(c[x], al, bh[2 * x], bh[2 * x + 1]);
-                mma_f16(c[x], ah, bl[2 * x], bl[2 * x + 1]);
-                mma_f16(c[x], ah, bh[2 * x], bh[2 * x + 1]);
+                mma_f16(c[x][0], ah, bh[2 * x], bh[2 * x + 1]);
+                mma_f16(c[x][1], al, bh[2 * x], bh[2 * x + 1]);
+                mma_f16(c[x][2], ah, bl[2 * x], bl[2 * x + 1]);
             }
         }
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) c[x][0][y] += c[x][1][y] + c[x][2][y];
         float *to = reinterpret_cast<float *>(smem + (u < 10 ? ChunkSmem::kKK : ChunkSmem::kQK));
         const float s = u < 10 ? 1.f / (kScaleK * kScaleK) : 1.f / kScaleK;   // Q K^T keeps the scale of q: P does
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             float *p = to + (16 * i + (lane >> 2)) * kLd + 16 * j + 8 * x + 2 * (lane & 3);
-            *reinterpret_cast<float2 *>(p) = make_float2(c[x][0] * s, c[x][1] * s);
-            *reinterpret_cast<float2 *>(p + 8 * kLd) = make_float2(c[x][2] * s, c[x][3] * s);
+            *reinterpret_cast<float2 *>(p) = make_float2(c[x][0][0] * s, c[x][0][1] * s);
+            *reinterpret_cast<float2 *>(p + 8 * kLd) = make_float2(c[x][0][2] * s, c[x][0][3] * s);
         }
     }
     const float *kkt = reinterpret_cast<const float *>(smem + ChunkSmem::kKK);
@@ -336,131 +467,183 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT + half * ChunkSmem::kTBytes);
         uint8_t *P = smem + ChunkSmem::kP + half * ChunkSmem::kPBytes;
         float *scratch = reinterpret_cast<float *>(smem + ChunkSmem::kScratch) + warp * 256;
+        auto head_sync = [&] { bar_sync(1 + half, 128); };
+        // what was copied out of this shared memory has been read
+        if (t128 == 0) bulk_wait_read();
         if (v0 > 0) gates_of(v0);
         __syncthreads();   // also: K K^T, Q K^T are complete, and K and Q are read
         if (on) {
             float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
             if (t128 < kC) gates[t128] = expf(G[half][t128].x + G[half][t128].y);
-            // M below the diagonal; P with its diagonal
-            for (int i = t128; i < kC * kC / 8; i += 128) {
-                const int t = i >> 3, s0 = (i & 7) * 8;
+            // M below the diagonal; P with its diagonal. Rows r and 63 - r have nine groups of 8 columns on or below
+            // the diagonal between them: eight lanes take one each, and an element each of the ninth.
+            const int lane8 = t128 & 7;
+#pragma unroll
+            for (int r = t128 >> 3; r < 32; r += 16) {
+                const int far = 63 - r, groups = 8 - (r >> 3);   // of row `far`
+                const int t = lane8 < groups ? far : r, grp = lane8 < groups ? lane8 : lane8 - groups, s0 = grp * 8;
+                const float2 g = G[half][t];
+                const float bt = beta[half][t];
                 float p[8], m[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[j] = m[j] = 0.f;
-                if (s0 <= t) {
+                for (int j = 0; j < 8; j += 4) {
+                    const float4 q = *reinterpret_cast<const float4 *>(qkt + t * kLd + s0 + j);
+                    const float4 k = *reinterpret_cast<const float4 *>(kkt + t * kLd + s0 + j);
+                    p[j] = q.x, p[j + 1] = q.y, p[j + 2] = q.z, p[j + 3] = q.w;
+                    m[j] = k.x, m[j + 1] = k.y, m[j + 2] = k.z, m[j + 3] = k.w;
+                }
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int s = s0 + j;
-                        const float e = s <= t ? __expf(diff(t, s)) : 0.f;   // at most 1: 2^-22 or so of it, and of 1
-                        p[j] = s <= t ? e * qkt[t * kLd + s] : 0.f;
-                        m[j] = s < t ? beta[half][t] * e * kkt[t * kLd + s] : 0.f;
-                    }
+                for (int j = 0; j < 8; j += 2) {
+                    const float4 gs = *reinterpret_cast<const float4 *>(&G[half][s0 + j]);   // of two columns
+                    const float e0 = __expf((g.x - gs.x) + (g.y - gs.y)), e1 = __expf((g.x - gs.z) + (g.y - gs.w));
+                    p[j] = s0 + j <= t ? e0 * p[j] : 0.f;   // e at most 1: 2^-22 or so of it, and of 1
+                    p[j + 1] = s0 + j + 1 <= t ? e1 * p[j + 1] : 0.f;
+                    m[j] = s0 + j < t ? bt * e0 * m[j] : 0.f;
+                    m[j + 1] = s0 + j + 1 < t ? bt * e1 * m[j + 1] : 0.f;
                 }
                 *reinterpret_cast<float4 *>(T + t * kLdT + s0) = make_float4(m[0], m[1], m[2], m[3]);
                 *reinterpret_cast<float4 *>(T + t * kLdT + s0 + 4) = make_float4(m[4], m[5], m[6], m[7]);
                 uint32_t h[4], l[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) split2(p[2 * j], p[2 * j + 1], h[j], l[j]);
-                *reinterpret_cast<uint4 *>(P + at128(t, i & 7)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(P + kC * 128 + at128(t, i & 7)) = make_uint4(l[0], l[1], l[2], l[3]);
+                *reinterpret_cast<uint4 *>(P + at128(t, grp)) = make_uint4(h[0], h[1], h[2], h[3]);
+                *reinterpret_cast<uint4 *>(P + kC * 128 + at128(t, grp)) = make_uint4(l[0], l[1], l[2], l[3]);
+                const int last = r >> 3, s = 8 * last + lane8;   // row r's group on the diagonal
+                const float e = __expf(diff(r, min(s, r)));
+                T[r * kLdT + s] = s < r ? beta[half][r] * e * kkt[r * kLd + s] : 0.f;
+                uint32_t hi, lo;
+                split2(s <= r ? e * qkt[r * kLd + s] : 0.f, 0.f, hi, lo);
+                *reinterpret_cast<uint16_t *>(P + at128(r, last) + 2 * lane8) = (uint16_t)hi;
+                *reinterpret_cast<uint16_t *>(P + kC * 128 + at128(r, last) + 2 * lane8) = (uint16_t)lo;
+                // the other group of a 16 x 16 block on the diagonal, in the one of the two rows where it is above it
+                const int above = r & 8 ? far : r;
+                if (lane8 < 2) *reinterpret_cast<uint4 *>(P + lane8 * kC * 128 + at128(above, (above >> 3) + 1)) = make_uint4(0, 0, 0, 0);
             }
-        }
-        __syncthreads();
-        // (I + M)^-1 by 16 x 16 blocks: the diagonal ones by substitution, a lane per column, ..
-        if (on && lane < 16) {
-            const float *m = T + 16 * q4 * kLdT + 16 * q4;
-            float x[16];
+            head_sync();
+            // (I + M)^-1. The 16 x 16 blocks on the diagonal by substitution, a lane per column, ..
+            if (lane < 16) {
+                const float *m = T + 16 * q4 * kLdT + 16 * q4;
+                float x[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float s = i == lane ? 1.f : 0.f;
+                for (int i = 0; i < 16; ++i) x[i] = i == lane ? 1.f : 0.f;
 #pragma unroll
-                for (int k = 0; k < i; ++k) s = fmaf(-m[i * kLdT + k], x[k], s);
-                x[i] = s;
+                for (int i = 1; i < 16; ++i)
+#pragma unroll
+                    for (int k = 0; k < i; k += 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(m + i * kLdT + k);
+                        x[i] = fmaf(-v.x, x[k], x[i]);
+                        if (k + 1 < i) x[i] = fmaf(-v.y, x[k + 1], x[i]);
+                        if (k + 2 < i) x[i] = fmaf(-v.z, x[k + 2], x[i]);
+                        if (k + 3 < i) x[i] = fmaf(-v.w, x[k + 3], x[i]);
+                    }
+                __syncwarp(0xffffu);
+                float *to = T + 16 * q4 * kLdT + 16 * q4 + lane;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) to[i * kLdT] = x[i];
             }
-            __syncwarp(0xffffu);
-            float *to = T + 16 * q4 * kLdT + 16 * q4 + lane;
+            head_sync();
+            // .. then the block below of each 32 x 32 block, and of the whole: -T_22 (M_21 T_11), 8 columns a warp,
+            // four of a row a lane (of two rows, in the second)
+            const int lr = lane & 15, lc = (lane >> 4) * 4;
+            auto add = [&](float *acc, const float *m, const float *u, int ldu) {   // acc += m[0..3] u[0..3][0..3]
+                const float4 f = *reinterpret_cast<const float4 *>(m);
+                const float mm[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to[i * kLdT] = x[i];
-        }
-        __syncthreads();
-        // .. then block row i: T_ij = -T_ii sum_{j<=k<i} M_ik T_kj, a warp per j; a lane holds 8 columns of a row
-        for (int i = 1; i < 4; ++i) {
-            const int j = q4, r = lane & 15, c = (lane >> 4) * 8;
-            float acc[8] = {};
-            if (on && j < i) {
-#pragma unroll 8
-                for (int k = 16 * j; k < 16 * i; ++k) {
-                    const float m = T[(16 * i + r) * kLdT + k];
-                    const float4 u = *reinterpret_cast<const float4 *>(T + k * kLdT + 16 * j + c);
-                    const float4 w = *reinterpret_cast<const float4 *>(T + k * kLdT + 16 * j + c + 4);
-                    acc[0] = fmaf(m, u.x, acc[0]), acc[1] = fmaf(m, u.y, acc[1]), acc[2] = fmaf(m, u.z, acc[2]);
-                    acc[3] = fmaf(m, u.w, acc[3]), acc[4] = fmaf(m, w.x, acc[4]), acc[5] = fmaf(m, w.y, acc[5]);
-                    acc[6] = fmaf(m, w.z, acc[6]), acc[7] = fmaf(m, w.w, acc[7]);
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = *reinterpret_cast<const float4 *>(u + k * ldu);
+                    acc[0] = fmaf(mm[k], v.x, acc[0]), acc[1] = fmaf(mm[k], v.y, acc[1]);
+                    acc[2] = fmaf(mm[k], v.z, acc[2]), acc[3] = fmaf(mm[k], v.w, acc[3]);
                 }
-                *reinterpret_cast<float4 *>(scratch + r * 16 + c) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                *reinterpret_cast<float4 *>(scratch + r * 16 + c + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-                __syncwarp();
+            };
+            auto put = [&](float *to, const float *v, float sign) {
+                *reinterpret_cast<float4 *>(to) = make_float4(sign * v[0], sign * v[1], sign * v[2], sign * v[3]);
+            };
+            {
+                const int d = 32 * (q4 >> 1), col = d + 8 * (q4 & 1) + lc;
+                float acc[4] = {};
 #pragma unroll
-                for (int x = 0; x < 8; ++x) acc[x] = 0.f;
+                for (int k = 0; k < 16; k += 4) add(acc, T + (d + 16 + lr) * kLdT + d + k, T + (d + k) * kLdT + col, kLdT);
+                put(scratch + lr * 8 + lc, acc, 1.f);
+                head_sync();   // M_21 is read
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const float m = -T[(16 * i + r) * kLdT + 16 * i + k];
-                    const float4 u = *reinterpret_cast<const float4 *>(scratch + k * 16 + c);
-                    const float4 w = *reinterpret_cast<const float4 *>(scratch + k * 16 + c + 4);
-                    acc[0] = fmaf(m, u.x, acc[0]), acc[1] = fmaf(m, u.y, acc[1]), acc[2] = fmaf(m, u.z, acc[2]);
-                    acc[3] = fmaf(m, u.w, acc[3]), acc[4] = fmaf(m, w.x, acc[4]), acc[5] = fmaf(m, w.y, acc[5]);
-                    acc[6] = fmaf(m, w.z, acc[6]), acc[7] = fmaf(m, w.w, acc[7]);
+                for (int x = 0; x < 4; ++x) acc[x] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) add(acc, T + (d + 16 + lr) * kLdT + d + 16 + k, scratch + k * 8 + lc, 8);
+                put(T + (d + 16 + lr) * kLdT + col, acc, -1.f);
+                head_sync();
+            }
+            {
+                const int col = 8 * q4 + lc;
+                float x0[4] = {}, x1[4] = {};   // rows lr, lr + 16
+#pragma unroll 2
+                for (int k = 8 * q4; k < 32; k += 4) {   // T_11 is zero above its diagonal
+                    add(x0, T + (32 + lr) * kLdT + k, T + k * kLdT + col, kLdT);
+                    add(x1, T + (48 + lr) * kLdT + k, T + k * kLdT + col, kLdT);
                 }
+                put(scratch + lr * 8 + lc, x0, 1.f);
+                put(scratch + (lr + 16) * 8 + lc, x1, 1.f);
+                head_sync();
+#pragma unroll
+                for (int x = 0; x < 4; ++x) x0[x] = x1[x] = 0.f;
+#pragma unroll 2
+                for (int k = 0; k < 16; k += 4) {
+                    add(x0, T + (32 + lr) * kLdT + 32 + k, scratch + k * 8 + lc, 8);
+                    add(x1, T + (48 + lr) * kLdT + 32 + k, scratch + k * 8 + lc, 8);
+                }
+#pragma unroll 2
+                for (int k = 16; k < 32; k += 4) add(x1, T + (48 + lr) * kLdT + 32 + k, scratch + k * 8 + lc, 8);
+                put(T + (32 + lr) * kLdT + col, x0, -1.f);
+                put(T + (48 + lr) * kLdT + col, x1, -1.f);
+                head_sync();
             }
-            __syncthreads();   // every M of the block row is read
-            if (on && j < i) {
-                float *to = T + (16 * i + r) * kLdT + 16 * j + c;
-                *reinterpret_cast<float4 *>(to) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                *reinterpret_cast<float4 *>(to + 4) = make_float4(acc[4], acc[5], acc[6], acc[7]);
-            }
-            __syncthreads();
-        }
-        // e^{G_63 - G} T b, whose product with R is W, into the workspace; T b itself in T's place, for P T b (a
-        // thread holds four 16-byte pieces of it meanwhile)
-        uint4 *to = reinterpret_cast<uint4 *>(a.tp + ((long long)chunk * a.value_heads + vh) * 2 * kTileT);
-        uint32_t th[4][4], tl[4][4];
-        if (on)
+            // e^{G_63 - G} T b, whose product with R is W, into the workspace; T b itself in T's place, for P T b (a
+            // thread holds four 16-byte pieces of it meanwhile)
+            uint8_t *to = a.tp + ((long long)chunk * a.value_heads + vh) * 2 * kTileT;
+            uint32_t th[4][4], tl[4][4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int i = t128 + 128 * x, t = i >> 3, s0 = (i & 7) * 8;
                 const float left = __expf(diff(kC - 1, t));
-                uint32_t wh[4], wl[4];
+                uint32_t wh[4] = {}, wl[4] = {};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int s = s0 + 2 * j;
-                    const float t0 = T[t * kLdT + s] * beta[half][s], t1 = T[t * kLdT + s + 1] * beta[half][s + 1];
-                    split2(t0, t1, th[x][j], tl[x][j]);
-                    split2(t0 * left, t1 * left, wh[j], wl[j]);
+                for (int j = 0; j < 4; ++j) th[x][j] = tl[x][j] = 0;
+                if (s0 <= t) {   // T holds nothing above its blocks on the diagonal, and zeros within them
+                    const float4 t0 = *reinterpret_cast<const float4 *>(T + t * kLdT + s0);
+                    const float4 t1 = *reinterpret_cast<const float4 *>(T + t * kLdT + s0 + 4);
+                    const float4 b0 = *reinterpret_cast<const float4 *>(&beta[half][s0]);
+                    const float4 b1 = *reinterpret_cast<const float4 *>(&beta[half][s0 + 4]);
+                    const float v[8] = {t0.x * b0.x, t0.y * b0.y, t0.z * b0.z, t0.w * b0.w,
+                                        t1.x * b1.x, t1.y * b1.y, t1.z * b1.z, t1.w * b1.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        split2(v[2 * j], v[2 * j + 1], th[x][j], tl[x][j]);
+                        split2(v[2 * j] * left, v[2 * j + 1] * left, wh[j], wl[j]);
+                    }
                 }
-                const int at = at128(t, i & 7) / 16;
-                to[at] = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-                to[kTileT / 16 + at] = make_uint4(wl[0], wl[1], wl[2], wl[3]);
+                const int at = at128(t, i & 7);
+                *reinterpret_cast<uint4 *>(to + at) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
+                *reinterpret_cast<uint4 *>(to + kTileT + at) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
             }
-        __syncthreads();
-        uint8_t *TB = reinterpret_cast<uint8_t *>(T);
-        if (on)
+            head_sync();
+            uint8_t *TB = reinterpret_cast<uint8_t *>(T);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int i = t128 + 128 * x, at = at128(i >> 3, i & 7);
                 *reinterpret_cast<uint4 *>(TB + at) = make_uint4(th[x][0], th[x][1], th[x][2], th[x][3]);
                 *reinterpret_cast<uint4 *>(TB + kC * 128 + at) = make_uint4(tl[x][0], tl[x][1], tl[x][2], tl[x][3]);
             }
-        __syncthreads();
-        // P T b: 16 rows a warp, the columns in pairs of 8; lower triangular as both are
-        float c[4][2][4] = {};
-        if (on)
+            head_sync();
+            // P T b: 16 rows a warp, the columns in pairs of 8; lower triangular as both are, so the two heads'
+            // blocks of rows run in opposite orders over the warp schedulers
+            const int rb = half ? 3 - q4 : q4;
+            float c[4][2][4] = {};
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int k = j; k < 4; ++k)
-                    if (k <= q4) {
+                    if (k <= rb) {
                         uint32_t ah[4], al[4], bh[4], bl[4];
-                        const uint32_t pa = smem_u32(P) + at128(16 * q4 + (lane & 15), 2 * k + (lane >> 4));
+                        const uint32_t pa = smem_u32(P) + at128(16 * rb + (lane & 15), 2 * k + (lane >> 4));
                         const uint32_t pb = smem_u32(TB) + at128(16 * k + (lane & 15), 2 * j + (lane >> 4));
                         ldsm4(pa, ah);
                         ldsm4(pa + kC * 128, al);
@@ -473,8 +656,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                             mma_f16(c[j][x], ah, bh[2 * x], bh[2 * x + 1]);
                         }
                     }
-        __syncwarp();   // a warp reads and writes its own rows of P
-        if (on)
+            __syncwarp();   // a warp reads and writes its own rows of P
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint32_t h[4], l[4];
@@ -483,21 +665,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                     split2(c[j][x][0], c[j][x][1], h[2 * x], l[2 * x]);
                     split2(c[j][x][2], c[j][x][3], h[2 * x + 1], l[2 * x + 1]);
                 }
-                const uint32_t at = smem_u32(P) + at128(16 * q4 + (lane & 15), 2 * j + (lane >> 4));
+                const uint32_t at = smem_u32(P) + at128(16 * rb + (lane & 15), 2 * j + (lane >> 4));
                 stsm4(at, h[0], h[1], h[2], h[3]);
                 stsm4(at + kC * 128, l[0], l[1], l[2], l[3]);
             }
-        __syncthreads();
-        if (on) {
-            constexpr int kHalf = kC * 128 / 16;   // 16-byte pieces of 64 rows
-#pragma unroll 4
-            for (int i = t128; i < 2 * kHalf; i += 128) {   // P T b below it, hi and lo
-                const int part = i / kHalf, x = i - part * kHalf;
-                to[(2 * part + 1) * kHalf + x] = reinterpret_cast<const uint4 *>(P + part * kC * 128)[x];
-            }
+            fence_async_smem();
+            head_sync();
+            if (t128 == 0)   // P T b below T b, hi and lo
+                for (int x = 0; x < 2; ++x) bulk_s2g(to + x * kTileT + kC * 128, P + x * kC * 128, kC * 128);
         }
-        __syncthreads();
     }
+    if (t128 == 0) bulk_wait_read();   // the shared memory stays until it is copied
+    if (last_cta) pdl_wait();
 }
 
 // ---- scan -------------------------------------------------------------------------------------------
@@ -607,23 +786,27 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem;
+    pdl_wait();   // this part's chunks, and with them the parts before
+    pdl_trigger();
     {
         int before = 0;
         for (int i = tid; i < b; i += kScanThreads) before += seq_chunks(a, i);
         if (before) atomicAdd(&S.first_chunk, before);   // integers: the order does not matter
     }
-    const int row0 = seq_first(a, b), rows = seq_rows(a, b), chunks = (rows + kC - 1) / kC;
+    const int all = seq_chunks(a, b), from = part_first(a, all, a.part), chunks = part_first(a, all, a.part + 1) - from;
+    const int row0 = seq_first(a, b) + from * kC, rows = seq_rows(a, b) - from * kC;   // from this part's first on
     const int wg = warp >> 2, r = 32 * (warp & 3) + lane, c0 = 32 * wg;
     const bool is_q = warp < 8 && (warp & 3) >= 2;
 
     // ---- the state: dim r, columns c0 .. c0 + 31
     float St[32];
+    const float *before = a.part > 0 ? a.delta_out : a.delta_in;
     const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN + c0) * kD + r;
     if (warp < 8) {
         float m = 0.f;
 #pragma unroll
         for (int j = 0; j < 32; ++j) {
-            St[j] = a.delta_in ? a.delta_in[s_at + (long long)j * kD] : 0.f;
+            St[j] = before ? __ldcg(before + s_at + (long long)j * kD) : 0.f;   // a launch beside this one wrote them
             m = fmaxf(m, fabsf(St[j]));
         }
 #pragma unroll
@@ -631,7 +814,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         if (lane == 0) atomicMax(&S.vmax[2], __float_as_int(m));   // not negative: ordered as integers
     }
     __syncthreads();
-    const long long chunk0 = S.first_chunk;
+    const long long chunk0 = S.first_chunk + from;
     float bound2 = __int_as_float(S.vmax[2]);   // of |S|^2, per value row
     bound2 = bound2 * bound2 * kD;
     __syncthreads();
@@ -715,7 +898,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             const Raw *p = static_cast<const Raw *>(a.qkv) + ch;
 #pragma unroll
             for (int i = 0; i < 19; ++i) {
-                const int x = min(max(c * kC + vt + i - 3, 0), rows - 1);
+                const int x = min(max(c * kC + vt + i - 3, from > 0 ? -3 : 0), rows - 1);
                 raw[i] = *reinterpret_cast<const Raw2 *>(p + (long long)(row0 + x) * a.qkv_stride);
             }
         };
@@ -732,7 +915,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                     x0[i] = raw[i].x, x1[i] = raw[i].y;
             }
             if (c + 1 < chunks) load_raw(c + 1);
-            if (c == 0 && vt == 0)   // the inputs before the sequence
+            if (from + c == 0 && vt == 0)   // the inputs before the sequence
 #pragma unroll
                 for (int i = 0; i < 3; ++i) {
                     float2 f = make_float2(0.f, 0.f);
@@ -846,7 +1029,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 tc_fence_after();
                 const float k0 = g * pow2(es) * pow2(-eu), s = pow2(eu) * (1.f / kScaleQ);
                 const int row = c * kC + t;
-                float4 *o = reinterpret_cast<float4 *>(a.o + ((long long)(row0 + row) * a.value_heads + vh) * kD + split * kN + c0);
+                float4 *o = reinterpret_cast<float4 *>(a.o + o_at(a, row0 + row, vh, split * kN + c0));
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     float x[16], y[16];
@@ -855,7 +1038,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                     if (row < rows)
 #pragma unroll
                         for (int j = 0; j < 16; j += 4)
-                            o[4 * hf + j / 4] = make_float4(fmaf(k0, x[j], y[j]) * s, fmaf(k0, x[j + 1], y[j + 1]) * s,
+                            o[8 * (4 * hf + j / 4)] = make_float4(fmaf(k0, x[j], y[j]) * s, fmaf(k0, x[j + 1], y[j + 1]) * s,
                                                             fmaf(k0, x[j + 2], y[j + 2]) * s, fmaf(k0, x[j + 3], y[j + 3]) * s);
                 }
             }
@@ -894,8 +1077,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
 // of every channel: after the other launches, so that the states may be updated in place.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) k_gdn_finish(const __grid_constant__ GdnArgs a, int norm_blocks) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = tid >> 5;
     if ((int)blockIdx.x >= norm_blocks) {
+        pdl_wait();
         const long long i = (long long)(blockIdx.x - norm_blocks) * kThreads + tid;
         if (i >= (long long)a.num_seqs * a.channels) return;
         const int b = (int)(i / a.channels), c = (int)(i - (long long)b * a.channels);
@@ -911,64 +1095,78 @@ __global__ void __launch_bounds__(kThreads) k_gdn_finish(const __grid_constant__
         for (int j = 0; j < 3; ++j) a.conv_out[((long long)b * 3 + j) * a.channels + c] = v[j];
         return;
     }
-    const int first = max(0, min(a.cu_rows[0], a.total_rows)), end = min(a.cu_rows[a.num_seqs], a.total_rows);
-    const long long units = (long long)max(0, end - first) * a.value_heads;
-    const uint2 wv = *reinterpret_cast<const uint2 *>(a.norm_w + 4 * lane);
-    const float w[4] = {bf16_lo(wv.x), bf16_hi(wv.x), bf16_lo(wv.y), bf16_hi(wv.y)};
-    constexpr int kAtOnce = 4;   // (row, head) pairs of a warp, one beside the other, on their way together
-    using Raw4 = typename std::conditional<kBf16, uint2, float4>::type;
-    using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
-    for (long long u0 = ((long long)blockIdx.x * kWarps + warp) * kAtOnce; u0 < units; u0 += (long long)norm_blocks * kWarps * kAtOnce) {
-        float4 o[kAtOnce];
-        Raw4 zr[kAtOnce];
-#pragma unroll
-        for (int x = 0; x < kAtOnce; ++x) {
-            const long long u = min(u0 + x, units - 1), r = first + u / a.value_heads;
-            const int vh = (int)(u % a.value_heads);
-            o[x] = *reinterpret_cast<const float4 *>(a.o + (r * a.value_heads + vh) * kD + 4 * lane);
-            zr[x] = *reinterpret_cast<const Raw4 *>(static_cast<const Raw *>(a.z) + r * a.z_stride + vh * kD + 4 * lane);
-        }
-#pragma unroll
-        for (int x = 0; x < kAtOnce; ++x) {
-            if (u0 + x >= units) break;
-            float z[4];
-            if constexpr (kBf16)
-                z[0] = bf16_lo(zr[x].x), z[1] = bf16_hi(zr[x].x), z[2] = bf16_lo(zr[x].y), z[3] = bf16_hi(zr[x].y);
-            else
-                z[0] = zr[x].x, z[1] = zr[x].y, z[2] = zr[x].z, z[3] = zr[x].w;
-            const float inv = rsqrtf(warp_sum(o[x].x * o[x].x + o[x].y * o[x].y + o[x].z * o[x].z + o[x].w * o[x].w) / kD + 1e-6f);
-            const float v0 = o[x].x * inv * w[0] * silu_fast(z[0]), v1 = o[x].y * inv * w[1] * silu_fast(z[1]);
-            const float v2 = o[x].z * inv * w[2] * silu_fast(z[2]), v3 = o[x].w * inv * w[3] * silu_fast(z[3]);
-            const long long at = ((first + (u0 + x) / a.value_heads) * a.value_heads + (u0 + x) % a.value_heads) * kD + 4 * lane;
-            if (a.out_bf16)
-                *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + at) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
-            else
-                *reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at) = make_float4(v0, v1, v2, v3);
+    const int w = blockIdx.x * kWarps + warp, warps = norm_blocks * kWarps;
+    if (a.parts == 1) {
+        pdl_wait();
+        const int first = max(0, min(a.cu_rows[0], a.total_rows)), end = min(a.cu_rows[a.num_seqs], a.total_rows);
+        gate_rows<kBf16>(a, first, end, w, warps);
+        return;
+    }
+    for (int p = a.parts - 2; p < a.parts; ++p) {   // the last but one while the scan of the last runs
+        if (p == a.parts - 1) pdl_wait();
+        for (int b = 0; b < a.num_seqs; ++b) {
+            const int chunks = seq_chunks(a, b), c0 = part_first(a, chunks, p), c1 = part_first(a, chunks, p + 1);
+            const int row0 = seq_first(a, b);
+            gate_rows<kBf16>(a, row0 + c0 * kC, row0 + min(seq_rows(a, b), c1 * kC), w, warps);
         }
     }
 }
 
 long long max_chunks(int num_seqs, int total_rows) { return (long long)total_rows / kC + num_seqs; }
 
+// Into how many parts the chunks go. With one, every launch has the machine to itself in turn. A scan that leaves
+// more than half of the SMs idle runs beside the launch that prepares the next part, on those SMs; a part more
+// costs about 10 us, and what hides is 1 us a chunk of every part but one: best near sqrt(chunks / 10).
+// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1234 us, 2 1163, 4 1105, 5 1074, 6 1127, 8 1130.
+int parts_of(const GdnArgs &a, int sms) {
+    if (2ll * kSplit * a.value_heads * a.num_seqs > sms) return 1;
+    const int chunks = a.total_rows / kC / a.num_seqs;
+    int parts = 1;
+    while (parts < 16 && 10 * (parts + 1) * (parts + 1) <= chunks) ++parts;
+    return parts;
+}
+
+template <class K, class... Args>
+cudaError_t launch_one(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, bool early, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = early ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <bool kBf16>
-cudaError_t launch(const GdnArgs &a, cudaStream_t st) {
-    cudaError_t e = cudaSuccess;
-    if (a.total_rows > 0) {
-        e = cudaFuncSetAttribute(k_gdn_chunks<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ChunkSmem::kBytes);
-        if (e != cudaSuccess) return e;
-        const dim3 grid((unsigned)max_chunks(a.num_seqs, a.total_rows), a.key_heads);
-        k_gdn_chunks<kBf16><<<grid, kThreads, ChunkSmem::kBytes, st>>>(a);
-        if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    }
-    e = cudaFuncSetAttribute(k_gdn_scan<kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem::kBytes + 1024);
+cudaError_t launch(GdnArgs a, cudaStream_t st) {
+    static SmemOnce chunks_smem, scan_smem;
+    cudaError_t e = chunks_smem.set(k_gdn_chunks<kBf16>, ChunkSmem::kBytes);
+    if (e == cudaSuccess) e = scan_smem.set(k_gdn_scan<kBf16>, ScanSmem::kBytes + 1024);
+    int dev = 0, sms = 0;
+    if (e == cudaSuccess) e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
-    k_gdn_scan<kBf16><<<dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem::kBytes + 1024, st>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const long long units = (long long)a.total_rows * a.value_heads, want = (units + 4 * kWarps - 1) / (4 * kWarps);
-    const int norm_blocks = (int)(want < 8 * 148 ? want : 8 * 148);   // 8 CTAs an SM
+    a.parts = parts_of(a, sms);
+    for (a.part = 0; a.part < a.parts; ++a.part) {
+        if (a.total_rows > 0) {
+            // a sequence's part has at most its chunks / parts, rounded up
+            const long long most = max_chunks(a.num_seqs, a.total_rows) / a.parts + (a.parts > 1 ? a.num_seqs : 0);
+            const dim3 grid((unsigned)most, a.key_heads + (a.part >= 2 ? kGateRows : 0));
+            e = launch_one(k_gdn_chunks<kBf16>, grid, kThreads, ChunkSmem::kBytes, st, a.part > 0, a);
+            if (e != cudaSuccess) return e;
+        }
+        e = launch_one(k_gdn_scan<kBf16>, dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem::kBytes + 1024, st,
+                       a.total_rows > 0, a);
+        if (e != cudaSuccess) return e;
+    }
+    const long long want = ((a.total_rows + 14ll) / 8 * a.value_heads + kWarps - 1) / kWarps;   // a warp 8 rows of a head
+    const int norm_blocks = a.total_rows == 0 ? 0 : (int)(want < 8ll * sms ? want : 8ll * sms);
     const long long conv_blocks = ((long long)a.num_seqs * a.channels + kThreads - 1) / kThreads;
-    k_gdn_finish<kBf16><<<(unsigned)(norm_blocks + conv_blocks), kThreads, 0, st>>>(a, norm_blocks);
-    return cudaGetLastError();
+    return launch_one(k_gdn_finish<kBf16>, dim3((unsigned)(norm_blocks + conv_blocks)), kThreads, 0, st, true, a, norm_blocks);
 }
 
 int check_shape(const nmoe_linear_attn_shape *s) {
@@ -990,7 +1188,7 @@ size_t carve(const nmoe_linear_attn_shape &s, int num_seqs, int total_rows, uint
         return p;
     };
     uint8_t *kq = take(chunks * s.key_heads * 2 * kTileX), *tp = take(chunks * s.value_heads * 2 * kTileT);
-    uint8_t *gates = take(chunks * s.value_heads * kGates), *o = take((size_t)total_rows * s.value_heads * kD * 4);
+    uint8_t *gates = take(chunks * s.value_heads * kGates), *o = take(((size_t)total_rows + 7) / 8 * 8 * s.value_heads * kD * 4);
     if (a != nullptr) {
         a->kq = kq;
         a->tp = tp;
@@ -999,8 +1197,6 @@ size_t carve(const nmoe_linear_attn_shape &s, int num_seqs, int total_rows, uint
     }
     return at;
 }
-
-bool aligned_to(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace
 }  // namespace nmoe
