@@ -457,8 +457,8 @@ size_t nmoe_full_attn_step_paged_workspace_bytes(const nmoe_full_attn_shape *sha
  * elements (0: packed; qkv and z rows 16-byte aligned). conv_in / conv_out f32
  * [num_seqs][3][channels], delta_in / delta_out f32 [num_seqs][value_heads][128][128] (in and
  * out may be the same buffer; in may be NULL: zeros, a new sequence). A sequence without rows
- * gets its states unchanged. out [total_rows][value_heads * 128] in out_dtype. Sums, states and
- * norms are fp32. workspace: nmoe_linear_attn_prefill_workspace_bytes(), 16-byte aligned, not
+ * gets its states unchanged. out [total_rows][value_heads * 128] in out_dtype; it overlaps no
+ * input. Sums, states and norms are fp32. workspace: nmoe_linear_attn_prefill_workspace_bytes(), 16-byte aligned, not
  * shared by calls that overlap. Allocates nothing; capturable. */
 typedef struct nmoe_linear_attn_shape {
     int key_heads, value_heads; /* value_heads a multiple of key_heads; Qwen3.6: 16 and 32 */

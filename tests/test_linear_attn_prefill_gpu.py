@@ -180,3 +180,29 @@ def test_no_rows_keep_the_states():
     p = Prompt([0, 0], 1, 1, torch.float32, seed=12)
     out, conv, delta = p.run()
     assert torch.equal(conv, p.conv) and torch.equal(delta, p.delta)
+
+
+@pytest.mark.parametrize("rows,dtype", [([9001], torch.bfloat16), ([17390, 30], torch.float32), ([5200, 0, 70, 5201], torch.float32)])
+def test_prompts_prepared_in_parts(rows, dtype):
+    """Long sequences that leave most of the machine idle: their chunks go in parts, each prepared while
+    the scan of the part before runs, the state handed on through memory. The state in place, one
+    sequence shorter than the parts are many, and the same from a captured graph, replayed twice."""
+    p = Prompt(rows, 1, 2, dtype, seed=13, spare=3)
+    a = p.run(in_place=True)
+    p.check(*a)
+    s = N.LinearAttnShape(1, 2)
+    ws = torch.empty(N.linear_attn_prefill_workspace_bytes(s, len(rows), p.total), dtype=torch.uint8, device="cuda")
+    out, conv, delta = torch.full_like(a[0], 7.0), torch.empty_like(p.conv), torch.empty_like(p.delta)
+    code = N.DTYPE_BF16 if dtype == torch.bfloat16 else N.DTYPE_F32
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        N.linear_attn_prefill(p.w, s, p.qkv, p.z, p.alpha, p.beta, p.cu, p.conv, p.delta, conv, delta, out, ws,
+                              x_dtype=code, out_dtype=N.DTYPE_F32, stream=side.cuda_stream)
+    for _ in range(2):
+        ws.fill_(255)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(a, (out, conv, delta)):
+            assert torch.equal(x, y)
