@@ -93,7 +93,9 @@ __device__ __forceinline__ int seq_rows(const GdnArgs &a, int b) {
 }
 __device__ __forceinline__ int seq_chunks(const GdnArgs &a, int b) { return (seq_rows(a, b) + kC - 1) / kC; }
 // first of the `chunks` chunks of a sequence that belongs to part p
-__device__ __forceinline__ int part_first(const GdnArgs &a, int chunks, int p) { return (int)((long long)chunks * p / a.parts); }
+__device__ __forceinline__ int part_first(const GdnArgs &a, int chunks, int p) {
+    return a.parts == 1 ? p * chunks : (int)((unsigned)chunks * p / (unsigned)a.parts);   // at most 2^25 chunks, 16 parts
+}
 
 // x = hi + lo in fp16, two values at a time: hi is x rounded to 11 bits by an integer addition, which fp16
 // holds as it is, so that lo comes out of one subtraction (unpacking a converted hi goes through the slow
@@ -226,27 +228,78 @@ __device__ __forceinline__ void gate_rows(const GdnArgs &a, long long first, lon
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// One thread of a converged warp issues (`one` != 0): M = 128, N = 64, fp16, fp32 sums.
+__device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t *bar, uint32_t one) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(one)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t idesc_f16(int a_mn, int b_mn) {
+    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(kN >> 3) << 17) | (8u << 24);
+}
+// rows are the sum's index, 64 columns a row; further columns `panel` bytes away
+__device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t panel) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+// Polls (a suspended wait wakes some hundred cycles later, five times a chunk). Bounded: a barrier that
+// never completes sets `stop`, and every later wait goes at once.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
+    for (uint32_t n = 0;; ++n) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if ((n & 1023) == 1023 && *stop) return false;
+        if (n >= kMaxSpins) {
+            *stop = 1;
+            return false;
+        }
+    }
+}
+
 // ---- chunks ---------------------------------------------------------------------------------------
 
 constexpr int kGateRows = 4;   // rows of the grid that norm the heads of an earlier part
-constexpr int kLd = 68;    // K K^T, Q K^T rows
 constexpr int kLdT = 68;   // T rows
 struct ChunkSmem {
     // K over Q, hi and lo; then, over them, the two heads' T (fp32, later T b's hi and lo in its place) and P's
     // (later P T b's) hi and lo
     static constexpr int kT = 0, kTBytes = kC * kLdT * 4, kP = 2 * kTBytes, kPBytes = 2 * kC * 128;
-    static constexpr int kScratch = kP + 2 * kPBytes;            // 16 x 16 a warp
-    static constexpr int kKK = kScratch + kWarps * 256 * 4, kQK = kKK + kC * kLd * 4;
-    static constexpr int kBytes = kQK + kC * kLd * 4;
+    static constexpr int kScratch = kP + 2 * kPBytes;            // 32 x 8 a warp
+    static constexpr int kBytes = kScratch + kWarps * 256 * 4 + 1024;   // and to align it
     static_assert(2 * kTileX <= kScratch, "K and Q end before what is used beside them");
 };
 
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constant__ GdnArgs a) {
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);   // the swizzle goes by the address
     __shared__ __align__(16) float2 G[2][kC];
     __shared__ __align__(16) float beta[2][kC];
-    __shared__ int scan[kWarps], found[2];
+    __shared__ int scan[kWarps], scan_all[kWarps], found[5], stop;
+    __shared__ uint64_t products;
+    __shared__ uint32_t tmem_at;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // Rows of the grid: the value heads' norm of part - 2, whose scan is complete, a quarter of a chunk each;
     // then the key heads. The last CTA returns when the scan of part - 1 has ended, and so does the launch:
@@ -260,34 +313,43 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     if (tid == 0) found[0] = -1;
     {
         const int chunk = blockIdx.x;
-        auto part_chunks = [&](int b) {
-            const int n = seq_chunks(a, b);
-            return part_first(a, n, part + 1) - part_first(a, n, part);
-        };
         const int per = (a.num_seqs + kThreads - 1) / kThreads;
         const int first = min(a.num_seqs, tid * per), last = min(a.num_seqs, first + per);
-        int own = 0;
-        for (int b = first; b < last; ++b) own += part_chunks(b);
-        int inc = own;
+        int own = 0, all = 0, row = 0, rows = 0, from = 0;   // chunks of this part, of all parts; the last sequence's
+        auto one = [&](int b) {
+            row = max(0, min(a.cu_rows[b], a.total_rows));
+            rows = max(0, min(a.cu_rows[b + 1], a.total_rows) - row);
+            const int n = (rows + kC - 1) / kC;
+            from = part_first(a, n, part);
+            all += n;
+            return part_first(a, n, part + 1) - from;
+        };
+        for (int b = first; b < last; ++b) own += one(b);
+        int inc = own, inc_all = all;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
+            const int v = __shfl_up_sync(0xffffffffu, inc, o), w = __shfl_up_sync(0xffffffffu, inc_all, o);
+            if (lane >= o) inc += v, inc_all += w;
         }
-        if (lane == 31) scan[warp] = inc;
+        if (lane == 31) scan[warp] = inc, scan_all[warp] = inc_all;
         __syncthreads();
-        int before = inc - own;
-        for (int w = 0; w < warp; ++w) before += scan[w];
-        if (chunk >= before && chunk < before + own)
-            for (int b = first; b < last; ++b) {
-                const int n = part_chunks(b);
-                if (chunk < before + n) {
-                    found[0] = b;
-                    found[1] = chunk - before + part_first(a, seq_chunks(a, b), part);
-                    break;
+        int before = inc - own, before_all = inc_all - all;
+        for (int w = 0; w < warp; ++w) before += scan[w], before_all += scan_all[w];
+        if (chunk >= before && chunk < before + own) {
+            all = before_all;
+            int b = first, n = own;
+            if (per > 1)
+                for (; b < last; ++b) {
+                    const int at = all;
+                    n = one(b);
+                    if (chunk < before + n) {
+                        all = at;
+                        break;
+                    }
+                    before += n;
                 }
-                before += n;
-            }
+            found[0] = b, found[1] = chunk - before + from, found[2] = row, found[3] = rows, found[4] = all;
+        }
         __syncthreads();
     }
     const int b = found[0];
@@ -295,34 +357,57 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         if (last_cta) pdl_wait();
         return;
     }
-    const int row0 = seq_first(a, b), in_seq = found[1] * kC, n = min(kC, seq_rows(a, b) - in_seq);
+    const int row0 = found[2], in_seq = found[1] * kC, n = min(kC, found[3] - in_seq);
     if (kh < 0) {
         gate_rows<kBf16>(a, row0 + in_seq, row0 + in_seq + n, (kh + kGateRows) * kWarps + warp, kGateRows * kWarps);
         return;
     }
-    // number in the workspace: over all chunks of all sequences
-    int chunk = blockIdx.x;
-    if (a.parts > 1) {
-        chunk = found[1];
-        for (int i = 0; i < b; ++i) chunk += seq_chunks(a, i);
+    const int chunk = found[4] + found[1];   // in the workspace: over all chunks of all sequences
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 64;" ::"r"(smem_u32(&tmem_at)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        mbar_init(&products, 1);
+        mbar_fence_init();
+        stop = 0;
     }
     const uint32_t sm = smem_u32(smem);
 
     const int ratio = a.value_heads / a.key_heads;
     const int half = warp >> 2, q4 = warp & 3, t128 = tid & 127;
     // G: the running sum of log g, in two floats (sums run to -1000 and beyond, and it is differences
-    // that count); a warp per head
-    auto gates_of = [&](int v0) {
-        if (q4 != 3 || v0 + half >= ratio) return;
+    // that count); a warp per head, on different schedulers, two tokens a lane
+    const bool gate_warp = warp == 3 || warp == 6;
+    using Raw1 = typename std::conditional<kBf16, uint16_t, float>::type;
+    Raw1 al_raw[2] = {}, be_raw[2] = {};
+    float a_log = 0.f;
+    uint16_t dt_raw = 0;
+    auto load_gates = [&](int v0) {
+        if (!gate_warp || v0 + half >= ratio) return;
         const int vh = kh * ratio + v0 + half;
-        const float rate = -expf(a.A_log[vh]), dt = bf16_to_f32(a.dt_bias[vh]);
+        a_log = a.A_log[vh];
+        dt_raw = a.dt_bias[vh];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const long long at = (long long)(row0 + in_seq + min(2 * lane + j, n - 1)) * a.ab_stride + vh;
+            al_raw[j] = static_cast<const Raw1 *>(a.alpha)[at];
+            be_raw[j] = static_cast<const Raw1 *>(a.beta)[at];
+        }
+    };
+    auto make_gates = [&](int v0) {
+        if (!gate_warp || v0 + half >= ratio) return;
+        const float rate = -expf(a_log), dt = bf16_to_f32(dt_raw);
         double g[2];
         float bt[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int t = 2 * lane + j;
-            const long long at = (long long)(row0 + in_seq + min(t, n - 1)) * a.ab_stride + vh;
-            const float al = load_x(a.alpha, at, kBf16), be = load_x(a.beta, at, kBf16);
+            float al, be;
+            if constexpr (kBf16)
+                al = bf16_to_f32(al_raw[j]), be = bf16_to_f32(be_raw[j]);
+            else
+                al = al_raw[j], be = be_raw[j];
             g[j] = t < n ? rate * softplus(al + dt) : 0.f;
             bt[j] = t < n ? sigmoidf_(be) : 0.f;
         }
@@ -358,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             w[0][j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (cq + j));
             w[1][j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ck + j));
         }
-        gates_of(0);   // while they are on their way
+        load_gates(0);
 #pragma unroll
         for (int side = 0; side < 2; ++side) {   // q, then k
             float x[11][4];
@@ -419,45 +504,28 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         }
     }
     fence_async_smem();
+    tc_fence_before();
     __syncthreads();
-    if (tid == 0)   // the tile images into the workspace, while K K^T is made of them
-        bulk_s2g(a.kq + ((long long)chunk * a.key_heads + kh) * 2 * kTileX, smem, 2 * kTileX);
-    // ---- K K^T and Q K^T, the 16 x 16 blocks on and below the diagonal: 20 of them over the warps
-    for (int u = warp; u < 20; u += kWarps) {
-        const int v = u % 10, i = v < 1 ? 0 : v < 3 ? 1 : v < 6 ? 2 : 3, j = v - i * (i + 1) / 2;
-        const int ra = u < 10 ? 0 : kC;   // K's rows, or Q's
-        float c[2][3][4] = {};   // hi hi, lo hi, hi lo: chains of their own
+    tc_fence_after();
+    const uint32_t tmem = tmem_at;
+    if (warp == 0) {
+        // K K^T over Q K^T: the products of [K; Q] with K, as the scan takes its operands; and the tile images
+        // into the workspace meanwhile
+        const uint32_t one = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        if (one) bulk_s2g(a.kq + ((long long)chunk * a.key_heads + kh) * 2 * kTileX, smem, 2 * kTileX);
 #pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {
-            uint32_t ah[4], al[4], bh[4], bl[4];
-            const uint32_t pa = at_kq(ra + 16 * i + (lane & 15), 2 * kk + (lane >> 4));
-            const uint32_t pb = at_kq(16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * kk + ((lane >> 3) & 1));
-            ldsm4(sm + pa, ah);
-            ldsm4(sm + kTileX + pa, al);
-            ldsm4(sm + pb, bh);
-            ldsm4(sm + kTileX + pb, bl);
+        for (int x = 0; x < 3; ++x)   // hi hi, lo hi, hi lo
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                mma_f16(c[x][0], ah, bh[2 * x], bh[2 * x + 1]);
-                mma_f16(c[x][1], al, bh[2 * x], bh[2 * x + 1]);
-                mma_f16(c[x][2], ah, bl[2 * x], bl[2 * x + 1]);
+            for (int k = 0; k < kD / 16; ++k) {
+                const uint32_t at = sm + (k >> 2) * kPanel + (k & 3) * 32;
+                mma_one(tm, sw128_desc(at + (x == 1) * kTileX), sw128_desc(at + (x == 2) * kTileX), idesc_f16(0, 0),
+                        x + k > 0 ? 1u : 0u, one);
             }
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) c[x][0][y] += c[x][1][y] + c[x][2][y];
-        float *to = reinterpret_cast<float *>(smem + (u < 10 ? ChunkSmem::kKK : ChunkSmem::kQK));
-        const float s = u < 10 ? 1.f / (kScaleK * kScaleK) : 1.f / kScaleK;   // Q K^T keeps the scale of q: P does
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            float *p = to + (16 * i + (lane >> 2)) * kLd + 16 * j + 8 * x + 2 * (lane & 3);
-            *reinterpret_cast<float2 *>(p) = make_float2(c[x][0][0] * s, c[x][0][1] * s);
-            *reinterpret_cast<float2 *>(p + 8 * kLd) = make_float2(c[x][0][2] * s, c[x][0][3] * s);
-        }
+        commit_one(&products, one);
     }
-    const float *kkt = reinterpret_cast<const float *>(smem + ChunkSmem::kKK);
-    const float *qkt = reinterpret_cast<const float *>(smem + ChunkSmem::kQK);
+    make_gates(0);
+    wait_bar(&products, 0, &stop);
+    tc_fence_after();
 
     // ---- the value heads of the key head, two at a time: four warps each
     auto diff = [&](int t, int s) { return (G[half][t].x - G[half][s].x) + (G[half][t].y - G[half][s].y); };
@@ -469,57 +537,63 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         float *scratch = reinterpret_cast<float *>(smem + ChunkSmem::kScratch) + warp * 256;
         auto head_sync = [&] { bar_sync(1 + half, 128); };
         // what was copied out of this shared memory has been read
-        if (t128 == 0) bulk_wait_read();
-        if (v0 > 0) gates_of(v0);
-        __syncthreads();   // also: K K^T, Q K^T are complete, and K and Q are read
+        if (v0 == 0 ? warp == 0 : t128 == 0) bulk_wait_read();
+        if (v0 > 0) {
+            load_gates(v0);
+            make_gates(v0);
+        }
+        __syncthreads();   // and the products that read K and Q are complete
+        // M below the diagonal, P with its diagonal, of both heads: a thread a row (of K K^T: M; of Q K^T: P) and 32
+        // columns, as the products lie in tensor memory. What is above the 32 x 32 blocks on the diagonal is not read.
+        const int t = 32 * (warp & 1) + lane, c0 = 32 * (warp >> 2);
+        if (c0 <= 32 * (warp & 1)) {
+            const bool is_q = warp & 2;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int s0 = c0 + 16 * hf;
+                float x[16];
+                tc_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + s0, reinterpret_cast<uint32_t *>(x));
+                tc_wait_ld();
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (v0 + h >= ratio) break;
+                    const float2 g = G[h][t];
+                    // Q K^T keeps the scale of q: P does
+                    const float scale = is_q ? 1.f / kScaleK : beta[h][t] * (1.f / (kScaleK * kScaleK));
+                    const int seen = t - s0 + (is_q ? 1 : 0);   // columns
+                    float y[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2) {
+                        const float4 gs = *reinterpret_cast<const float4 *>(&G[h][s0 + j]);   // of two columns
+                        const float e0 = __expf((g.x - gs.x) + (g.y - gs.y)), e1 = __expf((g.x - gs.z) + (g.y - gs.w));
+                        y[j] = j < seen ? scale * e0 * x[j] : 0.f;   // e at most 1: 2^-22 or so of it, and of 1
+                        y[j + 1] = j + 1 < seen ? scale * e1 * x[j + 1] : 0.f;
+                    }
+                    if (!is_q) {
+                        float *to = reinterpret_cast<float *>(smem + ChunkSmem::kT + h * ChunkSmem::kTBytes) + t * kLdT + s0;
+#pragma unroll
+                        for (int j = 0; j < 16; j += 4)
+                            *reinterpret_cast<float4 *>(to + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
+                    } else {
+                        uint8_t *to = smem + ChunkSmem::kP + h * ChunkSmem::kPBytes;
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) split2(y[8 * q + 2 * j], y[8 * q + 2 * j + 1], hi[j], lo[j]);
+                            const int at = at128(t, s0 / 8 + q);
+                            *reinterpret_cast<uint4 *>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                            *reinterpret_cast<uint4 *>(to + kC * 128 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
         if (on) {
             float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
-            if (t128 < kC) gates[t128] = expf(G[half][t128].x + G[half][t128].y);
-            // M below the diagonal; P with its diagonal. Rows r and 63 - r have nine groups of 8 columns on or below
-            // the diagonal between them: eight lanes take one each, and an element each of the ninth.
-            const int lane8 = t128 & 7;
-#pragma unroll
-            for (int r = t128 >> 3; r < 32; r += 16) {
-                const int far = 63 - r, groups = 8 - (r >> 3);   // of row `far`
-                const int t = lane8 < groups ? far : r, grp = lane8 < groups ? lane8 : lane8 - groups, s0 = grp * 8;
-                const float2 g = G[half][t];
-                const float bt = beta[half][t];
-                float p[8], m[8];
-#pragma unroll
-                for (int j = 0; j < 8; j += 4) {
-                    const float4 q = *reinterpret_cast<const float4 *>(qkt + t * kLd + s0 + j);
-                    const float4 k = *reinterpret_cast<const float4 *>(kkt + t * kLd + s0 + j);
-                    p[j] = q.x, p[j + 1] = q.y, p[j + 2] = q.z, p[j + 3] = q.w;
-                    m[j] = k.x, m[j + 1] = k.y, m[j + 2] = k.z, m[j + 3] = k.w;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const float4 gs = *reinterpret_cast<const float4 *>(&G[half][s0 + j]);   // of two columns
-                    const float e0 = __expf((g.x - gs.x) + (g.y - gs.y)), e1 = __expf((g.x - gs.z) + (g.y - gs.w));
-                    p[j] = s0 + j <= t ? e0 * p[j] : 0.f;   // e at most 1: 2^-22 or so of it, and of 1
-                    p[j + 1] = s0 + j + 1 <= t ? e1 * p[j + 1] : 0.f;
-                    m[j] = s0 + j < t ? bt * e0 * m[j] : 0.f;
-                    m[j + 1] = s0 + j + 1 < t ? bt * e1 * m[j + 1] : 0.f;
-                }
-                *reinterpret_cast<float4 *>(T + t * kLdT + s0) = make_float4(m[0], m[1], m[2], m[3]);
-                *reinterpret_cast<float4 *>(T + t * kLdT + s0 + 4) = make_float4(m[4], m[5], m[6], m[7]);
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) split2(p[2 * j], p[2 * j + 1], h[j], l[j]);
-                *reinterpret_cast<uint4 *>(P + at128(t, grp)) = make_uint4(h[0], h[1], h[2], h[3]);
-                *reinterpret_cast<uint4 *>(P + kC * 128 + at128(t, grp)) = make_uint4(l[0], l[1], l[2], l[3]);
-                const int last = r >> 3, s = 8 * last + lane8;   // row r's group on the diagonal
-                const float e = __expf(diff(r, min(s, r)));
-                T[r * kLdT + s] = s < r ? beta[half][r] * e * kkt[r * kLd + s] : 0.f;
-                uint32_t hi, lo;
-                split2(s <= r ? e * qkt[r * kLd + s] : 0.f, 0.f, hi, lo);
-                *reinterpret_cast<uint16_t *>(P + at128(r, last) + 2 * lane8) = (uint16_t)hi;
-                *reinterpret_cast<uint16_t *>(P + kC * 128 + at128(r, last) + 2 * lane8) = (uint16_t)lo;
-                // the other group of a 16 x 16 block on the diagonal, in the one of the two rows where it is above it
-                const int above = r & 8 ? far : r;
-                if (lane8 < 2) *reinterpret_cast<uint4 *>(P + lane8 * kC * 128 + at128(above, (above >> 3) + 1)) = make_uint4(0, 0, 0, 0);
-            }
-            head_sync();
+            // products that never came must not pass for an answer
+            if (t128 < kC) gates[t128] = stop ? NAN : expf(G[half][t128].x + G[half][t128].y);
             // (I + M)^-1. The 16 x 16 blocks on the diagonal by substitution, a lane per column, ..
             if (lane < 16) {
                 const float *m = T + 16 * q4 * kLdT + 16 * q4;
@@ -676,6 +750,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         }
     }
     if (t128 == 0) bulk_wait_read();   // the shared memory stays until it is copied
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 64;" ::"r"(tmem));
     if (last_cta) pdl_wait();
 }
 
@@ -696,56 +774,6 @@ struct ScanShared {
     int vmax[3], first_chunk, stop;
     uint32_t tmem;
 };
-
-// One thread of a converged warp issues (`one` != 0): M = 128, N = 64, fp16, fp32 sums.
-__device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(one)
-        : "memory");
-}
-__device__ __forceinline__ void commit_one(uint64_t *bar, uint32_t one) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-        "r"(one)
-        : "memory");
-}
-__device__ __forceinline__ uint32_t idesc_f16(int a_mn, int b_mn) {
-    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(kN >> 3) << 17) | (8u << 24);
-}
-// rows are the sum's index, 64 columns a row; further columns `panel` bytes away
-__device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t panel) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
-__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr)
-        : "memory");
-}
-// Polls (a suspended wait wakes some hundred cycles later, five times a chunk). Bounded: a barrier that
-// never completes sets `stop`, and every later wait goes at once.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    for (uint32_t n = 0;; ++n) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-        if ((n & 1023) == 1023 && *stop) return false;
-        if (n >= kMaxSpins) {
-            *stop = 1;
-            return false;
-        }
-    }
-}
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
 // The scale 2^-e for values whose square is at most `square`: they come below 2^13, so that fp16 holds
@@ -1117,7 +1145,9 @@ long long max_chunks(int num_seqs, int total_rows) { return (long long)total_row
 // Into how many parts the chunks go. With one, every launch has the machine to itself in turn. A scan that leaves
 // more than half of the SMs idle runs beside the launch that prepares the next part, on those SMs; a part more
 // costs about 10 us, and what hides is 1 us a chunk of every part but one: best near sqrt(chunks / 10).
-// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1234 us, 2 1163, 4 1105, 5 1074, 6 1127, 8 1130.
+// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1230 us, 3 1066, 5 1030, 6 1029, 8 1038, 16 1071.
+// The scan's CTAs come in clusters of two for their place only: those take the two SMs of a TPC. Beside an SM
+// that runs the other kernel a CTA of the scan took 20 % longer (1118 us in all, for 992 us in pairs).
 int parts_of(const GdnArgs &a, int sms) {
     if (2ll * kSplit * a.value_heads * a.num_seqs > sms) return 1;
     const int chunks = a.total_rows / kC / a.num_seqs;
@@ -1127,17 +1157,20 @@ int parts_of(const GdnArgs &a, int sms) {
 }
 
 template <class K, class... Args>
-cudaError_t launch_one(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, bool early, Args... args) {
+cudaError_t launch_one(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, bool early, int cluster, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = early ? 1 : 0;
+    cfg.numAttrs = early ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
@@ -1156,17 +1189,17 @@ cudaError_t launch(GdnArgs a, cudaStream_t st) {
             // a sequence's part has at most its chunks / parts, rounded up
             const long long most = max_chunks(a.num_seqs, a.total_rows) / a.parts + (a.parts > 1 ? a.num_seqs : 0);
             const dim3 grid((unsigned)most, a.key_heads + (a.part >= 2 ? kGateRows : 0));
-            e = launch_one(k_gdn_chunks<kBf16>, grid, kThreads, ChunkSmem::kBytes, st, a.part > 0, a);
+            e = launch_one(k_gdn_chunks<kBf16>, grid, kThreads, ChunkSmem::kBytes, st, a.part > 0, 1, a);
             if (e != cudaSuccess) return e;
         }
         e = launch_one(k_gdn_scan<kBf16>, dim3(kSplit, a.value_heads, a.num_seqs), kScanThreads, ScanSmem::kBytes + 1024, st,
-                       a.total_rows > 0, a);
+                       a.total_rows > 0, kSplit, a);
         if (e != cudaSuccess) return e;
     }
     const long long want = ((a.total_rows + 14ll) / 8 * a.value_heads + kWarps - 1) / kWarps;   // a warp 8 rows of a head
     const int norm_blocks = a.total_rows == 0 ? 0 : (int)(want < 8ll * sms ? want : 8ll * sms);
     const long long conv_blocks = ((long long)a.num_seqs * a.channels + kThreads - 1) / kThreads;
-    return launch_one(k_gdn_finish<kBf16>, dim3((unsigned)(norm_blocks + conv_blocks)), kThreads, 0, st, true, a, norm_blocks);
+    return launch_one(k_gdn_finish<kBf16>, dim3((unsigned)(norm_blocks + conv_blocks)), kThreads, 0, st, true, 1, a, norm_blocks);
 }
 
 int check_shape(const nmoe_linear_attn_shape *s) {
