@@ -55,7 +55,7 @@ int fail(int status, const char *fmt, ...) {
 constexpr int kD = 128, kC = 64;      // head dim, tokens of a chunk
 constexpr int kSplit = 2, kN = kD / kSplit;   // value columns of a scan CTA: 64
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kScanThreads = 448;     // warps 0-7: the rows, 8 and 13: MMAs (8 also the copies), 9-12: V
+constexpr int kScanThreads = 416;     // warps 0-7: the rows, 8: copies and MMAs, 9-12: V
 constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about 1 / 11 and 1 / 128
 
 // Tile images, the same in the workspace and in shared memory: rows of 128 bytes (64 fp16) in 16-byte
@@ -97,15 +97,42 @@ __device__ __forceinline__ int part_first(const GdnArgs &a, int chunks, int p) {
     return a.parts == 1 ? p * chunks : (int)((unsigned)chunks * p / (unsigned)a.parts);   // at most 2^25 chunks, 16 parts
 }
 
-// x = hi + lo in fp16, two values at a time: hi is x rounded to 11 bits by an integer addition, which fp16
-// holds as it is, so that lo comes out of one subtraction (unpacking a converted hi goes through the slow
-// conversion unit)
-__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) {
-    const float hx = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
-    const float hy = __uint_as_float((__float_as_uint(y) + 0x1000u) & 0xffffe000u);
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(hy), "f"(hx));
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(y - hy), "f"(x - hx));
+// Two floats in a register pair, one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
+__device__ __forceinline__ void unpair(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// x = hi + lo in fp16, two values at a time: hi is x rounded to 11 bits (Veltkamp's splitting: t = (2^13 + 1) x,
+// hi = t - (t - x)), which fp16 holds as it is, so that lo comes out of one subtraction (unpacking a
+// converted hi goes through the slow conversion unit)
+__device__ __forceinline__ void split2(uint64_t x, uint32_t &hi, uint32_t &lo) {
+    const uint64_t minus = pair(-1.f, -1.f), t = mul2(x, pair(8193.f, 8193.f));
+    const uint64_t h = fma2(fma2(x, minus, t), minus, t), l = fma2(h, minus, x);
+    float h0, h1, l0, l1;
+    unpair(h, h0, h1);
+    unpair(l, l0, l1);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(h1), "f"(h0));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(l1), "f"(l0));
+}
+__device__ __forceinline__ void split2(float x, float y, uint32_t &hi, uint32_t &lo) { split2(pair(x, y), hi, lo); }
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t *r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -228,7 +255,7 @@ __device__ __forceinline__ void gate_rows(const GdnArgs &a, long long first, lon
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// One thread of a converged warp issues (`one` != 0): M = 128, N = 64, fp16, fp32 sums.
+// One thread of a converged warp issues (`one` != 0): M = 128, fp16, fp32 sums.
 __device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t one) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
@@ -243,8 +270,8 @@ __device__ __forceinline__ void commit_one(uint64_t *bar, uint32_t one) {
         "r"(one)
         : "memory");
 }
-__device__ __forceinline__ uint32_t idesc_f16(int a_mn, int b_mn) {
-    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(kN >> 3) << 17) | (8u << 24);
+__device__ __forceinline__ uint32_t idesc_f16(int a_mn, int b_mn, int n) {
+    return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 // rows are the sum's index, 64 columns a row; further columns `panel` bytes away
 __device__ __forceinline__ uint64_t desc_rows(uint32_t addr, uint32_t panel) {
@@ -518,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
 #pragma unroll
             for (int k = 0; k < kD / 16; ++k) {
                 const uint32_t at = sm + (k >> 2) * kPanel + (k & 3) * 32;
-                mma_one(tm, sw128_desc(at + (x == 1) * kTileX), sw128_desc(at + (x == 2) * kTileX), idesc_f16(0, 0),
+                mma_one(tm, sw128_desc(at + (x == 1) * kTileX), sw128_desc(at + (x == 2) * kTileX), idesc_f16(0, 0, kC),
                         x + k > 0 ? 1u : 0u, one);
             }
         commit_one(&products, one);
@@ -785,8 +812,7 @@ __device__ __forceinline__ int exponent_of(float square) {
 
 // Threads 0-255: row r = 32 (warp % 4) + lane of the 128, columns 32 (warp / 4) .. + 31 of the CTA's 64.
 // Rows 0-63 are tokens (K's rows: R and W), rows 64-127 are tokens too (Q's rows: the output), and all of
-// them are dims of the state. Warps 9-12 convolve V a chunk ahead. Warps 8 and 13 issue half of the MMAs
-// each, into sums of their own: one thread issues one MMA in about 50 cycles, and these run 32.
+// them are dims of the state. Warp 8 issues the MMAs, warps 9-12 convolve V a chunk ahead.
 template <bool kBf16>
 __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
     using L = ScanSmem;
@@ -798,7 +824,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&S.kq_full[i], 1);
-        for (int i = 0; i < 3; ++i) mbar_init(&S.d[i], 2), S.vmax[i] = 0;   // a commit of either issuer
+        for (int i = 0; i < 3; ++i) mbar_init(&S.d[i], 1), S.vmax[i] = 0;
         mbar_init(&S.tp_full, 1);
         mbar_init(&S.r_ready, 4);   // the warps of rows 0-63
         mbar_init(&S.w_ready, 4);
@@ -827,15 +853,17 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     const bool is_q = warp < 8 && (warp & 3) >= 2;
 
     // ---- the state: dim r, columns c0 .. c0 + 31
-    float St[32];
+    uint64_t St[16];
     const float *before = a.part > 0 ? a.delta_out : a.delta_in;
     const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN + c0) * kD + r;
     if (warp < 8) {
         float m = 0.f;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            St[j] = before ? __ldcg(before + s_at + (long long)j * kD) : 0.f;   // a launch beside this one wrote them
-            m = fmaxf(m, fabsf(St[j]));
+        for (int j = 0; j < 16; ++j) {   // a launch beside this one may have written them
+            const float x = before ? __ldcg(before + s_at + (long long)(2 * j) * kD) : 0.f;
+            const float y = before ? __ldcg(before + s_at + (long long)(2 * j + 1) * kD) : 0.f;
+            St[j] = pair(x, y);
+            m = fmaxf(m, fmaxf(fabsf(x), fabsf(y)));
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -848,35 +876,33 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     __syncthreads();
     if (tid == 0) S.vmax[2] = 0;
 
-    if (warp == 8 || warp == 13) {
+    if (warp == 8) {
         // ---- copies and MMAs; every value is the same in all lanes
-        const uint32_t one = elect_lane();
-        const int second = __shfl_sync(0xffffffffu, warp == 13, 0), n = __shfl_sync(0xffffffffu, chunks, 0);
-        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0) + second * 3 * kN;
+        const uint32_t one = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int n = __shfl_sync(0xffffffffu, chunks, 0);
         const uint64_t keep = policy_evict_normal();
         auto copy_kq = [&](int c) {
-            if (!one || second) return;
+            if (!one) return;
             uint64_t *bar = &S.kq_full[c & 1];
             mbar_arrive_expect_tx(bar, L::kStage + kGates);
             bulk_g2s(smem + (c & 1) * L::kStage, a.kq + ((chunk0 + c) * a.key_heads + kh) * 2 * kTileX, L::kStage, bar, keep);
             bulk_g2s(smem + L::kGate + (c & 1) * kGates, a.gates + ((chunk0 + c) * a.value_heads + vh) * kGates, kGates, bar, keep);
         };
         auto copy_tp = [&](int c) {
-            if (!one || second) return;
+            if (!one) return;
             mbar_arrive_expect_tx(&S.tp_full, 2 * kTileT);
             bulk_g2s(smem + L::kTP, a.tp + ((chunk0 + c) * a.value_heads + vh) * 2 * kTileT, 2 * kTileT, &S.tp_full, keep);
         };
         auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop)); };
-        // The products of `steps` k-steps: the first issuer takes hi hi and half of lo hi, the second hi lo and
-        // the other half. A's and B's address of k-step k, part (0 hi, 1 lo).
-        auto issue = [&](uint32_t d, uint32_t idesc, auto steps, auto at_a, auto at_b) {
+        // The products of kSteps k-steps: A's hi with B's hi and lo, which lie side by side as 128 columns (one
+        // reading of A for both: these are bound by shared memory), then A's lo with B's hi onto the first 64.
+        // A's address of k-step k, part (0 hi, 1 lo); B's of k-step k.
+        auto issue = [&](uint32_t d, int a_mn, auto steps, auto at_a, auto at_b) {
             constexpr int kSteps = decltype(steps)::value;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k)
-                mma_one(d, at_a(k, 0), at_b(k, second), idesc, k > 0 ? 1u : 0u, one);
+            for (int k = 0; k < kSteps; ++k) mma_one(d, at_a(k, 0), at_b(k), idesc_f16(a_mn, 1, 2 * kN), k > 0 ? 1u : 0u, one);
 #pragma unroll
-            for (int k = 0; k < kSteps / 2; ++k)
-                mma_one(d, at_a(k + second * (kSteps / 2), 1), at_b(k + second * (kSteps / 2), 0), idesc, 1u, one);
+            for (int k = 0; k < kSteps; ++k) mma_one(d, at_a(k, 1), at_b(k), idesc_f16(a_mn, 1, kN), 1u, one);
         };
         if (n > 0) {
             copy_kq(0);
@@ -885,23 +911,23 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         }
         for (int c = 0; c < n; ++c) {
             const uint32_t st = sm + (c & 1) * L::kStage;
-            auto state_rows = [&](int k, int part) { return desc_rows(sm + L::kS + part * L::kTileS + k * 2048, 0); };
-            auto token_rows = [&](int k, int part) { return desc_rows(sm + L::kR + part * L::kTileR + k * 2048, 0); };
+            auto state_rows = [&](int k) { return desc_rows(sm + L::kS + k * 2048, L::kTileS); };
+            auto token_rows = [&](int k) { return desc_rows(sm + L::kR + k * 2048, L::kTileR); };
             if (!wait(&S.kq_full[c & 1], (c >> 1) & 1) || !wait(&S.s_ready, c & 1)) break;
             tc_fence_after();
-            issue(tm, idesc_f16(0, 1), std::integral_constant<int, kD / 16>{},
+            issue(tm, 0, std::integral_constant<int, kD / 16>{},
                   [&](int k, int part) { return sw128_desc(st + part * kTileX + (k >> 2) * kPanel + (k & 3) * 32); }, state_rows);
             commit_one(&S.d[0], one);
             // the state of chunk c was stored, so K^T W of chunk c - 1, the last that read its stage, is complete
             if (c > 0 && c + 1 < n) copy_kq(c + 1);
             if (!wait(&S.tp_full, c & 1) || !wait(&S.r_ready, c & 1)) break;
             tc_fence_after();
-            issue(tm + kN, idesc_f16(0, 1), std::integral_constant<int, kC / 16>{},
+            issue(tm + 2 * kN, 0, std::integral_constant<int, kC / 16>{},
                   [&](int k, int part) { return sw128_desc(sm + L::kTP + part * kTileT + k * 32); }, token_rows);
             commit_one(&S.d[1], one);
             if (!wait(&S.w_ready, c & 1)) break;
             tc_fence_after();
-            issue(tm + 2 * kN, idesc_f16(1, 1), std::integral_constant<int, kC / 16>{},
+            issue(tm + 4 * kN, 1, std::integral_constant<int, kC / 16>{},
                   [&](int k, int part) { return desc_rows(st + part * kTileX + k * 2048, kPanel); }, token_rows);
             commit_one(&S.d[2], one);
             if (c + 1 < n) copy_tp(c + 1);   // W is stored, so the products with T b are complete
@@ -974,12 +1000,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     } else {
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         // 16 columns (half hf of the thread's 32) of row `row` of an operand image, hi and lo `part` bytes apart
-        auto store_half = [&](uint32_t image, int part, int row, int hf, const float *v) {
+        auto store_half = [&](uint32_t image, int part, int row, int hf, const uint64_t *v) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 uint32_t h[4], l[4];
 #pragma unroll
-                for (int y = 0; y < 4; ++y) split2(v[8 * x + 2 * y], v[8 * x + 2 * y + 1], h[y], l[y]);
+                for (int y = 0; y < 4; ++y) split2(v[4 * x + y], h[y], l[y]);
                 uint8_t *to = smem + image + at128(row, 4 * wg + 2 * hf + x);
                 *reinterpret_cast<uint4 *>(to) = make_uint4(h[0], h[1], h[2], h[3]);
                 *reinterpret_cast<uint4 *>(to + part) = make_uint4(l[0], l[1], l[2], l[3]);
@@ -991,21 +1017,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
-        auto read_half = [&](int which, int hf, float *v) {   // 16 sums, of both issuers
-            float u[16];
-            tc_ld16(tmem + lanes + which * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(v));
-            tc_ld16(tmem + lanes + (3 + which) * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(u));
+        auto read_half = [&](int which, int hf, uint64_t *v) {   // 16 sums, of both halves of the product
+            float x[16], u[16];
+            tc_ld16(tmem + lanes + 2 * which * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(x));
+            tc_ld16(tmem + lanes + (2 * which + 1) * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(u));
             tc_wait_ld();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += u[j];
+            for (int j = 0; j < 8; ++j) v[j] = add2(pair(x[2 * j], x[2 * j + 1]), pair(u[2 * j], u[2 * j + 1]));
         };
         auto store_state = [&](int e) {
-            const float s = pow2(-e);
+            const uint64_t s = pair(pow2(-e), pow2(-e));
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                float v[16];
+                uint64_t v[8];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) v[j] = St[16 * hf + j] * s;
+                for (int j = 0; j < 8; ++j) v[j] = mul2(St[8 * hf + j], s);
                 store_half(L::kS, L::kTileS, r, hf, v);
             }
             signal(&S.s_ready);
@@ -1025,28 +1051,28 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             const float g = eg[t], keep = eg[kC - 1];
             if (!is_q) {
                 // R = V - e^G K S^T, scaled
-                const float k0 = g * pow2(es) * (1.f / kScaleK), s = pow2(-eu);
+                const float k0 = -g * pow2(es) * pow2(-eu) * (1.f / kScaleK), s = pow2(-eu);
+                const uint64_t kk = pair(k0, k0), ss = pair(s, s);
                 wait_bar(&S.d[0], c & 1, &S.stop);
                 tc_fence_after();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    float x[16], y[16];
+                    uint64_t x[8];
                     read_half(0, hf, x);
 #pragma unroll
-                    for (int j = 0; j < 16; j += 4) {
-                        const int piece = (c0 + 16 * hf + j) >> 2;
-                        const float4 v = *reinterpret_cast<const float4 *>(smem + L::kV + t * 256 + ((piece ^ (t & 15)) << 4));
-                        y[j] = (v.x - k0 * x[j]) * s, y[j + 1] = (v.y - k0 * x[j + 1]) * s;
-                        y[j + 2] = (v.z - k0 * x[j + 2]) * s, y[j + 3] = (v.w - k0 * x[j + 3]) * s;
+                    for (int j = 0; j < 8; j += 2) {
+                        const int piece = (c0 + 16 * hf + 2 * j) >> 2;
+                        const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(smem + L::kV + t * 256 + ((piece ^ (t & 15)) << 4));
+                        x[j] = fma2(kk, x[j], mul2(v.x, ss)), x[j + 1] = fma2(kk, x[j + 1], mul2(v.y, ss));
                     }
-                    store_half(L::kR, L::kTileR, t, hf, y);
+                    store_half(L::kR, L::kTileR, t, hf, x);
                 }
                 signal(&S.r_ready);
                 wait_bar(&S.d[1], c & 1, &S.stop);
                 tc_fence_after();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    float x[16];
+                    uint64_t x[8];
                     read_half(1, hf, x);
                     store_half(L::kR, L::kTileR, t, hf, x);   // W over R, which has been read
                 }
@@ -1056,18 +1082,22 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 wait_bar(&S.d[1], c & 1, &S.stop);   // and with it the product before it
                 tc_fence_after();
                 const float k0 = g * pow2(es) * pow2(-eu), s = pow2(eu) * (1.f / kScaleQ);
+                const uint64_t kk = pair(k0, k0), ss = pair(s, s);
                 const int row = c * kC + t;
                 float4 *o = reinterpret_cast<float4 *>(a.o + o_at(a, row0 + row, vh, split * kN + c0));
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    float x[16], y[16];
+                    uint64_t x[8], y[8];
                     read_half(0, hf, x);
                     read_half(1, hf, y);
                     if (row < rows)
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            o[8 * (4 * hf + j / 4)] = make_float4(fmaf(k0, x[j], y[j]) * s, fmaf(k0, x[j + 1], y[j + 1]) * s,
-                                                            fmaf(k0, x[j + 2], y[j + 2]) * s, fmaf(k0, x[j + 3], y[j + 3]) * s);
+                        for (int j = 0; j < 8; j += 2) {
+                            float4 f;
+                            unpair(mul2(fma2(kk, x[j], y[j]), ss), f.x, f.y);
+                            unpair(mul2(fma2(kk, x[j + 1], y[j + 1]), ss), f.z, f.w);
+                            o[8 * (4 * hf + j / 2)] = f;
+                        }
                 }
             }
             es = exponent_of(bound2);
@@ -1076,16 +1106,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             const float add = pow2(eu) * (1.f / kScaleK);
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
-                float x[16];
+                uint64_t x[8];
                 read_half(2, hf, x);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) St[16 * hf + j] = fmaf(St[16 * hf + j], keep, x[j] * add);
+                for (int j = 0; j < 8; ++j) St[8 * hf + j] = fma2(St[8 * hf + j], pair(keep, keep), mul2(x[j], pair(add, add)));
             }
             if (c + 1 < chunks) store_state(es);
         }
         const bool lost = S.stop;   // a copy or product that never came must not pass for an answer
 #pragma unroll
-        for (int j = 0; j < 32; ++j) a.delta_out[s_at + (long long)j * kD] = lost ? NAN : St[j];
+        for (int j = 0; j < 16; ++j) {
+            float x, y;
+            unpair(St[j], x, y);
+            a.delta_out[s_at + (long long)(2 * j) * kD] = lost ? NAN : x;
+            a.delta_out[s_at + (long long)(2 * j + 1) * kD] = lost ? NAN : y;
+        }
         tc_fence_before();
     }
     __syncthreads();
