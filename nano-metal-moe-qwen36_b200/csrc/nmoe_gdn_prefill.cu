@@ -173,6 +173,16 @@ __device__ __forceinline__ float silu_fast(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
     return x * r;
 }
+__device__ __forceinline__ uint64_t silu2(uint64_t x) {
+    float e0, e1, r0, r1;
+    unpair(mul2(x, pair(-1.4426950408889634f, -1.4426950408889634f)), e0, e1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
+    unpair(add2(pair(e0, e1), pair(1.f, 1.f)), e0, e1);
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(e0));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(e1));
+    return mul2(x, pair(r0, r1));
+}
 // byte offset of 16-byte piece p of row r: in a 128-byte row; in two panels of 128 rows
 __device__ __forceinline__ uint32_t at128(int r, int p) { return r * 128 + ((p ^ (r & 7)) << 4); }
 __device__ __forceinline__ uint32_t at_kq(int r, int p) { return (p >> 3) * kPanel + at128(r, p & 7); }
@@ -313,9 +323,8 @@ struct ChunkSmem {
     // K over Q, hi and lo; then, over them, the two heads' T (fp32, later T b's hi and lo in its place) and P's
     // (later P T b's) hi and lo
     static constexpr int kT = 0, kTBytes = kC * kLdT * 4, kP = 2 * kTBytes, kPBytes = 2 * kC * 128;
-    static constexpr int kScratch = kP + 2 * kPBytes;            // 32 x 8 a warp
-    static constexpr int kBytes = kScratch + kWarps * 256 * 4 + 1024;   // and to align it
-    static_assert(2 * kTileX <= kScratch, "K and Q end before what is used beside them");
+    static constexpr int kEnd = kP + 2 * kPBytes, kBytes = kEnd + 1024;   // and to align it
+    static_assert(2 * kTileX <= kEnd, "K and Q lie within");
 };
 
 template <bool kBf16>
@@ -323,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     extern __shared__ uint8_t raw_smem[];
     uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);   // the swizzle goes by the address
     __shared__ __align__(16) float2 G[2][kC];
-    __shared__ __align__(16) float beta[2][kC];
+    __shared__ __align__(16) float beta[2][kC], mid[2][kC / 2];   // mid: e^{G_31 - G_s}
     __shared__ int scan[kWarps], scan_all[kWarps], found[5], stop;
     __shared__ uint64_t products;
     __shared__ uint32_t tmem_at;
@@ -448,85 +457,100 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         const float h0 = (float)first, h1 = (float)inc;
         *reinterpret_cast<float4 *>(&G[half][2 * lane]) = make_float4(h0, (float)(first - h0), h1, (float)(inc - h1));
         *reinterpret_cast<float2 *>(&beta[half][2 * lane]) = make_float2(bt[0], bt[1]);
+        const double g31 = __shfl_sync(0xffffffffu, inc, 15);
+        if (lane < 16) *reinterpret_cast<float2 *>(&mid[half][2 * lane]) = make_float2(__expf((float)(g31 - first)), __expf((float)(g31 - inc)));
     };
 
-    // ---- convolution, SiLU and norm of q and k: a warp takes 8 tokens, a lane 4 channels of each. All rows
-    // are asked for first, wherever they lie; what is no row of the sequence is replaced after.
+    // ---- convolution, SiLU and norm of q and k: a warp takes 8 tokens, a lane 4 channels of each; four tokens of
+    // q or k at a time, the rows of the next four asked for before. Rows beyond the sequence's ends are asked
+    // for at its ends, and replaced.
     {
-        const int t0 = 8 * warp, cq = kh * kD + 4 * lane, ck = (a.key_heads + kh) * kD + 4 * lane;
         using Raw4 = typename std::conditional<kBf16, uint2, float4>::type;
         using Raw = typename std::conditional<kBf16, uint16_t, float>::type;
-        Raw4 xr[2][11];
+        const int t0 = 8 * warp;
+        Raw4 next[7];
+        uint2 w_next[4];
+        auto channel = [&](int side) { return (side * a.key_heads + kh) * kD + 4 * lane; };
+        auto load_rows = [&](int batch) {
+            const Raw *p = static_cast<const Raw *>(a.qkv) + channel(batch >> 1);
 #pragma unroll
-        for (int i = 0; i < 11; ++i) {
-            const int r = min(max(in_seq + t0 + i - 3, 0), in_seq + n - 1);
-            const Raw *p = static_cast<const Raw *>(a.qkv) + (long long)(row0 + r) * a.qkv_stride;
-            xr[0][i] = *reinterpret_cast<const Raw4 *>(p + cq);
-            xr[1][i] = *reinterpret_cast<const Raw4 *>(p + ck);
-        }
-        uint2 w[2][4];
+            for (int i = 0; i < 7; ++i) {
+                const int r = min(max(in_seq + t0 + 4 * (batch & 1) + i - 3, 0), in_seq + n - 1);
+                next[i] = *reinterpret_cast<const Raw4 *>(p + (long long)(row0 + r) * a.qkv_stride);
+            }
+            if ((batch & 1) == 0)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            w[0][j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (cq + j));
-            w[1][j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ck + j));
-        }
+                for (int j = 0; j < 4; ++j) w_next[j] = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (channel(batch >> 1) + j));
+        };
         load_gates(0);
+        load_rows(0);
+        uint64_t w[2][4];   // of two channels, by tap
 #pragma unroll
-        for (int side = 0; side < 2; ++side) {   // q, then k
-            float x[11][4];
+        for (int batch = 0; batch < 4; ++batch) {
+            const int side = batch >> 1, i0 = 4 * (batch & 1);
+            uint64_t x[7][2];
 #pragma unroll
-            for (int i = 0; i < 11; ++i) {
+            for (int i = 0; i < 7; ++i) {
                 if constexpr (kBf16) {
-                    x[i][0] = bf16_lo(xr[side][i].x), x[i][1] = bf16_hi(xr[side][i].x);
-                    x[i][2] = bf16_lo(xr[side][i].y), x[i][3] = bf16_hi(xr[side][i].y);
+                    x[i][0] = pair(bf16_lo(next[i].x), bf16_hi(next[i].x));
+                    x[i][1] = pair(bf16_lo(next[i].y), bf16_hi(next[i].y));
                 } else {
-                    x[i][0] = xr[side][i].x, x[i][1] = xr[side][i].y, x[i][2] = xr[side][i].z, x[i][3] = xr[side][i].w;
+                    x[i][0] = pair(next[i].x, next[i].y);
+                    x[i][1] = pair(next[i].z, next[i].w);
                 }
             }
-            if (in_seq == 0 && warp == 0) {   // the inputs before the sequence
+            if (i0 == 0)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint2 u = w_next[2 * j], v = w_next[2 * j + 1];
+                    w[j][0] = pair(bf16_lo(u.x), bf16_lo(v.x)), w[j][1] = pair(bf16_hi(u.x), bf16_hi(v.x));
+                    w[j][2] = pair(bf16_lo(u.y), bf16_lo(v.y)), w[j][3] = pair(bf16_hi(u.y), bf16_hi(v.y));
+                }
+            if (batch < 3) load_rows(batch + 1);
+            if (in_seq == 0 && warp == 0 && i0 == 0) {   // the inputs before the sequence
 #pragma unroll
                 for (int i = 0; i < 3; ++i) {
                     float4 c = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (a.conv_in != nullptr)
-                        c = *reinterpret_cast<const float4 *>(a.conv_in + ((long long)b * 3 + i) * a.channels + (side ? ck : cq));
-                    x[i][0] = c.x, x[i][1] = c.y, x[i][2] = c.z, x[i][3] = c.w;
+                        c = *reinterpret_cast<const float4 *>(a.conv_in + ((long long)b * 3 + i) * a.channels + channel(side));
+                    x[i][0] = pair(c.x, c.y), x[i][1] = pair(c.z, c.w);
                 }
             }
             const float scale = side ? kScaleK * 0.08838834764831845f : kScaleQ / kD;
+            uint64_t y[4][2];
+            float ss[4];
 #pragma unroll
-            for (int i0 = 0; i0 < 8; i0 += 4) {
-                float y[4][4], ss[4];
+            for (int i = 0; i < 4; ++i) {
+                uint64_t sum2 = 0;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    ss[i] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float s = x[i0 + i][j] * bf16_lo(w[side][j].x) + x[i0 + i + 1][j] * bf16_hi(w[side][j].x) +
-                                        x[i0 + i + 2][j] * bf16_lo(w[side][j].y) + x[i0 + i + 3][j] * bf16_hi(w[side][j].y);
-                        y[i][j] = t0 + i0 + i < n ? silu_fast(s) : 0.f;
-                        ss[i] = fmaf(y[i][j], y[i][j], ss[i]);
-                    }
+                for (int j = 0; j < 2; ++j) {
+                    const uint64_t v = fma2(x[i + 3][j], w[j][3], fma2(x[i + 2][j], w[j][2], fma2(x[i + 1][j], w[j][1], mul2(x[i][j], w[j][0]))));
+                    y[i][j] = t0 + i0 + i < n ? silu2(v) : 0;
+                    sum2 = fma2(y[i][j], y[i][j], sum2);
                 }
-                // the four sums over the warp together: a lane keeps half of them in each of two exchanges, so
-                // that lane l ends with that of token l & 3 and takes its root
-                const bool odd = lane & 1, upper = lane & 2;
-                const float a0 = (odd ? ss[1] : ss[0]) + __shfl_xor_sync(0xffffffffu, odd ? ss[0] : ss[1], 1);
-                const float a1 = (odd ? ss[3] : ss[2]) + __shfl_xor_sync(0xffffffffu, odd ? ss[2] : ss[3], 1);
-                float sum = (upper ? a1 : a0) + __shfl_xor_sync(0xffffffffu, upper ? a0 : a1, 2);
+                float s0, s1;
+                unpair(sum2, s0, s1);
+                ss[i] = s0 + s1;
+            }
+            // the four sums over the warp together: a lane keeps half of them in each of two exchanges, so
+            // that lane l ends with that of token l & 3 and takes its root
+            const bool odd = lane & 1, upper = lane & 2;
+            const float a0 = (odd ? ss[1] : ss[0]) + __shfl_xor_sync(0xffffffffu, odd ? ss[0] : ss[1], 1);
+            const float a1 = (odd ? ss[3] : ss[2]) + __shfl_xor_sync(0xffffffffu, odd ? ss[2] : ss[3], 1);
+            float sum = (upper ? a1 : a0) + __shfl_xor_sync(0xffffffffu, upper ? a0 : a1, 2);
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const float root = rsqrtf(sum / kD + 1e-12f) * scale;
+            for (int o = 4; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float root = rsqrtf(sum / kD + 1e-12f) * scale;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int t = t0 + i0 + i;
-                    const float inv = __shfl_sync(0xffffffffu, root, i);
-                    uint32_t h0, l0, h1, l1;
-                    const uint32_t at = at_kq(side ? t : kC + t, lane >> 1) + (lane & 1) * 8;
-                    split2(y[i][0] * inv, y[i][1] * inv, h0, l0);
-                    split2(y[i][2] * inv, y[i][3] * inv, h1, l1);
-                    *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h0, h1);
-                    *reinterpret_cast<uint2 *>(smem + kTileX + at) = make_uint2(l0, l1);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int t = t0 + i0 + i;
+                const float inv = __shfl_sync(0xffffffffu, root, i);
+                uint32_t h0, l0, h1, l1;
+                const uint32_t at = at_kq(side ? t : kC + t, lane >> 1) + (lane & 1) * 8;
+                split2(mul2(y[i][0], pair(inv, inv)), h0, l0);
+                split2(mul2(y[i][1], pair(inv, inv)), h1, l1);
+                *reinterpret_cast<uint2 *>(smem + at) = make_uint2(h0, h1);
+                *reinterpret_cast<uint2 *>(smem + kTileX + at) = make_uint2(l0, l1);
             }
         }
     }
@@ -561,7 +585,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         const int vh = kh * ratio + v0 + half;
         float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT + half * ChunkSmem::kTBytes);
         uint8_t *P = smem + ChunkSmem::kP + half * ChunkSmem::kPBytes;
-        float *scratch = reinterpret_cast<float *>(smem + ChunkSmem::kScratch) + warp * 256;
+        float *scratch = T + 32 + 8 * q4;   // 8 columns of T's quarter above the diagonal, which is not used otherwise
         auto head_sync = [&] { bar_sync(1 + half, 128); };
         // what was copied out of this shared memory has been read
         if (v0 == 0 ? warp == 0 : t128 == 0) bulk_wait_read();
@@ -570,48 +594,52 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             make_gates(v0);
         }
         __syncthreads();   // and the products that read K and Q are complete
-        // M below the diagonal, P with its diagonal, of both heads: a thread a row (of K K^T: M; of Q K^T: P) and 32
-        // columns, as the products lie in tensor memory. What is above the 32 x 32 blocks on the diagonal is not read.
-        const int t = 32 * (warp & 1) + lane, c0 = 32 * (warp >> 2);
-        if (c0 <= 32 * (warp & 1)) {
+        // M below the diagonal, P with its diagonal: a thread a row (of K K^T: M; of Q K^T: P), as the products lie in
+        // tensor memory, four warps a head. What is above the 32 x 32 blocks on the diagonal is not read. The block
+        // below them: e^{G_t - G_s} = e^{G_t - G_31} e^{G_31 - G_s}, neither above 1.
+        if (on) {
+            const int block = warp & 1, t = 32 * block + lane;
             const bool is_q = warp & 2;
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int s0 = c0 + 16 * hf;
+            const float2 g = G[half][t], g31 = G[half][31];
+            // Q K^T keeps the scale of q: P does
+            const float scale = is_q ? 1.f / kScaleK : beta[half][t] * (1.f / (kScaleK * kScaleK));
+            const float far = scale * __expf((g.x - g31.x) + (g.y - g31.y));
+#pragma unroll 1
+            for (int s0 = 0; s0 < 32 * block + 32; s0 += 16) {
                 float x[16];
+                uint64_t y[8];
                 tc_ld16(tmem + ((uint32_t)(32 * (warp & 3)) << 16) + s0, reinterpret_cast<uint32_t *>(x));
                 tc_wait_ld();
+                if (s0 < 32 * block) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (v0 + h >= ratio) break;
-                    const float2 g = G[h][t];
-                    // Q K^T keeps the scale of q: P does
-                    const float scale = is_q ? 1.f / kScaleK : beta[h][t] * (1.f / (kScaleK * kScaleK));
+                    for (int j = 0; j < 8; j += 2) {
+                        const ulonglong2 e = *reinterpret_cast<const ulonglong2 *>(&mid[half][s0 + 2 * j]);
+                        y[j] = mul2(mul2(pair(x[2 * j], x[2 * j + 1]), e.x), pair(far, far));
+                        y[j + 1] = mul2(mul2(pair(x[2 * j + 2], x[2 * j + 3]), e.y), pair(far, far));
+                    }
+                } else {
                     const int seen = t - s0 + (is_q ? 1 : 0);   // columns
-                    float y[16];
 #pragma unroll
                     for (int j = 0; j < 16; j += 2) {
-                        const float4 gs = *reinterpret_cast<const float4 *>(&G[h][s0 + j]);   // of two columns
+                        const float4 gs = *reinterpret_cast<const float4 *>(&G[half][s0 + j]);   // of two columns
                         const float e0 = __expf((g.x - gs.x) + (g.y - gs.y)), e1 = __expf((g.x - gs.z) + (g.y - gs.w));
-                        y[j] = j < seen ? scale * e0 * x[j] : 0.f;   // e at most 1: 2^-22 or so of it, and of 1
-                        y[j + 1] = j + 1 < seen ? scale * e1 * x[j + 1] : 0.f;
+                        // e at most 1: 2^-22 or so of it, and of 1
+                        y[j / 2] = pair(j < seen ? scale * e0 * x[j] : 0.f, j + 1 < seen ? scale * e1 * x[j + 1] : 0.f);
                     }
-                    if (!is_q) {
-                        float *to = reinterpret_cast<float *>(smem + ChunkSmem::kT + h * ChunkSmem::kTBytes) + t * kLdT + s0;
+                }
+                if (!is_q) {
+                    ulonglong2 *to = reinterpret_cast<ulonglong2 *>(T + t * kLdT + s0);
 #pragma unroll
-                        for (int j = 0; j < 16; j += 4)
-                            *reinterpret_cast<float4 *>(to + j) = make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]);
-                    } else {
-                        uint8_t *to = smem + ChunkSmem::kP + h * ChunkSmem::kPBytes;
+                    for (int j = 0; j < 4; ++j) to[j] = make_ulonglong2(y[2 * j], y[2 * j + 1]);
+                } else {
 #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            uint32_t hi[4], lo[4];
+                    for (int q = 0; q < 2; ++q) {
+                        uint32_t hi[4], lo[4];
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) split2(y[8 * q + 2 * j], y[8 * q + 2 * j + 1], hi[j], lo[j]);
-                            const int at = at128(t, s0 / 8 + q);
-                            *reinterpret_cast<uint4 *>(to + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                            *reinterpret_cast<uint4 *>(to + kC * 128 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                        }
+                        for (int j = 0; j < 4; ++j) split2(y[4 * q + j], hi[j], lo[j]);
+                        const int at = at128(t, s0 / 8 + q);
+                        *reinterpret_cast<uint4 *>(P + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *reinterpret_cast<uint4 *>(P + kC * 128 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
             }
@@ -664,12 +692,12 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 float acc[4] = {};
 #pragma unroll
                 for (int k = 0; k < 16; k += 4) add(acc, T + (d + 16 + lr) * kLdT + d + k, T + (d + k) * kLdT + col, kLdT);
-                put(scratch + lr * 8 + lc, acc, 1.f);
+                put(scratch + lr * kLdT + lc, acc, 1.f);
                 head_sync();   // M_21 is read
 #pragma unroll
                 for (int x = 0; x < 4; ++x) acc[x] = 0.f;
 #pragma unroll
-                for (int k = 0; k < 16; k += 4) add(acc, T + (d + 16 + lr) * kLdT + d + 16 + k, scratch + k * 8 + lc, 8);
+                for (int k = 0; k < 16; k += 4) add(acc, T + (d + 16 + lr) * kLdT + d + 16 + k, scratch + k * kLdT + lc, kLdT);
                 put(T + (d + 16 + lr) * kLdT + col, acc, -1.f);
                 head_sync();
             }
@@ -681,18 +709,18 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                     add(x0, T + (32 + lr) * kLdT + k, T + k * kLdT + col, kLdT);
                     add(x1, T + (48 + lr) * kLdT + k, T + k * kLdT + col, kLdT);
                 }
-                put(scratch + lr * 8 + lc, x0, 1.f);
-                put(scratch + (lr + 16) * 8 + lc, x1, 1.f);
+                put(scratch + lr * kLdT + lc, x0, 1.f);
+                put(scratch + (lr + 16) * kLdT + lc, x1, 1.f);
                 head_sync();
 #pragma unroll
                 for (int x = 0; x < 4; ++x) x0[x] = x1[x] = 0.f;
 #pragma unroll 2
                 for (int k = 0; k < 16; k += 4) {
-                    add(x0, T + (32 + lr) * kLdT + 32 + k, scratch + k * 8 + lc, 8);
-                    add(x1, T + (48 + lr) * kLdT + 32 + k, scratch + k * 8 + lc, 8);
+                    add(x0, T + (32 + lr) * kLdT + 32 + k, scratch + k * kLdT + lc, kLdT);
+                    add(x1, T + (48 + lr) * kLdT + 32 + k, scratch + k * kLdT + lc, kLdT);
                 }
 #pragma unroll 2
-                for (int k = 16; k < 32; k += 4) add(x1, T + (48 + lr) * kLdT + 32 + k, scratch + k * 8 + lc, 8);
+                for (int k = 16; k < 32; k += 4) add(x1, T + (48 + lr) * kLdT + 32 + k, scratch + k * kLdT + lc, kLdT);
                 put(T + (32 + lr) * kLdT + col, x0, -1.f);
                 put(T + (48 + lr) * kLdT + col, x1, -1.f);
                 head_sync();
