@@ -60,9 +60,11 @@ constexpr float kScaleK = 16.f, kScaleQ = 128.f;   // k and q elements are about
 
 // Tile images, the same in the workspace and in shared memory: rows of 128 bytes (64 fp16) in 16-byte
 // pieces, piece p of row r at p ^ (r & 7): the MMA's 128-byte swizzle, and 8 bank groups for an ldmatrix.
-constexpr int kPanel = 128 * 128;     // 128 rows: K over Q, T b over P T b
+constexpr int kPanel = 128 * 128;     // 128 rows
 constexpr int kTileX = 2 * kPanel;    // K over Q, one part (hi or lo): two panels of 64 dims
-constexpr int kTileT = kPanel;        // T b over P T b, one part
+constexpr int kTileZ = kPanel;        // Z, one part: 128 dims, 64 tokens
+constexpr int kTileP = kC * 128;      // P T b, one part: 64 tokens by 64
+constexpr int kTileZP = 2 * kTileZ + 2 * kTileP;   // Z hi, lo, then P T b hi, lo
 constexpr int kGates = kC * 4;        // e^{G_t}
 
 struct GdnArgs {
@@ -320,11 +322,11 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
 constexpr int kGateRows = 4;   // rows of the grid that norm the heads of an earlier part
 constexpr int kLdT = 68;   // T rows
 struct ChunkSmem {
-    // K over Q, hi and lo; then, over them, the two heads' T (fp32, later T b's hi and lo in its place) and P's
-    // (later P T b's) hi and lo
-    static constexpr int kT = 0, kTBytes = kC * kLdT * 4, kP = 2 * kTBytes, kPBytes = 2 * kC * 128;
-    static constexpr int kEnd = kP + 2 * kPBytes, kBytes = kEnd + 1024;   // and to align it
-    static_assert(2 * kTileX <= kEnd, "K and Q lie within");
+    // K over Q, hi and lo, two panels each: K stays; the heads' P hi and lo (later P T b's, then half of Z's lo) go
+    // where Q was, head h into panel h. Beside them T (fp32, later images in its place)
+    static constexpr int kT = 2 * kTileX, kTBytes = kC * kLdT * 4, kP = kTileP, kPStride = kPanel;
+    static constexpr int kBytes = kT + 2 * kTBytes + 1024;   // and to align it
+    static_assert(kT % 1024 == 0 && kTBytes % 1024 == 0 && kTBytes >= kTileZ, "images in T's place");
 };
 
 template <bool kBf16>
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     __shared__ __align__(16) float2 G[2][kC];
     __shared__ __align__(16) float beta[2][kC], mid[2][kC / 2];   // mid: e^{G_31 - G_s}
     __shared__ int scan[kWarps], scan_all[kWarps], found[5], stop;
-    __shared__ uint64_t products;
+    __shared__ uint64_t products, z_done[2];
     __shared__ uint32_t tmem_at;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // Rows of the grid: the value heads' norm of part - 2, whose scan is complete, a quarter of a chunk each;
@@ -400,11 +402,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     }
     const int chunk = found[4] + found[1];   // in the workspace: over all chunks of all sequences
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 64;" ::"r"(smem_u32(&tmem_at)));
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_at)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     if (tid == 0) {
         mbar_init(&products, 1);
+        mbar_init(&z_done[0], 1);
+        mbar_init(&z_done[1], 1);
         mbar_fence_init();
         stop = 0;
     }
@@ -584,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         const bool on = v0 + half < ratio;
         const int vh = kh * ratio + v0 + half;
         float *T = reinterpret_cast<float *>(smem + ChunkSmem::kT + half * ChunkSmem::kTBytes);
-        uint8_t *P = smem + ChunkSmem::kP + half * ChunkSmem::kPBytes;
+        uint8_t *P = smem + ChunkSmem::kP + half * ChunkSmem::kPStride;   // hi; lo kTileX behind it
         float *scratch = T + 32 + 8 * q4;   // 8 columns of T's quarter above the diagonal, which is not used otherwise
         auto head_sync = [&] { bar_sync(1 + half, 128); };
         // what was copied out of this shared memory has been read
@@ -604,7 +608,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
             // Q K^T keeps the scale of q: P does
             const float scale = is_q ? 1.f / kScaleK : beta[half][t] * (1.f / (kScaleK * kScaleK));
             const float far = scale * __expf((g.x - g31.x) + (g.y - g31.y));
-#pragma unroll 1
+#pragma unroll 2
             for (int s0 = 0; s0 < 32 * block + 32; s0 += 16) {
                 float x[16];
                 uint64_t y[8];
@@ -639,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                         for (int j = 0; j < 4; ++j) split2(y[4 * q + j], hi[j], lo[j]);
                         const int at = at128(t, s0 / 8 + q);
                         *reinterpret_cast<uint4 *>(P + at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-                        *reinterpret_cast<uint4 *>(P + kC * 128 + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                        *reinterpret_cast<uint4 *>(P + kTileX + at) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
             }
@@ -647,8 +651,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         __syncthreads();
         if (on) {
             float *gates = reinterpret_cast<float *>(a.gates + ((long long)chunk * a.value_heads + vh) * kGates);
-            // products that never came must not pass for an answer
-            if (t128 < kC) gates[t128] = stop ? NAN : expf(G[half][t128].x + G[half][t128].y);
+            if (t128 < kC) gates[t128] = expf(G[half][t128].x + G[half][t128].y);
             // (I + M)^-1. The 16 x 16 blocks on the diagonal by substitution, a lane per column, ..
             if (lane < 16) {
                 const float *m = T + 16 * q4 * kLdT + 16 * q4;
@@ -725,42 +728,37 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 put(T + (48 + lr) * kLdT + col, x1, -1.f);
                 head_sync();
             }
-            // e^{G_63 - G} T b, whose product with R is W, into the workspace; T b itself in T's place, for P T b (a
-            // thread holds four 16-byte pieces of it meanwhile)
-            uint8_t *to = a.tp + ((long long)chunk * a.value_heads + vh) * 2 * kTileT;
-            uint32_t th[4][4], tl[4][4];
+            // T b in T's place, for P T b (a thread holds four 16-byte pieces of it)
+            uint8_t *to = a.tp + ((long long)chunk * a.value_heads + vh) * kTileZP, *TB = reinterpret_cast<uint8_t *>(T);
+            uint64_t tb[4][4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int i = t128 + 128 * x, t = i >> 3, s0 = (i & 7) * 8;
-                const float left = __expf(diff(kC - 1, t));
-                uint32_t wh[4] = {}, wl[4] = {};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) th[x][j] = tl[x][j] = 0;
+                for (int j = 0; j < 4; ++j) tb[x][j] = 0;
                 if (s0 <= t) {   // T holds nothing above its blocks on the diagonal, and zeros within them
-                    const float4 t0 = *reinterpret_cast<const float4 *>(T + t * kLdT + s0);
-                    const float4 t1 = *reinterpret_cast<const float4 *>(T + t * kLdT + s0 + 4);
-                    const float4 b0 = *reinterpret_cast<const float4 *>(&beta[half][s0]);
-                    const float4 b1 = *reinterpret_cast<const float4 *>(&beta[half][s0 + 4]);
-                    const float v[8] = {t0.x * b0.x, t0.y * b0.y, t0.z * b0.z, t0.w * b0.w,
-                                        t1.x * b1.x, t1.y * b1.y, t1.z * b1.z, t1.w * b1.w};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        split2(v[2 * j], v[2 * j + 1], th[x][j], tl[x][j]);
-                        split2(v[2 * j] * left, v[2 * j + 1] * left, wh[j], wl[j]);
-                    }
+                    const ulonglong2 t0 = *reinterpret_cast<const ulonglong2 *>(T + t * kLdT + s0);
+                    const ulonglong2 t1 = *reinterpret_cast<const ulonglong2 *>(T + t * kLdT + s0 + 4);
+                    const ulonglong2 b0 = *reinterpret_cast<const ulonglong2 *>(&beta[half][s0]);
+                    const ulonglong2 b1 = *reinterpret_cast<const ulonglong2 *>(&beta[half][s0 + 4]);
+                    tb[x][0] = mul2(t0.x, b0.x), tb[x][1] = mul2(t0.y, b0.y);
+                    tb[x][2] = mul2(t1.x, b1.x), tb[x][3] = mul2(t1.y, b1.y);
                 }
-                const int at = at128(t, i & 7);
-                *reinterpret_cast<uint4 *>(to + at) = make_uint4(wh[0], wh[1], wh[2], wh[3]);
-                *reinterpret_cast<uint4 *>(to + kTileT + at) = make_uint4(wl[0], wl[1], wl[2], wl[3]);
             }
-            head_sync();
-            uint8_t *TB = reinterpret_cast<uint8_t *>(T);
+            auto put_tb = [&](bool decayed) {   // its hi and lo; with row t times e^{G_63 - G_t}
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int i = t128 + 128 * x, at = at128(i >> 3, i & 7);
-                *reinterpret_cast<uint4 *>(TB + at) = make_uint4(th[x][0], th[x][1], th[x][2], th[x][3]);
-                *reinterpret_cast<uint4 *>(TB + kC * 128 + at) = make_uint4(tl[x][0], tl[x][1], tl[x][2], tl[x][3]);
-            }
+                for (int x = 0; x < 4; ++x) {
+                    const int i = t128 + 128 * x, t = i >> 3, at = at128(t, i & 7);
+                    const float left = decayed ? __expf(diff(kC - 1, t)) : 1.f;
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split2(decayed ? mul2(tb[x][j], pair(left, left)) : tb[x][j], h[j], l[j]);
+                    *reinterpret_cast<uint4 *>(TB + at) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(TB + kTileP + at) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            };
+            head_sync();
+            put_tb(false);
             head_sync();
             // P T b: 16 rows a warp, the columns in pairs of 8; lower triangular as both are, so the two heads'
             // blocks of rows run in opposite orders over the warp schedulers
@@ -775,9 +773,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                         const uint32_t pa = smem_u32(P) + at128(16 * rb + (lane & 15), 2 * k + (lane >> 4));
                         const uint32_t pb = smem_u32(TB) + at128(16 * k + (lane & 15), 2 * j + (lane >> 4));
                         ldsm4(pa, ah);
-                        ldsm4(pa + kC * 128, al);
+                        ldsm4(pa + kTileX, al);
                         ldsm4t(pb, bh);
-                        ldsm4t(pb + kC * 128, bl);
+                        ldsm4t(pb + kTileP, bl);
 #pragma unroll
                         for (int x = 0; x < 2; ++x) {
                             mma_f16(c[j][x], al, bh[2 * x], bh[2 * x + 1]);
@@ -796,19 +794,66 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 }
                 const uint32_t at = smem_u32(P) + at128(16 * rb + (lane & 15), 2 * j + (lane >> 4));
                 stsm4(at, h[0], h[1], h[2], h[3]);
-                stsm4(at + kC * 128, l[0], l[1], l[2], l[3]);
+                stsm4(at + kTileX, l[0], l[1], l[2], l[3]);
             }
             fence_async_smem();
             head_sync();
-            if (t128 == 0)   // P T b below T b, hi and lo
-                for (int x = 0; x < 2; ++x) bulk_s2g(to + x * kTileT + kC * 128, P + x * kC * 128, kC * 128);
+            if (t128 == 0)
+                for (int x = 0; x < 2; ++x) bulk_s2g(to + 2 * kTileZ + x * kTileP, P + x * kTileX, kTileP);
+            // Z = K^T (e^{G_63 - G} T b), with which the state takes in R in one product
+            put_tb(true);
+            fence_async_smem();
+            tc_fence_before();
+            head_sync();
+            const uint32_t acc = tmem + kC + half * kC;
+            if (q4 == 0) {
+                tc_fence_after();
+                const uint32_t one = elect_lane(), tm = __shfl_sync(0xffffffffu, acc, 0);
+                const uint32_t tb_at = __shfl_sync(0xffffffffu, smem_u32(TB), 0);
+#pragma unroll
+                for (int x = 0; x < 3; ++x)   // hi hi, lo hi, hi lo
+#pragma unroll
+                    for (int k = 0; k < kC / 16; ++k)
+                        mma_one(tm, desc_rows(sm + (x == 1) * kTileX + k * 2048, kPanel), desc_rows(tb_at + (x == 2) * kTileP + k * 2048, 0),
+                                idesc_f16(1, 1, kC), x + k > 0 ? 1u : 0u, one);
+                commit_one(&z_done[half], one);
+            }
+            if (t128 == 0) bulk_wait_read();   // P T b, which Z's lo goes over
+            wait_bar(&z_done[half], (v0 >> 1) & 1, &stop);
+            tc_fence_after();
+            head_sync();
+            if (stop && t128 < kC) gates[t128] = NAN;   // products that never came must not pass for an answer
+            const int dim = 32 * q4 + lane;
+            uint8_t *z_lo = P + (dim >> 6) * kTileX;   // rows 0-63 where P's hi was, 64-127 where its lo was
+#pragma unroll
+            for (int c16 = 0; c16 < 4; ++c16) {
+                float x[16];
+                tc_ld16(acc + ((uint32_t)(32 * q4) << 16) + 16 * c16, reinterpret_cast<uint32_t *>(x));
+                tc_wait_ld();
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    uint32_t h[4], l[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split2(x[8 * q + 2 * j], x[8 * q + 2 * j + 1], h[j], l[j]);
+                    *reinterpret_cast<uint4 *>(TB + at128(dim, 2 * c16 + q)) = make_uint4(h[0], h[1], h[2], h[3]);
+                    *reinterpret_cast<uint4 *>(z_lo + at128(dim & 63, 2 * c16 + q)) = make_uint4(l[0], l[1], l[2], l[3]);
+                }
+            }
+            fence_async_smem();
+            tc_fence_before();
+            head_sync();
+            if (t128 == 0) {
+                bulk_s2g(to, TB, kTileZ);
+                bulk_s2g(to + kTileZ, P, kTileP);
+                bulk_s2g(to + kTileZ + kTileP, P + kTileX, kTileP);
+            }
         }
     }
     if (t128 == 0) bulk_wait_read();   // the shared memory stays until it is copied
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 64;" ::"r"(tmem));
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
     if (last_cta) pdl_wait();
 }
 
@@ -816,16 +861,23 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
 
 struct ScanSmem {
     static constexpr int kStage = 2 * kTileX;                       // K over Q of a chunk, hi and lo; two of them
-    static constexpr int kTP = 2 * kStage;                          // T b over P T b, hi and lo
-    static constexpr int kS = kTP + 2 * kTileT, kTileS = kD * 128;  // the state: [dim][64 columns], hi and lo
-    static constexpr int kR = kS + 2 * kTileS, kTileR = kC * 128;   // R, then W: [token][64 columns], hi and lo
-    static constexpr int kV = kR + 2 * kTileR;                      // V: [token][64 columns] fp32
-    static constexpr int kGate = kV + kC * kN * 4;                  // gates of two chunks
+    static constexpr int kZ = 2 * kStage;                           // Z, hi and lo
+    static constexpr int kS = kZ + 2 * kTileZ, kTileS = kD * 128;   // the state: [dim][64 columns], hi and lo
+    // R: [token][64 columns], hi and lo; before it V (fp32), every value in the bytes of the thread that makes R of it
+    static constexpr int kR = kS + 2 * kTileS, kTileR = kC * 128;
+    static constexpr int kP = kR + 2 * kTileR;                      // P T b, hi and lo
+    static constexpr int kGate = kP + 2 * kTileP;                   // gates of two chunks
     static constexpr int kBytes = kGate + 2 * kGates;
 };
 
+// byte of V's column c (a multiple of 2; 4 in a piece) of token t in R's place: 16 columns in two pieces each of
+// the hi and the lo image
+__device__ __forceinline__ uint32_t v_at(int t, int c) {
+    return ((c >> 3) & 1) * (kC * 128) + at128(t, 2 * (c >> 4) + ((c >> 2) & 1)) + (c & 3) * 4;
+}
+
 struct ScanShared {
-    uint64_t kq_full[2], tp_full, d[3], r_ready, w_ready, s_ready;
+    uint64_t kq_full[2], zp_full, d, zr, pr, r_ready, s_ready;   // d: [K; Q] S^T, zr: Z R, pr: P T b R
     int vmax[3], first_chunk, stop;
     uint32_t tmem;
 };
@@ -852,10 +904,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&S.kq_full[i], 1);
-        for (int i = 0; i < 3; ++i) mbar_init(&S.d[i], 1), S.vmax[i] = 0;
-        mbar_init(&S.tp_full, 1);
-        mbar_init(&S.r_ready, 4);   // the warps of rows 0-63
-        mbar_init(&S.w_ready, 4);
+        for (int i = 0; i < 3; ++i) S.vmax[i] = 0;
+        mbar_init(&S.d, 1);
+        mbar_init(&S.zr, 1);
+        mbar_init(&S.pr, 1);
+        mbar_init(&S.zp_full, 1);
+        mbar_init(&S.r_ready, 8);
         mbar_init(&S.s_ready, 8);
         mbar_fence_init();
         S.first_chunk = S.stop = 0;
@@ -916,26 +970,30 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             bulk_g2s(smem + (c & 1) * L::kStage, a.kq + ((chunk0 + c) * a.key_heads + kh) * 2 * kTileX, L::kStage, bar, keep);
             bulk_g2s(smem + L::kGate + (c & 1) * kGates, a.gates + ((chunk0 + c) * a.value_heads + vh) * kGates, kGates, bar, keep);
         };
-        auto copy_tp = [&](int c) {
+        auto zp = [&](int c) { return a.tp + ((chunk0 + c) * a.value_heads + vh) * kTileZP; };
+        auto copy_z = [&](int c) {
             if (!one) return;
-            mbar_arrive_expect_tx(&S.tp_full, 2 * kTileT);
-            bulk_g2s(smem + L::kTP, a.tp + ((chunk0 + c) * a.value_heads + vh) * 2 * kTileT, 2 * kTileT, &S.tp_full, keep);
+            mbar_arrive_expect_tx(&S.zp_full, kTileZP);
+            bulk_g2s(smem + L::kZ, zp(c), 2 * kTileZ, &S.zp_full, keep);
+        };
+        auto copy_p = [&](int c) {
+            if (one) bulk_g2s(smem + L::kP, zp(c) + 2 * kTileZ, 2 * kTileP, &S.zp_full, keep);
         };
         auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop)); };
         // The products of kSteps k-steps: A's hi with B's hi and lo, which lie side by side as 128 columns (one
         // reading of A for both: these are bound by shared memory), then A's lo with B's hi onto the first 64.
         // A's address of k-step k, part (0 hi, 1 lo); B's of k-step k.
-        auto issue = [&](uint32_t d, int a_mn, auto steps, auto at_a, auto at_b) {
+        auto issue = [&](uint32_t d, auto steps, auto at_a, auto at_b) {
             constexpr int kSteps = decltype(steps)::value;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) mma_one(d, at_a(k, 0), at_b(k), idesc_f16(a_mn, 1, 2 * kN), k > 0 ? 1u : 0u, one);
+            for (int k = 0; k < kSteps; ++k) mma_one(d, at_a(k, 0), at_b(k), idesc_f16(0, 1, 2 * kN), k > 0 ? 1u : 0u, one);
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) mma_one(d, at_a(k, 1), at_b(k), idesc_f16(a_mn, 1, kN), 1u, one);
+            for (int k = 0; k < kSteps; ++k) mma_one(d, at_a(k, 1), at_b(k), idesc_f16(0, 1, kN), 1u, one);
         };
         if (n > 0) {
             copy_kq(0);
-            copy_tp(0);
-            if (n > 1) copy_kq(1);
+            copy_z(0);
+            copy_p(0);
         }
         for (int c = 0; c < n; ++c) {
             const uint32_t st = sm + (c & 1) * L::kStage;
@@ -943,22 +1001,27 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             auto token_rows = [&](int k) { return desc_rows(sm + L::kR + k * 2048, L::kTileR); };
             if (!wait(&S.kq_full[c & 1], (c >> 1) & 1) || !wait(&S.s_ready, c & 1)) break;
             tc_fence_after();
-            issue(tm, 0, std::integral_constant<int, kD / 16>{},
+            issue(tm + (c & 1) * 2 * kN, std::integral_constant<int, kD / 16>{},
                   [&](int k, int part) { return sw128_desc(st + part * kTileX + (k >> 2) * kPanel + (k & 3) * 32); }, state_rows);
-            commit_one(&S.d[0], one);
-            // the state of chunk c was stored, so K^T W of chunk c - 1, the last that read its stage, is complete
-            if (c > 0 && c + 1 < n) copy_kq(c + 1);
-            if (!wait(&S.tp_full, c & 1) || !wait(&S.r_ready, c & 1)) break;
+            commit_one(&S.d, one);
+            // the other stage was last read by the product of the chunk before. The copies are timed to land while
+            // rows are at work: beside a product they take shared memory from it
+            if (c + 1 < n) copy_kq(c + 1);
+            if (!wait(&S.zp_full, c & 1) || !wait(&S.r_ready, c & 1)) break;
             tc_fence_after();
-            issue(tm + 2 * kN, 0, std::integral_constant<int, kC / 16>{},
-                  [&](int k, int part) { return sw128_desc(sm + L::kTP + part * kTileT + k * 32); }, token_rows);
-            commit_one(&S.d[1], one);
-            if (!wait(&S.w_ready, c & 1)) break;
-            tc_fence_after();
-            issue(tm + 4 * kN, 1, std::integral_constant<int, kC / 16>{},
-                  [&](int k, int part) { return desc_rows(st + part * kTileX + k * 2048, kPanel); }, token_rows);
-            commit_one(&S.d[2], one);
-            if (c + 1 < n) copy_tp(c + 1);   // W is stored, so the products with T b are complete
+            issue(tm + 4 * kN, std::integral_constant<int, kC / 16>{},
+                  [&](int k, int part) { return sw128_desc(sm + L::kZ + part * kTileZ + k * 32); }, token_rows);
+            commit_one(&S.zr, one);
+            // P T b as the lower 64 of 128 rows, where Q S^T is; the upper ones (R, which is before it) are not read
+            issue(tm + 6 * kN, std::integral_constant<int, kC / 16>{},
+                  [&](int k, int part) { return sw128_desc(sm + L::kP + (part - 1) * kTileP + k * 32); }, token_rows);
+            commit_one(&S.pr, one);
+            if (c + 1 < n) {
+                if (!wait(&S.zr, c & 1)) break;
+                copy_z(c + 1);
+                if (!wait(&S.pr, c & 1)) break;
+                copy_p(c + 1);
+            }
         }
     } else if (warp >= 9) {
         // ---- V of a chunk: a lane two of 32 channels (warps 9, 10: the first 32) and 16 tokens (lanes 0-15 the
@@ -969,12 +1032,12 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         const int vt = 32 * ((warp - 9) & 1) + 16 * (lane >> 4), vc = 32 * ((warp - 9) >> 1) + 2 * (lane & 15);
         const int ch = (2 * a.key_heads + vh) * kD + split * kN + vc;
         Raw2 raw[19];
-        float w0[4], w1[4];
+        uint64_t w[4];   // of both channels, by tap
         {
             const uint2 u = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * ch);
             const uint2 v = *reinterpret_cast<const uint2 *>(a.conv_w + 4ll * (ch + 1));
-            w0[0] = bf16_lo(u.x), w0[1] = bf16_hi(u.x), w0[2] = bf16_lo(u.y), w0[3] = bf16_hi(u.y);
-            w1[0] = bf16_lo(v.x), w1[1] = bf16_hi(v.x), w1[2] = bf16_lo(v.y), w1[3] = bf16_hi(v.y);
+            w[0] = pair(bf16_lo(u.x), bf16_lo(v.x)), w[1] = pair(bf16_hi(u.x), bf16_hi(v.x));
+            w[2] = pair(bf16_lo(u.y), bf16_lo(v.y)), w[3] = pair(bf16_hi(u.y), bf16_hi(v.y));
         }
         auto load_raw = [&](int c) {   // rows beyond the sequence's ends are asked for at its ends
             const Raw *p = static_cast<const Raw *>(a.qkv) + ch;
@@ -986,15 +1049,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         };
         if (chunks > 0) load_raw(0);
         for (int c = 0; c < chunks; ++c) {
-            float x0[19], x1[19];
-            float2 v[16];
+            uint64_t x[19], v[16];
             float m = 0.f;
 #pragma unroll
             for (int i = 0; i < 19; ++i) {
                 if constexpr (kBf16)
-                    x0[i] = bf16_lo(raw[i]), x1[i] = bf16_hi(raw[i]);
+                    x[i] = pair(bf16_lo(raw[i]), bf16_hi(raw[i]));
                 else
-                    x0[i] = raw[i].x, x1[i] = raw[i].y;
+                    x[i] = pair(raw[i].x, raw[i].y);
             }
             if (c + 1 < chunks) load_raw(c + 1);
             if (from + c == 0 && vt == 0)   // the inputs before the sequence
@@ -1003,27 +1065,25 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                     float2 f = make_float2(0.f, 0.f);
                     if (a.conv_in != nullptr)
                         f = *reinterpret_cast<const float2 *>(a.conv_in + ((long long)b * 3 + i) * a.channels + ch);
-                    x0[i] = f.x, x1[i] = f.y;
+                    x[i] = pair(f.x, f.y);
                 }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float y0 = x0[i] * w0[0] + x0[i + 1] * w0[1] + x0[i + 2] * w0[2] + x0[i + 3] * w0[3];
-                const float y1 = x1[i] * w1[0] + x1[i + 1] * w1[1] + x1[i + 2] * w1[2] + x1[i + 3] * w1[3];
-                const bool in = c * kC + vt + i < rows;
-                v[i] = make_float2(in ? silu_fast(y0) : 0.f, in ? silu_fast(y1) : 0.f);
-                m = fmaxf(m, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
+                const uint64_t y = fma2(x[i + 3], w[3], fma2(x[i + 2], w[2], fma2(x[i + 1], w[1], mul2(x[i], w[0]))));
+                v[i] = c * kC + vt + i < rows ? silu2(y) : 0;
+                float v0, v1;
+                unpair(v[i], v0, v1);
+                m = fmaxf(m, fmaxf(fabsf(v0), fabsf(v1)));
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            // over the values of the chunk before, once R is made of them
-            if (c > 0) wait_bar(&S.d[1], (c - 1) & 1, &S.stop);
+            // over R of the chunk before, once the products have read it
+            if (c > 0) wait_bar(&S.pr, (c - 1) & 1, &S.stop);
             if (lane == 0) atomicMax(&S.vmax[c % 3], __float_as_int(m));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int t = vt + i;
-                *reinterpret_cast<float2 *>(smem + L::kV + t * 256 + (((vc >> 2) ^ (t & 15)) << 4) + (vc & 3) * 4) = v[i];
-            }
-            bar_sync(1, 384);   // before chunk c
+            for (int i = 0; i < 16; ++i) *reinterpret_cast<uint64_t *>(smem + L::kR + v_at(vt + i, vc)) = v[i];
+            asm volatile("bar.arrive 1, 256;" ::: "memory");   // before chunk c
+            asm volatile("bar.arrive 2, 256;" ::: "memory");
         }
     } else {
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
@@ -1047,8 +1107,8 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         };
         auto read_half = [&](int which, int hf, uint64_t *v) {   // 16 sums, of both halves of the product
             float x[16], u[16];
-            tc_ld16(tmem + lanes + 2 * which * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(x));
-            tc_ld16(tmem + lanes + (2 * which + 1) * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(u));
+            tc_ld16(tmem + lanes + 2 * which * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(x));   // hi hi and lo hi
+            tc_ld16(tmem + lanes + (2 * which + 1) * kN + c0 + 16 * hf, reinterpret_cast<uint32_t *>(u));   // hi lo
             tc_wait_ld();
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = add2(pair(x[2 * j], x[2 * j + 1]), pair(u[2 * j], u[2 * j + 1]));
@@ -1069,7 +1129,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         if (chunks > 0) store_state(es);
         const int t = r & 63;   // this row's token
         for (int c = 0; c < chunks; ++c) {
-            bar_sync(1, 384);                        // V of the chunk is stored
+            // V of the chunk is stored. Q's rows, which only need its size, have a barrier of their own: they may
+            // still be busy with the output of the chunk before
+            bar_sync(is_q ? 2 : 1, 256);
             if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to for chunk c + 2
             const float vm = __int_as_float(S.vmax[c % 3]);
             bound2 += kC * vm * vm;                  // of the states of this chunk, and of the one it leaves
@@ -1081,55 +1143,24 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 // R = V - e^G K S^T, scaled
                 const float k0 = -g * pow2(es) * pow2(-eu) * (1.f / kScaleK), s = pow2(-eu);
                 const uint64_t kk = pair(k0, k0), ss = pair(s, s);
-                wait_bar(&S.d[0], c & 1, &S.stop);
+                wait_bar(&S.d, c & 1, &S.stop);
                 tc_fence_after();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     uint64_t x[8];
-                    read_half(0, hf, x);
+                    read_half(c & 1, hf, x);
 #pragma unroll
                     for (int j = 0; j < 8; j += 2) {
-                        const int piece = (c0 + 16 * hf + 2 * j) >> 2;
-                        const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(smem + L::kV + t * 256 + ((piece ^ (t & 15)) << 4));
+                        const ulonglong2 v = *reinterpret_cast<const ulonglong2 *>(smem + L::kR + v_at(t, c0 + 16 * hf + 2 * j));
                         x[j] = fma2(kk, x[j], mul2(v.x, ss)), x[j + 1] = fma2(kk, x[j + 1], mul2(v.y, ss));
                     }
                     store_half(L::kR, L::kTileR, t, hf, x);
                 }
-                signal(&S.r_ready);
-                wait_bar(&S.d[1], c & 1, &S.stop);
-                tc_fence_after();
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint64_t x[8];
-                    read_half(1, hf, x);
-                    store_half(L::kR, L::kTileR, t, hf, x);   // W over R, which has been read
-                }
-                signal(&S.w_ready);
-            } else {
-                // the output before its norm: e^G Q S^T + P U
-                wait_bar(&S.d[1], c & 1, &S.stop);   // and with it the product before it
-                tc_fence_after();
-                const float k0 = g * pow2(es) * pow2(-eu), s = pow2(eu) * (1.f / kScaleQ);
-                const uint64_t kk = pair(k0, k0), ss = pair(s, s);
-                const int row = c * kC + t;
-                float4 *o = reinterpret_cast<float4 *>(a.o + o_at(a, row0 + row, vh, split * kN + c0));
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    uint64_t x[8], y[8];
-                    read_half(0, hf, x);
-                    read_half(1, hf, y);
-                    if (row < rows)
-#pragma unroll
-                        for (int j = 0; j < 8; j += 2) {
-                            float4 f;
-                            unpair(mul2(fma2(kk, x[j], y[j]), ss), f.x, f.y);
-                            unpair(mul2(fma2(kk, x[j + 1], y[j + 1]), ss), f.z, f.w);
-                            o[8 * (4 * hf + j / 2)] = f;
-                        }
-                }
             }
+            signal(&S.r_ready);   // the rows of Q: P T b R of the chunk before is read
+            const float k0 = g * pow2(es) * pow2(-eu);
             es = exponent_of(bound2);
-            wait_bar(&S.d[2], c & 1, &S.stop);
+            wait_bar(&S.zr, c & 1, &S.stop);
             tc_fence_after();
             const float add = pow2(eu) * (1.f / kScaleK);
 #pragma unroll
@@ -1140,6 +1171,29 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 for (int j = 0; j < 8; ++j) St[8 * hf + j] = fma2(St[8 * hf + j], pair(keep, keep), mul2(x[j], pair(add, add)));
             }
             if (c + 1 < chunks) store_state(es);
+            if (is_q) {
+                // the output before its norm, e^G Q S^T + P U, while the next chunk's first product runs
+                wait_bar(&S.pr, c & 1, &S.stop);
+                tc_fence_after();
+                const float s = pow2(eu) * (1.f / kScaleQ);
+                const uint64_t kk = pair(k0, k0), ss = pair(s, s);
+                const int row = c * kC + t;
+                float4 *o = reinterpret_cast<float4 *>(a.o + o_at(a, row0 + row, vh, split * kN + c0));
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint64_t x[8], y[8];
+                    read_half(c & 1, hf, x);
+                    read_half(3, hf, y);
+                    if (row < rows)
+#pragma unroll
+                        for (int j = 0; j < 8; j += 2) {
+                            float4 f;
+                            unpair(mul2(fma2(kk, x[j], y[j]), ss), f.x, f.y);
+                            unpair(mul2(fma2(kk, x[j + 1], y[j + 1]), ss), f.z, f.w);
+                            o[8 * (4 * hf + j / 2)] = f;
+                        }
+                }
+            }
         }
         const bool lost = S.stop;   // a copy or product that never came must not pass for an answer
 #pragma unroll
@@ -1153,9 +1207,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     }
     __syncthreads();
     if (S.stop && warp == 8) {   // copies in flight land before the shared memory goes (each wait bounded)
-        for (int i = 0; i < 2; ++i)
+        for (int i = 0; i < 3; ++i)
             for (int p = 0; p < 2; ++p)
-                for (int k = 0; k < 1000 && !mbar_try_wait_sleep(&S.kq_full[i], p, 1000); ++k) {}
+                for (int k = 0; k < 1000 && !mbar_try_wait_sleep(i < 2 ? &S.kq_full[i] : &S.zp_full, p, 1000); ++k) {}
     }
     __syncthreads();
     tc_fence_after();
@@ -1283,7 +1337,7 @@ size_t carve(const nmoe_linear_attn_shape &s, int num_seqs, int total_rows, uint
         at += (n + 255) & ~(size_t)255;
         return p;
     };
-    uint8_t *kq = take(chunks * s.key_heads * 2 * kTileX), *tp = take(chunks * s.value_heads * 2 * kTileT);
+    uint8_t *kq = take(chunks * s.key_heads * 2 * kTileX), *tp = take(chunks * s.value_heads * kTileZP);
     uint8_t *gates = take(chunks * s.value_heads * kGates), *o = take(((size_t)total_rows + 7) / 8 * 8 * s.value_heads * kD * 4);
     if (a != nullptr) {
         a->kq = kq;
