@@ -319,7 +319,7 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
 
 // ---- chunks ---------------------------------------------------------------------------------------
 
-constexpr int kGateRows = 4;   // rows of the grid that norm the heads of an earlier part
+constexpr int kGateRows = 8;   // rows of the grid that norm the heads of an earlier part
 constexpr int kLdT = 68;   // T rows
 struct ChunkSmem {
     // K over Q, hi and lo, two panels each: K stays; the heads' P hi and lo (later P T b's, then half of Z's lo) go
@@ -339,11 +339,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     __shared__ uint64_t products, z_done[2];
     __shared__ uint32_t tmem_at;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // Rows of the grid: the value heads' norm of part - 2, whose scan is complete, a quarter of a chunk each;
-    // then the key heads. The last CTA returns when the scan of part - 1 has ended, and so does the launch:
-    // what waits for it has all of the parts before.
-    const int gating = a.part >= 2 ? kGateRows : 0;
-    const int kh = (int)blockIdx.y - gating, part = kh < 0 ? a.part - 2 : a.part;
+    // Rows of the grid: the key heads, and spread among them (waiting for memory, where the others wait for the
+    // arithmetic) the value heads' norm of part - 2, whose scan is complete, an eighth of a chunk each. The last CTA
+    // returns when the scan of part - 1 has ended, and so does the launch: what waits for it has all of the
+    // parts before.
+    const int gating = a.part >= 2 ? kGateRows : 0, y = blockIdx.y;
+    const int gate = y * gating / (int)gridDim.y;   // norm rows before this one
+    const bool is_gate = (y + 1) * gating / (int)gridDim.y > gate;
+    const int kh = y - gate, part = is_gate ? a.part - 2 : a.part;
     const bool last_cta = a.part > 0 && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
     pdl_trigger();
 
@@ -396,8 +399,9 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         return;
     }
     const int row0 = found[2], in_seq = found[1] * kC, n = min(kC, found[3] - in_seq);
-    if (kh < 0) {
-        gate_rows<kBf16>(a, row0 + in_seq, row0 + in_seq + n, (kh + kGateRows) * kWarps + warp, kGateRows * kWarps);
+    if (is_gate) {
+        gate_rows<kBf16>(a, row0 + in_seq, row0 + in_seq + n, gate * kWarps + warp, kGateRows * kWarps);
+        if (last_cta) pdl_wait();
         return;
     }
     const int chunk = found[4] + found[1];   // in the workspace: over all chunks of all sequences
@@ -1262,7 +1266,7 @@ long long max_chunks(int num_seqs, int total_rows) { return (long long)total_row
 // Into how many parts the chunks go. With one, every launch has the machine to itself in turn. A scan that leaves
 // more than half of the SMs idle runs beside the launch that prepares the next part, on those SMs; a part more
 // costs about 10 us, and what hides is 1 us a chunk of every part but one: best near sqrt(chunks / 10).
-// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1230 us, 3 1066, 5 1030, 6 1029, 8 1038, 16 1071.
+// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1052 us, 3 895, 4 875, 5 859, 6 876, 8 893, 16 992.
 // The scan's CTAs come in clusters of two for their place only: those take the two SMs of a TPC. Beside an SM
 // that runs the other kernel a CTA of the scan took 20 % longer (1118 us in all, for 992 us in pairs).
 int parts_of(const GdnArgs &a, int sms) {
