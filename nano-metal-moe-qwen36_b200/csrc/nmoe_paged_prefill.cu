@@ -62,9 +62,7 @@ constexpr int kInfo = 8;        // ring of tile masks
 struct Shared {
     uint64_t full[10], empty[10], landed, s_full[2], p_ready[2][2], o_done, done, q_ready;
     uint32_t info[kInfo][5];          // valid positions of a tile, then whether all are
-    long long scan[kThreads / 32];
-    long long unit_off;
-    int unit_seq;
+    int scan[kThreads / 32], unit_off, unit_seq;
     float row_max[2][2][kRows];       // of a row's two halves, by the parity of the tile
     uint32_t tmem;
     int stop;                         // a bounded wait has run out
@@ -74,16 +72,27 @@ template <int D>
 struct Cfg {
     static constexpr int kQB = kRows * D * 2;
     static constexpr int kStageB = 64 * D * 2;              // half a K or V tile
-    static constexpr int kStages = D == 256 ? 5 : 10;
+    // At head_dim 256 a CTA has the SM, and two S tiles so that the next one's product runs beside the softmax. At
+    // 128 a tile's products take half of that and its softmax, a chain of waits, as long as ever: two CTAs share
+    // the SM, an S tile each, and one's products run beside the other's softmax. Seven packed prompts of 1 to 3000
+    // rows, 24 query and 4 KV heads, behind up to 8191 positions: 270 us, for 331 us with one CTA an SM
+    static constexpr int kCtas = D == 256 ? 1 : 2, kBufs = D == 256 ? 2 : 1;
+    static constexpr int kStages = D == 256 ? 5 : 4;
     static constexpr int kRing = kQB, kShared = kQB + kStages * kStageB;   // offsets in shared memory
     static constexpr int kSmem = kShared + (int)sizeof(Shared);
-    static_assert(kSmem <= 232448, "shared memory of a CTA");
-    static constexpr uint32_t kO = 0, kS = D;               // TMEM columns: O, then two S tiles of 128
+    static_assert(kSmem <= (kCtas == 1 ? 232448 : 115712), "shared memory of a CTA");
+    static constexpr uint32_t kO = 0, kS = D;               // TMEM columns: O, then the S tiles of 128
+    static constexpr uint32_t kTmem = D + kBufs * kTile;
+    static_assert(kTmem * kCtas == 512, "tensor memory of the SM");
     static constexpr int kOutB = D * 4 + 16;                // a row of O on its way out
     static_assert(kRows * kOutB <= kQB + kStages * kStageB, "the output rows reuse the queries and the ring");
-    // the stage that holds K tile j, V tile j of n
-    __device__ static uint32_t k_stage(int j) { return j == 0 ? 0 : 2 * j - 1; }
-    __device__ static uint32_t v_stage(int j, int n) { return j == n - 1 ? 2 * j + 1 : 2 * j + 2; }
+    // the stage that holds K tile j, V tile j of n: K 0, K 1, V 0, K 2, V 1, .. with two S tiles, K 0, V 0, K 1, .. with one
+    __device__ static uint32_t k_stage(int j) { return kBufs == 1 ? 2 * j : j == 0 ? 0 : 2 * j - 1; }
+    __device__ static uint32_t v_stage(int j, int n) { return kBufs == 1 || j == n - 1 ? 2 * j + 1 : 2 * j + 2; }
+    // column of the 16 positions i of P: in the place of the scores that they are made of, by the thread that read them
+    __device__ static uint32_t p_at(uint32_t i) { return 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 8 * (i & 1); }
+    // which 32 of a thread's 64 columns are handed over first (0) and second (1)
+    __device__ static constexpr int order(int x) { return kBufs == 1 ? 1 - x : x; }
 };
 
 __device__ __forceinline__ uint32_t cluster_addr(const void *p, int rank) {
@@ -414,7 +423,7 @@ struct Copier {
 };
 
 template <int D>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefill_pairs(const __grid_constant__ PrefillArgs a) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kCtas) k_prefill_pairs(const __grid_constant__ PrefillArgs a) {
     using C = Cfg<D>;
     extern __shared__ __align__(1024) uint8_t raw[];   // the only shared memory: queries, ring, the rest
     cg::cluster_group cluster = cg::this_cluster();
@@ -424,48 +433,101 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
     const int rank = (int)cluster.block_rank();
     const int per_cta = kRows / a.group, per_unit = 2 * per_cta;   // tokens
 
-    // ---- the unit: (sequence, query tile, KV head), the last tiles (the longest) of a sequence first
-    const int unit = blockIdx.x >> 1, kvh = unit % a.kv_heads;
-    const long long want = unit / a.kv_heads;
+    // ---- the unit: (sequence, query tile, KV head), in the order of how many tiles of positions they walk over, the
+    // most first: units are handed to SMs as these become free, and a long one begun last would run alone. The
+    // length of this one by bisection over how many units are at least as long, each sequence's by one division;
+    // by every warp for itself, a lane a sequence, or by the CTA when there are more than 32.
+    const int unit = blockIdx.x >> 1, kvh = unit % a.kv_heads, want = unit / a.kv_heads;
     if (tid == 0) {
         S.unit_seq = -1;
         S.stop = 0;
     }
     {
-        const int per = (a.num_seqs + kThreads - 1) / kThreads;
-        const int first = min(a.num_seqs, tid * per), last = min(a.num_seqs, first + per);
-        auto tiles = [&](int b) {
-            const int lo = max(0, a.cu_rows[b]), hi = min(a.total_rows, a.cu_rows[b + 1]);
-            return hi > lo ? (hi - lo + per_unit - 1) / per_unit : 0;
+        const bool small = a.num_seqs <= 32;
+        const int first = small ? lane : tid, step = small ? 32 : kThreads;
+        auto load_rows = [&](int b) { return max(0, min(a.total_rows, a.cu_rows[b + 1]) - max(0, a.cu_rows[b])); };
+        const int rows0 = first < a.num_seqs ? load_rows(first) : 0, len0 = first < a.num_seqs ? a.kv_lens[first] : 0;
+        auto rows_of = [&](int b) { return b == first ? rows0 : load_rows(b); };
+        auto len_of = [&](int b) { return b == first ? len0 : a.kv_lens[b]; };
+        // of sequence b: its units, and of them the first that walks over `tiles` tiles or more (they grow)
+        auto units = [&](int b) { return (int)(((unsigned)rows_of(b) + per_unit - 1) / per_unit); };
+        auto from = [&](int b, int n, int tiles) {
+            if (tiles <= 0 || n == 0) return 0;
+            const long long len = len_of(b), need = (long long)(tiles - 1) * kTile + 1;   // positions
+            if (min(len, (long long)a.c.capacity) < need) return n;
+            const long long rows = need - (len - rows_of(b));   // of the sequence's rows, that many
+            return rows <= 0 ? 0 : min((int)(((unsigned)rows + per_unit - 1) / per_unit) - 1, n - 1);
         };
-        long long own = 0;
-        for (int b = first; b < last; ++b) own += tiles(b);
-        long long inc = own;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += v;
-        }
-        if (lane == 31) S.scan[warp] = inc;
-        __syncthreads();
-        long long before = inc - own;
-        for (int w = 0; w < warp; ++w) before += S.scan[w];
-        if (want >= before && want < before + own)
-            for (int b = first; b < last; ++b) {
-                const int n = tiles(b);
-                if (want < before + n) {
-                    S.unit_seq = b;
-                    S.unit_off = n - 1 - (want - before);
-                    break;
-                }
-                before += n;
+        auto combine = [&](int v, auto add) {
+            if (small) return v;
+            if (lane == 0) S.scan[warp] = v;
+            __syncthreads();
+            v = S.scan[0];
+            for (int w = 1; w < kThreads / 32; ++w) v = add ? v + S.scan[w] : max(v, S.scan[w]);
+            __syncthreads();
+            return v;
+        };
+        auto at_least = [&](int tiles) {
+            int v = 0;
+            for (int b = first; b < a.num_seqs; b += step) {
+                const int n = units(b);
+                v += n - from(b, n, tiles);
             }
+            return combine(__reduce_add_sync(0xffffffffu, v), true);
+        };
+        int lo = 0, hi = 0, longer = 0;   // at_least(lo) > want >= at_least(hi) = longer
+        if (at_least(0) > want) {
+            {   // the longest there is
+                int most = 0;
+                for (int b = first; b < a.num_seqs; b += step) most = max(most, (int)min((long long)max(0, len_of(b)), (long long)a.c.capacity));
+                hi = (combine(__reduce_max_sync(0xffffffffu, most), false) + kTile - 1) / kTile + 1;
+            }
+            while (hi - lo > 1) {
+                const int mid = lo + (hi - lo) / 2, n = at_least(mid);
+                if (n > want)
+                    lo = mid;
+                else
+                    hi = mid, longer = n;
+            }
+            // of the units of length lo, the (want - longer)-th
+            int own = 0;
+            auto same = [&](int b, int *k) {
+                const int n = units(b);
+                *k = from(b, n, lo);
+                return from(b, n, lo + 1) - *k;
+            };
+            int k;
+            for (int b = first; b < a.num_seqs; b += step) own += same(b, &k);
+            int before = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += v;
+            }
+            if (!small) {
+                if (lane == 31) S.scan[warp] = before;
+                __syncthreads();
+                for (int w = 0; w < warp; ++w) before += S.scan[w];
+            }
+            before -= own;
+            const int nth = want - longer;
+            if (nth >= before && nth < before + own && (!small || warp == 0))
+                for (int b = first; b < a.num_seqs; b += step) {
+                    const int n = same(b, &k);
+                    if (nth < before + n) {
+                        S.unit_seq = b;
+                        S.unit_off = k + nth - before;
+                        break;
+                    }
+                    before += n;
+                }
+        }
         __syncthreads();
     }
     const int b = S.unit_seq;
     if (b < 0) return;   // both CTAs of the pair: there are fewer units than the grid has room for
     const int lo = max(0, a.cu_rows[b]), rows_b = min(a.total_rows, a.cu_rows[b + 1]) - lo;
-    const int tok0 = (int)S.unit_off * per_unit;          // first token of the pair in the sequence
+    const int tok0 = S.unit_off * per_unit;          // first token of the pair in the sequence
     const long long len64 = a.kv_lens[b];
     const long long seq0 = len64 - rows_b;                // position of the sequence's first row
     const int len = (int)max(0ll, min(len64, (long long)a.c.capacity));
@@ -492,7 +554,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
         mbar_fence_init();
     }
     if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)));
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem)), "n"(C::kTmem));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
     tc_fence_before();
@@ -549,26 +611,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 return x < C::kStages ? wait(&S.full[x], round) : wait(&S.full[x - C::kStages], round ^ 1);
             };
             auto qk = [&](int j) {
-                const uint32_t at = ring_at + s * C::kStageB, d = tm + C::kS + (j & 1) * kTile;
+                const uint32_t at = ring_at + s * C::kStageB, d = tm + C::kS + j % C::kBufs * kTile;
 #pragma unroll
                 for (uint32_t i = 0; i < D / 16; ++i)
                     mma2_ss(d, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
                             desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u, one);
                 commit2(&S.empty[s], one);
-                commit2(&S.s_full[j & 1], one);
+                commit2(&S.s_full[j % C::kBufs], one);
                 next();
             };
             // P V of tile j, the two quarters of P that the softmax hands over first, then the others
             auto pv = [&](int j) {
-                const uint32_t at = ring_at + s * C::kStageB, p = tm + C::kS + (j & 1) * kTile;
+                const uint32_t at = ring_at + s * C::kStageB, p = tm + C::kS + j % C::kBufs * kTile;
 #pragma unroll
                 for (uint32_t x = 0; x < 2; ++x) {
-                    if (!wait(&S.p_ready[j & 1][x], (j >> 1) & 1)) return false;
+                    if (!wait(&S.p_ready[j % C::kBufs][x], j / C::kBufs & 1)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (uint32_t y = 0; y < 4; ++y) {
-                        const uint32_t i = 2 * x + (y & 1) + 4 * (y >> 1);
-                        mma2_ts(tm + C::kO, p + 8 * i,
+                        const uint32_t i = 2 * C::order(x) + (y & 1) + 4 * (y >> 1);
+                        mma2_ts(tm + C::kO, p + C::p_at(i),
                                 desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1u << v_shift) - 1)) * 2048, v_rows * 128),
                                 id_o, (j > 0 || x + y > 0) ? 1u : 0u, one);
                     }
@@ -578,18 +640,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 next();
                 return true;
             };
-            // S 0, S 1, P V 0, S 2, P V 1, ..: S of tile j + 1 runs while tile j is in the softmax. What was
-            // copied is waited for ahead of P, so that P V j and S j + 2 follow it at once.
+            // S 0, S 1, P V 0, S 2, P V 1, ..: S of tile j + 1 runs while tile j is in the softmax (with one S tile:
+            // S 0, P V 0, S 1, ..). What was copied is waited for ahead of P, so that P V and the next S follow it at
+            // once.
             bool ok = wait(&S.q_ready, 0) && full(0);
             tc_fence_after();
             if (ok) qk(0);
-            if (ok && n > 1 && (ok = full(0))) {
+            if (C::kBufs == 2 && ok && n > 1 && (ok = full(0))) {
                 tc_fence_after();
                 qk(1);
             }
             for (int j = 0; j < n && ok; ++j) {
-                ok = full(0) && (j + 2 >= n || full(1)) && pv(j);
-                if (ok && j + 2 < n) qk(j + 2);
+                ok = full(0) && (j + C::kBufs >= n || full(1)) && pv(j);
+                if (ok && j + C::kBufs < n) qk(j + C::kBufs);
             }
             if (ok) commit2(&S.done, one);
         }
@@ -608,36 +671,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
             // the first position that some row of this warp does not see
             const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
             for (int j = 0; j < n_tiles; ++j) {
-                wait_bar(&S.s_full[j & 1], (j >> 1) & 1, &S.stop);
+                wait_bar(&S.s_full[j % C::kBufs], j / C::kBufs & 1, &S.stop);
                 tc_fence_after();
-                const uint32_t st = tmem + lanes + C::kS + (j & 1) * kTile;
-                float s[64];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) tc_ld32(st + 64 * wg + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
-                tc_wait_ld();
+                const uint32_t st = tmem + lanes + C::kS + j % C::kBufs * kTile + 64 * wg;
                 const uint32_t *info = S.info[j % kInfo];
-                if ((j + 1) * kTile > seen || !info[4]) {
-                    const int n = pos - j * kTile - 64 * wg;   // columns 0..n of this half are seen
+                const bool masked = (j + 1) * kTile > seen || !info[4];
+                const int n = pos - j * kTile - 64 * wg;   // columns 0..n of this half are seen
+                auto mask32 = [&](int c, float *s) {
+                    if (!masked) return;
+                    const int k = n - 32 * c;
+                    const uint32_t w = info[2 * wg + c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int k = n - 32 * c;
-                        const uint32_t w = info[2 * wg + c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
+                    for (int i = 0; i < 32; ++i) s[i] = w >> i & 1u ? s[i] : -INFINITY;
+                };
+                auto max32 = [&](const float *s) {
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) s[32 * c + i] = w >> i & 1u ? s[32 * c + i] : -INFINITY;
-                    }
+                    for (int i = 4; i < 28; i += 8)
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[i + x], s[i + 4 + x]);
+                    return max3(max3(mx[0], mx[1], mx[2]), mx[3], fmaxf(fmaxf(s[28], s[29]), fmaxf(s[30], s[31])));
+                };
+                // two CTAs an SM have registers for 32 columns a thread: the first 32 are read a second time
+                float s[C::kCtas == 1 ? 64 : 32];
+                float top;
+                if constexpr (C::kCtas == 1) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) tc_ld32(st + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+                    tc_wait_ld();
+                    mask32(0, s);
+                    mask32(1, s + 32);
+                    top = fmaxf(max32(s), max32(s + 32));
+                } else {
+                    tc_ld32(st, reinterpret_cast<uint32_t *>(s));
+                    tc_wait_ld();
+                    mask32(0, s);
+                    top = max32(s);
+                    tc_ld32(st + 32, reinterpret_cast<uint32_t *>(s));
+                    tc_wait_ld();
+                    mask32(1, s);
+                    top = fmaxf(top, max32(s));
                 }
-                float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                for (int i = 4; i < 60; i += 8)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[i + x], s[i + 4 + x]);
-#pragma unroll
-                for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[60 + x]);
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 S.row_max[j & 1][wg][r_cta] = top;
-                tc_fence_before();
-                pair_sync(quad);   // the other half's maximum; and its scores are read: P may go over them
-                tc_fence_after();
+                pair_sync(quad);   // the other half's maximum
                 top = fmaxf(top, S.row_max[j & 1][wg ^ 1][r_cta]);
                 const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
                 const float mn = grow ? top : m;
@@ -666,20 +742,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {   // 32 columns at a time into the MMAs' hands
+                    constexpr int kHeld = C::kCtas == 1 ? 32 : 0;
+                    const int h = C::order(x);
+                    if (C::kCtas == 2 && x == 1) {
+                        tc_ld32(st, reinterpret_cast<uint32_t *>(s));
+                        tc_wait_ld();
+                        mask32(0, s);
+                    }
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float e0, e1;
-                        unpack_f32x2(add_f32x2(pack_f32x2(s[32 * x + 2 * i], s[32 * x + 2 * i + 1]), neg), e0, e1);
+                        unpack_f32x2(add_f32x2(pack_f32x2(s[kHeld * x + 2 * i], s[kHeld * x + 2 * i + 1]), neg), e0, e1);
                         e0 = ex2f(e0), e1 = ex2f(e1);
                         sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
                         p[i] = pack2_bf16(e0, e1);
                     }
-                    tc_st16(st + 32 * wg + 16 * x, p);
+                    tc_st16(st + 32 * h, p);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) signal_cluster(p_bar + (j & 1) * 16 + x * 8);
+                    if (lane == 0) signal_cluster(p_bar + j % C::kBufs * 16 + x * 8);
                 }
                 float s0, s1;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
@@ -761,7 +844,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1) k_prefi
     }
     cluster.sync();   // neither CTA leaves while the other may still signal it
     tc_fence_after();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(C::kTmem));
 }
 
 bool query_map(CUtensorMap *m, const uint16_t *base, int d, long long rows) {

@@ -258,6 +258,20 @@ def test_prefill_one_prompt(rows):
     check_prefill(p, prefill(p))
 
 
+@pytest.mark.parametrize("batch", [32, 33, 400])
+@pytest.mark.parametrize("shape", [(6, 1, 128, 64), (4, 2, 256, 64)])
+def test_prefill_many_sequences(shape, batch):
+    """Units in the order of their lengths, over sequences of all kinds: empty ones, ones of a few
+    rows behind long prefixes, several units of one length and of none (rows before position 0)."""
+    hq, hk, d, rotary = shape
+    rows = [(7 * i * i + 3 * i) % 23 if i % 5 else 0 if i % 2 else 60 + i % 70 for i in range(batch)]
+    past = [(i * 37) % 300 if i % 3 else -(i % 11) if i % 4 else 0 for i in range(batch)]
+    past = [max(x, -r) if r else max(x, 0) for x, r in zip(past, rows)]
+    p = Packed(rows, past, 16, hq, hk, d, rotary, seed=26, spare_rows=2, tail=float("nan"))
+    append(p)
+    check_prefill(p, prefill(p))
+
+
 def test_prefill_long_context_few_rows():
     p = Packed([3, 40], [20000, 9000], 64, 16, 2, 256, 64, seed=22, tail=float("nan"))
     append(p)
