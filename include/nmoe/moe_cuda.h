@@ -381,15 +381,17 @@ typedef struct nmoe_full_attn_shape {
                               multiplied with sigmoid(gate); 0: [query] per head               */
     float rope_theta;      /* > 0: pair t turns by position * theta^(-2 t / rotary_dims); the angle
                               is reduced in 64 bits                                            */
-    float norm_eps;        /* >= 0: x * rsqrt(mean(x^2) + eps) * (w + 1), w = q_norm / k_norm (bf16
+    float norm_eps;        /* > 0: x * rsqrt(mean(x^2) + eps) * (w + 1), w = q_norm / k_norm (bf16
                               [head_dim]); a NULL norm weight leaves the head as it is         */
 } nmoe_full_attn_shape;
 /* Keys and values in pages: element (page, row, head, dim) is at page * page_stride +
  * row * row_stride + head * head_stride + dim (strides in elements, multiples of 8, the same
  * for k and v), so [page][row][head][dim] and [page][head][row][dim] both fit. Position p of
  * sequence b lies in page block_table[b * table_stride + p / page_size], row p % page_size, for
- * p < max_pages * page_size (at most 2^31 - 1 positions). An entry outside [0, num_pages) is no
- * page: nothing is written there, and its positions are left out of every softmax. */
+ * p < max_pages * page_size (at most 2^31 - 257 positions; table_stride 0: one row for all). An
+ * entry outside [0, num_pages) is no page: nothing is written there, and its positions are left
+ * out of every softmax. Sequences may share pages that no call writes; where two rows of a call
+ * are appended to one place, which of them it holds is not defined. */
 typedef struct nmoe_paged_kv {
     uint16_t *k, *v;             /* bf16 */
     int64_t page_stride, row_stride, head_stride;
@@ -414,8 +416,8 @@ int nmoe_full_attn_append_paged(const nmoe_full_attn_weights *w, const nmoe_full
  * positions 0..p of its sequence, scores times `scale` (0: 1 / sqrt(head_dim)). q:
  * [total_rows][q_heads][head_dim, or 2 head_dim when gated] in x_dtype, row r at r * q_stride
  * elements (0: packed); normalised with q_norm and rotated here (w->k_norm is not read). out:
- * bf16 [total_rows][q_heads][head_dim]. Queries, probabilities and the cache meet in bf16
- * tensor-core products with fp32 sums. A row that sees no position (a negative position, or no
+ * bf16 [total_rows][q_heads][head_dim]; it overlaps no input. Queries, probabilities and the
+ * cache meet in bf16 tensor-core products with fp32 sums. A row that sees no position (a negative position, or no
  * page) gets zeros. kv_lens beyond max_pages * page_size: the positions past it do not exist.
  * A NaN or infinity in a position reaches only rows of its own sequence. workspace:
  * nmoe_full_attn_prefill_paged_workspace_bytes(), not shared by calls that overlap.
@@ -432,7 +434,7 @@ size_t nmoe_full_attn_prefill_paged_workspace_bytes(const nmoe_full_attn_shape *
  * are appended (as by nmoe_full_attn_append_paged) and its query attends to the positions
  * 0..kv_lens[b] - 1. k_new and v_new may both be NULL: the cache then holds them already. q,
  * k_new, v_new as above with one row per sequence; out [batch][q_heads][head_dim] in out_dtype
- * (F32 or BF16). Queries and probabilities are split into bf16 parts, so sums are as exact as
+ * (F32 or BF16); it overlaps no input. Queries and probabilities are split into bf16 parts, so sums are as exact as
  * in fp32 (out_dtype F32) or to about 2^-17 (BF16). kv_lens[b] < 1, or beyond max_pages *
  * page_size: zeros, nothing appended. workspace: nmoe_full_attn_step_paged_workspace_bytes(),
  * 16-byte aligned, not shared by calls that overlap. Two launches; allocates nothing; capturable
@@ -458,7 +460,11 @@ size_t nmoe_full_attn_step_paged_workspace_bytes(const nmoe_full_attn_shape *sha
  * [num_seqs][3][channels], delta_in / delta_out f32 [num_seqs][value_heads][128][128] (in and
  * out may be the same buffer; in may be NULL: zeros, a new sequence). A sequence without rows
  * gets its states unchanged. out [total_rows][value_heads * 128] in out_dtype; it overlaps no
- * input. Sums, states and norms are fp32. workspace: nmoe_linear_attn_prefill_workspace_bytes(), 16-byte aligned, not
+ * input. Sums, states and norms are fp32, for values and states up to 1e14 in magnitude; what the
+ * products read carries 22 bits (of what is below 2^-15 of a head's largest value or state in a
+ * chunk, 2^-38 of that). Rows go
+ * in chunks of 64 from a sequence's first on: a NaN or infinity reaches the rows of its own chunk
+ * and all behind them, and no other sequence. workspace: nmoe_linear_attn_prefill_workspace_bytes(), 16-byte aligned, not
  * shared by calls that overlap. Allocates nothing; capturable. */
 typedef struct nmoe_linear_attn_shape {
     int key_heads, value_heads; /* value_heads a multiple of key_heads; Qwen3.6: 16 and 32 */

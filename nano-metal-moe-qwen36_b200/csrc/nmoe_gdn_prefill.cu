@@ -8,26 +8,30 @@
 // M_ts = b_t e^{G_t-G_s} k_t . k_s (s < t). Then, with P_ts = e^{G_t-G_s} q_t . k_s (s <= t),
 //     O = e^G Q S^T + P U,   S' = e^{G_63} S + sum_t (e^{G_63-G_t} u_t) k_t^T
 //
-// Since P U = (P T b) (V - e^G K S^T), U and P U come out of one product.
+// With R = V - e^G K S^T, U = T b R, so P U = (P T b) R and, with Z = K^T (e^{G_63 - G} T b),
+//     S'^T = e^{G_63} S^T + Z R:
+// all that meets the state is one product with [K; Q] and, after R is made of it, one with [Z; P T b].
 //
-// Three launches. k_gdn_chunks, a CTA per (chunk, key head): convolution and norms of q and k, K K^T and
-// Q K^T, T b and P T b of its value heads; nothing here depends on the state. k_gdn_scan, a CTA per
+// Three kinds of launch. k_gdn_chunks, a CTA per (chunk, key head): convolution and norms of q and k, K K^T and
+// Q K^T, P T b and Z of its value heads; nothing here depends on the state. k_gdn_scan, a CTA per
 // (sequence, value head, 64 of the 128 value columns): the recurrence over the chunks; the columns of
 // the state never mix, so the CTAs of a head share nothing. k_gdn_finish: gated norm and conv states.
+// Long sequences that leave SMs idle go in parts: the preparation of a part and the norm of an earlier one run on
+// those SMs beside the scan of the part between (see parts_of).
 //
 // Arithmetic: every product's operands are split into two fp16 parts, x = hi + lo (22 bits), and the
-// products hi hi, hi lo, lo hi summed in fp32, so that states are as exact as with fp32 operands (1e-7 of
-// their norm). fp16 has the range of 2^40 only: k, q and P are scaled by constants, the state and U by a
-// power of two that follows a bound on them (|u| <= max |v| + |S|, |S'|^2 <= |S|^2 + sum v^2, row by row,
-// since |k| <= 1 and b <= 1).
+// products hi hi, hi lo, lo hi summed in fp32, so that states are as exact as with fp32 operands (4e-7 of
+// their norm). fp16 has the range of 2^40 only: k, q, P and Z are scaled by constants (Z's columns, like
+// k, are no longer than one: what a token leaves in the state after contractions), the state and R by a power of two
+// that follows a bound on them (|u| <= max |v| + |S|, |S'|^2 <= e^{2 G_63} |S|^2 + sum v^2, row by row, since |k| <= 1
+// and b <= 1).
 //
-// The scan is a chain of three products a chunk, 128 rows high, on tcgen05: [K; Q] S^T (128 x 64 x 128),
-// [e^{G_63 - G} T b; P T b] R (128 x 64 x 64), whose upper half is W = e^{G_63 - G} U, and K^T W
-// (128 x 64 x 64); between them eight warps
-// read the sums from tensor memory, a thread per row and 32 columns, and write the next operand as rows
-// of 128 bytes, which the MMA takes as they are (MN-major). The warp tensor instructions needed the
-// fragments through registers, 3 KB of shared memory traffic a cycle's worth of products, and ran
-// 3.4 us a chunk for half the columns. What bounds it: the chain's latency.
+// The scan is a chain of two products a chunk, 128 rows high, on tcgen05: [K; Q] S^T (128 x 64 x 128) and Z R
+// (128 x 64 x 64); P T b R follows beside the work on the state. Between them eight warps read the sums from tensor
+// memory, a thread per row and 32 columns, and write the next operand as rows of 128 bytes, which the MMA takes as
+// they are (MN-major). What bounds it: the chain's latency, 4500 cycles a chunk, of which the products, bound by
+// shared memory's bandwidth, take 1800. Measured, 16 key and 32 value heads, bf16: 16384 rows 842 us (preparation,
+// scan and norm one after the other: 1052), of which 75 us are the first part's preparation.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -78,6 +82,7 @@ struct GdnArgs {
     void *out;
     int num_seqs, total_rows, key_heads, value_heads, channels, x_bf16, out_bf16;
     int part, parts;   // of every sequence's chunks: those that a launch takes
+    int room;          // chunks that the workspace holds: as many as there are when cu_rows does not decrease
     // workspace, per chunk and head: K over Q, hi and lo; T b over P T b, hi and lo; gates; and O
     uint8_t *kq, *tp, *gates;
     float *o;
@@ -405,6 +410,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
         return;
     }
     const int chunk = found[4] + found[1];   // in the workspace: over all chunks of all sequences
+    if ((unsigned)chunk >= (unsigned)a.room) {
+        if (last_cta) pdl_wait();
+        return;
+    }
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(smem_u32(&tmem_at)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -933,7 +942,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         for (int i = tid; i < b; i += kScanThreads) before += seq_chunks(a, i);
         if (before) atomicAdd(&S.first_chunk, before);   // integers: the order does not matter
     }
-    const int all = seq_chunks(a, b), from = part_first(a, all, a.part), chunks = part_first(a, all, a.part + 1) - from;
+    const int all = seq_chunks(a, b), from = part_first(a, all, a.part);
     const int row0 = seq_first(a, b) + from * kC, rows = seq_rows(a, b) - from * kC;   // from this part's first on
     const int wg = warp >> 2, r = 32 * (warp & 3) + lane, c0 = 32 * wg;
     const bool is_q = warp < 8 && (warp & 3) >= 2;
@@ -956,7 +965,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         if (lane == 0) atomicMax(&S.vmax[2], __float_as_int(m));   // not negative: ordered as integers
     }
     __syncthreads();
-    const long long chunk0 = S.first_chunk + from;
+    const long long chunk0 = (long long)S.first_chunk + from;
+    const int here = part_first(a, all, a.part + 1) - from;
+    const int chunks = chunk0 < 0 || chunk0 + here > a.room ? 0 : here;   // not beyond the workspace, whatever cu_rows holds
     float bound2 = __int_as_float(S.vmax[2]);   // of |S|^2, per value row
     bound2 = bound2 * bound2 * kD;
     __syncthreads();
@@ -1138,11 +1149,13 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             bar_sync(is_q ? 2 : 1, 256);
             if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to for chunk c + 2
             const float vm = __int_as_float(S.vmax[c % 3]);
-            bound2 += kC * vm * vm;                  // of the states of this chunk, and of the one it leaves
-            const int eu = exponent_of(bound2) + 1;  // max |v| + |S| <= 9/8 sqrt(bound2)
+            // of the states of this chunk; the one it leaves has decayed, so that what was large is forgotten
+            const float before2 = bound2, in2 = kC * vm * vm;
+            const int eu = exponent_of(before2 + in2) + 1;   // max |v| + |S| <= 9/8 of its root
             const float *eg = reinterpret_cast<const float *>(smem + L::kGate + (c & 1) * kGates);
             wait_bar(&S.kq_full[c & 1], (c >> 1) & 1, &S.stop);
             const float g = eg[t], keep = eg[kC - 1];
+            bound2 = keep * keep * before2 + in2;
             if (!is_q) {
                 // R = V - e^G K S^T, scaled
                 const float k0 = -g * pow2(es) * pow2(-eu) * (1.f / kScaleK), s = pow2(-eu);
@@ -1305,6 +1318,7 @@ cudaError_t launch(GdnArgs a, cudaStream_t st) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return e;
     a.parts = parts_of(a, sms);
+    a.room = (int)max_chunks(a.num_seqs, a.total_rows);
     for (a.part = 0; a.part < a.parts; ++a.part) {
         if (a.total_rows > 0) {
             // a sequence's part has at most its chunks / parts, rounded up
@@ -1420,7 +1434,7 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     a.out_bf16 = out_dtype == NMOE_DTYPE_BF16;
     if (workspace == nullptr || !aligned_to(workspace, 16)) return fail(NMOE_EINVAL, "workspace is NULL or not aligned");
-    if (max_chunks(num_seqs, total_rows) > 2147483647ll || a.value_heads > 65535)
+    if (max_chunks(num_seqs, total_rows) > 2147483647ll || total_rows > 2147483647 - kC || a.value_heads > 65535)
         return fail(NMOE_EINVAL, "too many rows or sequences");
     carve(*shape, num_seqs, total_rows, static_cast<uint8_t *>(workspace), &a);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

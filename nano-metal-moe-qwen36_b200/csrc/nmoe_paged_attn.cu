@@ -62,8 +62,8 @@ int check_paged_kv(const nmoe_paged_kv *kv, PagedDev *d) {
         return full_attn_fail(NMOE_EINVAL, "the cache or one of its pointers is NULL");
     if (kv->num_pages < 1 || kv->page_size < 1 || kv->max_pages < 1 || kv->table_stride < 0)
         return full_attn_fail(NMOE_EINVAL, "num_pages, page_size and max_pages must be positive");
-    if ((long long)kv->max_pages * kv->page_size > 2147483647ll - 64)
-        return full_attn_fail(NMOE_EINVAL, "max_pages * page_size exceeds 2^31 - 65 positions");
+    if ((long long)kv->max_pages * kv->page_size > 2147483647ll - 256)   // the end of the last tile is an int too
+        return full_attn_fail(NMOE_EINVAL, "max_pages * page_size exceeds 2^31 - 257 positions");
     if (!aligned_to(kv->k, 16) || !aligned_to(kv->v, 16) || !aligned_to(kv->block_table, 4))
         return full_attn_fail(NMOE_EINVAL, "pages must be 16-byte aligned, the block table 4-byte");
     if (((kv->page_stride | kv->row_stride | kv->head_stride) & 7) != 0 || kv->page_stride < 0 ||

@@ -14,10 +14,14 @@
 // from shared memory to keep the tensor cores busy, the pair 31 and 95.
 //
 // Softmax: two threads per query row (warps 0-7, 64 columns each) read its 128 scores from tensor
-// memory, keep the running maximum and sum in fp32, and write P back as bf16 over the scores. O is rescaled only
+// memory, keep the running maximum and sum in fp32, and write P back as bf16 over the scores. Queries and P are
+// rounded to bf16, the type of the pages, since an MMA's operands have one type: the output is off by 0.0025 of its
+// norm, of which its own rounding is 0.0017; two bf16 parts of either would double the products. O is rescaled only
 // when a row's maximum has grown by more than 2^8 since the last time: O and the sum carry the same
 // reference, so the result does not depend on which one it is. While S of tile j is in the softmax,
-// the tensor cores run S of tile j + 1 and P V of tile j - 1.
+// the tensor cores run S of tile j + 1 and P V of tile j - 1. Measured: a prompt of 16384 rows, 16 query and 2 KV heads
+// of 256: 1.59 ms in a burst, 1.38 PFLOP/s (of the visible pairs; the tiles on the diagonal are computed whole); held for
+// seconds, under the power limit, 1.81 ms.
 //
 // Pages: a warp of each CTA copies boxes of page rows by TMA (the rows of a box lie in one page, as
 // a tile's 64 positions may lie in many). Positions behind a sequence's end, and pages that are

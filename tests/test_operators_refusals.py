@@ -40,7 +40,7 @@ REFUSED = [
     (dict(kv_heads=0), ALL), (dict(rotary=48), ALL), (dict(rotary=8), ALL), (dict(rotary=512), ALL), (dict(rotary=-16), ALL),
     (dict(theta=0.0), ALL), (dict(theta=float("nan")), ALL), (dict(eps=0.0), ALL), (dict(eps=float("nan")), ALL),
     (dict(gated=2), ALL), (dict(pages=0), ALL), (dict(page_size=0), ALL), (dict(max_pages=0), ALL),
-    (dict(max_pages=1 << 27), ALL), (dict(k=None), ALL), (dict(v=None), ALL), (dict(table=None), ALL), (dict(table=A + 2), ALL),
+    (dict(max_pages=1 << 27), ALL), (dict(page_size=1, max_pages=(1 << 31) - 256), ALL), (dict(k=None), ALL), (dict(v=None), ALL), (dict(table=None), ALL), (dict(table=A + 2), ALL),
     (dict(k=A + 8), ALL), (dict(ps=8193), ALL), (dict(rs=4), ALL), (dict(hs=-256), ALL), (dict(ts=-1), ALL),
     (dict(x_dtype=N.DTYPE_Q4), ALL), (dict(n=-1), ALL), (dict(lens=None), ALL),
     (dict(rows=-1), ["append", "prefill"]), (dict(cu=None), ["append", "prefill"]), (dict(cu=A + 1), ["append", "prefill"]),
