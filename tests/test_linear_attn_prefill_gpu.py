@@ -206,3 +206,27 @@ def test_prompts_prepared_in_parts(rows, dtype):
         torch.cuda.synchronize()
         for x, y in zip(a, (out, conv, delta)):
             assert torch.equal(x, y)
+
+
+def test_two_streams_with_workspaces_of_their_own():
+    """Two calls at once, one of them in parts, give what each gives alone."""
+    a, b = Prompt([9001], 1, 2, torch.bfloat16, seed=14), Prompt([700, 64, 1300], 4, 8, torch.float32, seed=15)
+    alone = [p.run() for p in (a, b)]
+    calls = []
+    for p, code in ((a, N.DTYPE_BF16), (b, N.DTYPE_F32)):
+        s = N.LinearAttnShape(p.hk, p.hv)
+        ws = torch.full((N.linear_attn_prefill_workspace_bytes(s, len(p.rows), p.total),), 255, dtype=torch.uint8, device="cuda")
+        outs = [(torch.full((p.total, p.hv * 128), 7.0, device="cuda"), torch.empty_like(p.conv), torch.empty_like(p.delta))
+                for _ in range(4)]
+        calls.append((p, s, ws, outs, torch.cuda.Stream(), code))
+    torch.cuda.synchronize()
+    for i in range(4):
+        for p, s, ws, outs, stream, code in calls:
+            out, conv, delta = outs[i]
+            N.linear_attn_prefill(p.w, s, p.qkv, p.z, p.alpha, p.beta, p.cu, p.conv, p.delta, conv, delta, out, ws,
+                                  x_dtype=code, out_dtype=N.DTYPE_F32, stream=stream.cuda_stream)
+    torch.cuda.synchronize()
+    for want, (_, _, _, outs, _, _) in zip(alone, calls):
+        for got in outs:
+            for x, y in zip(want, got):
+                assert torch.equal(x, y)
