@@ -913,7 +913,18 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     __shared__ ScanShared S;
     uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x, vh = blockIdx.y, b = blockIdx.z, kh = vh / (a.value_heads / a.key_heads);
+    const int split = blockIdx.x, vh = blockIdx.y, kh = vh / (a.value_heads / a.key_heads);
+    // The longest sequences first, as far as a lane a sequence goes: CTAs begin as SMs become free
+    int b = blockIdx.z;
+    if (a.num_seqs > 1 && a.num_seqs <= 32) {
+        const int n = lane < a.num_seqs ? seq_chunks(a, lane) : -1;
+        int rank = 0;
+        for (int i = 0; i < a.num_seqs; ++i) {
+            const int v = __shfl_sync(0xffffffffu, n, i);
+            rank += v > n || (v == n && i < lane);
+        }
+        b = __ffs(__ballot_sync(0xffffffffu, lane < a.num_seqs && rank == b)) - 1;
+    }
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&S.kq_full[i], 1);
@@ -935,8 +946,10 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = S.tmem;
-    pdl_wait();   // this part's chunks, and with them the parts before
-    pdl_trigger();
+    // This part's chunks, and with them the parts before, are complete: for the warp that copies them, and from the
+    // second part on for the state too. The inputs were there when the first part's chunks were begun.
+    if (a.part > 0 || warp == 8) pdl_wait();
+    if (warp == 8) pdl_trigger();
     {
         int before = 0;
         for (int i = tid; i < b; i += kScanThreads) before += seq_chunks(a, i);
@@ -1332,7 +1345,7 @@ cudaError_t launch(GdnArgs a, cudaStream_t st) {
         if (e != cudaSuccess) return e;
     }
     const long long want = ((a.total_rows + 14ll) / 8 * a.value_heads + kWarps - 1) / kWarps;   // a warp 8 rows of a head
-    const int norm_blocks = a.total_rows == 0 ? 0 : (int)(want < 8ll * sms ? want : 8ll * sms);
+    const int norm_blocks = a.total_rows == 0 ? 0 : (int)(want < 2ll * sms ? want : 2ll * sms);
     const long long conv_blocks = ((long long)a.num_seqs * a.channels + kThreads - 1) / kThreads;
     return launch_one(k_gdn_finish<kBf16>, dim3((unsigned)(norm_blocks + conv_blocks)), kThreads, 0, st, true, 1, a, norm_blocks);
 }
