@@ -437,55 +437,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
     const int rank = (int)cluster.block_rank();
     const int per_cta = kRows / a.group, per_unit = 2 * per_cta;   // tokens
 
-    // ---- the unit: (sequence, query tile, KV head), in the order of how many tiles of positions they walk over, the
-    // most first: units are handed to SMs as these become free, and a long one begun last would run alone. The
-    // length of this one by bisection over how many units are at least as long, each sequence's by one division;
-    // by every warp for itself, a lane a sequence, or by the CTA when there are more than 32.
+    // ---- the unit: (sequence, query tile, KV head). Units are handed to SMs as these become free, so a long one that
+    // begins last would run alone. Up to 32 sequences, a lane each: in the order of how many tiles of positions they
+    // walk over, the most first. The length of this one by bisection over how many units are at least as long, each
+    // sequence's by one division; by every warp for itself. More sequences: by sequence, the last tiles (the
+    // longest) first, since a bisection over them costs every unit microseconds.
     const int unit = blockIdx.x >> 1, kvh = unit % a.kv_heads, want = unit / a.kv_heads;
+    auto rows_of = [&](int b) { return max(0, min(a.total_rows, a.cu_rows[b + 1]) - max(0, a.cu_rows[b])); };
+    auto units_of = [&](int rows) { return (int)(((unsigned)rows + per_unit - 1) / per_unit); };
     if (tid == 0) {
         S.unit_seq = -1;
         S.stop = 0;
     }
-    {
-        const bool small = a.num_seqs <= 32;
-        const int first = small ? lane : tid, step = small ? 32 : kThreads;
-        auto load_rows = [&](int b) { return max(0, min(a.total_rows, a.cu_rows[b + 1]) - max(0, a.cu_rows[b])); };
-        const int rows0 = first < a.num_seqs ? load_rows(first) : 0, len0 = first < a.num_seqs ? a.kv_lens[first] : 0;
-        auto rows_of = [&](int b) { return b == first ? rows0 : load_rows(b); };
-        auto len_of = [&](int b) { return b == first ? len0 : a.kv_lens[b]; };
-        // of sequence b: its units, and of them the first that walks over `tiles` tiles or more (they grow)
-        auto units = [&](int b) { return (int)(((unsigned)rows_of(b) + per_unit - 1) / per_unit); };
-        auto from = [&](int b, int n, int tiles) {
-            if (tiles <= 0 || n == 0) return 0;
-            const long long len = len_of(b), need = (long long)(tiles - 1) * kTile + 1;   // positions
-            if (min(len, (long long)a.c.capacity) < need) return n;
-            const long long rows = need - (len - rows_of(b));   // of the sequence's rows, that many
-            return rows <= 0 ? 0 : min((int)(((unsigned)rows + per_unit - 1) / per_unit) - 1, n - 1);
+    if (a.num_seqs <= 32) {
+        const bool own = lane < a.num_seqs;
+        const int rows = own ? rows_of(lane) : 0, units = units_of(rows);
+        const long long len = own ? a.kv_lens[lane] : 0, there = max(0ll, min(len, (long long)a.c.capacity));
+        auto from = [&](int tiles) {   // of this lane's units, the first that walks over `tiles` tiles or more (they grow)
+            if (tiles <= 0 || units == 0) return 0;
+            const long long need = (long long)(tiles - 1) * kTile + 1;   // positions
+            if (there < need) return units;
+            const long long r = need - (len - rows);   // of the sequence's rows, that many
+            return r <= 0 ? 0 : min(units_of((int)r) - 1, units - 1);
         };
-        auto combine = [&](int v, auto add) {
-            if (small) return v;
-            if (lane == 0) S.scan[warp] = v;
-            __syncthreads();
-            v = S.scan[0];
-            for (int w = 1; w < kThreads / 32; ++w) v = add ? v + S.scan[w] : max(v, S.scan[w]);
-            __syncthreads();
-            return v;
-        };
-        auto at_least = [&](int tiles) {
-            int v = 0;
-            for (int b = first; b < a.num_seqs; b += step) {
-                const int n = units(b);
-                v += n - from(b, n, tiles);
-            }
-            return combine(__reduce_add_sync(0xffffffffu, v), true);
-        };
-        int lo = 0, hi = 0, longer = 0;   // at_least(lo) > want >= at_least(hi) = longer
+        auto at_least = [&](int tiles) { return (int)__reduce_add_sync(0xffffffffu, units - from(tiles)); };
         if (at_least(0) > want) {
-            {   // the longest there is
-                int most = 0;
-                for (int b = first; b < a.num_seqs; b += step) most = max(most, (int)min((long long)max(0, len_of(b)), (long long)a.c.capacity));
-                hi = (combine(__reduce_max_sync(0xffffffffu, most), false) + kTile - 1) / kTile + 1;
-            }
+            // at_least(lo) > want >= at_least(hi) = longer
+            int lo = 0, hi = ((int)__reduce_max_sync(0xffffffffu, (int)there) + kTile - 1) / kTile + 1, longer = 0;
             while (hi - lo > 1) {
                 const int mid = lo + (hi - lo) / 2, n = at_least(mid);
                 if (n > want)
@@ -494,40 +472,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
                     hi = mid, longer = n;
             }
             // of the units of length lo, the (want - longer)-th
-            int own = 0;
-            auto same = [&](int b, int *k) {
-                const int n = units(b);
-                *k = from(b, n, lo);
-                return from(b, n, lo + 1) - *k;
-            };
-            int k;
-            for (int b = first; b < a.num_seqs; b += step) own += same(b, &k);
-            int before = own;
+            const int k = from(lo), same = from(lo + 1) - k;
+            int before = same;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const int v = __shfl_up_sync(0xffffffffu, before, o);
                 if (lane >= o) before += v;
             }
-            if (!small) {
-                if (lane == 31) S.scan[warp] = before;
-                __syncthreads();
-                for (int w = 0; w < warp; ++w) before += S.scan[w];
+            before -= same;
+            const int nth = want - longer - before;
+            if (warp == 0 && nth >= 0 && nth < same) {
+                S.unit_seq = lane;
+                S.unit_off = k + nth;
             }
-            before -= own;
-            const int nth = want - longer;
-            if (nth >= before && nth < before + own && (!small || warp == 0))
-                for (int b = first; b < a.num_seqs; b += step) {
-                    const int n = same(b, &k);
-                    if (nth < before + n) {
-                        S.unit_seq = b;
-                        S.unit_off = k + nth - before;
-                        break;
-                    }
-                    before += n;
-                }
         }
+    } else {
+        const int per = (a.num_seqs + kThreads - 1) / kThreads;
+        const int first = min(a.num_seqs, tid * per), last = min(a.num_seqs, first + per);
+        int own = 0;
+        for (int b = first; b < last; ++b) own += units_of(rows_of(b));
+        int before = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += v;
+        }
+        if (lane == 31) S.scan[warp] = before;
         __syncthreads();
+        before -= own;
+        for (int w = 0; w < warp; ++w) before += S.scan[w];
+        if (want >= before && want < before + own)
+            for (int b = first; b < last; ++b) {
+                const int n = units_of(rows_of(b));
+                if (want < before + n) {
+                    S.unit_seq = b;
+                    S.unit_off = n - 1 - (want - before);
+                    break;
+                }
+                before += n;
+            }
     }
+    __syncthreads();
     const int b = S.unit_seq;
     if (b < 0) return;   // both CTAs of the pair: there are fewer units than the grid has room for
     const int lo = max(0, a.cu_rows[b]), rows_b = min(a.total_rows, a.cu_rows[b + 1]) - lo;
