@@ -76,27 +76,27 @@ template <int D>
 struct Cfg {
     static constexpr int kQB = kRows * D * 2;
     static constexpr int kStageB = 64 * D * 2;              // half a K or V tile
-    // At head_dim 256 a CTA has the SM, and two S tiles so that the next one's product runs beside the softmax. At
-    // 128 a tile's products take half of that and its softmax, a chain of waits, as long as ever: two CTAs share
-    // the SM, an S tile each, and one's products run beside the other's softmax. Seven packed prompts of 1 to 3000
-    // rows, 24 query and 4 KV heads, behind up to 8191 positions: 270 us, for 331 us with one CTA an SM
-    static constexpr int kCtas = D == 256 ? 1 : 2, kBufs = D == 256 ? 2 : 1;
+    // A step is what goes through the softmax at a time: at head_dim 256 a tile, at 128 half of one (32 of each
+    // CTA's 64 positions). Two steps' scores lie in tensor memory, so that the next one's product runs beside the
+    // softmax. At 256 a CTA has the SM; at 128 a step's products take a quarter of that time and its softmax, a chain
+    // of waits, is what lasts: two CTAs share the SM. Seven packed prompts of 1 to 3000 rows, 24 query and 4 KV
+    // heads, behind up to 8191 positions: 248 us; with whole tiles, one at a time, 265 us, and with one CTA
+    // an SM 331 us
+    static constexpr int kCtas = D == 256 ? 1 : 2, kHalves = D == 256 ? 1 : 2;
+    static constexpr int kCols = 64 / kHalves, kStep = 2 * kCols;   // columns of a thread, of a step
     static constexpr int kStages = D == 256 ? 5 : 4;
     static constexpr int kRing = kQB, kShared = kQB + kStages * kStageB;   // offsets in shared memory
     static constexpr int kSmem = kShared + (int)sizeof(Shared);
     static_assert(kSmem <= (kCtas == 1 ? 232448 : 115712), "shared memory of a CTA");
-    static constexpr uint32_t kO = 0, kS = D;               // TMEM columns: O, then the S tiles of 128
-    static constexpr uint32_t kTmem = D + kBufs * kTile;
+    static constexpr uint32_t kO = 0, kS = D;               // TMEM columns: O, then two steps' scores
+    static constexpr uint32_t kTmem = D + 2 * kStep;
     static_assert(kTmem * kCtas == 512, "tensor memory of the SM");
     static constexpr int kOutB = D * 4 + 16;                // a row of O on its way out
     static_assert(kRows * kOutB <= kQB + kStages * kStageB, "the output rows reuse the queries and the ring");
-    // the stage that holds K tile j, V tile j of n: K 0, K 1, V 0, K 2, V 1, .. with two S tiles, K 0, V 0, K 1, .. with one
-    __device__ static uint32_t k_stage(int j) { return kBufs == 1 ? 2 * j : j == 0 ? 0 : 2 * j - 1; }
-    __device__ static uint32_t v_stage(int j, int n) { return kBufs == 1 || j == n - 1 ? 2 * j + 1 : 2 * j + 2; }
-    // column of the 16 positions i of P: in the place of the scores that they are made of, by the thread that read them
-    __device__ static uint32_t p_at(uint32_t i) { return 64 * (i >> 2) + 32 * ((i >> 1) & 1) + 8 * (i & 1); }
-    // which 32 of a thread's 64 columns are handed over first (0) and second (1)
-    __device__ static constexpr int order(int x) { return kBufs == 1 ? 1 - x : x; }
+    // the stage that holds K tile j, V tile j of n, in the order in which they are read: K 0, K 1, V 0, K 2, V 1, .. by
+    // steps of a tile, K 0, V 0, K 1, V 1, .. by halves
+    __device__ static uint32_t k_stage(int j) { return kHalves == 2 ? 2 * j : j == 0 ? 0 : 2 * j - 1; }
+    __device__ static uint32_t v_stage(int j, int n) { return kHalves == 2 || j == n - 1 ? 2 * j + 1 : 2 * j + 2; }
 };
 
 __device__ __forceinline__ uint32_t cluster_addr(const void *p, int rank) {
@@ -449,7 +449,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
         S.unit_seq = -1;
         S.stop = 0;
     }
-    if (a.num_seqs <= 32) {
+    if (a.num_seqs == 1) {   // its last units are its longest
+        const int units = units_of(rows_of(0));
+        if (tid == 0 && want < units) {
+            S.unit_seq = 0;
+            S.unit_off = units - 1 - want;
+        }
+    } else if (a.num_seqs <= 32) {
         const bool own = lane < a.num_seqs;
         const int rows = own ? rows_of(lane) : 0, units = units_of(rows);
         const long long len = own ? a.kv_lens[lane] : 0, there = max(0ll, min(len, (long long)a.c.capacity));
@@ -585,63 +591,67 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             const uint32_t q_at = smem_u32(q_smem), ring_at = smem_u32(ring);
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
             const int n = __shfl_sync(0xffffffffu, n_tiles, 0);
-            const uint32_t id_s = idesc2(kTile, 0), id_o = idesc2(D, 1);
+            const uint32_t id_s = idesc2(C::kStep, 0), id_o = idesc2(D, 1);
+            const int steps = n * C::kHalves;
             // V in shared memory: [box][panel][rows][64], one box when the warp copies
             const uint32_t v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop));
             };
-            uint32_t s = 0, round = 0;   // the stage that the next MMAs read, and the parity of its use
-            auto next = [&] {
-                if (++s == C::kStages) s = 0, round ^= 1;
+            // the stages that the next K and V tile are read from, and the parity of their filling
+            uint32_t k_at = 0, k_round = 0, v_at = C::v_stage(0, n), v_round = 0;
+            auto advance = [&](uint32_t &at, uint32_t &round, uint32_t by) {
+                at += by;
+                if (at >= C::kStages) at -= C::kStages, round ^= 1;
             };
-            auto full = [&](uint32_t ahead) {   // the stage `ahead` of the next one has been filled
-                const uint32_t x = s + ahead;
-                return x < C::kStages ? wait(&S.full[x], round) : wait(&S.full[x - C::kStages], round ^ 1);
-            };
-            auto qk = [&](int j) {
-                const uint32_t at = ring_at + s * C::kStageB, d = tm + C::kS + j % C::kBufs * kTile;
+            // S of step t: of its tile (half x)
+            auto qk = [&](int t) {
+                const int j = t / C::kHalves, x = t % C::kHalves;
+                const uint32_t at = ring_at + k_at * C::kStageB + x * 32 * 128;
 #pragma unroll
                 for (uint32_t i = 0; i < D / 16; ++i)
-                    mma2_ss(d, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
+                    mma2_ss(tm + C::kS + (t & 1) * C::kStep, desc_k(q_at + (i >> 2) * (kRows * 128) + (i & 3) * 32),
                             desc_k(at + (i >> 2) * 8192 + (i & 3) * 32), id_s, i > 0 ? 1u : 0u, one);
-                commit2(&S.empty[s], one);
-                commit2(&S.s_full[j % C::kBufs], one);
-                next();
+                if (x == C::kHalves - 1) {
+                    commit2(&S.empty[k_at], one);
+                    advance(k_at, k_round, C::k_stage(j + 1) - C::k_stage(j));
+                }
+                commit2(&S.s_full[t & 1], one);
             };
-            // P V of tile j, the two quarters of P that the softmax hands over first, then the others
-            auto pv = [&](int j) {
-                const uint32_t at = ring_at + s * C::kStageB, p = tm + C::kS + j % C::kBufs * kTile;
+            // P V of step t, in the 32 positions of each CTA's half that the softmax hands over together. The 16
+            // positions i of P lie over the scores that they were made of
+            auto pv = [&](int t) {
+                const int j = t / C::kHalves, x = t % C::kHalves;
+                const uint32_t at = ring_at + v_at * C::kStageB;
+                const uint32_t p = tm + C::kS + (t & 1) * C::kStep;
 #pragma unroll
-                for (uint32_t x = 0; x < 2; ++x) {
-                    if (!wait(&S.p_ready[j % C::kBufs][x], j / C::kBufs & 1)) return false;
+                for (uint32_t h = 0; h < 2 / C::kHalves; ++h) {
+                    if (!wait(&S.p_ready[t & 1][h], t >> 1 & 1)) return false;
                     tc_fence_after();
 #pragma unroll
                     for (uint32_t y = 0; y < 4; ++y) {
-                        const uint32_t i = 2 * C::order(x) + (y & 1) + 4 * (y >> 1);
-                        mma2_ts(tm + C::kO, p + C::p_at(i),
+                        const uint32_t i = 2 * (C::kHalves == 2 ? x : h) + (y & 1) + 4 * (y >> 1);
+                        mma2_ts(tm + C::kO, p + C::kCols * (y >> 1) + 32 * h + 8 * (y & 1),
                                 desc_mn(at + (i >> v_shift) * (v_rows * D) + (i & ((1u << v_shift) - 1)) * 2048, v_rows * 128),
-                                id_o, (j > 0 || x + y > 0) ? 1u : 0u, one);
+                                id_o, (t > 0 || h + y > 0) ? 1u : 0u, one);
                     }
                 }
-                commit2(&S.empty[s], one);
+                if (x == C::kHalves - 1) {
+                    commit2(&S.empty[v_at], one);
+                    advance(v_at, v_round, C::v_stage(j + 1, n) - C::v_stage(j, n));
+                }
                 commit2(&S.o_done, one);
-                next();
                 return true;
             };
-            // S 0, S 1, P V 0, S 2, P V 1, ..: S of tile j + 1 runs while tile j is in the softmax (with one S tile:
-            // S 0, P V 0, S 1, ..). What was copied is waited for ahead of P, so that P V and the next S follow it at
-            // once.
-            bool ok = wait(&S.q_ready, 0) && full(0);
-            tc_fence_after();
-            if (ok) qk(0);
-            if (C::kBufs == 2 && ok && n > 1 && (ok = full(0))) {
+            // S 0, S 1, P V 0, S 2, P V 1, ..: S of step t + 1 runs while step t is in the softmax. What was
+            // copied is waited for ahead of P, so that P V t and S t + 2 follow it at once.
+            bool ok = wait(&S.q_ready, 0);
+            for (int t = -2; t < steps && ok; ++t) {
+                if (t >= 0 && t % C::kHalves == 0) ok = wait(&S.full[v_at], v_round);
+                if (t + 2 < steps && (t + 2) % C::kHalves == 0) ok = ok && wait(&S.full[k_at], k_round);
                 tc_fence_after();
-                qk(1);
-            }
-            for (int j = 0; j < n && ok; ++j) {
-                ok = full(0) && (j + C::kBufs >= n || full(1)) && pv(j);
-                if (ok && j + C::kBufs < n) qk(j + C::kBufs);
+                if (t >= 0 && ok) ok = pv(t);
+                if (t + 2 < steps && ok) qk(t + 2);
             }
             if (ok) commit2(&S.done, one);
         }
@@ -659,62 +669,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             const uint32_t p_bar = cluster_addr(&S.p_ready[0][0], 0);
             // the first position that some row of this warp does not see
             const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
-            for (int j = 0; j < n_tiles; ++j) {
-                wait_bar(&S.s_full[j % C::kBufs], j / C::kBufs & 1, &S.stop);
+            for (int t = 0; t < n_tiles * C::kHalves; ++t) {
+                const int j = t / C::kHalves, x0 = t % C::kHalves;
+                wait_bar(&S.s_full[t & 1], t >> 1 & 1, &S.stop);
                 tc_fence_after();
-                const uint32_t st = tmem + lanes + C::kS + j % C::kBufs * kTile + 64 * wg;
+                const uint32_t st = tmem + lanes + C::kS + (t & 1) * C::kStep + C::kCols * wg;
+                float s[C::kCols];
+#pragma unroll
+                for (int c = 0; c < C::kCols / 32; ++c) tc_ld32(st + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+                tc_wait_ld();
                 const uint32_t *info = S.info[j % kInfo];
-                const bool masked = (j + 1) * kTile > seen || !info[4];
-                const int n = pos - j * kTile - 64 * wg;   // columns 0..n of this half are seen
-                auto mask32 = [&](int c, float *s) {
-                    if (!masked) return;
-                    const int k = n - 32 * c;
-                    const uint32_t w = info[2 * wg + c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
+                if ((j + 1) * kTile > seen || !info[4]) {
+                    const int n = pos - j * kTile - 64 * wg - 32 * x0;   // columns 0..n of this thread's are seen
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[i] = w >> i & 1u ? s[i] : -INFINITY;
-                };
-                auto max32 = [&](const float *s) {
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
+                    for (int c = 0; c < C::kCols / 32; ++c) {
+                        const int k = n - 32 * c;
+                        const uint32_t w = info[2 * wg + x0 + c] & (k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1u);
 #pragma unroll
-                    for (int i = 4; i < 28; i += 8)
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[i + x], s[i + 4 + x]);
-                    return max3(max3(mx[0], mx[1], mx[2]), mx[3], fmaxf(fmaxf(s[28], s[29]), fmaxf(s[30], s[31])));
-                };
-                // two CTAs an SM have registers for 32 columns a thread: the first 32 are read a second time
-                float s[C::kCtas == 1 ? 64 : 32];
-                float top;
-                if constexpr (C::kCtas == 1) {
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) tc_ld32(st + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
-                    tc_wait_ld();
-                    mask32(0, s);
-                    mask32(1, s + 32);
-                    top = fmaxf(max32(s), max32(s + 32));
-                } else {
-                    tc_ld32(st, reinterpret_cast<uint32_t *>(s));
-                    tc_wait_ld();
-                    mask32(0, s);
-                    top = max32(s);
-                    tc_ld32(st + 32, reinterpret_cast<uint32_t *>(s));
-                    tc_wait_ld();
-                    mask32(1, s);
-                    top = fmaxf(top, max32(s));
+                        for (int i = 0; i < 32; ++i) s[32 * c + i] = w >> i & 1u ? s[32 * c + i] : -INFINITY;
+                    }
                 }
-                S.row_max[j & 1][wg][r_cta] = top;
-                pair_sync(quad);   // the other half's maximum
-                top = fmaxf(top, S.row_max[j & 1][wg ^ 1][r_cta]);
+                float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < C::kCols - 4; i += 8)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) mx[x] = max3(mx[x], s[i + x], s[i + 4 + x]);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) mx[x] = fmaxf(mx[x], s[C::kCols - 4 + x]);
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                S.row_max[t & 1][wg][r_cta] = top;
+                pair_sync(quad);   // the other part's maximum
+                top = fmaxf(top, S.row_max[t & 1][wg ^ 1][r_cta]);
                 const bool grow = top > m + 8.0f || (m == -INFINITY && top > m);
                 const float mn = grow ? top : m;
                 const float base = mn == -INFINITY ? 0.f : mn;
-                const bool scale_o = j > 0 && __any_sync(0xffffffffu, grow);
+                const bool scale_o = t > 0 && __any_sync(0xffffffffu, grow);
                 const float c = grow ? ex2f(m - base) : 1.0f;
                 l *= c;
                 m = mn;
                 if (scale_o) {
-                    // P V of tile j - 1 is the last that added to O; that of tile j - 2 is complete, since S of
-                    // tile j, issued after it, is
-                    wait_bar(&S.o_done, (j - 1) & 1, &S.stop);
+                    // P V of step t - 1 is the last that added to O; that of step t - 2 is complete, since S of
+                    // step t, issued after it, is
+                    wait_bar(&S.o_done, (t - 1) & 1, &S.stop);
                     tc_fence_after();
 #pragma unroll 1
                     for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
@@ -730,28 +726,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
                 const uint64_t neg = pack_f32x2(-base, -base);
                 uint64_t sum[2] = {0, 0};
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {   // 32 columns at a time into the MMAs' hands
-                    constexpr int kHeld = C::kCtas == 1 ? 32 : 0;
-                    const int h = C::order(x);
-                    if (C::kCtas == 2 && x == 1) {
-                        tc_ld32(st, reinterpret_cast<uint32_t *>(s));
-                        tc_wait_ld();
-                        mask32(0, s);
-                    }
+                for (int x = 0; x < C::kCols / 32; ++x) {   // 32 columns at a time into the MMAs' hands
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         float e0, e1;
-                        unpack_f32x2(add_f32x2(pack_f32x2(s[kHeld * x + 2 * i], s[kHeld * x + 2 * i + 1]), neg), e0, e1);
+                        unpack_f32x2(add_f32x2(pack_f32x2(s[32 * x + 2 * i], s[32 * x + 2 * i + 1]), neg), e0, e1);
                         e0 = ex2f(e0), e1 = ex2f(e1);
                         sum[i & 1] = add_f32x2(sum[i & 1], pack_f32x2(e0, e1));
                         p[i] = pack2_bf16(e0, e1);
                     }
-                    tc_st16(st + 32 * h, p);
+                    tc_st16(st + 32 * x, p);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) signal_cluster(p_bar + j % C::kBufs * 16 + x * 8);
+                    if (lane == 0) signal_cluster(p_bar + (t & 1) * 16 + x * 8);
                 }
                 float s0, s1;
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
@@ -759,7 +748,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             }
             wait_bar(&S.done, 0, &S.stop);
             tc_fence_after();
-            float(*sums)[kRows] = S.row_max[n_tiles & 1];   // the parity that the last tile left alone
+            float(*sums)[kRows] = S.row_max[n_tiles * C::kHalves & 1];   // the parity that the last step left alone
             sums[wg][r_cta] = l;
             pair_sync(quad);
             l += sums[wg ^ 1][r_cta];
