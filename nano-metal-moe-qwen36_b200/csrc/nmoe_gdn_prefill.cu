@@ -1168,7 +1168,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             const float *eg = reinterpret_cast<const float *>(smem + L::kGate + (c & 1) * kGates);
             wait_bar(&S.kq_full[c & 1], (c >> 1) & 1, &S.stop);
             const float g = eg[t], keep = eg[kC - 1];
-            bound2 = keep * keep * before2 + in2;
+            bound2 = keep * before2 * keep + in2;   // in this order: keep^2 alone may be zero when the state is not
             if (!is_q) {
                 // R = V - e^G K S^T, scaled
                 const float k0 = -g * pow2(es) * pow2(-eu) * (1.f / kScaleK), s = pow2(-eu);

@@ -112,6 +112,33 @@ def test_slow_and_fast_decay_and_alike_keys():
     p.check(*p.run())
 
 
+def test_a_large_state_that_decays_with_nothing_new():
+    """A state of 1e6 that loses 23 decades a chunk while every value is zero.
+
+    Operands are held to an absolute error too. Scaled so that 2^12 <= B 2^-e < 2^13, B the bound
+    sqrt(128) max|S| on them, an element is off by half of fp16's least step, 2^-25 2^e; with e one
+    larger for R that is 2^-36 B at most. An output element before its norm is a sum over 64 tokens of
+    R's elements, each times a product of q, contractions and k: at most |q| = 128^-1/2. So it is
+    off by 64 * 128^-1/2 * 2^-36 * 128^1/2 max|S| = 2^-30 max|S|, and by less again through S itself:
+    2^-29 max|S|. The norm divides by the row's root mean square r and passes on at most twice
+    that; r follows from the 64-bit output y / (w silu(z)), whose mean square is r^2 / (r^2 + 1e-6)."""
+    p = Prompt([200], 1, 1, torch.float32, seed=16)
+    p.qkv[:, 256:] = 0
+    p.conv[:, :, 256:] = 0
+    p.delta *= 2e7
+    p.w["A_log"][:], p.w["dt_bias"][:] = 0.0, 0.0
+    p.alpha[:] = 0.24
+    out, conv, delta = p.run()
+    c64, d64 = p.conv.double().clone(), p.delta.double().clone()
+    ref = gdn(p.w, 1, 1, p.cu_host, p.qkv, p.z, p.alpha, p.beta, c64, d64)
+    gate = (p.w["norm_w"].double() * torch.nn.functional.silu(p.z.double())).abs()
+    m = (ref / gate).pow(2).mean(1, keepdim=True)
+    r = (1e-6 * m / (1 - m) + 1e-6).sqrt()
+    tol = TOL * float(ref.abs().max()) + 2 * 2.0 ** -29 * float(p.delta.abs().max()) / r * gate
+    assert bool(((out.double() - ref).abs() <= tol).all())
+    assert float((delta.double() - d64).abs().max()) <= 1e-20
+
+
 def test_zero_keys():
     p = Prompt([80], 1, 1, torch.float32, seed=8, fresh=True)
     p.qkv[20:50] = 0
