@@ -76,6 +76,12 @@ def test_lengths(rows):
     p.check(*p.run())
 
 
+@pytest.mark.parametrize("count", [32, 33, 300])
+def test_many_sequences(count):
+    p = Prompt([(11 * i * i + 5 * i) % 7 if i % 9 else 60 + i % 70 for i in range(count)], 1, 2, torch.bfloat16, seed=17, spare=1)
+    p.check(*p.run())
+
+
 def test_full_geometry_and_new_sequences():
     p = Prompt([100, 33], 16, 32, torch.bfloat16, seed=3, fresh=True)
     p.check(*p.run(torch.bfloat16, null_in=True))
