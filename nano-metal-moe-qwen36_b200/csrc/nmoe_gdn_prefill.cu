@@ -914,17 +914,6 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     uint8_t *smem = raw_smem + ((1024 - (smem_u32(raw_smem) & 1023)) & 1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int split = blockIdx.x, vh = blockIdx.y, kh = vh / (a.value_heads / a.key_heads);
-    // The longest sequences first, as far as a lane a sequence goes: CTAs begin as SMs become free
-    int b = blockIdx.z;
-    if (a.num_seqs > 1 && a.num_seqs <= 32) {
-        const int n = lane < a.num_seqs ? seq_chunks(a, lane) : -1;
-        int rank = 0;
-        for (int i = 0; i < a.num_seqs; ++i) {
-            const int v = __shfl_sync(0xffffffffu, n, i);
-            rank += v > n || (v == n && i < lane);
-        }
-        b = __ffs(__ballot_sync(0xffffffffu, lane < a.num_seqs && rank == b)) - 1;
-    }
     const uint32_t sm = smem_u32(smem);
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) mbar_init(&S.kq_full[i], 1);
@@ -942,6 +931,19 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&S.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    // The sequence, and the chunks of those before it. The longest first, as far as a lane a sequence goes: CTAs
+    // begin as SMs become free
+    int b = blockIdx.z, first_chunk = 0;
+    if (a.num_seqs <= 32) {
+        const int n = lane < a.num_seqs ? seq_chunks(a, lane) : -1;
+        int rank = 0;
+        for (int i = 0; i < a.num_seqs; ++i) {
+            const int v = __shfl_sync(0xffffffffu, n, i);
+            rank += v > n || (v == n && i < lane);
+        }
+        b = __ffs(__ballot_sync(0xffffffffu, lane < a.num_seqs && rank == b)) - 1;
+        first_chunk = __reduce_add_sync(0xffffffffu, lane < b ? n : 0);
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -950,41 +952,21 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     // second part on for the state too. The inputs were there when the first part's chunks were begun.
     if (a.part > 0 || warp == 8) pdl_wait();
     if (warp == 8) pdl_trigger();
-    {
+    if (a.num_seqs > 32) {
         int before = 0;
         for (int i = tid; i < b; i += kScanThreads) before += seq_chunks(a, i);
         if (before) atomicAdd(&S.first_chunk, before);   // integers: the order does not matter
+        __syncthreads();
+        first_chunk = S.first_chunk;
     }
     const int all = seq_chunks(a, b), from = part_first(a, all, a.part);
     const int row0 = seq_first(a, b) + from * kC, rows = seq_rows(a, b) - from * kC;   // from this part's first on
     const int wg = warp >> 2, r = 32 * (warp & 3) + lane, c0 = 32 * wg;
     const bool is_q = warp < 8 && (warp & 3) >= 2;
 
-    // ---- the state: dim r, columns c0 .. c0 + 31
-    uint64_t St[16];
-    const float *before = a.part > 0 ? a.delta_out : a.delta_in;
-    const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN + c0) * kD + r;
-    if (warp < 8) {
-        float m = 0.f;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {   // a launch beside this one may have written them
-            const float x = before ? __ldcg(before + s_at + (long long)(2 * j) * kD) : 0.f;
-            const float y = before ? __ldcg(before + s_at + (long long)(2 * j + 1) * kD) : 0.f;
-            St[j] = pair(x, y);
-            m = fmaxf(m, fmaxf(fabsf(x), fabsf(y)));
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) atomicMax(&S.vmax[2], __float_as_int(m));   // not negative: ordered as integers
-    }
-    __syncthreads();
-    const long long chunk0 = (long long)S.first_chunk + from;
+    const long long chunk0 = (long long)first_chunk + from;
     const int here = part_first(a, all, a.part + 1) - from;
     const int chunks = chunk0 < 0 || chunk0 + here > a.room ? 0 : here;   // not beyond the workspace, whatever cu_rows holds
-    float bound2 = __int_as_float(S.vmax[2]);   // of |S|^2, per value row
-    bound2 = bound2 * bound2 * kD;
-    __syncthreads();
-    if (tid == 0) S.vmax[2] = 0;
 
     if (warp == 8) {
         // ---- copies and MMAs; every value is the same in all lanes
@@ -1114,6 +1096,27 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             asm volatile("bar.arrive 2, 256;" ::: "memory");
         }
     } else {
+        // ---- the state: dim r, columns c0 .. c0 + 31; and a bound of |S|^2, per value row
+        uint64_t St[16];
+        const float *before = a.part > 0 ? a.delta_out : a.delta_in;
+        const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN + c0) * kD + r;
+        float bound2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {   // a launch beside this one may have written them
+            const float x = before ? __ldcg(before + s_at + (long long)(2 * j) * kD) : 0.f;
+            const float y = before ? __ldcg(before + s_at + (long long)(2 * j + 1) * kD) : 0.f;
+            St[j] = pair(x, y);
+            bound2 = fmaxf(bound2, fmaxf(fabsf(x), fabsf(y)));
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) bound2 = fmaxf(bound2, __shfl_xor_sync(0xffffffffu, bound2, o));
+        if (lane == 0) atomicMax(&S.vmax[2], __float_as_int(bound2));   // not negative: ordered as integers
+        bar_sync(3, 256);
+        bound2 = __int_as_float(S.vmax[2]);
+        bound2 = bound2 * bound2 * kD;
+        bar_sync(3, 256);
+        if (tid == 0) S.vmax[2] = 0;   // V of chunk 2 adds to it after the product with R of chunk 1
+
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         // 16 columns (half hf of the thread's 32) of row `row` of an operand image, hi and lo `part` bytes apart
         auto store_half = [&](uint32_t image, int part, int row, int hf, const uint64_t *v) {
