@@ -334,6 +334,9 @@ struct ChunkSmem {
     static_assert(kT % 1024 == 0 && kTBytes % 1024 == 0 && kTBytes >= kTileZ, "images in T's place");
 };
 
+// A chunk of a key head: the products that meet tokens with tokens only. What bounds it: instructions, issued 40 % of
+// the time by the 16 warps that shared memory leaves room for (three CTAs an SM at 80 registers a thread spilled and
+// gained nothing); 832 CTAs 77 us. K stays in shared memory from the convolution to Z.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constant__ GdnArgs a) {
     extern __shared__ uint8_t raw_smem[];
@@ -904,7 +907,7 @@ __device__ __forceinline__ int exponent_of(float square) {
 }
 
 // Threads 0-255: row r = 32 (warp % 4) + lane of the 128, columns 32 (warp / 4) .. + 31 of the CTA's 64.
-// Rows 0-63 are tokens (K's rows: R and W), rows 64-127 are tokens too (Q's rows: the output), and all of
+// Rows 0-63 are tokens (K's rows: R), rows 64-127 are tokens too (Q's rows: the output), and all of
 // them are dims of the state. Warp 8 issues the MMAs, warps 9-12 convolve V a chunk ahead.
 template <bool kBf16>
 __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_constant__ GdnArgs a) {
@@ -1251,8 +1254,9 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
 
 // ---- finish -------------------------------------------------------------------------------------------
 
-// Gated RMS norm of every (row, value head), a warp each; then (the last blocks) the last three inputs
-// of every channel: after the other launches, so that the states may be updated in place.
+// Gated RMS norm of every value head, 8 rows a warp; then (the last blocks) the last three inputs of every
+// channel: after the other launches, so that the states may be updated in place. HBM bound: 4065 rows of 32 heads in
+// fp32, 200 MB, 43 us; more warps an SM had to spill and took 55.
 template <bool kBf16>
 __global__ void __launch_bounds__(kThreads) k_gdn_finish(const __grid_constant__ GdnArgs a, int norm_blocks) {
     const int tid = threadIdx.x, warp = tid >> 5;

@@ -14,7 +14,8 @@
 // positions of every tile with its own ring of copies (16 rows of K, 16 of V, by TMA) and its own
 // running maximum and sum; warps join through shared memory at the end of a pair, and pieces of
 // one pair join in a second launch. Beginning and ending a pair costs a piece about four tiles' time, and
-// counts as that much on the line.
+// counts as that much on the line. Measured: 64 sequences of 32768 (2 KV heads of 256, bf16) 655 us, 6.5 TB/s; 37
+// of up to 16384 (32 heads over 4 of 128, fp32) 64 us with the join, 54 of it here, 4.2 TB/s; one of 4096 12 us.
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -156,7 +157,7 @@ constexpr int kAppendThreads = 256, kAppendRows = 8;
 // A CTA takes rows_per_cta rows (1 when there are few, so that they spread over the SMs): one (cos, sin)
 // table per row for all its heads, then a warp per (row, head, k or v). HBM bound: the operands of a
 // warp's first units are asked for before the rows' sequences, positions and angles are found, which
-// takes three dependent reads.
+// takes three dependent reads. 32768 rows of 2 KV heads of 256: 35 us, 0.57 of the copy rate; 4095 rows 14 us.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_constant__ AppendArgs a) {
     constexpr int E = D / 32, kAtOnce = 4;
@@ -648,7 +649,8 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
 }
 
 // The pieces of one (pair, query head), or zeros for a sequence without positions. The plan is
-// recomputed while the step kernel runs (it reads only the lengths).
+// recomputed while the step kernel runs (it reads only the lengths). 512 threads, since one pair may have all 148
+// pieces and their reads are what it waits for.
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) k_step_join(const __grid_constant__ StepArgs a) {
     constexpr int kLanes = D / 4, kSets = kJoinThreads / kLanes;
