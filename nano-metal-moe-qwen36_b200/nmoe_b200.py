@@ -615,19 +615,26 @@ def _int32(t, n, name):
 
 
 def _rows(t, rows, width, dtype, name):
-    """Row stride in elements of a [rows][width] operand whose rows are contiguous."""
+    """Row stride in elements of a [rows][width] operand whose rows are contiguous and lie apart. Rows
+    that overlap, broadcast ones among them, are refused: the library takes a stride of 0 for packed rows."""
     if t.dtype not in _dtypes().get(dtype, ()):
         raise NmoeError(EINVAL, f"{name}: element type {t.dtype} does not match the dtype argument {dtype}")
     if t.dim() == 2:
         n, w = t.shape
         stride, inner = t.stride()
-        if n >= rows and w == width and (inner == 1 or width == 1):
-            return stride if n > 1 else width
+        fits = n >= rows and w == width and (inner == 1 or width == 1)
+    else:
+        fits = t.dim() > 2 and t.shape[0] >= rows > 0 and t[0].numel() == width and t[0].is_contiguous()
+        stride = t.stride(0) if t.dim() > 0 else 0
     if rows == 0:
         return width
-    if t.dim() < 2 or t.shape[0] < rows or t[0].numel() != width or not t[0].is_contiguous():
+    if not fits:
         raise NmoeError(EINVAL, f"{name} must hold at least {rows} rows of {width} contiguous elements")
-    return t.stride(0) if t.shape[0] > 1 else width
+    if rows == 1:   # one row is read: any stride
+        return width
+    if stride < width:
+        raise NmoeError(EINVAL, f"{name}: rows of {width} elements are {stride} apart; expanded or overlapping rows are not taken")
+    return stride
 
 
 def _output(t, n, dtype, name="out"):
