@@ -648,8 +648,8 @@ def _states(t, n, name):
 
 
 def _workspace(t, need):
-    if need and (t is None or t.numel() * t.element_size() < need):
-        raise NmoeError(EINVAL, f"workspace of at least {need} bytes needed")
+    if need and (t is None or not t.is_contiguous() or t.numel() * t.element_size() < need):
+        raise NmoeError(EINVAL, f"a contiguous workspace of at least {need} bytes is needed")
 
 
 class PagedKV:

@@ -107,3 +107,15 @@ def test_one_row_has_any_stride(on_host):
         assert N._rows(t, 1, 256, N.DTYPE_BF16, "x") == 256
     assert N._rows(wide[:, :256], 3, 256, N.DTYPE_BF16, "x") == 1024
     assert N._rows(wide[:, :256].unflatten(1, (2, 128)), 3, 256, N.DTYPE_BF16, "x") == 1024
+
+
+@pytest.mark.parametrize("name", ["prefill", "step", "linear"])
+def test_workspaces_with_holes_are_refused(on_host, name):
+    """A workspace counts as large as its elements only when they lie together."""
+    x = operands()[name]
+    n = x["workspace"].numel()
+    for t in (torch.zeros(1, dtype=torch.uint8).expand(n), torch.zeros(8, dtype=torch.uint8)[::2].expand(n // 4, 4)):
+        x["workspace"] = t
+        with pytest.raises(N.NmoeError) as e:
+            call(name, x)
+        assert e.value.status == N.EINVAL
