@@ -668,11 +668,14 @@ class PagedKV:
             raise NmoeError(EINVAL, "block_table must be int32 [sequences][max_pages], the last stride 1")
         _on_device((k, v, block_table))
         self.k, self.v, self.block_table = k, v, block_table
+        self._device = _dtypes()["device"]()
         self._fits = (k.shape[2], k.shape[3], block_table.shape[0])
         self.host = PagedKVHost(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), k.shape[0],
                                 k.shape[1], block_table.data_ptr(), block_table.shape[1], block_table.stride(0))
 
     def _check(self, shape, seqs):
+        if self._device != _dtypes()["device"]():   # another one may be current by now
+            raise NmoeError(EINVAL, "the cache is not on the current CUDA device")
         heads, dim, rows = self._fits
         if heads != shape.kv_heads or dim != shape.head_dim:
             raise NmoeError(EINVAL, f"pages of {heads} KV heads of {dim} do not fit the shape")

@@ -119,3 +119,24 @@ def test_workspaces_with_holes_are_refused(on_host, name):
         with pytest.raises(N.NmoeError) as e:
             call(name, x)
         assert e.value.status == N.EINVAL
+
+
+class Elsewhere(torch.Tensor):
+    """A tensor that says it is on device 5."""
+
+    def get_device(self):
+        return 5
+
+
+@pytest.mark.parametrize("name", ["append", "prefill", "step"])
+def test_a_cache_of_another_device_is_refused(on_host, monkeypatch, name):
+    """The cache is checked at the call, not only where it was made: the current device may be another one by then."""
+    monkeypatch.setitem(N._dtypes(), "device", lambda: 5)
+    seqs = ROWS if name == "step" else 1
+    far = N.PagedKV(*(bf16(4, 16, 2, 128).as_subclass(Elsewhere) for _ in range(2)),
+                    torch.zeros(seqs, 2, dtype=torch.int32).as_subclass(Elsewhere))
+    monkeypatch.setitem(N._dtypes(), "device", lambda: -1)
+    monkeypatch.setitem(globals(), "cache", lambda n: far)
+    with pytest.raises(N.NmoeError) as e:
+        call(name, operands()[name])
+    assert e.value.status == N.EINVAL
