@@ -461,8 +461,8 @@ size_t nmoe_full_attn_step_paged_workspace_bytes(const nmoe_full_attn_shape *sha
  * out may be the same buffer; in may be NULL: zeros, a new sequence). A sequence without rows
  * gets its states unchanged. out [total_rows][value_heads * 128] in out_dtype; it overlaps no
  * input. Sums, states and norms are fp32, for values and states up to 1e14 in magnitude; what the
- * products read carries 22 bits (what is below 2^-10 of a head's largest value or state in a
- * chunk: to 2^-32 of that). Rows go
+ * products read carries 22 bits (what is below 2^-10 of the largest value or state that a head has
+ * in a chunk or the two before it: to 2^-32 of that). Rows go
  * in chunks of 64 from a sequence's first on: a NaN or infinity reaches the rows of its own chunk
  * and all behind them, and no other sequence. workspace: nmoe_linear_attn_prefill_workspace_bytes(), 16-byte aligned, not
  * shared by calls that overlap. Allocates nothing; capturable. */

@@ -24,7 +24,7 @@
 // their norm). fp16 has the range of 2^40 only: k, q, P and Z are scaled by constants (Z's columns, like
 // k, are no longer than one: what a token leaves in the state after contractions), the state and R by a power of two
 // that follows a bound on them (|u| <= max |v| + |S|, |S'|^2 <= e^{2 G_63} |S|^2 + sum v^2, row by row, since |k| <= 1
-// and b <= 1).
+// and b <= 1), from the largest element that the state had a chunk or two ago.
 //
 // The scan is a chain of two products a chunk, 128 rows high, on tcgen05: [K; Q] S^T (128 x 64 x 128) and Z R
 // (128 x 64 x 64); P T b R follows beside the work on the state. Between them eight warps read the sums from tensor
@@ -896,6 +896,7 @@ struct ScanShared {
     uint64_t kq_full[2], zp_full, d, zr, pr, r_ready, s_ready;   // d: [K; Q] S^T, zr: Z R, pr: P T b R
     int vmax[3], first_chunk, stop;
     uint32_t tmem;
+    __align__(16) float s_max[2][8];   // largest |S| of a row warp, of the state before a chunk, by the chunk's parity
 };
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((127 + e) << 23); }
@@ -1103,22 +1104,33 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         uint64_t St[16];
         const float *before = a.part > 0 ? a.delta_out : a.delta_in;
         const long long s_at = (((long long)b * a.value_heads + vh) * kD + split * kN + c0) * kD + r;
-        float bound2 = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {   // a launch beside this one may have written them
             const float x = before ? __ldcg(before + s_at + (long long)(2 * j) * kD) : 0.f;
             const float y = before ? __ldcg(before + s_at + (long long)(2 * j + 1) * kD) : 0.f;
             St[j] = pair(x, y);
-            bound2 = fmaxf(bound2, fmaxf(fabsf(x), fabsf(y)));
         }
+        // The largest |S| of the CTA before chunk c: every warp leaves its own, and reads all of them once it has met
+        // a product that all have signalled for since
+        auto leave_max = [&](int c) {
+            float m = 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) bound2 = fmaxf(bound2, __shfl_xor_sync(0xffffffffu, bound2, o));
-        if (lane == 0) atomicMax(&S.vmax[2], __float_as_int(bound2));   // not negative: ordered as integers
+            for (int j = 0; j < 16; ++j) {
+                float x, y;
+                unpair(St[j], x, y);
+                m = fmaxf(m, fmaxf(fabsf(x), fabsf(y)));
+            }
+            m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));   // not negative: ordered as integers
+            if (lane == 0) S.s_max[c & 1][warp] = m;
+        };
+        auto square_of = [&](int c) {   // of a value row's norm, at most
+            const float4 x = *reinterpret_cast<const float4 *>(S.s_max[c & 1]), y = *reinterpret_cast<const float4 *>(S.s_max[c & 1] + 4);
+            const float m = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
+            return m * m * kD;
+        };
+        leave_max(0);
         bar_sync(3, 256);
-        bound2 = __int_as_float(S.vmax[2]);
-        bound2 = bound2 * bound2 * kD;
-        bar_sync(3, 256);
-        if (tid == 0) S.vmax[2] = 0;   // V of chunk 2 adds to it after the product with R of chunk 1
+        float bound2 = square_of(0);
 
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         // 16 columns (half hf of the thread's 32) of row `row` of an operand image, hi and lo `part` bytes apart
@@ -1168,13 +1180,11 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             bar_sync(is_q ? 2 : 1, 256);
             if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to for chunk c + 2
             const float vm = __int_as_float(S.vmax[c % 3]);
-            // of the states of this chunk; the one it leaves has decayed, so that what was large is forgotten
             const float before2 = bound2, in2 = kC * vm * vm;
             const int eu = exponent_of(before2 + in2) + 1;   // max |v| + |S| <= 9/8 of its root
             const float *eg = reinterpret_cast<const float *>(smem + L::kGate + (c & 1) * kGates);
             wait_bar(&S.kq_full[c & 1], (c >> 1) & 1, &S.stop);
             const float g = eg[t], keep = eg[kC - 1];
-            bound2 = keep * before2 * keep + in2;   // in this order: keep^2 alone may be zero when the state is not
             if (!is_q) {
                 // R = V - e^G K S^T, scaled
                 const float k0 = -g * pow2(es) * pow2(-eu) * (1.f / kScaleK), s = pow2(-eu);
@@ -1195,7 +1205,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             }
             signal(&S.r_ready);   // the rows of Q: P T b R of the chunk before is read
             const float k0 = g * pow2(es) * pow2(-eu);
-            es = exponent_of(bound2);
+            es = exponent_of(keep * before2 * keep + in2);   // in this order: keep^2 alone may be zero when the state is not
             wait_bar(&S.zr, c & 1, &S.stop);
             tc_fence_after();
             const float add = pow2(eu) * (1.f / kScaleK);
@@ -1206,7 +1216,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
 #pragma unroll
                 for (int j = 0; j < 8; ++j) St[8 * hf + j] = fma2(St[8 * hf + j], pair(keep, keep), mul2(x[j], pair(add, add)));
             }
-            if (c + 1 < chunks) store_state(es);
+            if (c + 1 < chunks) {
+                store_state(es);
+                leave_max(c + 1);
+                // The next chunk's bound goes by the state before this one, known by now (on the way to the state's
+                // scale it would have cost 1.4 % of 16384 rows): by its decay alone it would keep what the rule
+                // itself has erased, and the small parts of what is left would be lost
+                bound2 = keep * fminf(before2, square_of(c)) * keep + in2;
+            }
             if (is_q) {
                 // the output before its norm, e^G Q S^T + P U, while the next chunk's first product runs
                 wait_bar(&S.pr, c & 1, &S.stop);

@@ -1,0 +1,41 @@
+"""nmoe_linear_attn_prefill where magnitudes change on the way, against the 64-bit statement; the
+tolerances are those of test_linear_attn_prefill_gpu."""
+import pytest
+import torch
+
+import nmoe_b200 as N  # noqa: F401  (the extension has to be there)
+from operators_ref import gdn
+from test_linear_attn_prefill_gpu import TOL, Prompt
+
+pytestmark = pytest.mark.gpu
+
+
+def statement(p):
+    conv, delta = p.conv.double().clone(), p.delta.double().clone()
+    return gdn(p.w, p.hk, p.hv, p.cu_host, p.qkv, p.z, p.alpha, p.beta, conv, delta), conv, delta
+
+
+@pytest.mark.parametrize("dims,rows", [(8, 640), (128, 1500)])
+@pytest.mark.parametrize("size", [1.0, 1e5, 1e7])
+def test_a_large_start_that_the_rule_erases(dims, rows, size):
+    """16 large values, then ordinary ones, without decay: keys along the first `dims` axes in turn and
+    a step of 0.999, so that a visit to a key leaves a thousandth of what its column of the state held.
+
+    What a visit rounds, 2^-24 of the column or 2^-32 of the largest value of a chunk and of the two
+    before it, is erased by the next visits too. A large column is visited 8 times or more before the rows that
+    are compared: 1e7 * 1e-3^8 is nothing. So their error is that of ordinary values, whatever the start was."""
+    p = Prompt([rows], 1, 1, torch.float32, seed=21, fresh=True)
+    p.w["conv_w"].zero_()
+    p.w["conv_w"][:, 3] = 1.0
+    p.w["A_log"].zero_(), p.w["dt_bias"].zero_()
+    p.qkv[:, 128:256] = 0
+    t = torch.arange(rows, device="cuda")
+    p.qkv[t, 128 + t % dims] = 10.0
+    p.qkv[:16, 256:] = p.qkv[:16, 256:].abs() * size
+    p.alpha[:], p.beta[:] = -12.0, 7.0
+    out, conv, delta = p.run()
+    ref, c64, d64 = statement(p)
+    assert torch.equal(conv.double(), c64)
+    assert float((delta.double() - d64).abs().max()) <= TOL * float(d64.abs().max())
+    late = slice(rows * 3 // 4, rows)
+    assert float((out.double() - ref)[late].abs().max()) <= TOL * float(ref[late].abs().max())
