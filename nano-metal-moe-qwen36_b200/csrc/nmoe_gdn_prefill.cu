@@ -464,7 +464,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
                 al = bf16_to_f32(al_raw[j]), be = bf16_to_f32(be_raw[j]);
             else
                 al = al_raw[j], be = be_raw[j];
-            g[j] = t < n ? rate * softplus(al + dt) : 0.f;
+            const float lg = t < n ? rate * softplus(al + dt) : 0.f;
+            // e^-1000 is zero too, and sums of it keep the decays beside it: with 1e12 or an infinity, the differences
+            // between the tokens behind would be lost, or NaN
+            g[j] = lg < -1000.f ? -1000.f : lg;
             bt[j] = t < n ? sigmoidf_(be) : 0.f;
         }
         double inc = g[0] + g[1];

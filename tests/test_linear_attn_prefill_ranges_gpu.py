@@ -39,3 +39,15 @@ def test_a_large_start_that_the_rule_erases(dims, rows, size):
     assert float((delta.double() - d64).abs().max()) <= TOL * float(d64.abs().max())
     late = slice(rows * 3 // 4, rows)
     assert float((out.double() - ref)[late].abs().max()) <= TOL * float(ref[late].abs().max())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_decays_that_forget_everything(dtype):
+    """A gate so large, up to infinity, that nothing of the state is left: what follows in the same chunk goes on
+    from there, with the small decays between its own tokens. And gates of -inf: no decay at all."""
+    p = Prompt([150, 40], 1, 2, dtype, seed=22)
+    for row, size in ((5, 1e4), (20, 1e12), (37, 1e30), (64, 3e38), (80, float("inf")), (81, float("inf")), (127, 1e9), (160, 2e20)):
+        p.alpha[row] = size
+    p.alpha[100, 1] = float("inf")
+    p.alpha[30:34] = p.alpha[90] = float("-inf")
+    p.check(*p.run())
