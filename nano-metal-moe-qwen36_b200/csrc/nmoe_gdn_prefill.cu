@@ -82,6 +82,7 @@ struct GdnArgs {
     void *out;
     int num_seqs, total_rows, key_heads, value_heads, channels, x_bf16, out_bf16;
     int part, parts;   // of every sequence's chunks: those that a launch takes
+    uint32_t tries;    // of a wait of the scan, before it gives up
     int room;          // chunks that the workspace holds: as many as there are when cu_rows does not decrease
     // workspace, per chunk and head: K over Q, hi and lo; T b over P T b, hi and lo; gates; and O
     uint8_t *kq, *tp, *gates;
@@ -171,6 +172,12 @@ __device__ __forceinline__ uint32_t elect_lane() {
     uint32_t one;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
     return one;
+}
+// After a wait that ran out: what a barrier still counts, copies or products, lands before its memory goes. Of
+// either parity, as one of them is in flight; bounded too.
+__device__ __forceinline__ void settle(uint64_t *bar) {
+    for (int p = 0; p < 2; ++p)
+        for (int k = 0; k < 1000 && !mbar_try_wait_sleep(bar, p, 1000); ++k) {}
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 // x / (1 + e^-x) with the hardware's exponential and reciprocal: a few 2^-23 of it
@@ -305,7 +312,7 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t *r) {
 }
 // Polls (a suspended wait wakes some hundred cycles later, five times a chunk). Bounded: a barrier that
 // never completes sets `stop`, and every later wait goes at once.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t tries = kMaxSpins) {
     for (uint32_t n = 0;; ++n) {
         uint32_t ok;
         asm volatile(
@@ -315,7 +322,7 @@ __device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatil
             : "memory");
         if (ok) return true;
         if ((n & 1023) == 1023 && *stop) return false;
-        if (n >= kMaxSpins) {
+        if (n >= tries) {
             *stop = 1;
             return false;
         }
@@ -871,6 +878,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_gdn_chunks(const __grid_constan
     if (t128 == 0) bulk_wait_read();   // the shared memory stays until it is copied
     tc_fence_before();
     __syncthreads();
+    if (stop && warp == 0) {
+        settle(&products);
+        settle(&z_done[0]);
+        settle(&z_done[1]);
+    }
     tc_fence_after();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));
     if (last_cta) pdl_wait();
@@ -896,7 +908,7 @@ __device__ __forceinline__ uint32_t v_at(int t, int c) {
 }
 
 struct ScanShared {
-    uint64_t kq_full[2], zp_full, d, zr, pr, r_ready, s_ready;   // d: [K; Q] S^T, zr: Z R, pr: P T b R
+    uint64_t kq_full[2], zp_full, d, zr, pr, r_ready, s_ready, v_ready;   // d: [K; Q] S^T, zr: Z R, pr: P T b R
     int vmax[3], first_chunk, stop;
     uint32_t tmem;
     __align__(16) float s_max[2][8];   // largest |S| of a row warp, of the state before a chunk, by the chunk's parity
@@ -931,6 +943,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         mbar_init(&S.zp_full, 1);
         mbar_init(&S.r_ready, 8);
         mbar_init(&S.s_ready, 8);
+        mbar_init(&S.v_ready, 4);
         mbar_fence_init();
         S.first_chunk = S.stop = 0;
     }
@@ -975,6 +988,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
     const int here = part_first(a, all, a.part + 1) - from;
     const int chunks = chunk0 < 0 || chunk0 + here > a.room ? 0 : here;   // not beyond the workspace, whatever cu_rows holds
 
+    auto wait_for = [&](uint64_t *bar, uint32_t parity) { return wait_bar(bar, parity, &S.stop, a.tries); };
     if (warp == 8) {
         // ---- copies and MMAs; every value is the same in all lanes
         const uint32_t one = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -996,7 +1010,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         auto copy_p = [&](int c) {
             if (one) bulk_g2s(smem + L::kP, zp(c) + 2 * kTileZ, 2 * kTileP, &S.zp_full, keep);
         };
-        auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop)); };
+        auto wait = [&](uint64_t *bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_for(bar, parity)); };
         // The products of kSteps k-steps: A's hi with B's hi and lo, which lie side by side as 128 columns (one
         // reading of A for both: these are bound by shared memory), then A's lo with B's hi onto the first 64.
         // A's address of k-step k, part (0 hi, 1 lo); B's of k-step k.
@@ -1095,12 +1109,14 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             // over R of the chunk before, once the products have read it
-            if (c > 0) wait_bar(&S.pr, (c - 1) & 1, &S.stop);
+            if (c > 0) wait_for(&S.pr, (c - 1) & 1);
             if (lane == 0) atomicMax(&S.vmax[c % 3], __float_as_int(m));
 #pragma unroll
             for (int i = 0; i < 16; ++i) *reinterpret_cast<uint64_t *>(smem + L::kR + v_at(vt + i, vc)) = v[i];
-            asm volatile("bar.arrive 1, 256;" ::: "memory");   // before chunk c
-            asm volatile("bar.arrive 2, 256;" ::: "memory");
+            // a barrier whose waits are bounded: arrivals at a named one, once they no longer wait for the rows, would
+            // leave the rows waiting
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S.v_ready);
         }
     } else {
         // ---- the state: dim r, columns c0 .. c0 + 31; and a bound of |S|^2, per value row
@@ -1178,21 +1194,19 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
         if (chunks > 0) store_state(es);
         const int t = r & 63;   // this row's token
         for (int c = 0; c < chunks; ++c) {
-            // V of the chunk is stored. Q's rows, which only need its size, have a barrier of their own: they may
-            // still be busy with the output of the chunk before
-            bar_sync(is_q ? 2 : 1, 256);
+            wait_for(&S.v_ready, c & 1);   // V of the chunk is stored; Q's rows only need its size
             if (tid == 0) S.vmax[(c + 2) % 3] = 0;   // of chunk c - 1: read by all; next added to for chunk c + 2
             const float vm = __int_as_float(S.vmax[c % 3]);
             const float before2 = bound2, in2 = kC * vm * vm;
             const int eu = exponent_of(before2 + in2) + 1;   // max |v| + |S| <= 9/8 of its root
             const float *eg = reinterpret_cast<const float *>(smem + L::kGate + (c & 1) * kGates);
-            wait_bar(&S.kq_full[c & 1], (c >> 1) & 1, &S.stop);
+            wait_for(&S.kq_full[c & 1], (c >> 1) & 1);
             const float g = eg[t], keep = eg[kC - 1];
             if (!is_q) {
                 // R = V - e^G K S^T, scaled
                 const float k0 = -g * pow2(es) * pow2(-eu) * (1.f / kScaleK), s = pow2(-eu);
                 const uint64_t kk = pair(k0, k0), ss = pair(s, s);
-                wait_bar(&S.d, c & 1, &S.stop);
+                wait_for(&S.d, c & 1);
                 tc_fence_after();
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
@@ -1209,7 +1223,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             signal(&S.r_ready);   // the rows of Q: P T b R of the chunk before is read
             const float k0 = g * pow2(es) * pow2(-eu);
             es = exponent_of(keep * before2 * keep + in2);   // in this order: keep^2 alone may be zero when the state is not
-            wait_bar(&S.zr, c & 1, &S.stop);
+            wait_for(&S.zr, c & 1);
             tc_fence_after();
             const float add = pow2(eu) * (1.f / kScaleK);
 #pragma unroll
@@ -1229,7 +1243,7 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
             }
             if (is_q) {
                 // the output before its norm, e^G Q S^T + P U, while the next chunk's first product runs
-                wait_bar(&S.pr, c & 1, &S.stop);
+                wait_for(&S.pr, c & 1);
                 tc_fence_after();
                 const float s = pow2(eu) * (1.f / kScaleQ);
                 const uint64_t kk = pair(k0, k0), ss = pair(s, s);
@@ -1251,21 +1265,33 @@ __global__ void __launch_bounds__(kScanThreads, 1) k_gdn_scan(const __grid_const
                 }
             }
         }
-        const bool lost = S.stop;   // a copy or product that never came must not pass for an answer
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
             float x, y;
             unpair(St[j], x, y);
-            a.delta_out[s_at + (long long)(2 * j) * kD] = lost ? NAN : x;
-            a.delta_out[s_at + (long long)(2 * j + 1) * kD] = lost ? NAN : y;
+            a.delta_out[s_at + (long long)(2 * j) * kD] = x;
+            a.delta_out[s_at + (long long)(2 * j + 1) * kD] = y;
         }
         tc_fence_before();
     }
     __syncthreads();
-    if (S.stop && warp == 8) {   // copies in flight land before the shared memory goes (each wait bounded)
-        for (int i = 0; i < 3; ++i)
-            for (int p = 0; p < 2; ++p)
-                for (int k = 0; k < 1000 && !mbar_try_wait_sleep(i < 2 ? &S.kq_full[i] : &S.zp_full, p, 1000); ++k) {}
+    if (S.stop) {
+        // A copy or product that never came must not pass for an answer: this part's outputs, and the state that it
+        // leaves, and with it all behind
+        const int n = min(rows, chunks * kC);
+        for (int i = tid; i < n * (kN / 4); i += kScanThreads)
+            *reinterpret_cast<float4 *>(a.o + o_at(a, row0 + i / (kN / 4), vh, split * kN + 4 * (i % (kN / 4)))) =
+                make_float4(NAN, NAN, NAN, NAN);
+        for (int i = tid; i < kN * kD; i += kScanThreads)
+            a.delta_out[(((long long)b * a.value_heads + vh) * kD + split * kN) * kD + i] = NAN;
+        if (warp == 8) {
+            settle(&S.kq_full[0]);
+            settle(&S.kq_full[1]);
+            settle(&S.zp_full);
+            settle(&S.d);
+            settle(&S.zr);
+            settle(&S.pr);
+        }
     }
     __syncthreads();
     tc_fence_after();
@@ -1473,6 +1499,7 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
     a.channels = (int)ch;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     a.out_bf16 = out_dtype == NMOE_DTYPE_BF16;
+    a.tries = wait_tries();
     if (workspace == nullptr || !aligned_to(workspace, 16)) return fail(NMOE_EINVAL, "workspace is NULL or not aligned");
     if (max_chunks(num_seqs, total_rows) > 2147483647ll || total_rows > 2147483647 - kC || a.value_heads > 65535)
         return fail(NMOE_EINVAL, "too many rows or sequences");

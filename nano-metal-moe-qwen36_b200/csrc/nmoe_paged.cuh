@@ -11,6 +11,7 @@
 
 #include "nmoe/moe_cuda.h"
 #include "nmoe_common.cuh"
+#include "nmoe_sm100.cuh"
 
 namespace nmoe {
 
@@ -179,6 +180,9 @@ int check_x(const char *what, const void *p, int x_dtype, long long stride, long
 // on), and the logarithm of the warps that share a row.
 void rows_a_cta(int want, int *rows, int *share_log);
 int device_sm_count(int *sms);
+// Tries of a wait on the device before it gives up and its outputs become NaN: kMaxSpins, or what NMOE_WAIT_TRIES
+// says (for tests: 0 gives up at once).
+uint32_t wait_tries();
 using TensorMapEncode = PFN_cuTensorMapEncodeTiled_v12000;
 TensorMapEncode tensor_map_encode();
 // Pages as a 5D tensor (64 columns, page rows, panels of 64 columns, heads, pages); boxes of `rows`

@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include "nmoe_paged.cuh"
 #include "nmoe_sm100.cuh"
@@ -110,6 +111,11 @@ int device_sm_count(int *sms) {
         cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         return full_attn_fail(NMOE_ECUDA, "no CUDA device");
     return NMOE_OK;
+}
+
+uint32_t wait_tries() {
+    const char *t = getenv("NMOE_WAIT_TRIES");
+    return t != nullptr ? (uint32_t)strtoul(t, nullptr, 10) : kMaxSpins;
 }
 
 TensorMapEncode tensor_map_encode() {
