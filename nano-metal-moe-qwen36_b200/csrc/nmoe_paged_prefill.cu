@@ -56,6 +56,7 @@ struct PrefillArgs {
     float scale;   // softmax scale times log2(e)
     int num_seqs, total_rows, kv_heads, group, gated, x_bf16;
     int box_rows, box_shift;   // rows of a TMA box: 16, 32 or 64, or 0: no TMA
+    uint32_t tries, nap;       // of a wait before it gives up, and the ns that each may take
 };
 
 constexpr int kThreads = 352;   // warps 0-7 softmax, 8 copies Q and K, 9 MMA, 10 copies V
@@ -118,24 +119,24 @@ __device__ __forceinline__ void arrive_tx_cluster(uint32_t bar, uint32_t bytes) 
     asm volatile("mbarrier.arrive.expect_tx.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
 }
-// Bounded wait: a barrier that never completes sets `stop` and lets every later wait go at once.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop) {
-    for (uint32_t n = 0;; ++n) {
+// Bounded wait: a barrier that never completes sets `stop` in both CTAs of the pair, which depend on each other, and
+// lets every later wait of theirs go at once.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile int *stop, uint32_t tries, uint32_t nap) {
+    for (uint32_t n = 0; n < tries; ++n) {
         uint32_t ok;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(nap)
             : "memory");
         if (ok) return true;
         if (*stop) return false;
-        if (n >= (1u << 16)) {
-            *stop = 1;
-            return false;
-        }
     }
+    for (int r = 0; r < 2; ++r)
+        asm volatile("st.shared::cluster.u32 [%0], 1;" ::"r"(cluster_addr(const_cast<int *>(stop), r)) : "memory");
+    return false;
 }
 // A box of page rows: coordinates (column 0, row, panel of 64 columns, head, page).
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap *map, int panel, int row, int head, int page,
@@ -336,10 +337,12 @@ struct Copier {
         }
         __syncwarp();
     }
-    __device__ __forceinline__ uint32_t acquire(uint32_t n) const {   // the n-th stage filled
-        const uint32_t s = n % Cfg<D>::kStages;
-        wait_bar(&S->empty[s], ((n / Cfg<D>::kStages) & 1) ^ 1, &S->stop);
-        return s;
+    __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) const {
+        return __all_sync(0xffffffffu, wait_bar(bar, parity, &S->stop, a.tries, a.nap));
+    }
+    __device__ __forceinline__ bool acquire(uint32_t n, uint32_t *s) const {   // the n-th stage filled
+        *s = n % Cfg<D>::kStages;
+        return wait(&S->empty[*s], ((n / Cfg<D>::kStages) & 1) ^ 1);
     }
     // Positions p0 .. p0 + n - 1, columns c0 .. c0 + 64 panels - 1, by the warp's own loads and stores.
     __device__ __forceinline__ void by_hand(const uint16_t *src, uint8_t *dst, int p0, int n, int c0, int panels,
@@ -364,16 +367,18 @@ struct Copier {
         fence_async_smem();
         __syncwarp();
     }
-    // This CTA's 64 positions of the tile's K: panels of [64 rows][64 columns].
-    __device__ __forceinline__ void keys(int tile, uint32_t n) {
+    // This CTA's 64 positions of the tile's K: panels of [64 rows][64 columns]. False: a wait has run out, and nothing
+    // more may be copied.
+    __device__ __forceinline__ bool keys(int tile, uint32_t n) {
         mask(tile);
-        const uint32_t s = acquire(n);
+        uint32_t s;
+        if (!acquire(n, &s)) return false;
         uint8_t *dst = ring + s * Cfg<D>::kStageB;
         const uint32_t bar = cluster_addr(&S->full[s], 0);
         if (a.box_rows == 0) {
             by_hand(a.c.k, dst, tile * kTile + 64 * rank, 64, 0, D / 64, false);
             if (lane == 0) arrive_cluster(bar);
-            return;
+            return true;
         }
         const int per = 64 >> a.box_shift, first = rank * per;
         const uint32_t mine = (boxes >> first) & ((1u << per) - 1u);
@@ -387,17 +392,19 @@ struct Copier {
                 for (int p = 0; p < D / 64; ++p) tma_box(at + p * 8192, &a.k_map, p, row, kvh, page, bar);
             }
         }
+        return true;
     }
     // This CTA's half of the columns of all of the tile's V. One copy a box: [box][panel][rows][64].
-    __device__ __forceinline__ void values(int tile, uint32_t n) {
-        const uint32_t s = acquire(n);
+    __device__ __forceinline__ bool values(int tile, uint32_t n) {
+        uint32_t s;
+        if (!acquire(n, &s)) return false;
         uint8_t *dst = ring + s * Cfg<D>::kStageB;
         const uint32_t bar = cluster_addr(&S->full[s], 0);
         constexpr int kPanels = D / 128;
         if (a.box_rows == 0) {
             by_hand(a.c.v, dst, tile * kTile, kTile, rank * (D / 2), kPanels, true);
             if (lane == 0) arrive_cluster(bar);
-            return;
+            return true;
         }
         const bool clean = __popc(boxes) == kTile >> a.box_shift && (tile + 1) * kTile <= len;
         const uint32_t bytes = __popc(boxes) * a.box_rows * 128 * kPanels;
@@ -407,7 +414,7 @@ struct Copier {
         if (page >= 0)
             tma_box(smem_u32(dst) + lane * a.box_rows * 128 * kPanels, &a.v_map, rank * kPanels, row, kvh, page, to);
         if (!clean) {
-            wait_bar(&S->landed, landed & 1, &S->stop);
+            if (!wait(&S->landed, landed & 1)) return false;
             ++landed;
             // rows that are no positions: a box's rows [exist, box_rows), or all of them
             for (int i = 0; i < kTile >> a.box_shift; ++i) {
@@ -422,6 +429,7 @@ struct Copier {
             __syncwarp();
             if (lane == 0) arrive_cluster(bar);
         }
+        return true;
     }
     uint32_t landed = 0;
 };
@@ -563,7 +571,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             if (a.box_rows > 0) cp.look_ahead(0);
             for (int j = 0; j < n_tiles; ++j) {
                 cp.begin(j, j + 1 < n_tiles);
-                cp.keys(j, C::k_stage(j));
+                if (!cp.keys(j, C::k_stage(j))) break;
                 if (j == 0) {
                     asm volatile("griddepcontrol.wait;" ::: "memory");   // the prepared queries
                     if (lane == 0) {
@@ -582,7 +590,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
         if (a.box_rows > 0 && n_tiles > 0) cp.look_ahead(0);
         for (int j = 0; j < n_tiles; ++j) {
             cp.begin(j, j + 1 < n_tiles);
-            cp.values(j, C::v_stage(j, n_tiles));
+            if (!cp.values(j, C::v_stage(j, n_tiles))) break;
         }
     } else if (warp == 9) {
         if (rank == 0 && n_tiles > 0) {
@@ -596,7 +604,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             // V in shared memory: [box][panel][rows][64], one box when the warp copies
             const uint32_t v_rows = a.box_rows > 0 ? a.box_rows : kTile, v_shift = a.box_rows > 0 ? a.box_shift - 4 : 3;
             auto wait = [&](uint64_t *bar, uint32_t parity) {
-                return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop));
+                return __all_sync(0xffffffffu, wait_bar(bar, parity, &S.stop, a.tries, a.nap));
             };
             // the stages that the next K and V tile are read from, and the parity of their filling
             uint32_t k_at = 0, k_round = 0, v_at = C::v_stage(0, n), v_round = 0;
@@ -671,7 +679,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             const int seen = __reduce_min_sync(0xffffffffu, live ? pos + 1 : 0x7fffffff);
             for (int t = 0; t < n_tiles * C::kHalves; ++t) {
                 const int j = t / C::kHalves, x0 = t % C::kHalves;
-                wait_bar(&S.s_full[t & 1], t >> 1 & 1, &S.stop);
+                wait_bar(&S.s_full[t & 1], t >> 1 & 1, &S.stop, a.tries, a.nap);
                 tc_fence_after();
                 const uint32_t st = tmem + lanes + C::kS + (t & 1) * C::kStep + C::kCols * wg;
                 float s[C::kCols];
@@ -710,7 +718,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
                 if (scale_o) {
                     // P V of step t - 1 is the last that added to O; that of step t - 2 is complete, since S of
                     // step t, issued after it, is
-                    wait_bar(&S.o_done, (t - 1) & 1, &S.stop);
+                    wait_bar(&S.o_done, (t - 1) & 1, &S.stop, a.tries, a.nap);
                     tc_fence_after();
 #pragma unroll 1
                     for (int x = wg * (D / 2); x < (wg + 1) * (D / 2); x += 32) {
@@ -746,7 +754,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
                 unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
                 l += s0 + s1;
             }
-            wait_bar(&S.done, 0, &S.stop);
+            wait_bar(&S.done, 0, &S.stop, a.tries, a.nap);
             tc_fence_after();
             float(*sums)[kRows] = S.row_max[n_tiles * C::kHalves & 1];   // the parity that the last step left alone
             sums[wg][r_cta] = l;
@@ -755,7 +763,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
         }
         // ---- O / l through shared memory (the MMAs have read the queries and the ring for the last
         // time), so that a warp gates and stores a row of D at a time
-        const float inv = S.stop ? NAN : l == 0.f ? 0.f : 1.0f / l;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
         uint8_t *rows_out = q_smem + quad * 32 * C::kOutB;
         if (n_tiles > 0) {
             uint8_t *to = rows_out + lane * C::kOutB;
@@ -812,13 +820,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
             store_rows(std::true_type{});
         else
             store_rows(std::false_type{});
+        if (*static_cast<volatile int *>(&S.stop)) {   // a copy or product that never came must not pass for an answer
+            __syncwarp();
+            for (int i = first; i < mine; ++i) {
+                const int rr = quad * 32 + i, tok = rr / a.group, h = kvh * a.group + rr - tok * a.group;
+                for (int d = lane; d < D; d += 32) a.out[(((long long)lo + my_tok0 + tok) * heads + h) * D + d] = 0x7fc0;
+            }
+        }
         tc_fence_before();
     }
     __syncthreads();
-    if (S.stop && (warp == 8 || warp == 10)) {   // copies in flight land before the shared memory goes (each wait bounded)
-        int go_on = 0;
-        for (int s = 0; s < C::kStages; ++s)
-            for (int n = 0; n < 1000 && !mbar_try_wait_sleep(&S.full[s], go_on, 1000); ++n) {}
+    if (S.stop && warp == 8) {
+        // what is in flight lands before the shared and the tensor memory go: of either parity of each barrier, as
+        // one of them is in flight; bounded too
+        auto settle = [&](uint64_t *bar) {
+            for (int p = 0; p < 2; ++p)
+                for (int n = 0; n < 1000 && !mbar_try_wait_sleep(bar, p, 1000); ++n) {}
+        };
+        for (int s = 0; s < C::kStages; ++s) settle(&S.full[s]), settle(&S.empty[s]);
+        settle(&S.landed);
+        settle(&S.q_ready);
+        settle(&S.o_done);
     }
     cluster.sync();   // neither CTA leaves while the other may still signal it
     tc_fence_after();
@@ -904,6 +926,9 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.gated = shape->gated;
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     a.q_ready = static_cast<uint16_t *>(workspace);
+    const uint32_t tries = wait_tries();
+    a.tries = (tries + 63) / 64;   // of up to 20 us each
+    a.nap = tries < 20000 ? tries : 20000;
     int sms = 0;
     if ((rc = device_sm_count(&sms)) != NMOE_OK) return rc;
     rows_a_cta(total_rows / (4 * sms), &a.prep_rows, &a.share_log);

@@ -3,8 +3,9 @@ call ends, what it could not compute is NaN and never a number, and the next cal
 import pytest
 import torch
 
-from operators_ref import gdn
+from operators_ref import Packed, gdn
 from test_linear_attn_prefill_gpu import TOL, Prompt
+from test_paged_attn_gpu import H, append, check_prefill, prefill
 
 pytestmark = pytest.mark.gpu
 FEW = [1, 10, 40, 100, 300]   # tries that may or may not be enough
@@ -36,3 +37,23 @@ def test_linear_attn_prefill(monkeypatch, rows, tries):
         assert bool(lost.all()) and bool(gone[[b for b, r in enumerate(rows) if r]].all())
     assert torch.equal(d[[b for b, r in enumerate(rows) if not r]], p.delta[[b for b, r in enumerate(rows) if not r]])
     p.check(*p.run())
+
+
+@pytest.mark.parametrize("page", [16, 64, 7])
+@pytest.mark.parametrize("shape", [(16, 2, 256, 64), (6, 1, 128, 128)])
+@pytest.mark.parametrize("tries", [0] + FEW)
+def test_full_attn_prefill(monkeypatch, shape, page, tries):
+    p = Packed([130, 0, 70, 300], [0, 5, 200, 900], page, *shape, seed=32, spare_rows=3, tail=float("nan"))
+    append(p)
+    ref, mass, reach = p.attention()
+    monkeypatch.setenv("NMOE_WAIT_TRIES", str(tries))
+    out = prefill(p)
+    torch.cuda.synchronize()
+    monkeypatch.delenv("NMOE_WAIT_TRIES")
+    n = sum(p.rows)
+    tol = H * ref.abs() + (H + 2 * H * reach) * mass + 1e-30   # as in check_prefill
+    lost = all_or_nan(out.view(p.total, p.hq, p.d)[:n], ref[:n], tol[:n])
+    assert bool((out[n:] == 7.0).all())
+    if tries == 0:
+        assert bool(lost.all())
+    check_prefill(p, prefill(p))
