@@ -236,6 +236,7 @@ struct StepArgs {
     void *out;
     float scale;   // softmax scale times log2(e)
     int batch, kv_heads, group, gated, x_bf16, out_bf16, ctas, boxed;
+    uint32_t tries;   // of a wait, before it gives up
 };
 
 // Warps a CTA: what a scheduler needs to hide a step's chain of products behind another warp's, as far as
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
     const uint32_t sq = smem_u32(smem) + Cfg::kQ;
     uint32_t it = 0;   // stages this warp has filled
     uint32_t used = 0;
-    bool lost = false;
+    bool lost = false;   // a wait has run out: this warp copies and waits no more, and its sums are NaN
 
     while (true) {
         // tiles t0 .. t1 - 1 of this pair; none when the piece holds no more than the pair's cost
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
         if (steps > 0) {
         page_next = page_of(0);
         int issued = 0;
-        for (; issued < kStages && issued < steps; ++issued) issue(issued);
+        for (; issued < kStages && issued < steps && !lost; ++issued) issue(issued);
 
         // ---- the queries of the group, prepared, scaled and split into bf16 parts
         if (tid < a.rot.half) cs[tid] = rotary_cs(freq, len - 1);
@@ -493,10 +494,10 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
 #pragma unroll
         for (int n = 0; n < D / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
 
-        for (int i = 0; i < steps; ++i) {
+        for (int i = 0; i < steps && !lost; ++i) {
             const int s = used % kStages;
-            lost |= !mbar_wait_spin(&bars[warp][s], (used / kStages) & 1);
-            __syncwarp();
+            lost = !__all_sync(0xffffffffu, mbar_wait_spin(&bars[warp][s], (used / kStages) & 1, a.tries));
+            if (lost) break;
             const int base = (t0 + i) * kTile + 16 * warp;
             uint32_t lv = live[warp][s];
             const uint32_t ks = ring + s * Cfg::kStageB, vs = ks + Cfg::kHalfB;
@@ -652,6 +653,9 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
             if (nt == 0) break;
         }
     }
+    if (lost)   // copies in flight land before the shared memory goes: of either parity, as one is in flight; bounded too
+        for (int s = 0; s < 2 * kStages; ++s)
+            for (int n = 0; n < 1000 && !mbar_try_wait_sleep(&bars[warp][s >> 1], s & 1, 1000); ++n) {}
 }
 
 // The pieces of one (pair, query head), or zeros for a sequence without positions. The plan is
@@ -847,6 +851,7 @@ extern "C" int nmoe_full_attn_step_paged(const nmoe_full_attn_weights *w, const 
     a.part = static_cast<float *>(workspace);
     a.out = out;
     a.scale = (scale == 0.f ? 1.0f / sqrtf((float)shape->head_dim) : scale) * 1.4426950408889634f;
+    a.tries = wait_tries();
     a.batch = batch;
     a.kv_heads = shape->kv_heads;
     a.group = shape->q_heads / shape->kv_heads;

@@ -63,10 +63,10 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint64
     return true;
 }
 // A wait for the CTA's own copies, bounded by its number of tries.
-__device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity) {
-    for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n)
-        if (n >= kMaxSpins) return false;
-    return true;
+__device__ __forceinline__ bool mbar_wait_spin(uint64_t *bar, uint32_t parity, uint32_t tries) {
+    for (uint32_t n = 0; n < tries; ++n)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
 }
 // Sleeping wait for the grouped GEMM's role warps: each try suspends up to 20 us.
 __device__ __forceinline__ bool mbar_wait_sleep(uint64_t *bar, uint32_t parity, uint64_t deadline) {

@@ -5,7 +5,7 @@ import torch
 
 from operators_ref import Packed, gdn
 from test_linear_attn_prefill_gpu import TOL, Prompt
-from test_paged_attn_gpu import H, append, check_prefill, prefill
+from test_paged_attn_gpu import H, append, check_prefill, check_step, prefill, step
 
 pytestmark = pytest.mark.gpu
 FEW = [1, 10, 40, 100, 300]   # tries that may or may not be enough
@@ -57,3 +57,20 @@ def test_full_attn_prefill(monkeypatch, shape, page, tries):
     if tries == 0:
         assert bool(lost.all())
     check_prefill(p, prefill(p))
+
+
+@pytest.mark.parametrize("page", [16, 7])
+@pytest.mark.parametrize("shape", [(16, 2, 256, 64), (6, 1, 128, 128)])
+@pytest.mark.parametrize("tries", [0] + FEW)
+def test_full_attn_step(monkeypatch, shape, page, tries):
+    p = Packed([1] * 6, [0, 63, 5000, 64, 17, 1200], page, *shape, torch.float32, seed=33, tail=float("nan"))
+    monkeypatch.setenv("NMOE_WAIT_TRIES", str(tries))
+    out = step(p, torch.float32)
+    torch.cuda.synchronize()
+    monkeypatch.delenv("NMOE_WAIT_TRIES")
+    again = step(p, torch.float32)   # appends what the first call may not have come to
+    check_step(p, again)
+    ref, mass, _ = p.attention()
+    lost = all_or_nan(out.view(6, p.hq, p.d), ref, 2e-5 * mass.amax(-1, keepdim=True) + 1e-30)   # as in check_step
+    if tries == 0:
+        assert bool(lost.all())
