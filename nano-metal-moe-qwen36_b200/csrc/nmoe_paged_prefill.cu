@@ -528,7 +528,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
     }
     __syncthreads();
     const int b = S.unit_seq;
-    if (b < 0) return;   // both CTAs of the pair: there are fewer units than the grid has room for
+    if (b < 0) {   // both CTAs of the pair: there are fewer units than the grid has room for
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+    }
     const int lo = max(0, a.cu_rows[b]), rows_b = min(a.total_rows, a.cu_rows[b + 1]) - lo;
     const int tok0 = S.unit_off * per_unit;          // first token of the pair in the sequence
     const long long len64 = a.kv_lens[b];
@@ -585,6 +588,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, Cfg<D>::kC
                 }
             }
         }
+        // Every CTA waits, those that need no queries too, so that this launch never ends before the one that
+        // prepares them: a call behind this one may use the workspace
+        asm volatile("griddepcontrol.wait;" ::: "memory");
     } else if (warp == 10) {
         Copier<D> cp{a, &S, ring, b, kvh, rank, lane, len};
         if (a.box_rows > 0 && n_tiles > 0) cp.look_ahead(0);
