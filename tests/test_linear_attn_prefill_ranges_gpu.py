@@ -51,3 +51,64 @@ def test_decays_that_forget_everything(dtype):
     p.alpha[100, 1] = float("inf")
     p.alpha[30:34] = p.alpha[90] = float("-inf")
     p.check(*p.run())
+
+
+@pytest.mark.parametrize("heads,rows,dtype,out_dtype", [
+    ((16, 32), [6000], torch.bfloat16, torch.bfloat16), ((4, 4), [5000, 6100], torch.float32, torch.bfloat16),
+    ((2, 6), [5900, 3], torch.bfloat16, torch.float32)])
+def test_parts_of_several_key_heads(heads, rows, dtype, out_dtype):
+    """Three parts or more of a prompt: the norm of an earlier part runs in rows of the grid between those of the key
+    heads, whatever their number."""
+    p = Prompt(rows, *heads, dtype, seed=23, spare=2)
+    p.check(*p.run(out_dtype))
+
+
+@pytest.mark.parametrize("heads", [(1, 3), (2, 6), (1, 5)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_odd_numbers_of_value_heads_a_key_head(heads, dtype):
+    p = Prompt([1, 70, 0, 130, 64], *heads, dtype, seed=24, spare=1)
+    p.check(*p.run())
+
+
+@pytest.mark.parametrize("scale", [1e9, 1e13])
+def test_large_values(scale):
+    p = Prompt([150, 0, 70], 1, 2, torch.float32, seed=25, scale=scale)
+    p.conv *= scale
+    p.check(*p.run())
+
+
+@pytest.mark.parametrize("rows", [[100, 130, 70], [100] * 20 + [130] + [50] * 20, [9000, 9100, 9003]])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_what_is_not_finite_stays_in_its_sequence(rows, bad):
+    """Every operand of one row set to NaN or an infinity, each in a sequence of its own kind: the other sequences give
+    the same bits, and so do the chunks before it."""
+    at = rows.index(max(rows)) if len(rows) > 3 else 1
+    for which in ("qkv", "z", "alpha", "beta", "state"):
+        p = Prompt(rows, 1, 2, torch.float32, seed=26)
+        clean = p.run()
+        first = p.cu_host[at] + 70
+        if which == "state":
+            p.delta[at, 1, 3, 5] = bad
+            p.conv[at, 1, 7] = bad
+            first = p.cu_host[at]
+        else:
+            getattr(p, which)[first] = bad
+            if which == "qkv":
+                p.qkv[first, 1:] = 1.0   # one channel of a query
+        out, conv, delta = p.run()
+        end = p.cu_host[at + 1]
+        before = p.cu_host[at] + (first - p.cu_host[at]) // 64 * 64
+        assert torch.equal(out[:before], clean[0][:before]) and torch.equal(out[end:], clean[0][end:]), which
+        others = [b for b in range(len(rows)) if b != at]
+        assert torch.equal(conv[others], clean[1][others]) and torch.equal(delta[others], clean[2][others]), which
+
+
+def test_rows_in_front_of_the_first_sequence():
+    """cu_rows need not begin at zero: what lies in front belongs to no sequence."""
+    p = Prompt([11, 70, 5], 1, 2, torch.float32, seed=27, spare=2)
+    p.cu_host = [c + 7 for c in [0, 60, 60, 79]]
+    p.cu = torch.tensor(p.cu_host, dtype=torch.int32, device="cuda")
+    out, conv, delta = p.run()
+    assert bool((out[:7] == 7.0).all())
+    out[:7] = 0   # the statement's value for rows that it does not compute
+    p.check(out, conv, delta)

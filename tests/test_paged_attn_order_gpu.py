@@ -5,7 +5,7 @@ import torch
 
 import nmoe_b200 as N
 from operators_ref import Packed
-from test_paged_attn_gpu import append, check_prefill, prefill, shape_of
+from test_paged_attn_gpu import append, check_pages, check_prefill, prefill, shape_of
 
 pytestmark = pytest.mark.gpu
 
@@ -33,3 +33,21 @@ def test_prefill_behind_one_in_which_no_row_sees_anything(rows, cu):
     for out in outs:
         assert torch.equal(out, outs[0])
     check_prefill(p, outs[0])
+
+
+@pytest.mark.parametrize("heads", [(16, 2, 256, 64), (6, 1, 128, 128)])
+def test_rows_in_front_of_the_first_sequence(heads):
+    """cu_rows need not begin at zero: what lies in front belongs to no sequence."""
+    p = Packed([130, 0, 45], [20, 3, 0], 16, *heads, seed=73, tail=float("nan"))
+    before, want = (p.k.clone(), p.v.clone()), p.append()
+    q, out = p.q.clone(), torch.full((p.total + 9, p.hq * p.d), 7.0, dtype=torch.bfloat16, device="cuda")
+    front = lambda t: torch.cat([torch.full((9, t.shape[1]), float("nan"), dtype=t.dtype, device="cuda"), t])  # noqa: E731
+    p.q, p.k_new, p.v_new = front(p.q), front(p.k_new), front(p.v_new)
+    p.cu += 9
+    p.total += 9
+    append(p)
+    check_pages(p, want, before)
+    prefill(p, out=out)
+    assert bool((out[:9] == 7.0).all())
+    p.q, p.cu, p.total = q, p.cu - 9, p.total - 9
+    check_prefill(p, out[9:])
