@@ -459,7 +459,7 @@ size_t nmoe_full_attn_step_paged_workspace_bytes(const nmoe_full_attn_shape *sha
  * elements (0: packed; qkv and z rows 16-byte aligned). conv_in / conv_out f32
  * [num_seqs][3][channels], delta_in / delta_out f32 [num_seqs][value_heads][128][128] (in and
  * out may be the same buffer; in may be NULL: zeros, a new sequence). A sequence without rows
- * gets its states unchanged. out [total_rows][value_heads * 128] in out_dtype; it overlaps no
+ * gets its states unchanged (num_seqs: at most 65535). out [total_rows][value_heads * 128] in out_dtype; it overlaps no
  * input. Sums, states and norms are fp32, for values and states up to 1e14 in magnitude; what the
  * products read carries 22 bits (what is below 2^-10 of the largest value or state that a head has
  * in a chunk or the two before it: to 2^-32 of that). Rows go

@@ -5,7 +5,8 @@
 // Inside a chunk (G_t: the sum of log g up to t, S the state before it) the rank-one updates are
 //     u_t = b_t (v_t - e^{G_t} S k_t - sum_{s<t} e^{G_t-G_s} (k_t . k_s) u_s)
 // a unit lower triangular system: U = T b (V - e^G K S^T), T = (I + M)^{-1},
-// M_ts = b_t e^{G_t-G_s} k_t . k_s (s < t). Then, with P_ts = e^{G_t-G_s} q_t . k_s (s <= t),
+// M_ts = b_t e^{G_t-G_s} k_t . k_s (s < t): the WY form of a product of rank-one updates (Bischof and Van Loan 1987),
+// for the delta rule in chunks as in Yang et al. 2024. Then, with P_ts = e^{G_t-G_s} q_t . k_s (s <= t),
 //     O = e^G Q S^T + P U,   S' = e^{G_63} S + sum_t (e^{G_63-G_t} u_t) k_t^T
 //
 // With R = V - e^G K S^T, U = T b R, so P U = (P T b) R and, with Z = K^T (e^{G_63 - G} T b),
@@ -29,9 +30,10 @@
 // The scan is a chain of two products a chunk, 128 rows high, on tcgen05: [K; Q] S^T (128 x 64 x 128) and Z R
 // (128 x 64 x 64); P T b R follows beside the work on the state. Between them eight warps read the sums from tensor
 // memory, a thread per row and 32 columns, and write the next operand as rows of 128 bytes, which the MMA takes as
-// they are (MN-major). What bounds it: the chain's latency, 4500 cycles a chunk, of which the products, bound by
-// shared memory's bandwidth, take 1800. Measured, 16 key and 32 value heads, bf16: 16384 rows 842 us (preparation,
-// scan and norm one after the other: 1052), of which 75 us are the first part's preparation.
+// they are (MN-major). What bounds it: the chain's latency, 4600 cycles a chunk, of which the products, bound by
+// shared memory's bandwidth, take 1800; and the preparation, which needs more of the machine than the scan (57 ms of an
+// SM against 38 at 16384 rows). Measured, 16 key and 32 value heads, bf16: 16384 rows 857 us (preparation, scan and
+// norm one after the other: 1061), of which 78 us are the first part's preparation.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdarg.h>
@@ -84,7 +86,7 @@ struct GdnArgs {
     int part, parts;   // of every sequence's chunks: those that a launch takes
     uint32_t tries;    // of a wait of the scan, before it gives up
     int room;          // chunks that the workspace holds: as many as there are when cu_rows does not decrease
-    // workspace, per chunk and head: K over Q, hi and lo; T b over P T b, hi and lo; gates; and O
+    // workspace, per chunk and head: K over Q, hi and lo; Z, hi and lo, and P T b, hi and lo; gates; and O
     uint8_t *kq, *tp, *gates;
     float *o;
 };
@@ -1345,7 +1347,9 @@ long long max_chunks(int num_seqs, int total_rows) { return (long long)total_row
 // Into how many parts the chunks go. With one, every launch has the machine to itself in turn. A scan that leaves
 // more than half of the SMs idle runs beside the launch that prepares the next part, on those SMs; a part more
 // costs about 10 us, and what hides is 1 us a chunk of every part but one: best near sqrt(chunks / 10).
-// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1052 us, 3 895, 4 875, 5 859, 6 876, 8 893, 16 992.
+// 16384 rows, 16 key and 32 value heads (64 scan CTAs): 1 part 1061 us, 3 892, 4 866, 5 849, 6 862, 8 883, 16 979;
+// 4 and 8 heads: 1 part 781 us, 3 720, 5 721, 8 717, 16 749; 1 and 2 heads, with little to hide: 1 part 667 us, 3 670,
+// 5 674, 8 690, so the rule costs 1 % there.
 // The scan's CTAs come in clusters of two for their place only: those take the two SMs of a TPC. Beside an SM
 // that runs the other kernel a CTA of the scan took 20 % longer (1118 us in all, for 992 us in pairs).
 int parts_of(const GdnArgs &a, int sms) {
@@ -1501,7 +1505,7 @@ extern "C" int nmoe_linear_attn_prefill(const nmoe_linear_attn_weights *w, const
     a.out_bf16 = out_dtype == NMOE_DTYPE_BF16;
     a.tries = wait_tries();
     if (workspace == nullptr || !aligned_to(workspace, 16)) return fail(NMOE_EINVAL, "workspace is NULL or not aligned");
-    if (max_chunks(num_seqs, total_rows) > 2147483647ll || total_rows > 2147483647 - kC || a.value_heads > 65535)
+    if (max_chunks(num_seqs, total_rows) > 2147483647ll || total_rows > 2147483647 - kC)
         return fail(NMOE_EINVAL, "too many rows or sequences");
     carve(*shape, num_seqs, total_rows, static_cast<uint8_t *>(workspace), &a);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

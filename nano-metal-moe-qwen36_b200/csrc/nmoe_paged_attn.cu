@@ -14,8 +14,10 @@
 // positions of every tile with its own ring of copies (16 rows of K, 16 of V, by TMA) and its own
 // running maximum and sum; warps join through shared memory at the end of a pair, and pieces of
 // one pair join in a second launch. Beginning and ending a pair costs a piece about four tiles' time, and
-// counts as that much on the line. Measured: 64 sequences of 32768 (2 KV heads of 256, bf16) 655 us, 6.5 TB/s; 37
-// of up to 16384 (32 heads over 4 of 128, fp32) 64 us with the join, 54 of it here, 4.2 TB/s; one of 4096 12 us.
+// counts as that much on the line. Measured: 64 sequences of 32768 (2 KV heads of 256, bf16) 655 us, 6.5 TB/s; 64 of
+// 8192 187 us, with an fp32 output, three parts, 232 us; 37 of up to 16384 (32 heads over 4 of 128, fp32) 64 us with
+// the join, 55 of it here, 4.2 TB/s; one of 4096 14 us with the join. Pages that are no multiple of 16 rows are copied row
+// by row, each waited for: 64 of 8192 2.2 ms.
 #include <cuda_runtime.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -161,9 +163,10 @@ struct AppendArgs {
 constexpr int kAppendThreads = 256, kAppendRows = 8;
 
 // A CTA takes rows_per_cta rows (1 when there are few, so that they spread over the SMs): one (cos, sin)
-// table per row for all its heads, then a warp per (row, head, k or v). HBM bound: the operands of a
-// warp's first units are asked for before the rows' sequences, positions and angles are found, which
-// takes three dependent reads. 32768 rows of 2 KV heads of 256: 35 us, 0.57 of the copy rate; 4095 rows 14 us.
+// table per row for all its heads, then a warp per (row, head, k or v). The operands of a warp's first units are
+// asked for before the rows' sequences, positions and angles are found, which takes three dependent reads and two
+// barriers: these, in CTAs that live for 8 rows, are what bounds it (the barrier is the first stall, DRAM moves at 0.39
+// of the copy rate). 32768 rows of 2 KV heads of 256: 35 us, 20.6 at the copy rate; 4095 rows 14 us.
 template <int D, bool kBf16>
 __global__ void __launch_bounds__(kAppendThreads) k_append_paged(const __grid_constant__ AppendArgs a) {
     constexpr int E = D / 32, kAtOnce = 4;
@@ -602,7 +605,7 @@ __global__ void __launch_bounds__(StepCfg<D>::kThreads, 1) k_step_paged(const __
         l += __shfl_xor_sync(0xffffffffu, l, 2);
         if (lost) l = NAN;   // a copy that never landed must not pass for an answer
 
-        // ---- join the four warps through the (drained) ring
+        // ---- join the warps through the (drained) ring
         __syncthreads();
         float *so = reinterpret_cast<float *>(smem) + (warp * kGroupMax + (lane >> 2)) * D + 2 * (lane & 3);
 #pragma unroll

@@ -14,14 +14,15 @@
 // from shared memory to keep the tensor cores busy, the pair 31 and 95.
 //
 // Softmax: two threads per query row (warps 0-7, 64 columns each) read its 128 scores from tensor
-// memory, keep the running maximum and sum in fp32, and write P back as bf16 over the scores. Queries and P are
+// memory, keep the running maximum and sum (Milakov and Gimelshein 2018) in fp32, and write P back as bf16 over the scores. Queries and P are
 // rounded to bf16, the type of the pages, since an MMA's operands have one type: the output is off by 0.0025 of its
 // norm, of which its own rounding is 0.0017; two bf16 parts of either would double the products. O is rescaled only
 // when a row's maximum has grown by more than 2^8 since the last time: O and the sum carry the same
 // reference, so the result does not depend on which one it is. While S of tile j is in the softmax,
 // the tensor cores run S of tile j + 1 and P V of tile j - 1. Measured: a prompt of 16384 rows, 16 query and 2 KV heads
-// of 256: 1.59 ms in a burst, 1.38 PFLOP/s (of the visible pairs; the tiles on the diagonal are computed whole); held for
-// seconds, under the power limit, 1.81 ms.
+// of 256: 1.77 ms held for seconds, under the power limit, 1.24 PFLOP/s (of the visible pairs; the tiles on the diagonal
+// are computed whole); one call alone 1.54 ms, 1.42 PFLOP/s. Pages that no box fits (below): 4096 rows 870 us with 7
+// rows a page, 198 us with 16.
 //
 // Pages: a warp of each CTA copies boxes of page rows by TMA (the rows of a box lie in one page, as
 // a tile's 64 positions may lie in many). Positions behind a sequence's end, and pages that are
@@ -42,7 +43,7 @@ namespace nmoe {
 namespace {
 
 struct PrefillArgs {
-    CUtensorMap k_map, v_map;   // pages as 4D tensors, boxes of 64 columns x box_rows
+    CUtensorMap k_map, v_map;   // pages as 5D tensors (page_map), boxes of box_rows rows and one or more panels of 64 columns
     CUtensorMap q_map;          // prepared queries, boxes of 64 columns x 128 rows
     uint16_t *q_ready;
     int prep_rows, share_log;
@@ -80,9 +81,9 @@ struct Cfg {
     // A step is what goes through the softmax at a time: at head_dim 256 a tile, at 128 half of one (32 of each
     // CTA's 64 positions). Two steps' scores lie in tensor memory, so that the next one's product runs beside the
     // softmax. At 256 a CTA has the SM; at 128 a step's products take a quarter of that time and its softmax, a chain
-    // of waits, is what lasts: two CTAs share the SM. Seven packed prompts of 1 to 3000 rows, 24 query and 4 KV
-    // heads, behind up to 8191 positions: 248 us; with whole tiles, one at a time, 265 us, and with one CTA
-    // an SM 331 us
+    // of waits, is what lasts: two CTAs share the SM (at 80 registers a thread, 32 bytes of which are spilled).
+    // Seven packed prompts of 1 to 3000 rows, 24 query and 4 KV heads, behind up to 8191 positions: 252 us; when
+    // these were compared, at 250, with whole tiles, one at a time, 265 us, and with one CTA an SM 331 us
     static constexpr int kCtas = D == 256 ? 1 : 2, kHalves = D == 256 ? 1 : 2;
     static constexpr int kCols = 64 / kHalves, kStep = 2 * kCols;   // columns of a thread, of a step
     static constexpr int kStages = D == 256 ? 5 : 4;
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(kPrepThreads) k_prefill_queries(const __grid_c
 }
 
 // A warp that copies one unit's K tiles, or its V tiles, into the ring. The ring's stages are taken
-// in the order of the MMAs (K 0, K 1, V 0, K 2, V 1, ..), so each of the two warps knows its stages.
+// in the order of the MMAs (Cfg::k_stage, v_stage), so each of the two warps knows its stages.
 template <int D>
 struct Copier {
     const PrefillArgs &a;
@@ -933,7 +934,7 @@ extern "C" int nmoe_full_attn_prefill_paged(const nmoe_full_attn_weights *w, con
     a.x_bf16 = x_dtype == NMOE_DTYPE_BF16;
     a.q_ready = static_cast<uint16_t *>(workspace);
     const uint32_t tries = wait_tries();
-    a.tries = (tries + 63) / 64;   // of up to 20 us each
+    a.tries = tries / 64 + (tries % 64 != 0);   // of up to 20 us each
     a.nap = tries < 20000 ? tries : 20000;
     int sms = 0;
     if ((rc = device_sm_count(&sms)) != NMOE_OK) return rc;
